@@ -439,6 +439,109 @@ neon_status neon_attn_prefill(const uint16_t* q, const uint16_t* k_cache,
                               uint16_t* out, int M, int Hq, int Hkv, int D,
                               int T_max, int window, void* stream);
 
+/* ---- paged KV cache ------------------------------------------------------ */
+/* A cache of fixed-size pages that sequences hold in any number and order: a
+ * sequence's token t sits in page page_table[b][t / page_size], row
+ * t % page_size.  The caller allocates the pools and hands out the pages; a
+ * page may be read by several sequences (a shared prefix), and is written by
+ * neon_paged_append only. */
+enum {
+  NEON_KV_BF16 = 0,  /* k, v: bf16 [n_pages][n_kv_heads][page_size][head_dim]        */
+  NEON_KV_MXFP4 = 1  /* k, v: codes [n_pages][n_kv_heads][page_size][head_dim / 2],
+                      * low nibble = even element; k_scales, v_scales: E8M0
+                      * [n_pages][n_kv_heads][page_size][head_dim / 32]               */
+};
+typedef struct neon_paged_kv {
+  void *k, *v;                  /* device, 16-byte aligned                            */
+  uint8_t *k_scales, *v_scales; /* device, 16-byte aligned; NULL for NEON_KV_BF16     */
+  int32_t format;               /* NEON_KV_*                                          */
+  int32_t n_pages;
+  int32_t page_size;            /* a power of two from 16 to 65536                    */
+  int32_t n_kv_heads;
+  int32_t head_dim;             /* 64 or 128                                          */
+} neon_paged_kv;
+
+/* The paged calls take the rows of B sequences one after another:
+ *   q_start [B + 1]  device int32: sequence b's rows are q_start[b] ..
+ *                    q_start[b + 1] - 1 (none when equal).  NULL: one row per
+ *                    sequence, row b (then n_rows == B).
+ *   kv_len [B]       device int32: the sequence's tokens in the cache, those
+ *                    rows included: its last row has position kv_len[b] - 1.
+ *   page_table       device int32 [B][max_pages]; entries past a sequence's
+ *                    pages are not read.
+ * Rows from q_start[B] to n_rows - 1 (padding) and the rows of a sequence with
+ * kv_len 0 (a free place of the batch) are left as they are.  A sequence whose numbers do not fit (rows outside [0, n_rows], kv_len below its
+ * rows or above max_pages * page_size, a position >= n_pos) is left out, a page
+ * id outside [0, n_pages) drops what it would hold (append, gather) or hides
+ * its keys (attention), and neon_device_check then returns NEON_EINVAL.  (The
+ * reference has no counterpart: it has no model code.) */
+
+/* Rotates and appends: qkv rows [n_rows] of (Hq + 2 n_kv_heads) head_dim bf16,
+ * `qkv_stride` elements apart (a multiple of 8; 16-byte aligned), hold the q,
+ * k and v heads of the projection.  q and k are rotated as neon_rope_yarn does
+ * (table [2][n_pos][head_dim / 2] from neon_rope_table, 16-byte aligned; NULL:
+ * not rotated), q goes to q_out [n_rows][Hq][head_dim] (not overlapping qkv;
+ * Hq may be 0 and q_out then NULL), k and v into the pages.  MXFP4 pages take
+ * the fp32 values: per 32 elements along head_dim the scale is
+ * 2^(floor(log2 amax) - 2), doubled when amax's significand exceeds 1.75, each
+ * element the nearest E2M1 value (ties to even); a block with a non-finite
+ * value gets the scale 0xFF (NaN), a zero block 127. */
+neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t* qkv, int64_t qkv_stride,
+                              const float* table, int n_pos, const int32_t* q_start,
+                              const int32_t* kv_len, const int32_t* page_table, int max_pages,
+                              uint16_t* q_out, int n_rows, int B, int Hq, void* stream);
+
+/* Reads rows back: the positions that neon_paged_append writes for the same
+ * arguments, as bf16 (MXFP4: exact), into k_out, v_out
+ * [n_rows][n_kv_heads][head_dim].  With q_start the running sum of kv_len, the
+ * whole sequences. */
+neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t* q_start,
+                              const int32_t* kv_len, const int32_t* page_table, int max_pages,
+                              uint16_t* k_out, uint16_t* v_out, int n_rows, int B, void* stream);
+
+/* Causal GQA attention over the pages, with per-head sinks (bf16 [Hq], or NULL
+ * for none): q rows [n_rows], `q_stride` elements apart (a multiple of 8,
+ * 16-byte aligned; rotated, head h at h head_dim); the row at position p sees
+ * keys 0 .. p, the last `window` of them when window > 0.  out
+ * [n_rows][Hq head_dim] bf16, 16-byte aligned; a row that sees no key gets 0.
+ * Hq a multiple of n_kv_heads, at most 64 query heads per KV head.  Any number
+ * of rows per sequence: decode steps, drafts and prompt chunks in one call.
+ *   workspace, counters  as neon_attn_decode: neon_paged_attn_workspace(...)
+ *                        bytes of any contents and
+ *                        neon_paged_attn_counters(...) bytes, zero before
+ *                        their first use and left zero by every call. */
+size_t neon_paged_attn_workspace(int n_rows, int B, int Hq, int n_kv_heads, int head_dim);
+size_t neon_paged_attn_counters(int n_rows, int B, int Hq, int n_kv_heads, int head_dim);
+neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                            const uint16_t* sinks, const int32_t* q_start, const int32_t* kv_len,
+                            const int32_t* page_table, int max_pages, uint16_t* out, int n_rows,
+                            int B, int Hq, int window, void* workspace, size_t workspace_bytes,
+                            int32_t* counters, size_t counter_bytes, void* stream);
+
+/* One draw per row of logits (device fp32, rows `stride` >= V elements apart),
+ * each row with its own settings and its own random number u[b] in [0, 1):
+ *   w_i = exp((l_i - max l) / temperature[b]) in 64 bits;
+ *   tokens in the order of (l descending, index ascending): the first top_k[b]
+ *   are kept (0 or less: all); of these the shortest prefix whose mass is at
+ *   least top_p[b] of theirs; of these the tokens with w_i >= min_p[b] (the
+ *   maximum has w = 1);
+ *   out_ids[b] = the lowest kept index whose running sum of w, in index order,
+ *   exceeds u[b] times the kept mass.
+ * Masses are held as multiples of 2^-44 of the maximum's (2^-(62 - log2 V)
+ * past 2^18 tokens): a token below half of that is never drawn.
+ * temperature 0: the maximum (the lowest of equal ones).  NaN counts as -inf; a
+ * row with nothing above -inf gives -1.  Each parameter array is device data
+ * [B]; temperature NULL means 1, top_k / top_p / min_p NULL off.  A row with a
+ * parameter outside its range (temperature < 0 or infinite, top_p outside
+ * (0, 1], min_p outside [0, 1], u outside [0, 1), a NaN) gives -1 and
+ * neon_device_check NEON_EINVAL.  V up to 2^24.  workspace:
+ * neon_sample_rows_workspace(B, V) bytes, 16-byte aligned, any contents. */
+size_t neon_sample_rows_workspace(int B, int V);
+neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
+                             const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, const float* u, int32_t* out_ids,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,6 +40,8 @@ EXPORTS = (
     "neon_rope_table", "neon_moe_layer_workspace", "neon_attn_decode_workspace",
     "neon_attn_decode_counters", "neon_sample_workspace", "neon_moe_prefill_workspace",
     "neon_seq_add", "neon_seq_remove",
+    "neon_paged_append", "neon_paged_gather", "neon_paged_attn", "neon_paged_attn_workspace",
+    "neon_paged_attn_counters", "neon_sample_rows", "neon_sample_rows_workspace",
 )
 
 
@@ -60,6 +62,13 @@ class Config(C.Structure):
 
     def as_dict(self):
         return {n: getattr(self, n) for n, _ in self._fields_}
+
+
+class PagedKVStruct(C.Structure):
+    """neon_paged_kv."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p)] + [(n, C.c_int32) for n in (
+                    "format", "n_pages", "page_size", "n_kv_heads", "head_dim")]
 
 
 _lib = None
@@ -124,6 +133,11 @@ def lib():
             "neon_gemv_bf16_mfma": [_P, _P, _P, _P, _I, _I, _I, _P],
             "neon_device_check": [_P],
             "neon_moe_layer_noalloc": [_P] * 13 + [_I] * 5 + [_F, _F, _P],
+            "neon_paged_append": [_P, _P, _I64, _P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _P],
+            "neon_paged_gather": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _P],
+            "neon_paged_attn": [_P, _P, _I64, _P, _P, _P, _P, _I, _P] + [_I] * 4 +
+                               [_P, _SZ, _P, _SZ, _P],
+            "neon_sample_rows": [_P, _I64, _I, _I] + [_P] * 7 + [_SZ, _P],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -134,7 +148,10 @@ def lib():
                            "neon_attn_decode_workspace": [_I] * 6,
                            "neon_attn_decode_counters": [_I] * 2,
                            "neon_sample_workspace": [_I] * 2,
-                           "neon_moe_prefill_workspace": [_I] * 6}.items():
+                           "neon_moe_prefill_workspace": [_I] * 6,
+                           "neon_paged_attn_workspace": [_I] * 5,
+                           "neon_paged_attn_counters": [_I] * 5,
+                           "neon_sample_rows_workspace": [_I] * 2}.items():
             f = getattr(L, name)
             f.argtypes = args
             f.restype = _SZ
@@ -368,6 +385,181 @@ def sample_logits(logits, B, V, temperature, top_p, seed, pos, out_ids, stream=N
     _check(lib().neon_sample(_ptr(logits), B, V, temperature, top_p, seed, _ptr(pos),
                              _ptr(out_ids), _ptr(workspace), _nbytes(workspace),
                              _stream(stream)))
+
+
+KV_BF16, KV_MXFP4 = 0, 1
+
+
+class PagedKV:
+    """A paged KV cache over the caller's pools (neon_paged_kv).
+
+    k, v: bf16 [n_pages][n_kv_heads][page_size][head_dim]; or, with k_scales
+    and v_scales (uint8 [..][head_dim / 32]), MXFP4 codes (uint8 [..][head_dim / 2])."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        mx = k_scales is not None
+        pools = (k, v, k_scales, v_scales) if mx or v_scales is not None else (k, v)
+        if any(t is None or t.dim() != 4 for t in pools):
+            raise ValueError("PagedKV: pools are [n_pages][n_kv_heads][page_size][..], MXFP4 ones "
+                             "with scales for both")
+        n_pages, heads, page, width = k.shape
+        dim = width * 2 if mx else width
+        if tuple(v.shape) != tuple(k.shape) or \
+                any(tuple(t.shape) != (n_pages, heads, page, dim // 32) for t in pools[2:]):
+            raise ValueError("PagedKV: k, v (and their scales) must have matching shapes")
+        if any(t.element_size() != (1 if mx else 2) for t in pools):
+            raise ValueError("PagedKV: bf16 pools have 2-byte elements, MXFP4 codes and scales 1")
+        self.pools = pools  # keeps them alive
+        self.device = k.device
+        self.format = KV_MXFP4 if mx else KV_BF16
+        self.n_kv_heads, self.head_dim = heads, dim
+        self.struct = PagedKVStruct(*(_ptr(t) for t in pools), *(() if mx else (None, None)),
+                                    self.format, n_pages, page, heads, dim)
+        self.ref = C.addressof(self.struct)
+
+
+def paged_kv(k, v, k_scales=None, v_scales=None) -> PagedKV:
+    return PagedKV(k, v, k_scales, v_scales)
+
+
+def _sized(t, dtype_bytes, n, name, device):
+    """t as this many elements of this size on this device, or ValueError: the
+    library trusts the sizes that the paged calls derive from other tensors."""
+    if t.element_size() != dtype_bytes or t.numel() < n or t.device != device:
+        raise ValueError(f"{name}: needs {n} elements of {dtype_bytes} bytes on {device}, has "
+                         f"{t.numel()} of {t.element_size()} on {t.device}")
+
+
+def _on_current(device):
+    """The calls go to the current device: tensors elsewhere are refused."""
+    if device.type != "cuda" or device.index != _torch_cuda().current_device():
+        raise ValueError(f"tensors on {device}: the call runs on the current HIP device")
+
+
+def _torch_cuda():
+    import torch
+    return torch.cuda
+
+
+def _row_stride(x, name):
+    """Rows of a 2-D or dense 3-D tensor, and the elements between them (a
+    slice of wider rows is fine)."""
+    inner = x.stride()[1:] if x.dim() > 1 else ()
+    want = {2: (1,), 3: (x.shape[2] if x.dim() == 3 else 0, 1)}.get(x.dim())
+    if want is None or any(s != w and n > 1 for s, w, n in zip(inner, want, x.shape[1:])):
+        raise ValueError(f"{name}: rows of contiguous elements, [n_rows][width] or "
+                         "[n_rows][heads][head_dim]")
+    width = x.numel() // x.shape[0] if x.shape[0] else 0
+    return x.shape[0], (x.stride(0) if x.shape[0] > 1 else width), width
+
+
+def _paged_rows(kv, q_start, kv_len, page_table, n_rows):
+    _on_current(kv.device)
+    B = kv_len.shape[0]
+    if page_table.dim() != 2:
+        raise ValueError("page_table: [B][max_pages]")
+    _sized(kv_len, 4, B, "kv_len", kv.device)
+    _sized(page_table, 4, B * page_table.shape[1], "page_table", kv.device)
+    if page_table.shape[0] != B:
+        raise ValueError("page_table: one row per sequence of kv_len")
+    if q_start is not None:
+        _sized(q_start, 4, B + 1, "q_start", kv.device)
+    elif n_rows != B:
+        raise ValueError("without q_start there is one row per sequence")
+    return B, page_table.shape[1]
+
+
+def paged_append(kv, qkv, table, q_start, kv_len, page_table, q_out, Hq, stream=None):
+    """Rotates q and k of the rows qkv [n_rows][(Hq + 2 n_kv_heads) head_dim]
+    and appends k and v to the pages (neon_paged_append).  table: from
+    rope_table, fp32 [2][n_pos][head_dim / 2], or None (no rotation)."""
+    n, stride, width = _row_stride(qkv, "qkv")
+    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
+    D = kv.head_dim
+    _sized(qkv, 2, n * (Hq + 2 * kv.n_kv_heads) * D, "qkv", kv.device)
+    if n and width < (Hq + 2 * kv.n_kv_heads) * D:
+        raise ValueError("qkv: rows of (Hq + 2 n_kv_heads) head_dim")
+    if Hq:
+        _sized(q_out, 2, n * Hq * D, "q_out", kv.device)
+    n_pos = 0
+    if table is not None:
+        if table.dim() != 3 or table.shape[0] != 2 or table.shape[2] != D // 2:
+            raise ValueError("table: [2][n_pos][head_dim / 2]")
+        n_pos = table.shape[1]
+        _sized(table, 4, n_pos * D, "table", kv.device)
+    _check(lib().neon_paged_append(kv.ref, qkv.data_ptr(), stride, _ptr(table), n_pos,
+                                   _ptr(q_start), _ptr(kv_len), _ptr(page_table), max_pages,
+                                   _ptr(q_out), n, B, Hq, _stream(stream)))
+
+
+def paged_gather(kv, q_start, kv_len, page_table, k_out, v_out, stream=None):
+    """The rows that paged_append writes for the same arguments, as bf16, into
+    k_out and v_out [n_rows][n_kv_heads][head_dim] (neon_paged_gather)."""
+    n = k_out.shape[0]
+    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        _sized(t, 2, n * kv.n_kv_heads * kv.head_dim, name, kv.device)
+    _check(lib().neon_paged_gather(kv.ref, _ptr(q_start), _ptr(kv_len), _ptr(page_table),
+                                   max_pages, _ptr(k_out), _ptr(v_out), n, B, _stream(stream)))
+
+
+def paged_attn_workspace(n_rows, B, Hq, Hkv, D):
+    """(workspace bytes, counter bytes) of neon_paged_attn."""
+    L = lib()
+    return (L.neon_paged_attn_workspace(n_rows, B, Hq, Hkv, D),
+            L.neon_paged_attn_counters(n_rows, B, Hq, Hkv, D))
+
+
+def paged_attn(kv, q, sinks, q_start, kv_len, page_table, out, Hq, window=0, stream=None,
+               workspace=None, counters=None):
+    """Attention of the rows q [n_rows][Hq head_dim] over the pages
+    (neon_paged_attn).  counters: zero-filled once by the caller (each call
+    leaves it zero)."""
+    n, stride, width = _row_stride(q, "q")
+    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
+    D = kv.head_dim
+    _sized(q, 2, n * Hq * D, "q", kv.device)
+    if n and width < Hq * D:
+        raise ValueError("q: rows of Hq head_dim")
+    _sized(out, 2, n * Hq * D, "out", kv.device)
+    if sinks is not None:
+        _sized(sinks, 2, Hq, "sinks", kv.device)
+    if workspace is None or counters is None:
+        wb, cb = paged_attn_workspace(n, B, Hq, kv.n_kv_heads, D)
+        if workspace is None:
+            workspace = _workspace(wb)
+        if counters is None:
+            counters = _workspace(cb, zero=True)
+    _check(lib().neon_paged_attn(kv.ref, q.data_ptr(), stride, _ptr(sinks), _ptr(q_start),
+                                 _ptr(kv_len), _ptr(page_table), max_pages, _ptr(out), n, B, Hq,
+                                 window, _ptr(workspace), _nbytes(workspace), _ptr(counters),
+                                 _nbytes(counters), _stream(stream)))
+
+
+def sample_rows_workspace(B, V):
+    return lib().neon_sample_rows_workspace(B, V)
+
+
+def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, min_p=None,
+                stream=None, workspace=None):
+    """One draw per row of logits [B][V] (fp32; rows may be a slice of wider
+    ones) from the random numbers u [B], each parameter a device array [B] or
+    None (neon_sample_rows)."""
+    if logits.dim() != 2:
+        raise ValueError("logits: [B][V]")
+    _on_current(logits.device)
+    B, V = logits.shape
+    _, stride, _ = _row_stride(logits, "logits")
+    _sized(logits, 4, B * V, "logits", logits.device)
+    for t, name in ((u, "u"), (out_ids, "out_ids"), (temperature, "temperature"),
+                    (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p")):
+        if t is not None:
+            _sized(t, 4, B, name, logits.device)
+    if workspace is None:
+        workspace = _workspace(sample_rows_workspace(B, V))
+    _check(lib().neon_sample_rows(logits.data_ptr(), stride, B, V, _ptr(temperature), _ptr(top_k),
+                                  _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(out_ids),
+                                  _ptr(workspace), _nbytes(workspace), _stream(stream)))
 
 
 PREFILL_BATCHED, PREFILL_STEPWISE, PREFILL_CHUNKED, PREFILL_MX8 = 0, 1, 2, 3

@@ -1722,6 +1722,15 @@ extern "C" neon_status neon_device_check(void* stream) {
   if (bits & kDevErrSyncTimeout)
     KFAIL(NEON_EHIP, "a grid-wide wait inside a kernel-level call timed out (status bits 0x%x); "
           "its results are invalid", bits);
+  if (bits & kDevErrPagedRows)
+    KFAIL(NEON_EINVAL, "a paged call saw row starts or lengths outside its buffers (status bits "
+          "0x%x); that sequence was left out", bits);
+  if (bits & kDevErrPageId)
+    KFAIL(NEON_EINVAL, "a paged call needed a page id outside [0, n_pages) (status bits 0x%x); "
+          "that page's rows were dropped or hidden", bits);
+  if (bits & kDevErrSampleParam)
+    KFAIL(NEON_EINVAL, "neon_sample_rows saw a row's parameter out of range (status bits 0x%x); "
+          "that row's id is -1", bits);
   KFAIL(NEON_EINVAL, "a kernel-level call saw an expert id outside [0, E) (status bits 0x%x); "
         "that slot was dropped", bits);
 }
@@ -2226,5 +2235,163 @@ extern "C" neon_status neon_attn_prefill(const uint16_t* q, const uint16_t* k_ca
   if (!kBatchedPrefillEnabled)
     KFAIL(NEON_ESTATE, "neon_attn_prefill: the batched prompt pass is switched off");
   launch_attn_prefill(q, k_cache, v_cache, sinks, out, M, Hq, Hkv, T_max, window, S(stream));
+  KLAUNCHED();
+}
+
+// ---- paged KV cache ---------------------------------------------------------
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The cache and the batch of a paged call; false (with the reason in `why`)
+// when they are not ones that the kernels take.
+static bool paged_args(const neon_paged_kv* kv, const int32_t* q_start, const int32_t* kv_len,
+                       const int32_t* page_table, int max_pages, int n_rows, int B, PagedKv& c,
+                       PagedRows& r, const char*& why) {
+  why = "null pointer";
+  if (!kv || !kv->k || !kv->v || !kv_len || !page_table) return false;
+  why = "format";
+  if (kv->format != NEON_KV_BF16 && kv->format != NEON_KV_MXFP4) return false;
+  const bool f4 = kv->format == NEON_KV_MXFP4;
+  why = "k_scales and v_scales belong to NEON_KV_MXFP4";
+  if (f4 != (kv->k_scales != nullptr) || f4 != (kv->v_scales != nullptr)) return false;
+  why = "pools must be 16-byte aligned";
+  if (!aligned16(kv->k) || !aligned16(kv->v) || !aligned16(kv->k_scales) ||
+      !aligned16(kv->v_scales))
+    return false;
+  why = "page_size must be a power of two from 16 to 65536";
+  const int ps = kv->page_size;
+  if (ps < 16 || ps > 65536 || (ps & (ps - 1)) != 0) return false;
+  why = "head_dim must be 64 or 128";
+  if (kv->head_dim != 64 && kv->head_dim != 128) return false;
+  why = "n_pages, n_kv_heads or max_pages";
+  if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 1024 || max_pages < 1) return false;
+  why = "n_rows or B (B 1 to 65535, n_rows up to 2^24, n_rows == B without q_start)";
+  if (B < 1 || B > 65535 || n_rows < 0 || n_rows > (1 << 24) || (!q_start && n_rows != B))
+    return false;
+  c.k = (uint8_t*)kv->k; c.v = (uint8_t*)kv->v;
+  c.ks = kv->k_scales; c.vs = kv->v_scales;
+  c.n_pages = kv->n_pages; c.page_log2 = __builtin_ctz((unsigned)ps);
+  c.Hkv = kv->n_kv_heads; c.D = kv->head_dim;
+  r.q_start = q_start; r.kv_len = kv_len; r.table = page_table;
+  r.max_pages = max_pages; r.n_rows = n_rows; r.B = B;
+  r.err = nullptr;
+  return true;
+}
+
+extern "C" neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t* qkv,
+                                         int64_t qkv_stride, const float* table, int n_pos,
+                                         const int32_t* q_start, const int32_t* kv_len,
+                                         const int32_t* page_table, int max_pages,
+                                         uint16_t* q_out, int n_rows, int B, int Hq,
+                                         void* stream) {
+  PagedKv c;
+  PagedRows r;
+  const char* why;
+  if (!paged_args(kv, q_start, kv_len, page_table, max_pages, n_rows, B, c, r, why))
+    KFAIL(NEON_EINVAL, "neon_paged_append: %s", why);
+  if (!qkv || Hq < 0 || Hq > 65535 || (Hq > 0 && !q_out))
+    KFAIL(NEON_EINVAL, "neon_paged_append: null pointer or Hq=%d", Hq);
+  if (qkv_stride < (int64_t)(Hq + 2 * c.Hkv) * c.D || qkv_stride % 8 || !aligned16(qkv) ||
+      !aligned16(q_out) || !aligned16(table))
+    KFAIL(NEON_EINVAL, "neon_paged_append: rows must be 16-byte aligned, a multiple of 8 elements "
+          "and at least (Hq + 2 n_kv_heads) head_dim apart");
+  if (table && n_pos < 1) KFAIL(NEON_EINVAL, "neon_paged_append: n_pos=%d", n_pos);
+  if (n_rows == 0) return NEON_OK;
+  r.err = device_status_word();
+  launch_paged_append(c, r, qkv, qkv_stride, table,
+                      table ? table + (size_t)n_pos * (c.D / 2) : nullptr, n_pos, q_out, Hq,
+                      S(stream));
+  KLAUNCHED();
+}
+
+extern "C" neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t* q_start,
+                                         const int32_t* kv_len, const int32_t* page_table,
+                                         int max_pages, uint16_t* k_out, uint16_t* v_out,
+                                         int n_rows, int B, void* stream) {
+  PagedKv c;
+  PagedRows r;
+  const char* why;
+  if (!paged_args(kv, q_start, kv_len, page_table, max_pages, n_rows, B, c, r, why))
+    KFAIL(NEON_EINVAL, "neon_paged_gather: %s", why);
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+    KFAIL(NEON_EINVAL, "neon_paged_gather: k_out and v_out must be given, 16-byte aligned");
+  if (n_rows == 0) return NEON_OK;
+  r.err = device_status_word();
+  launch_paged_gather(c, r, k_out, v_out, S(stream));
+  KLAUNCHED();
+}
+
+static bool paged_attn_shape_ok(int n_rows, int B, int Hq, int Hkv, int D) {
+  return n_rows >= 0 && n_rows <= (1 << 24) && B >= 1 && B <= 65535 && Hkv >= 1 && Hkv <= 1024 &&
+         Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 64 && (D == 64 || D == 128);
+}
+
+extern "C" size_t neon_paged_attn_workspace(int n_rows, int B, int Hq, int n_kv_heads,
+                                            int head_dim) {
+  if (!paged_attn_shape_ok(n_rows, B, Hq, n_kv_heads, head_dim)) return 0;
+  return 0;
+}
+
+extern "C" size_t neon_paged_attn_counters(int n_rows, int B, int Hq, int n_kv_heads,
+                                           int head_dim) {
+  if (!paged_attn_shape_ok(n_rows, B, Hq, n_kv_heads, head_dim)) return 0;
+  return 0;
+}
+
+extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* q,
+                                       int64_t q_stride, const uint16_t* sinks,
+                                       const int32_t* q_start, const int32_t* kv_len,
+                                       const int32_t* page_table, int max_pages, uint16_t* out,
+                                       int n_rows, int B, int Hq, int window, void* workspace,
+                                       size_t workspace_bytes, int32_t* counters,
+                                       size_t counter_bytes, void* stream) {
+  PagedAttnArgs a;
+  const char* why;
+  if (!paged_args(kv, q_start, kv_len, page_table, max_pages, n_rows, B, a.kv, a.r, why))
+    KFAIL(NEON_EINVAL, "neon_paged_attn: %s", why);
+  if (!paged_attn_shape_ok(n_rows, B, Hq, a.kv.Hkv, a.kv.D))
+    KFAIL(NEON_EINVAL, "neon_paged_attn: Hq=%d must be a multiple of n_kv_heads=%d, at most 64 "
+          "per KV head", Hq, a.kv.Hkv);
+  if (!q || !out || !aligned16(q) || !aligned16(out) || q_stride % 8 ||
+      q_stride < (int64_t)Hq * a.kv.D || window < 0)
+    KFAIL(NEON_EINVAL, "neon_paged_attn: q and out must be given, 16-byte aligned, q rows a "
+          "multiple of 8 elements and at least Hq head_dim apart, window >= 0");
+  const size_t need = neon_paged_attn_workspace(n_rows, B, Hq, a.kv.Hkv, a.kv.D);
+  const size_t needc = neon_paged_attn_counters(n_rows, B, Hq, a.kv.Hkv, a.kv.D);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    KFAIL(NEON_EINVAL, "neon_paged_attn: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace_bytes, need);
+  if (needc > 0 && (!counters || counter_bytes < needc || !aligned16(counters)))
+    KFAIL(NEON_EINVAL, "neon_paged_attn: counters of %zu bytes, %zu needed (16-byte aligned)",
+          counter_bytes, needc);
+  if (n_rows == 0) return NEON_OK;
+  a.r.err = device_status_word();
+  a.q = q; a.q_stride = q_stride; a.sinks = sinks; a.out = out; a.Hq = Hq; a.window = window;
+  launch_paged_attn(a, S(stream));
+  KLAUNCHED();
+}
+
+extern "C" size_t neon_sample_rows_workspace(int B, int V) {
+  if (B < 1 || B > 65535 || V < 1 || V > (1 << 24)) return 0;
+  return 0;
+}
+
+extern "C" neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
+                                        const float* temperature, const int32_t* top_k,
+                                        const float* top_p, const float* min_p, const float* u,
+                                        int32_t* out_ids, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  if (!logits || !u || !out_ids) KFAIL(NEON_EINVAL, "neon_sample_rows: null pointer");
+  if (B < 1 || B > 65535 || V < 1 || V > (1 << 24) || stride < V)
+    KFAIL(NEON_EINVAL, "neon_sample_rows: bad shape B=%d V=%d stride=%lld", B, V,
+          (long long)stride);
+  const size_t need = neon_sample_rows_workspace(B, V);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    KFAIL(NEON_EINVAL, "neon_sample_rows: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace_bytes, need);
+  SampleRowsArgs a;
+  a.logits = logits; a.stride = stride; a.B = B; a.V = V;
+  a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
+  a.ids = out_ids; a.err = device_status_word();
+  launch_sample_rows(a, S(stream));
   KLAUNCHED();
 }

@@ -144,6 +144,9 @@ void launch_gemv_o_router(const GemvArgs& o, const RouterArgs& r, hipStream_t st
 // when its input breaks a precondition it can only see on the device.
 constexpr int32_t kDevErrExpertId = 1;      // an expert id outside [0, E)
 constexpr int32_t kDevErrSyncTimeout = 2;   // a grid-wide wait gave up (results invalid)
+constexpr int32_t kDevErrPagedRows = 4;     // q_start / kv_len of a paged batch out of range
+constexpr int32_t kDevErrPageId = 8;        // a page id outside [0, n_pages) where a page is needed
+constexpr int32_t kDevErrSampleParam = 16;  // a row's sampling parameter out of range
 // polls a grid-wide wait makes before it gives up (~1 s)
 constexpr int kMoeSpinLimit = 1 << 20;
 
@@ -394,5 +397,57 @@ inline size_t mx8_scale_bytes(size_t rows, int K) { return rows * (size_t)mx8_sc
 void launch_mx8_quant_lines(const uint16_t* x, int64_t rows, int K, uint8_t* q, uint32_t* qs,
                             hipStream_t st);
 void launch_moe_prefill(const MoePrefillArgs& a, hipStream_t st);
+
+// ---- paged KV cache (neon_paged.hip) ------------------------------------------
+// Pages [n_pages][Hkv][page][D] (bf16), or codes [..][D/2] and E8M0 scales
+// [..][D/32] (MXFP4); page a power of two >= 16, D 64 or 128.
+struct PagedKv {
+  uint8_t *k, *v;    // bf16 rows or MXFP4 codes
+  uint8_t *ks, *vs;  // MXFP4 scales (NULL: bf16)
+  int n_pages, page_log2, Hkv, D;
+};
+// The rows of B sequences, one after another: sequence b's are q_start[b] ..
+// q_start[b + 1] - 1 (NULL: row b alone), the last of them at position
+// kv_len[b] - 1.
+struct PagedRows {
+  const int32_t *q_start, *kv_len;
+  const int32_t* table;  // page ids [B][max_pages]
+  int max_pages, n_rows, B;
+  int32_t* err;          // status word (kDevErr* bits)
+};
+// qkv rows [n_rows][stride] (Hq q heads, Hkv k heads, Hkv v heads): q rotated
+// into q_out [n_rows][Hq][D], k rotated and v into the pages; cos_t / sin_t
+// [n_pos][D/2], or NULL for no rotation
+void launch_paged_append(const PagedKv& kv, const PagedRows& r, const uint16_t* qkv, int64_t stride,
+                         const float* cos_t, const float* sin_t, int n_pos, uint16_t* q_out, int Hq,
+                         hipStream_t st);
+// the rows of the batch as the cache holds them, [n_rows][Hkv][D] bf16
+void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out, uint16_t* v_out,
+                         hipStream_t st);
+struct PagedAttnArgs {
+  PagedKv kv;
+  PagedRows r;
+  const uint16_t* q;      // rotated q [n_rows][q_stride] (head h at h D)
+  int64_t q_stride;
+  const uint16_t* sinks;  // [Hq] or NULL
+  uint16_t* out;          // [n_rows][Hq D]
+  int Hq, window;
+};
+void launch_paged_attn(const PagedAttnArgs& a, hipStream_t st);
+
+// ---- sampling with a setting per row (neon_sample_rows.hip) --------------------
+struct SampleRowsArgs {
+  const float* logits;  // [B][stride]
+  int64_t stride;
+  int B, V;
+  // per row, each NULL for "off" (temperature: 1)
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  const float* u;  // [B] uniform in [0, 1)
+  int32_t* ids;    // [B]
+  int32_t* err;
+};
+void launch_sample_rows(const SampleRowsArgs& a, hipStream_t st);
 
 }  // namespace neon
