@@ -468,10 +468,11 @@ typedef struct neon_paged_kv {
  *   kv_len [B]       device int32: the sequence's tokens in the cache, those
  *                    rows included: its last row has position kv_len[b] - 1.
  *   page_table       device int32 [B][max_pages]; entries past a sequence's
- *                    pages are not read.
+ *                    pages, and before those that a window reaches, are not
+ *                    read.
  * Rows from q_start[B] to n_rows - 1 (padding) and the rows of a sequence with
  * kv_len 0 (a free place of the batch) are left as they are.  A sequence whose numbers do not fit (rows outside [0, n_rows], kv_len below its
- * rows or above max_pages * page_size, a position >= n_pos) is left out, a page
+ * rows or above max_pages * page_size or 2^30, a position >= n_pos) is left out, a page
  * id outside [0, n_pages) drops what it would hold (append, gather) or hides
  * its keys (attention), and neon_device_check then returns NEON_EINVAL.  (The
  * reference has no counterpart: it has no model code.) */

@@ -2264,8 +2264,8 @@ static bool paged_args(const neon_paged_kv* kv, const int32_t* q_start, const in
   if (kv->head_dim != 64 && kv->head_dim != 128) return false;
   why = "n_pages, n_kv_heads or max_pages";
   if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 1024 || max_pages < 1) return false;
-  why = "n_rows or B (B 1 to 65535, n_rows up to 2^24, n_rows == B without q_start)";
-  if (B < 1 || B > 65535 || n_rows < 0 || n_rows > (1 << 24) || (!q_start && n_rows != B))
+  why = "n_rows or B (B 1 to 65535, n_rows up to 2^23, n_rows == B without q_start)";
+  if (B < 1 || B > 65535 || n_rows < 0 || n_rows > (1 << 23) || (!q_start && n_rows != B))
     return false;
   c.k = (uint8_t*)kv->k; c.v = (uint8_t*)kv->v;
   c.ks = kv->k_scales; c.vs = kv->v_scales;
@@ -2321,20 +2321,21 @@ extern "C" neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t*
 }
 
 static bool paged_attn_shape_ok(int n_rows, int B, int Hq, int Hkv, int D) {
-  return n_rows >= 0 && n_rows <= (1 << 24) && B >= 1 && B <= 65535 && Hkv >= 1 && Hkv <= 1024 &&
-         Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 64 && (D == 64 || D == 128);
+  return n_rows >= 0 && n_rows <= (1 << 23) && B >= 1 && B <= 65535 && Hkv >= 1 && Hkv <= 1024 &&
+         Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 64 && (D == 64 || D == 128) &&
+         paged_attn_fits(n_rows, B, Hq, Hkv);
 }
 
 extern "C" size_t neon_paged_attn_workspace(int n_rows, int B, int Hq, int n_kv_heads,
                                             int head_dim) {
   if (!paged_attn_shape_ok(n_rows, B, Hq, n_kv_heads, head_dim)) return 0;
-  return 0;
+  return paged_attn_workspace(head_dim);
 }
 
 extern "C" size_t neon_paged_attn_counters(int n_rows, int B, int Hq, int n_kv_heads,
                                            int head_dim) {
   if (!paged_attn_shape_ok(n_rows, B, Hq, n_kv_heads, head_dim)) return 0;
-  return 0;
+  return paged_attn_counters();
 }
 
 extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* q,
@@ -2350,7 +2351,7 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
     KFAIL(NEON_EINVAL, "neon_paged_attn: %s", why);
   if (!paged_attn_shape_ok(n_rows, B, Hq, a.kv.Hkv, a.kv.D))
     KFAIL(NEON_EINVAL, "neon_paged_attn: Hq=%d must be a multiple of n_kv_heads=%d, at most 64 "
-          "per KV head", Hq, a.kv.Hkv);
+          "per KV head, and n_rows=%d fit a launch", Hq, a.kv.Hkv, n_rows);
   if (!q || !out || !aligned16(q) || !aligned16(out) || q_stride % 8 ||
       q_stride < (int64_t)Hq * a.kv.D || window < 0)
     KFAIL(NEON_EINVAL, "neon_paged_attn: q and out must be given, 16-byte aligned, q rows a "
@@ -2366,6 +2367,7 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
   if (n_rows == 0) return NEON_OK;
   a.r.err = device_status_word();
   a.q = q; a.q_stride = q_stride; a.sinks = sinks; a.out = out; a.Hq = Hq; a.window = window;
+  a.part = (float*)workspace; a.arrive = counters;
   launch_paged_attn(a, S(stream));
   KLAUNCHED();
 }

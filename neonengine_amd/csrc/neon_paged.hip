@@ -17,14 +17,15 @@ namespace neon {
 // ---------------------------------------------------------------------------
 // Whether sequence b's rows and length are ones that the buffers hold (device
 // data: checked before anything is addressed with it).  A sequence of length 0
-// is a free place of the batch: it has no rows to take.
+// is a free place of the batch: it has no rows to take.  Lengths up to 2^30
+// keep every index below within an int.
 __device__ __forceinline__ bool paged_seq(const PagedRows& r, int page_log2, int b, int& start,
                                           int& n, int& len) {
   start = r.q_start != nullptr ? r.q_start[b] : b;
   const int end = r.q_start != nullptr ? r.q_start[b + 1] : b + 1;
   len = r.kv_len[b];
   n = end - start;
-  return start >= 0 && n >= 0 && end <= r.n_rows && len >= n &&
+  return start >= 0 && n >= 0 && end <= r.n_rows && len >= n && len <= (1 << 30) &&
          (int64_t)len <= ((int64_t)r.max_pages << page_log2);
 }
 
@@ -257,80 +258,527 @@ void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out,
 }
 
 // ---------------------------------------------------------------------------
-// Attention: one wave per (row, query head), 64 keys at a time: lane = key for
-// the scores, lane = output dims for P V, running maximum and sum in fp32.
+// Attention
+//
+// For a KV head g the query rows of a sequence are its (token, head of the
+// group) pairs r = i G + (h mod G), so one read of a key or value serves the
+// G heads and as many tokens as a tile of rows holds.  A unit of work is
+// (sequence, tile of R rows, KV head); its keys are cut into chunks of one
+// size for the whole call, and a block takes a chunk of a unit.
+//
+// The chunk is chosen on the device from the lengths that are there: W = sum of
+// (row tiles x keys) over the sequences, chunk = W Hkv / target rounded up, so
+// that about `target` blocks of equal work exist whatever the lengths are (a
+// batch of one long and many short sequences fills the chip as evenly as equal
+// ones).  Every wave finds its block's place by itself, lane = sequence, so
+// there is no planning launch and nothing on the host depends on the lengths.
+//   blocks  <= W Hkv / chunk + units <= target + units: the host's grid;
+//   blocks of units with more than one chunk (ceil(x) <= 2 x for x > 1)
+//           <= 2 target: their partial results have slots in the workspace.
+// A unit with one chunk is finished by its block.  Of several, each block
+// leaves (o, m, l) in its slot and arrives on the unit's counter; the last to
+// arrive joins them (stores and loads at agent scope, as in k_attn_split).
 // ---------------------------------------------------------------------------
-template <int D, bool F4>
-__global__ __launch_bounds__(64) void k_paged_attn(PagedAttnArgs a) {
-  __shared__ float qs[D];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  int b, pos;
-  if (!paged_row(a.r, a.kv.page_log2, row, b, pos)) return;
-  const int g = h / (a.Hq / a.kv.Hkv);
-  for (int d = lane; d < D; d += 64) qs[d] = bf2f(a.q[(int64_t)row * a.q_stride + (int64_t)h * D + d]);
-  __syncthreads();
-  const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-  const float scale = D == 64 ? 0.125f : 0.08838834764831845f;
-  float m = -INFINITY, l = 0.0f, o[D / 64];
-  for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-  const int32_t* table = a.r.table + (int64_t)b * a.r.max_pages;
-  for (int k0 = lo; k0 <= pos; k0 += 64) {
-    const int key = k0 + lane;
-    int id = key <= pos ? table[key >> a.kv.page_log2] : -1;
-    const bool seen = (unsigned)id < (unsigned)a.kv.n_pages;
-    if (key <= pos && !seen) flag_dev_err(a.r.err, kDevErrPageId);
-    float s = -INFINITY;
-    if (seen) {
-      const int64_t at = paged_row_at(a.kv, id, g, key);
-      float dot = 0.0f;
-      for (int d0 = 0; d0 < D; d0 += 8) {
-        float kf[8];
-        unpack8f(paged_load8<F4>(a.kv.k, a.kv.ks, at, D, d0), kf);
-        for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(qs[d0 + e], kf[e], dot);
-      }
-      s = dot * scale;
-    }
-    const float mn = fmaxf(m, wave_max(s));
-    if (mn == -INFINITY) continue;
-    const float al = neon_expf(m - mn), p = neon_expf(s - mn);
-    l = l * al + wave_sum(p);
-    m = mn;
-    for (int e = 0; e < D / 64; ++e) o[e] *= al;
-    for (int j = 0; j < 64; ++j) {
-      const int idj = __shfl(seen ? id : -1, j);
-      const float pj = __shfl(p, j);
-      if (idj < 0) continue;
-      const int64_t at = paged_row_at(a.kv, idj, g, k0 + j);
-      for (int e = 0; e < D / 64; ++e) {
-        const int d = lane + 64 * e;
-        float v;
-        if constexpr (F4) {
-          const uint32_t c = a.kv.v[at * (D / 2) + (d >> 1)] >> (4 * (d & 1));
-          v = __uint_as_float(
-              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(
-                                               c & 15u, __uint_as_float((uint32_t)a.kv.vs[at * (D / 32) + (d >> 5)] << 23), 0))
-              << 16);
-        } else {
-          v = bf2f(reinterpret_cast<const uint16_t*>(a.kv.v)[at * D + d]);
-        }
-        o[e] = __builtin_fmaf(pj, v, o[e]);
-      }
-    }
+constexpr int kPaTarget = 1024;   // blocks of equal work to aim at: 4 per CU
+constexpr int kPaArrive = 16;     // ints from one arrival counter to the next
+constexpr int kPaMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef float pf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pbf8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ pf4 pa_mfma(const uint4& a, const uint4& b, pf4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pbf8, a),
+                                                 __builtin_bit_cast(pbf8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A block's work: keys [k0, k1) of a unit, all wave-uniform.
+struct PaWork {
+  int b, start, n, len;  // the sequence, its rows and tokens
+  int row0;              // the tile's first (token, head) row
+  int lo, k0, k1;        // lo: the first key that any row of the tile sees
+  int chunks, slot;      // of the unit; the slot of its chunk 0
+  int c;
+};
+
+// rows and length of a sequence as the attention takes them (0 rows: none)
+__device__ __forceinline__ int pa_seq(const PagedAttnArgs& a, int b, int& start, int& len, bool flag) {
+  int n;
+  if (!paged_seq(a.r, a.kv.page_log2, b, start, n, len)) {
+    if (flag && len != 0) flag_dev_err(a.r.err, kDevErrPagedRows);
+    return 0;
   }
-  if (a.sinks != nullptr) {
-    const float sk = bf2f(a.sinks[h]), M = fmaxf(m, sk);
-    const float al = m == -INFINITY ? 0.0f : neon_expf(m - M);
-    l = l * al + neon_expf(sk - M);
-    for (int e = 0; e < D / 64; ++e) o[e] *= al;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int e = 0; e < D / 64; ++e)
-    a.out[((int64_t)row * a.Hq + h) * D + lane + 64 * e] = f2bf(o[e] * inv);
+  return len > 0 ? n : 0;
 }
 
+// Keys that any row tile of a sequence may take, its first key rounded down to
+// a multiple of ALIGN.
+template <int R, int ALIGN>
+__device__ __forceinline__ int pa_span(const PagedAttnArgs& a, int G, int len) {
+  if (a.window <= 0 || a.window >= len) return len;
+  return min(len, a.window + (R - 1) / G + ALIGN);
+}
+
+// The work of block `idx` (of every KV head alike); false when there is none.
+// ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
+// multiples of 128).
+template <int R, int ALIGN, int MINC>
+__device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool flag, PaWork& w) {
+  const int lane = threadIdx.x & 63;
+  const int G = a.Hq / a.kv.Hkv;
+  const int per = (a.r.B + 63) >> 6;  // consecutive sequences of a lane
+  const int b0 = lane * per, b1 = min(b0 + per, a.r.B);
+  float work = 0.0f;
+  for (int b = b0; b < b1; ++b) {
+    int start, len;
+    const int n = pa_seq(a, b, start, len, flag);
+    work += (float)((n * G + R - 1) / R) * (float)pa_span<R, ALIGN>(a, G, len);
+  }
+  // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
+  // 2^30 on no sequence is longer than a chunk.
+  const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / kPaTarget);
+  const int chunk = max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127);
+  // blocks and slots of the sequences, in order.  Row starts that overlap (an
+  // error that no single sequence shows) can sum to more blocks than the grid
+  // has: the clamp lies above every grid and keeps the sums of 64 lanes in an int.
+  int blocks = 0, slots = 0;
+  for (int b = b0; b < b1; ++b) {
+    int start, len;
+    const int n = pa_seq(a, b, start, len, false);
+    const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
+    const int nb = (n * G + R - 1) / R * nc;
+    blocks = min(blocks + nb, kPaMaxBlocks);
+    slots += nc > 1 ? nb : 0;
+  }
+  int blocks_to = blocks, slots_to = slots;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(blocks_to, o), y = __shfl_up(slots_to, o);
+    if (lane >= o) {
+      blocks_to += x;
+      slots_to += y;
+    }
+  }
+  const uint64_t mine = __ballot(idx < blocks_to);
+  if (mine == 0) return false;
+  const int owner = __builtin_ctzll(mine);
+  // the owner lane's sequences, one by one
+  int at = __builtin_amdgcn_readlane(blocks_to - blocks, owner);
+  int slot = __builtin_amdgcn_readlane(slots_to - slots, owner);
+  for (int b = owner * per; b < min(owner * per + per, a.r.B); ++b) {
+    int start, len;
+    const int n = uni(pa_seq(a, b, start, len, false));
+    start = uni(start);
+    len = uni(len);
+    const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
+    const int nb = (n * G + R - 1) / R * nc;
+    if (idx < at + nb) {
+      const int tile = (idx - at) / nc;
+      w.b = b; w.start = start; w.n = n; w.len = len;
+      w.c = (idx - at) % nc;
+      w.row0 = tile * R;
+      w.slot = slot + tile * nc;
+      const int last = min(w.row0 + R, n * G) - 1;
+      const int pos0 = len - n + w.row0 / G, pos1 = len - n + last / G;
+      w.lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+      const int from = w.lo / ALIGN * ALIGN;
+      w.chunks = (pos1 + 1 - from + chunk - 1) / chunk;
+      w.k0 = from + w.c * chunk;
+      w.k1 = min(w.k0 + chunk, pos1 + 1);
+      return w.c < w.chunks;
+    }
+    at += nb;
+    slot += nc > 1 ? nb : 0;
+  }
+  return false;
+}
+
+// How the kernels take a 16-key step of a wave: S^T = K Q^T with
+// v_mfma_f32_16x16x32_bf16 (A: lane c = lane % 16 a key, group g = lane / 16
+// eight dims; B: lane c a query row), so lane (g, c) holds the scores of row c
+// for the keys 4 g + i, which is also how the second product's B operand wants
+// them: O^T = V^T P^T over 32 keys k = 8 g + j, j < 4 the key 4 g + j of the
+// first 16 and j >= 4 that of the second.  Its A operand needs eight keys'
+// values of one dim in a lane: lane c reads the dims (D/16) c .. of its eight
+// keys and two 16-bit halves are paired by a byte permute, so nothing goes
+// through LDS or other lanes.  The results of row c for the dims (D/4) g ..
+// are in lane (g, c), with the running maximum and sum of row c.
+
+// A wave's two 16-key steps as they come from memory.
+template <int D, bool F4>
+struct PaTile;
+template <int D>
+struct PaTile<D, false> {
+  uint4 k[2][D / 32];      // dims 32 n + 8 g ..
+  uint32_t v[2][4][D / 32];  // keys 4 g + i, dims (D/16) c ..
+};
+template <int D>
+struct PaTile<D, true> {
+  uint32_t k[2][D / 32];     // codes of dims (D/4) g ..
+  uint32_t v[2][4];          // codes of keys 4 g + i, dims (D/16) c ..
+  uint32_t ks[2];            // scale of the key's block
+  uint32_t vs[2][D / 32];    // scales of the keys 4 g .. 4 g + 3
+};
+
+template <int D>
+__device__ __forceinline__ void pa_load(PaTile<D, false>& t, const PagedKv& kv, int g, int c,
+                                        const int64_t (&at)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint8_t* kp = kv.k + at[s] * (2 * D);
+    const uint8_t* vp = kv.v + at[s] * (2 * D);
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+      t.k[s][n] = *reinterpret_cast<const uint4*>(kp + (uint32_t)(c * 2 * D + 64 * n + 16 * g));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* p = vp + (uint32_t)((4 * g + i) * 2 * D + (D / 8) * c);
+      if constexpr (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        t.v[s][i][0] = x.x; t.v[s][i][1] = x.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        t.v[s][i][0] = x.x; t.v[s][i][1] = x.y; t.v[s][i][2] = x.z; t.v[s][i][3] = x.w;
+      }
+    }
+  }
+}
+template <int D>
+__device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, int g, int c,
+                                        const int64_t (&at)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint8_t* kp = kv.k + at[s] * (D / 2);
+    const uint8_t* vp = kv.v + at[s] * (D / 2);
+    const uint8_t* ksp = kv.ks + at[s] * (D / 32);
+    const uint8_t* vsp = kv.vs + at[s] * (D / 32);
+    t.ks[s] = ksp[(uint32_t)(c * (D / 32) + (D == 64 ? g >> 1 : g))];
+    if constexpr (D == 64) {
+      const uint2 x = *reinterpret_cast<const uint2*>(kp + (uint32_t)(c * 32 + 8 * g));
+      t.k[s][0] = x.x; t.k[s][1] = x.y;
+      const uint2 y = *reinterpret_cast<const uint2*>(vsp + (uint32_t)(8 * g));
+      t.vs[s][0] = y.x; t.vs[s][1] = y.y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        t.v[s][i] = *reinterpret_cast<const uint16_t*>(vp + (uint32_t)((4 * g + i) * 32 + 2 * c));
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(kp + (uint32_t)(c * 64 + 16 * g));
+      t.k[s][0] = x.x; t.k[s][1] = x.y; t.k[s][2] = x.z; t.k[s][3] = x.w;
+      const uint4 y = *reinterpret_cast<const uint4*>(vsp + (uint32_t)(16 * g));
+      t.vs[s][0] = y.x; t.vs[s][1] = y.y; t.vs[s][2] = y.z; t.vs[s][3] = y.w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        t.v[s][i] = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)((4 * g + i) * 64 + 4 * c));
+    }
+  }
+}
+
+// operand n of a 16-key step's keys: the dims that pa_query gives B
+template <int D>
+__device__ __forceinline__ uint4 pa_key(const PaTile<D, false>& t, int s, int n) { return t.k[s][n]; }
+template <int D>
+__device__ __forceinline__ uint4 pa_key(const PaTile<D, true>& t, int s, int n) {
+  return mx4_to_bf16x8(t.k[s][n], t.ks[s]);
+}
+template <int D, bool F4>
+__device__ __forceinline__ int pa_query_dim(int n, int g) {
+  return F4 ? (D / 4) * g + 8 * n : 32 * n + 8 * g;
+}
+// values of key 4 g + i, dims (D/16) c ..
+template <int D>
+__device__ __forceinline__ void pa_value(const PaTile<D, false>& t, int s, int i, int,
+                                         uint32_t (&v)[D / 32]) {
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n) v[n] = t.v[s][i][n];
+}
+template <int D>
+__device__ __forceinline__ void pa_value(const PaTile<D, true>& t, int s, int i, int c,
+                                         uint32_t (&v)[D / 32]) {
+  // scale byte i (D/32) + (block of the dims) of the four keys' bytes
+  const int at = i * (D / 32);
+  const uint32_t b = (t.vs[s][at >> 2] >> (8 * (at & 3))) >> (8 * (D == 64 ? c >> 3 : c >> 2));
+  const float sc = __uint_as_float((b & 0xFFu) << 23);
+  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 0));
+  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 1));
+  if constexpr (D == 128) {
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 2));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 3));
+  }
+}
+
+// Joins o (unnormalised, with maximum m in log2 units and sum l) with the sink
+// and gives the factor that finishes it: 0 where nothing was seen.
+__device__ __forceinline__ float pa_finish(const PagedAttnArgs& a, int h, float m, float l) {
+  if (a.sinks == nullptr) return l == 0.0f ? 0.0f : 1.0f / l;
+  const float sk = bf2f(a.sinks[h]) * kLog2e, M = fmaxf(m, sk);
+  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  const float den = l * f + __builtin_amdgcn_exp2f(sk - M);
+  return den == 0.0f ? 0.0f : f / den;
+}
+
+__device__ __forceinline__ uint64_t pa_pair(float x, float y) {
+  return (uint64_t)__float_as_uint(x) | ((uint64_t)__float_as_uint(y) << 32);
+}
+__device__ __forceinline__ void pa_store_agent(float* p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), pa_pair(x, y), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 pa_load_agent(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Few rows: 16 per unit, four waves that share nothing but the result, each
+// with every fourth 32 keys of the chunk, straight from memory into the
+// operands' registers and one step ahead of the products.
+template <int D, bool F4>
+__global__ __launch_bounds__(256) void k_paged_attn(PagedAttnArgs a) {
+  constexpr int R = 16, E = D / 16;
+  __shared__ __align__(16) float so[4][R][D + 4];
+  __shared__ float sm[4][R], sl[4][R];
+  __shared__ int merge_here;
+  const int h = blockIdx.x % a.kv.Hkv;
+  PaWork w;
+  if (!pa_work<R, 32, 256>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int G = a.Hq / a.kv.Hkv;
+  // the lane's query row
+  const int r = w.row0 + c, rows = w.n * G;
+  const bool has = r < rows;
+  const int tok = has ? r / G : 0, hq = h * G + (has ? r % G : 0);
+  const int pos = w.len - w.n + tok;
+  const int k_hi = has ? pos + 1 : 0;
+  const int k_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  // keys that every row of the tile sees
+  const int t_last = (min(w.row0 + R, rows) - 1) / G;
+  const int all_hi = w.len - w.n + w.row0 / G + 1;
+  const int all_lo = a.window > 0 ? max(0, w.len - w.n + t_last - a.window + 1) : 0;
+  uint4 q[D / 32];
+  {
+    const uint16_t* qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      q[n] = *reinterpret_cast<const uint4*>(qp + pa_query_dim<D, F4>(n, g));
+      if (!has) q[n] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  const float c2 = (D == 64 ? 0.125f : 0.08838834764831845f) * kLog2e;
+  pf4 o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+
+  const int tiles = (w.k1 - w.k0 + 31) >> 5;
+  const int n_it = (tiles - wave + 3) >> 2;  // this wave's
+  const int32_t* table = a.r.table + (int64_t)w.b * a.r.max_pages;
+  // page ids of the 16-key steps of 32 iterations, one per lane: -1 past the
+  // keys and where the table's entry is no page
+  auto load_ids = [&](int it) {
+    const int key = w.k0 + 32 * (wave + 4 * (it + (lane >> 1))) + 16 * (lane & 1);
+    int id = -1;
+    if (key < w.k1 && key + 16 > w.lo) {  // pages before the window may be gone
+      id = table[key >> a.kv.page_log2];
+      if ((unsigned)id >= (unsigned)a.kv.n_pages) {
+        id = -1;
+        flag_dev_err(a.r.err, kDevErrPageId);
+      }
+    }
+    return id;
+  };
+  const int page_mask = (1 << a.kv.page_log2) - 1;
+  auto load_tile = [&](PaTile<D, F4>& t, int it, int ids, int (&id)[2]) {
+    const int kb = w.k0 + 32 * (wave + 4 * it);
+    int64_t at[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      id[s] = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + s);
+      at[s] = (((int64_t)max(id[s], 0) * a.kv.Hkv + h) << a.kv.page_log2) +
+              ((kb + 16 * s) & page_mask);
+    }
+    pa_load<D>(t, a.kv, g, c, at);
+  };
+  auto step = [&](const PaTile<D, F4>& t, int it, const int (&id)[2]) {
+    const int kb = w.k0 + 32 * (wave + 4 * it);
+    const bool full = kb >= all_lo && kb + 32 <= all_hi && (id[0] | id[1]) >= 0;
+    float sv[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      pf4 acc = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n) acc = pa_mfma(pa_key<D>(t, s, n), q[n], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sv[s][i] = acc[i];
+        if (!full) {
+          const int key = kb + 16 * s + 4 * g + i;
+          if (key < k_lo || key >= k_hi || id[s] < 0) sv[s][i] = -INFINITY;
+        }
+      }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
+                     fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3]))) * c2;
+    mx = fmaxf(mx, xor_lane<16>(mx));
+    mx = fmaxf(mx, xor_lane<32>(mx));
+    if (__any(mx > m)) {  // rarely, once a row has seen some keys
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= f;
+      m = mn;
+    }
+    const float me = m == -INFINITY ? 0.0f : m;
+    uint32_t hi[4], lo[4];  // P in two bf16 terms
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[s][i], c2, -me));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[s][i + 1], c2, -me));
+        l += p0;
+        l += p1;
+        const uint32_t x = pack_bf2(p0, p1);
+        hi[2 * s + i / 2] = x;
+        lo[2 * s + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
+      }
+    uint32_t v[2][4][D / 32];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pa_value<D>(t, s, i, c, v[s][i]);
+        if (!full) {  // rows that hold no key of the sequence may hold anything
+          const int key = kb + 16 * s + 4 * g + i;
+          const bool none = key >= w.k1 || key < w.lo || id[s] < 0;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) v[s][i][n] = none ? 0u : v[s][i][n];
+        }
+      }
+    const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      uint32_t f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        f[k] = __builtin_amdgcn_perm(v[k >> 1][2 * (k & 1) + 1][e >> 1], v[k >> 1][2 * (k & 1)][e >> 1],
+                                     e & 1 ? 0x07060302u : 0x05040100u);
+      const uint4 vf = make_uint4(f[0], f[1], f[2], f[3]);
+      o[e] = pa_mfma(vf, ph, o[e]);
+      o[e] = pa_mfma(vf, pl, o[e]);
+    }
+  };
+  if (n_it > 0) {
+    PaTile<D, F4> ta, tb;
+    int ida[2], idb[2];
+    int ids = load_ids(0);
+    load_tile(ta, 0, ids, ida);
+    for (int it = 0; it < n_it; it += 2) {
+      // unconditional loads (past the last step, that one again): a load under
+      // a condition is waited for where the paths join
+      int nx = min(it + 1, n_it - 1);
+      load_tile(tb, nx, ids, idb);
+      step(ta, it, ida);
+      if (it + 1 >= n_it) break;
+      nx = min(it + 2, n_it - 1);
+      if ((nx & 31) == 0) ids = load_ids(nx);  // 32 is even: only here
+      load_tile(ta, nx, ids, ida);
+      step(tb, it + 1, idb);
+    }
+  }
+  l += xor_lane<16>(l);
+  l += xor_lane<32>(l);
+  // the four waves' states
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < E; e += 4)
+      *reinterpret_cast<float4*>(&so[wave][c][(D / 4) * g + E * i + e]) =
+          make_float4(o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]);
+  if (g == 0) {
+    sm[wave][c] = m;
+    sl[wave][c] = l;
+  }
+  __syncthreads();
+  // thread: row tr, dims td .. td + E - 1
+  const int tr = tid >> 4, td = (tid & 15) * E;
+  float M = fmaxf(fmaxf(sm[0][tr], sm[1][tr]), fmaxf(sm[2][tr], sm[3][tr]));
+  float L = 0.0f, x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.0f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float f = sm[v][tr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[v][tr] - M);
+    L = __builtin_fmaf(sl[v][tr], f, L);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = __builtin_fmaf(so[v][tr][td + e], f, x[e]);
+  }
+  const int row = w.row0 + tr;
+  if (w.chunks > 1) {
+    const int64_t first = ((int64_t)w.slot * a.kv.Hkv + h);
+    float* po = a.part + (first + (int64_t)w.c * a.kv.Hkv) * R * (D + 2);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) pa_store_agent(po + tr * D + td + e, x[e], x[e + 1]);
+    if ((tid & 15) == 0) pa_store_agent(po + R * D + 2 * tr, M, L);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
+    __syncthreads();
+    int32_t* ctr = a.arrive + first * kPaArrive;
+    if (tid == 0)
+      merge_here = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                   w.chunks - 1;
+    __syncthreads();
+    if (!merge_here) return;
+    if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    M = -INFINITY;
+    L = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.0f;
+    const float* p0 = a.part + first * R * (D + 2);
+    const int64_t step_c = (int64_t)a.kv.Hkv * R * (D + 2);
+    for (int j = 0; j < w.chunks; ++j) {
+      const float2 ml = pa_load_agent(p0 + j * step_c + R * D + 2 * tr);
+      const float mn = fmaxf(M, ml.x);
+      const float fo = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+      const float fn = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+      L = L * fo + ml.y * fn;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 y = pa_load_agent(p0 + j * step_c + tr * D + td + e);
+        x[e] = x[e] * fo + y.x * fn;
+        x[e + 1] = x[e + 1] * fo + y.y * fn;
+      }
+      M = mn;
+    }
+  }
+  if (row >= rows) return;
+  const int head = h * G + row % G;
+  const float fin = pa_finish(a, head, M, L);
+  uint16_t* dst = a.out + ((int64_t)(w.start + row / G) * a.Hq + head) * D + td;
+#pragma unroll
+  for (int e = 0; e < E; e += 4)
+    *reinterpret_cast<uint2*>(dst + e) = make_uint2(pack_bf2(x[e] * fin, x[e + 1] * fin),
+                                                    pack_bf2(x[e + 2] * fin, x[e + 3] * fin));
+}
+
+// Units of R rows that n_rows rows of B sequences can make (per KV head).
+static int64_t pa_units(int n_rows, int B, int G, int R) {
+  return (int64_t)n_rows * G / R + B;
+}
+
+static int64_t pa_blocks(int n_rows, int B, int Hq, int Hkv) {
+  return (kPaTarget / Hkv + 1 + pa_units(n_rows, B, Hq / Hkv, 16)) * Hkv;
+}
+
+bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {
+  return pa_blocks(n_rows, B, Hq, Hkv) < kPaMaxBlocks;
+}
+size_t paged_attn_workspace(int D) { return (size_t)(2 * kPaTarget) * 16 * (D + 2) * 4; }
+size_t paged_attn_counters() { return (size_t)(2 * kPaTarget) * kPaArrive * 4; }
+
 void launch_paged_attn(const PagedAttnArgs& a, hipStream_t st) {
-  const dim3 grid(a.r.n_rows, a.Hq);
-#define PA(D, F4) hipLaunchKernelGGL((k_paged_attn<D, F4>), grid, dim3(64), 0, st, a)
+  const dim3 grid((unsigned)pa_blocks(a.r.n_rows, a.r.B, a.Hq, a.kv.Hkv));
+#define PA(D, F4) hipLaunchKernelGGL((k_paged_attn<D, F4>), grid, dim3(256), 0, st, a)
   if (a.kv.D == 64) {
     if (a.kv.ks != nullptr) PA(64, true); else PA(64, false);
   } else {

@@ -290,6 +290,25 @@ def test_attention_bad_pages_are_hidden(lens):
     check(got, ref, mag, 0x1357)
 
 
+def test_pages_behind_the_window_may_be_gone():
+    """Their table entries are not looked at, their memory is poison."""
+    torch_cuda()
+    for mx, lens, page, window in ((False, [(1, 1000), (3, 333)], 16, 128),
+                                   (True, [(70, 900), (1, 129)], 32, 100)):
+        bt, q, sk = attn_case(mx, 64, 16, 2, page, lens, window, seed=15)
+        ref, mag = attention(bt, f32(q), sk, window)
+        for b, (n, t) in enumerate(lens):
+            gone = max(0, t - n - window + 1) // page
+            ids = bt.table[b, :gone].copy()
+            bt.k[ids], bt.v[ids] = (0x77, 0x77) if mx else (0x7FC1, 0x7FC1)
+            if mx:
+                bt.ks[ids] = bt.vs[ids] = 255
+            bt.table[b, :gone] = -1
+        got = run_attn(bt, q, sk, window)
+        ne.device_check()
+        check(got, ref, mag, 0x1357)
+
+
 def test_attention_nothing_visible_gives_zero():
     """Every page of a sequence hidden, with and without sinks."""
     torch_cuda()

@@ -46,7 +46,7 @@ CACHE = [dict(k=None), dict(v=None), dict(k=P + 8), dict(v=P + 2), dict(format=2
          dict(n_kv_heads=0), dict(n_kv_heads=-2), dict(head_dim=32), dict(head_dim=96),
          dict(head_dim=256)]
 ROWS = [dict(kv_len=None), dict(pages=None), dict(max_pages=0), dict(B=0), dict(B=-1),
-        dict(B=65536), dict(n_rows=-1), dict(n_rows=(1 << 24) + 1), dict(q_start=None, n_rows=3, B=2)]
+        dict(B=65536), dict(n_rows=-1), dict(n_rows=(1 << 23) + 1), dict(q_start=None, n_rows=3, B=2)]
 
 
 @pytest.mark.parametrize("bad", CACHE + ROWS, ids=str)
@@ -86,7 +86,7 @@ def test_gather_refusals(bad):
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(q=P + 4), dict(out=None), dict(out=P + 8), dict(stride=248),
     dict(stride=260), dict(Hq=3), dict(Hq=1), dict(Hq=0), dict(Hq=130, stride=1 << 20),
-    dict(window=-1)], ids=str)
+    dict(window=-1), dict(n_rows=1 << 22, Hq=64, n_kv_heads=64, stride=4096)], ids=str)
 def test_attn_refusals(bad):
     assert attn(**bad) == ne.NEON_EINVAL
 
