@@ -2329,7 +2329,7 @@ static bool paged_attn_shape_ok(int n_rows, int B, int Hq, int Hkv, int D) {
 extern "C" size_t neon_paged_attn_workspace(int n_rows, int B, int Hq, int n_kv_heads,
                                             int head_dim) {
   if (!paged_attn_shape_ok(n_rows, B, Hq, n_kv_heads, head_dim)) return 0;
-  return paged_attn_workspace(head_dim);
+  return paged_attn_workspace(n_rows, Hq, n_kv_heads, head_dim);
 }
 
 extern "C" size_t neon_paged_attn_counters(int n_rows, int B, int Hq, int n_kv_heads,

@@ -434,11 +434,12 @@ struct PagedAttnArgs {
   int Hq, window;
   float* part;            // partial results of split units (paged_attn_workspace)
   int32_t* arrive;        // their counters, 0 at launch and left at 0
+  int few;                // set by the launcher
 };
-size_t paged_attn_workspace(int D);
+size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D);
 size_t paged_attn_counters();
 bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv);  // the launch's grid holds them
-void launch_paged_attn(const PagedAttnArgs& a, hipStream_t st);
+void launch_paged_attn(PagedAttnArgs a, hipStream_t st);
 
 // ---- sampling with a setting per row (neon_sample_rows.hip) --------------------
 struct SampleRowsArgs {

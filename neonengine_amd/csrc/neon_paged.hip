@@ -280,6 +280,8 @@ void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out,
 // arrive joins them (stores and loads at agent scope, as in k_attn_split).
 // ---------------------------------------------------------------------------
 constexpr int kPaTarget = 1024;   // blocks of equal work to aim at: 4 per CU
+constexpr int kPmTarget = 512;    // of the many-row kernel: 2 per CU
+constexpr int kPaFew = 32;        // (token, head) rows per KV head of the few-row kernel
 constexpr int kPaArrive = 16;     // ints from one arrival counter to the next
 constexpr int kPaMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
 constexpr float kLog2e = 1.4426950408889634f;
@@ -301,14 +303,16 @@ struct PaWork {
   int c;
 };
 
-// rows and length of a sequence as the attention takes them (0 rows: none)
+// Rows and length of a sequence as a kernel takes them (0 rows: none): FEW the
+// ones of up to a.few (token, head) rows per KV head, otherwise the longer ones.
+template <bool FEW>
 __device__ __forceinline__ int pa_seq(const PagedAttnArgs& a, int b, int& start, int& len, bool flag) {
   int n;
   if (!paged_seq(a.r, a.kv.page_log2, b, start, n, len)) {
     if (flag && len != 0) flag_dev_err(a.r.err, kDevErrPagedRows);
     return 0;
   }
-  return len > 0 ? n : 0;
+  return len > 0 && (n * (a.Hq / a.kv.Hkv) <= a.few) == FEW ? n : 0;
 }
 
 // Keys that any row tile of a sequence may take, its first key rounded down to
@@ -322,7 +326,7 @@ __device__ __forceinline__ int pa_span(const PagedAttnArgs& a, int G, int len) {
 // The work of block `idx` (of every KV head alike); false when there is none.
 // ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
 // multiples of 128).
-template <int R, int ALIGN, int MINC>
+template <bool FEW, int R, int ALIGN, int MINC, int TARGET>
 __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool flag, PaWork& w) {
   const int lane = threadIdx.x & 63;
   const int G = a.Hq / a.kv.Hkv;
@@ -331,12 +335,12 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   float work = 0.0f;
   for (int b = b0; b < b1; ++b) {
     int start, len;
-    const int n = pa_seq(a, b, start, len, flag);
+    const int n = pa_seq<FEW>(a, b, start, len, flag);
     work += (float)((n * G + R - 1) / R) * (float)pa_span<R, ALIGN>(a, G, len);
   }
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
-  const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / kPaTarget);
+  const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
   const int chunk = max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127);
   // blocks and slots of the sequences, in order.  Row starts that overlap (an
   // error that no single sequence shows) can sum to more blocks than the grid
@@ -344,7 +348,7 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   int blocks = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
     int start, len;
-    const int n = pa_seq(a, b, start, len, false);
+    const int n = pa_seq<FEW>(a, b, start, len, false);
     const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
     const int nb = (n * G + R - 1) / R * nc;
     blocks = min(blocks + nb, kPaMaxBlocks);
@@ -366,13 +370,14 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   int slot = __builtin_amdgcn_readlane(slots_to - slots, owner);
   for (int b = owner * per; b < min(owner * per + per, a.r.B); ++b) {
     int start, len;
-    const int n = uni(pa_seq(a, b, start, len, false));
+    const int n = uni(pa_seq<FEW>(a, b, start, len, false));
     start = uni(start);
     len = uni(len);
     const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
     const int nb = (n * G + R - 1) / R * nc;
     if (idx < at + nb) {
-      const int tile = (idx - at) / nc;
+      // the last tiles first: they see the most keys
+      const int tile = nb / nc - 1 - (idx - at) / nc;
       w.b = b; w.start = start; w.n = n; w.len = len;
       w.c = (idx - at) % nc;
       w.row0 = tile * R;
@@ -528,18 +533,50 @@ __device__ __forceinline__ float2 pa_load_agent(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
+// Joins the E values of a row that the chunks' blocks left (of the same launch:
+// agent-scope loads), with its (m, l) pairs.
+template <int E>
+__device__ __forceinline__ void pa_join(const float* po, const float* pml, int64_t step, int chunks,
+                                        float& M, float& L, float (&x)[E]) {
+  M = -INFINITY;
+  L = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.0f;
+  for (int j = 0; j < chunks; ++j) {
+    const float2 ml = pa_load_agent(pml + j * step);
+    const float mn = fmaxf(M, ml.x);
+    const float fo = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+    const float fn = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    L = L * fo + ml.y * fn;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 y = pa_load_agent(po + j * step + e);
+      x[e] = x[e] * fo + y.x * fn;
+      x[e + 1] = x[e + 1] * fo + y.y * fn;
+    }
+    M = mn;
+  }
+}
+template <int E>
+__device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], float fin) {
+#pragma unroll
+  for (int e = 0; e < E; e += 4)
+    *reinterpret_cast<uint2*>(dst + e) = make_uint2(pack_bf2(x[e] * fin, x[e + 1] * fin),
+                                                    pack_bf2(x[e + 2] * fin, x[e + 3] * fin));
+}
+
 // Few rows: 16 per unit, four waves that share nothing but the result, each
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers and one step ahead of the products.
 template <int D, bool F4>
-__global__ __launch_bounds__(256) void k_paged_attn(PagedAttnArgs a) {
+__global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
   constexpr int R = 16, E = D / 16;
   __shared__ __align__(16) float so[4][R][D + 4];
   __shared__ float sm[4][R], sl[4][R];
   __shared__ int merge_here;
   const int h = blockIdx.x % a.kv.Hkv;
   PaWork w;
-  if (!pa_work<R, 32, 256>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
+  if (!pa_work<true, R, 32, 256, kPaTarget>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int G = a.Hq / a.kv.Hkv;
@@ -730,55 +767,389 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedAttnArgs a) {
     __syncthreads();
     if (!merge_here) return;
     if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    M = -INFINITY;
-    L = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.0f;
     const float* p0 = a.part + first * R * (D + 2);
-    const int64_t step_c = (int64_t)a.kv.Hkv * R * (D + 2);
-    for (int j = 0; j < w.chunks; ++j) {
-      const float2 ml = pa_load_agent(p0 + j * step_c + R * D + 2 * tr);
-      const float mn = fmaxf(M, ml.x);
-      const float fo = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
-      const float fn = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-      L = L * fo + ml.y * fn;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 y = pa_load_agent(p0 + j * step_c + tr * D + td + e);
-        x[e] = x[e] * fo + y.x * fn;
-        x[e + 1] = x[e + 1] * fo + y.y * fn;
-      }
-      M = mn;
-    }
+    pa_join<E>(p0 + tr * D + td, p0 + R * D + 2 * tr, (int64_t)a.kv.Hkv * R * (D + 2), w.chunks, M, L,
+               x);
   }
   if (row >= rows) return;
   const int head = h * G + row % G;
-  const float fin = pa_finish(a, head, M, L);
-  uint16_t* dst = a.out + ((int64_t)(w.start + row / G) * a.Hq + head) * D + td;
-#pragma unroll
-  for (int e = 0; e < E; e += 4)
-    *reinterpret_cast<uint2*>(dst + e) = make_uint2(pack_bf2(x[e] * fin, x[e + 1] * fin),
-                                                    pack_bf2(x[e + 2] * fin, x[e + 3] * fin));
+  pa_write<E>(a.out + ((int64_t)(w.start + row / G) * a.Hq + head) * D + td, x,
+              pa_finish(a, head, M, L));
 }
 
-// Units of R rows that n_rows rows of B sequences can make (per KV head).
+// Many rows: 128 per unit, 32 of each wave (two tiles of 16), 64 keys at a time
+// through LDS, where the four waves share them.  K rows lie as they are, their
+// 16-byte words exchanged by the key's low bits, so the 16 lanes that read one
+// word of 16 keys touch every bank once.  V lies as pairs: dword (m, d) holds
+// the values of the keys 2 m and 2 m + 1, paired once when a tile is written
+// instead of by every wave, so a lane's four 16-byte reads are its A operands.
+// MXFP4 pages are expanded when a tile is written.  The next tile's loads are
+// on their way while a tile is used, and LDS holds two.
+// P is rounded to bf16, and the row sums come from the same rounded values (a
+// product with ones), so the rounding cancels where a row's weights share it.
+template <int D>
+struct PmStage {  // a thread's part of a tile on its way
+  uint4 k[D / 32], v[2][D / 64];
+};
+
+template <int D, bool F4>
+__global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
+  constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
+  __shared__ __align__(16) uint4 kt[2][64 * W];
+  __shared__ __align__(16) uint32_t vt[2][32 * D];
+  __shared__ int merge_here;
+  const int h = blockIdx.x % a.kv.Hkv;
+  PaWork w;
+  if (!pa_work<false, R, 64, 512, kPmTarget>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int G = a.Hq / a.kv.Hkv, rows = w.n * G, pos0 = w.len - w.n;
+  const float c2 = (D == 64 ? 0.125f : 0.08838834764831845f) * kLog2e;
+  uint4 q[2][D / 32];
+  int k_hi[2], k_lo[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r = w.row0 + 32 * wave + 16 * t + c;
+    const bool has = r < rows;
+    const int tok = has ? r / G : 0, hq = h * G + (has ? r % G : 0);
+    k_hi[t] = has ? pos0 + tok + 1 : 0;
+    k_lo[t] = a.window > 0 ? max(0, pos0 + tok - a.window + 1) : 0;
+    const uint16_t* qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      q[t][n] = *reinterpret_cast<const uint4*>(qp + 32 * n + 8 * g);
+      if (!has) q[t][n] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  // of the wave's 32 rows: the keys that all see, and that any sees
+  const int r_first = w.row0 + 32 * wave, r_last = min(r_first + 32, rows) - 1;
+  const bool idle = r_first >= rows;
+  const int all_hi = idle ? 0 : pos0 + r_first / G + 1;
+  const int any_hi = idle ? 0 : pos0 + r_last / G + 1;
+  const int all_lo = a.window > 0 && !idle ? max(0, pos0 + r_last / G - a.window + 1) : 0;
+  const int any_lo = a.window > 0 && !idle ? max(0, pos0 + r_first / G - a.window + 1) : 0;
+
+  const int n_it = (w.k1 - w.k0 + 63) >> 6;
+  const int32_t* table = a.r.table + (int64_t)w.b * a.r.max_pages;
+  // page ids of the 16-key groups of 16 tiles, one per lane, as in the other kernel
+  auto load_ids = [&](int it) {
+    const int key = w.k0 + 64 * it + 16 * lane;
+    int id = -1;
+    if (key < w.k1 && key + 16 > w.lo) {
+      id = table[key >> a.kv.page_log2];
+      if ((unsigned)id >= (unsigned)a.kv.n_pages) {
+        id = -1;
+        flag_dev_err(a.r.err, kDevErrPageId);
+      }
+    }
+    return id;
+  };
+  const int page_mask = (1 << a.kv.page_log2) - 1;
+  auto group_at = [&](int it, int ids, int grp) {  // rows of the group's first key
+    const int id = max(__builtin_amdgcn_readlane(ids, 4 * (it & 15) + grp), 0);
+    return (((int64_t)id * a.kv.Hkv + h) << a.kv.page_log2) +
+           ((w.k0 + 64 * it + 16 * grp) & page_mask);
+  };
+  // bit grp: the tile's group has no page
+  auto dead_groups = [&](int it, int ids) {
+    uint32_t dead = 0;
+#pragma unroll
+    for (int grp = 0; grp < 4; ++grp)
+      dead |= (uint32_t)(__builtin_amdgcn_readlane(ids, 4 * (it & 15) + grp) < 0) << grp;
+    return dead;
+  };
+  // A tile's loads.  bf16: K word tid % W of keys tid / W + (256 / W) j; V
+  // words tid % 8 (+ 8 j) of the keys 2 m, 2 m + 1, m = tid / 8.  MXFP4: K codes
+  // of D/4 dims of key tid / 4 in k[0] and their scale in k[1].x; V codes of 8
+  // dims of the keys 2 m, 2 m + 1 (D = 128: of 16) and the two scales.
+  auto load_tile = [&](PmStage<D>& t, int it, int ids) {
+    const int m2 = (tid >> 3 & 7) * 2;  // the pair's first key within its group (= wave)
+    const int64_t va = group_at(it, ids, wave);
+    if constexpr (F4) {
+      const int kk = tid >> 2 & 15, part = tid & 3;
+      const uint8_t* kp = a.kv.k + va * (D / 2);
+      const uint8_t* vp = a.kv.v + va * (D / 2);
+      t.k[1].x = (a.kv.ks + va * (D / 32))[(uint32_t)(kk * (D / 32) + (D == 64 ? part >> 1 : part))];
+      const uint8_t* vs = a.kv.vs + va * (D / 32);
+      const uint32_t sat = (uint32_t)(m2 * (D / 32) + (D == 64 ? (tid & 7) >> 2 : (tid & 7) >> 1));
+      t.k[1].y = vs[sat];
+      t.k[1].z = vs[sat + D / 32];
+      if constexpr (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(kp + (uint32_t)(kk * 32 + 8 * part));
+        t.k[0].x = x.x; t.k[0].y = x.y;
+        t.v[0][0].x = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)(m2 * 32 + 4 * (tid & 7)));
+        t.v[1][0].x = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)(m2 * 32 + 32 + 4 * (tid & 7)));
+      } else {
+        t.k[0] = *reinterpret_cast<const uint4*>(kp + (uint32_t)(kk * 64 + 16 * part));
+        const uint2 x = *reinterpret_cast<const uint2*>(vp + (uint32_t)(m2 * 64 + 8 * (tid & 7)));
+        const uint2 y = *reinterpret_cast<const uint2*>(vp + (uint32_t)(m2 * 64 + 64 + 8 * (tid & 7)));
+        t.v[0][0].x = x.x; t.v[0][0].y = x.y;
+        t.v[1][0].x = y.x; t.v[1][0].y = y.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int key = tid / W + (256 / W) * j;  // its group is the wave's
+        const int64_t ka = group_at(it, ids, uni(key >> 4));
+        t.k[j] = *reinterpret_cast<const uint4*>(a.kv.k + ka * (2 * D) +
+                                                 (uint32_t)((key & 15) * 2 * D + 16 * (tid % W)));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j)
+          t.v[i][j] = *reinterpret_cast<const uint4*>(
+              a.kv.v + va * (2 * D) + (uint32_t)((m2 + i) * 2 * D + 16 * ((tid & 7) + 8 * j)));
+    }
+  };
+  auto put_k = [&](int buf, int key, int word, const uint4& x) {
+    kt[buf][key * W + (word ^ (key & 7))] = x;
+  };
+  auto put_pairs = [&](int buf, int m, int d0, const uint4& x, const uint4& y) {
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    uint32_t z[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      z[2 * i] = __builtin_amdgcn_perm(ys[i], xs[i], 0x05040100u);
+      z[2 * i + 1] = __builtin_amdgcn_perm(ys[i], xs[i], 0x07060302u);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(&vt[buf][m * D + d0]);
+    dst[0] = make_uint4(z[0], z[1], z[2], z[3]);
+    dst[1] = make_uint4(z[4], z[5], z[6], z[7]);
+  };
+  auto write_tile = [&](const PmStage<D>& t, int it, int ids) {
+    const int buf = it & 1, m = tid >> 3, kb = w.k0 + 64 * it;
+    // values of rows that hold no key of the sequence may be anything
+    const bool edge = kb < w.lo || kb + 64 > w.k1;
+    const bool dead = __builtin_amdgcn_readlane(ids, 4 * (it & 15) + wave) < 0;
+    bool none[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = kb + 2 * m + i;
+      none[i] = dead || (edge && (key < w.lo || key >= w.k1));
+    }
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (F4) {
+      const int key = tid >> 2, part = tid & 3;
+      const uint32_t kc[4] = {t.k[0].x, t.k[0].y, t.k[0].z, t.k[0].w};
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) put_k(buf, key, part * (D / 32) + j, mx4_to_bf16x8(kc[j], t.k[1].x));
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const uint4 x = mx4_to_bf16x8(j == 0 ? t.v[0][0].x : t.v[0][0].y, t.k[1].y);
+        const uint4 y = mx4_to_bf16x8(j == 0 ? t.v[1][0].x : t.v[1][0].y, t.k[1].z);
+        put_pairs(buf, m, 8 * ((tid & 7) * (D / 64) + j), none[0] ? zero : x, none[1] ? zero : y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) put_k(buf, tid / W + (256 / W) * j, tid % W, t.k[j]);
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j)
+        put_pairs(buf, m, 8 * ((tid & 7) + 8 * j), none[0] ? zero : t.v[0][j], none[1] ? zero : t.v[1][j]);
+    }
+  };
+
+  pf4 o[2][E], l[2];
+  float m[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[t][e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    l[t] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    m[t] = -INFINITY;
+  }
+  const uint4 ones = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
+
+  auto compute = [&](int it, uint32_t dead) {
+    const int kb = w.k0 + 64 * it, buf = it & 1;
+    if (kb >= any_hi || kb + 64 <= any_lo) return;
+    const bool full = kb >= all_lo && kb + 64 <= all_hi && dead == 0;
+    pf4 s[2][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 kf[D / 32];
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n) kf[n] = kt[buf][(16 * k + c) * W + ((4 * n + g) ^ (c & 7))];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t][k] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) s[t][k] = pa_mfma(kf[n], q[t][n], s[t][k]);
+      }
+    }
+    if (!full) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = kb + 16 * k + 4 * g + i;
+            if (key < k_lo[t] || key >= k_hi[t] || (dead >> k & 1)) s[t][k][i] = -INFINITY;
+          }
+    }
+    uint4 p[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mx = fmaxf(mx, fmaxf(fmaxf(s[t][k][0], s[t][k][1]), fmaxf(s[t][k][2], s[t][k][3])));
+      mx *= c2;
+      mx = fmaxf(mx, xor_lane<16>(mx));
+      mx = fmaxf(mx, xor_lane<32>(mx));
+      if (__any(mx > m[t])) {
+        const float mn = fmaxf(m[t], mx);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[t][e] *= f;
+        l[t] *= f;
+        m[t] = mn;
+      }
+      const float me = m[t] == -INFINITY ? 0.0f : m[t];
+      uint32_t pw[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+          pw[2 * k + i / 2] =
+              pack_bf2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i], c2, -me)),
+                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i + 1], c2, -me)));
+      p[t][0] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+      p[t][1] = make_uint4(pw[4], pw[5], pw[6], pw[7]);
+      l[t] = pa_mfma(ones, p[t][0], l[t]);
+      l[t] = pa_mfma(ones, p[t][1], l[t]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e0 = 0; e0 < E; e0 += 4) {
+        uint4 x[4];  // pair j of the lane's keys, dims E c + e0 ..
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[j] = *reinterpret_cast<const uint4*>(
+              &vt[buf][(16 * k + 8 * (j >> 1) + 2 * g + (j & 1)) * D + E * c + e0]);
+        const uint4 f[4] = {make_uint4(x[0].x, x[1].x, x[2].x, x[3].x),
+                            make_uint4(x[0].y, x[1].y, x[2].y, x[3].y),
+                            make_uint4(x[0].z, x[1].z, x[2].z, x[3].z),
+                            make_uint4(x[0].w, x[1].w, x[2].w, x[3].w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) o[t][e0 + e] = pa_mfma(f[e], p[t][k], o[t][e0 + e]);
+      }
+  };
+
+  PmStage<D> st;
+  int ids = load_ids(0);
+  load_tile(st, 0, ids);
+  for (int it = 0; it < n_it; ++it) {
+    write_tile(st, it, ids);
+    const uint32_t dead = dead_groups(it, ids);
+    const int nx = min(it + 1, n_it - 1);
+    if ((nx & 15) == 0 && nx > it) ids = load_ids(nx);
+    load_tile(st, nx, ids);
+    lds_barrier();  // the tile is written; the one before it was read before this
+    compute(it, dead);
+  }
+
+  // lane (g, c): row c of each tile, dims (D/4) g ..
+  if (w.chunks == 1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = r_first + 16 * t + c;
+      if (r >= rows) continue;
+      const int head = h * G + r % G;
+      const float fin = pa_finish(a, head, m[t], l[t][0]);
+      uint16_t* dst = a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + (D / 4) * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<uint2*>(dst + E * i + e) =
+              make_uint2(pack_bf2(o[t][e][i] * fin, o[t][e + 1][i] * fin),
+                         pack_bf2(o[t][e + 2][i] * fin, o[t][e + 3][i] * fin));
+    }
+    return;
+  }
+  const int64_t first = (int64_t)w.slot * a.kv.Hkv + h;
+  const int64_t step_c = (int64_t)a.kv.Hkv * R * (D + 2);
+  float* p0 = a.part + first * R * (D + 2);
+  float* po = p0 + w.c * step_c;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r = 32 * wave + 16 * t + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        pa_store_agent(po + r * D + (D / 4) * g + E * i + e, o[t][e][i], o[t][e + 1][i]);
+    if (g == 0) pa_store_agent(po + R * D + 2 * r, m[t], l[t][0]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
+  __syncthreads();
+  int32_t* ctr = a.arrive + first * kPaArrive;
+  if (tid == 0)
+    merge_here = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 w.chunks - 1;
+  __syncthreads();
+  if (!merge_here) return;
+  if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int r0 = tid >> 4; r0 < R; r0 += 16) {  // 16 threads of a row, E dims each
+    const int r = w.row0 + r0, td = (tid & 15) * E;
+    if (r >= rows) break;
+    float M, L, x[E];
+    pa_join<E>(p0 + r0 * D + td, p0 + R * D + 2 * r0, step_c, w.chunks, M, L, x);
+    const int head = h * G + r % G;
+    pa_write<E>(a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + td, x,
+                pa_finish(a, head, M, L));
+  }
+}
+
+// Units of R rows that n_rows rows of up to B sequences can make (per KV head).
 static int64_t pa_units(int n_rows, int B, int G, int R) {
   return (int64_t)n_rows * G / R + B;
 }
-
-static int64_t pa_blocks(int n_rows, int B, int Hq, int Hkv) {
-  return (kPaTarget / Hkv + 1 + pa_units(n_rows, B, Hq / Hkv, 16)) * Hkv;
+// Blocks of the two launches (0: no row can be of that kind).  One row per
+// sequence has G rows; with row starts the host does not know, and launches
+// both unless all rows together are few.
+static int64_t pa_few_blocks(const PagedRows& r, int Hq, int Hkv) {
+  if (r.q_start == nullptr && Hq / Hkv > kPaFew) return 0;
+  return (kPaTarget / Hkv + 1 + pa_units(r.n_rows, r.B, Hq / Hkv, 16)) * Hkv;
+}
+static int64_t pa_many_blocks(const PagedRows& r, int Hq, int Hkv) {
+  const int64_t G = Hq / Hkv;
+  if (r.q_start == nullptr ? G <= kPaFew : r.n_rows * G <= kPaFew) return 0;
+  const int64_t most = r.n_rows * G / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
+  return (kPmTarget / Hkv + 1 + pa_units(r.n_rows, (int)(most < r.B ? most : r.B), (int)G, 128)) *
+         Hkv;
 }
 
 bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {
-  return pa_blocks(n_rows, B, Hq, Hkv) < kPaMaxBlocks;
+  PagedRows r{};
+  static const int32_t given = 0;
+  r.q_start = &given;
+  r.n_rows = n_rows;
+  r.B = B;
+  return pa_few_blocks(r, Hq, Hkv) < kPaMaxBlocks && pa_many_blocks(r, Hq, Hkv) < kPaMaxBlocks;
 }
-size_t paged_attn_workspace(int D) { return (size_t)(2 * kPaTarget) * 16 * (D + 2) * 4; }
+// The two launches use the same places, one after the other.
+size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D) {
+  const size_t few = (size_t)(2 * kPaTarget) * 16, many = (size_t)(2 * kPmTarget) * 128;
+  return ((int64_t)n_rows * (Hq / Hkv) <= kPaFew ? few : many) * (D + 2) * 4;
+}
 size_t paged_attn_counters() { return (size_t)(2 * kPaTarget) * kPaArrive * 4; }
 
-void launch_paged_attn(const PagedAttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)pa_blocks(a.r.n_rows, a.r.B, a.Hq, a.kv.Hkv));
-#define PA(D, F4) hipLaunchKernelGGL((k_paged_attn<D, F4>), grid, dim3(256), 0, st, a)
+void launch_paged_attn(PagedAttnArgs a, hipStream_t st) {
+  a.few = kPaFew;
+  const int64_t few = pa_few_blocks(a.r, a.Hq, a.kv.Hkv), many = pa_many_blocks(a.r, a.Hq, a.kv.Hkv);
+#define PA(D, F4)                                                                              \
+  do {                                                                                         \
+    if (few)                                                                                   \
+      hipLaunchKernelGGL((k_paged_attn_few<D, F4>), dim3((unsigned)few), dim3(256), 0, st, a); \
+    if (many)                                                                                  \
+      hipLaunchKernelGGL((k_paged_attn_many<D, F4>), dim3((unsigned)many), dim3(256), 0, st, a); \
+  } while (0)
   if (a.kv.D == 64) {
     if (a.kv.ks != nullptr) PA(64, true); else PA(64, false);
   } else {
