@@ -2374,7 +2374,7 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
 
 extern "C" size_t neon_sample_rows_workspace(int B, int V) {
   if (B < 1 || B > 65535 || V < 1 || V > (1 << 24)) return 0;
-  return 0;
+  return sample_rows_workspace(B, V);
 }
 
 extern "C" neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
@@ -2393,7 +2393,7 @@ extern "C" neon_status neon_sample_rows(const float* logits, int64_t stride, int
   SampleRowsArgs a;
   a.logits = logits; a.stride = stride; a.B = B; a.V = V;
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
-  a.ids = out_ids; a.err = device_status_word();
+  a.ids = out_ids; a.workspace = workspace; a.err = device_status_word();
   launch_sample_rows(a, S(stream));
   KLAUNCHED();
 }

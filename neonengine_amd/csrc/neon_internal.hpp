@@ -453,7 +453,10 @@ struct SampleRowsArgs {
   const float* u;  // [B] uniform in [0, 1)
   int32_t* ids;    // [B]
   int32_t* err;
+  void* workspace;
+  int chunk, chunks;  // set by the launcher
 };
-void launch_sample_rows(const SampleRowsArgs& a, hipStream_t st);
+size_t sample_rows_workspace(int B, int V);
+void launch_sample_rows(SampleRowsArgs a, hipStream_t st);
 
 }  // namespace neon

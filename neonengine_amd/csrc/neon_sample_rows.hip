@@ -27,24 +27,65 @@ __device__ __forceinline__ uint32_t sr_key(float l) {
   const uint32_t b = __float_as_uint(l + 0.0f);  // -0 + 0 = +0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float sr_logit(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
 constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 
+// ---------------------------------------------------------------------------
+// A row is cut into chunks of one block each.  The order is searched in bins of
+// 1/16 of T below the maximum (512 of them; what lies further down has mass 0):
+//   k_sr_max    chunk maxima
+//   k_sr_hist   per chunk the count and mass of every bin; the row's last block
+//               sums them and finds the bins that the top_k-th token and the
+//               token at top_p's goal can lie in
+//   k_sr_pick   per chunk the mass of the bins above those, which is kept
+//               whatever the exact places are, and the tokens of those bins (the
+//               candidates, some hundreds of a large vocabulary); the row's last
+//               block finds the two places among the candidates, then the chunk
+//               that holds the draw, then the token in it
+// A row of one chunk is one launch with the same steps.  Nothing but the chunks'
+// partial results crosses launches, at agent scope, so that the last block reads
+// what the others wrote without a launch in between.
+// Bound: three reads of the logits (the later two from the caches) and, for many
+// rows, one 64-bit exponential per token and pass.
+// ---------------------------------------------------------------------------
+constexpr int kSrThreads = 512;
+constexpr int kSrBins = 512;   // one per thread in the scan
+constexpr int kSrCap = 8192;   // candidates of a row that are listed
+constexpr float kSrBinsPerT = 16.0f;
+
+// A row's parameters as the kernels use them.
 struct SrRow {
-  float m;       // the row's maximum
+  const float* l;
+  int V;
+  float m;       // the maximum
+  float bin_t;   // bins per unit of the logits
   double inv_t;  // 1 / T
   double scale;  // 2^S
-  double min_p;
+  double min_p, p, u;
+  int k;         // 0: all
+  uint64_t best; // key and ~index of the maximum
 };
-__device__ __forceinline__ double sr_weight(const SrRow& r, uint32_t key) {
-  const float l = sr_logit(key);
+__device__ __forceinline__ double sr_weight(const SrRow& r, float l) {
   if (l == r.m) return 1.0;  // also where both are infinite
   return exp(((double)l - (double)r.m) * r.inv_t);
 }
-__device__ __forceinline__ u64 sr_mass(const SrRow& r, uint32_t key) {
-  return (u64)__builtin_rint(sr_weight(r, key) * r.scale);
+__device__ __forceinline__ u64 sr_mass(const SrRow& r, float l) {
+  return (u64)__builtin_rint(sr_weight(r, l) * r.scale);
+}
+// mass under min_p's limit: 0 below it
+__device__ __forceinline__ u64 sr_kept_mass(const SrRow& r, float l) {
+  const double w = sr_weight(r, l);
+  return w >= r.min_p ? (u64)__builtin_rint(w * r.scale) : 0;
+}
+// Falls with l, never rises: each step rounds monotonically.
+__device__ __forceinline__ int sr_bin(const SrRow& r, float l) {
+  if (l == r.m) return 0;
+  const float x = (r.m - l) * r.bin_t;
+  return x < (float)kSrBins ? (int)x : kSrBins;  // a NaN goes to the end
+}
+__device__ __forceinline__ float sr_clean(float l) { return l != l ? -INFINITY : l + 0.0f; }
+// unique, and in the order of the tokens: larger logit, then lower index
+__device__ __forceinline__ u64 sr_place(float l, int i) {
+  return ((u64)sr_key(l) << 32) | (uint32_t)~i;
 }
 
 __device__ __forceinline__ double sr_scale(int V) {
@@ -52,18 +93,41 @@ __device__ __forceinline__ double sr_scale(int V) {
   return lg <= 18 ? 0x1p44 : __builtin_ldexp(1.0, 62 - lg);
 }
 
+__device__ __forceinline__ u64 sr_get(const u64* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void sr_put(u64* p, u64 v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 __device__ __forceinline__ u64 sr_block_sum(u64 v, u64* red) {
+#pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   u64 t = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) t += red[w];
+#pragma unroll
+  for (int w = 0; w < kSrThreads / 64; ++w) t += red[w];
   return t;
 }
-// sums of the threads before this one
+__device__ __forceinline__ u64 sr_block_max(u64 v, u64* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 x = __shfl_xor(v, o);
+    v = x > v ? x : v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSrThreads / 64; ++w) v = red[w] > v ? red[w] : v;
+  return v;
+}
+// sum of the threads before this one
 __device__ __forceinline__ u64 sr_block_before(u64 v, u64* red) {
   u64 x = v;
+#pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const u64 y = __shfl_up(x, o);
     if ((int)(threadIdx.x & 63) >= o) x += y;
@@ -75,163 +139,555 @@ __device__ __forceinline__ u64 sr_block_before(u64 v, u64* red) {
   return x - v;
 }
 
-// A row's parameters; false (flagged) where one is out of range.
-__device__ __forceinline__ bool sr_params(const SampleRowsArgs& a, int b, float& t, int& k, float& p,
-                                          float& mp, float& u) {
-  t = a.temperature != nullptr ? a.temperature[b] : 1.0f;
-  k = a.top_k != nullptr ? a.top_k[b] : 0;
-  p = a.top_p != nullptr ? a.top_p[b] : 1.0f;
-  mp = a.min_p != nullptr ? a.min_p[b] : 0.0f;
-  u = a.u[b];
+// What the scan of the bins finds.
+struct SrFound {
+  int lo, hi;     // bins that top_p's token can lie in: everything before lo is kept
+  int bin_k;      // bin of the top_k-th token, kSrBins where none is cut
+  u64 base;       // mass before lo
+  u64 before_k;   // mass before bin_k
+  u64 mass_k;     // mass of the top_k tokens, where bin_k cuts none
+  u64 need_k;     // tokens of bin_k that are among the top_k
+};
+
+struct SrShared {
+  u64 red[16];
+  u64 list[kSrCap];
+  u64 mass[kSrBins], any[256];
+  uint32_t count[kSrBins];
+  SrFound found;
+  u64 s_u64[2];
+  int s_int[4];
+};
+
+// Reads row b's parameters; false where one is out of range.
+__device__ __forceinline__ bool sr_params(const SampleRowsArgs& a, int b, SrRow& r, bool& greedy) {
+  const float t = a.temperature != nullptr ? a.temperature[b] : 1.0f;
+  const float p = a.top_p != nullptr ? a.top_p[b] : 1.0f;
+  const float mp = a.min_p != nullptr ? a.min_p[b] : 0.0f;
+  const float u = a.u[b];
+  const int k = a.top_k != nullptr ? a.top_k[b] : 0;
+  r.l = a.logits + (int64_t)b * a.stride;
+  r.V = a.V;
+  r.k = k > 0 && k < a.V ? k : 0;
+  r.p = (double)p;
+  r.min_p = (double)mp;
+  r.u = (double)u;
+  r.inv_t = 1.0 / (double)t;
+  r.bin_t = (float)r.inv_t * kSrBinsPerT;
+  r.scale = sr_scale(a.V);
+  greedy = t == 0.0f;
   return t >= 0.0f && t < INFINITY && p > 0.0f && p <= 1.0f && mp >= 0.0f && mp <= 1.0f &&
          u >= 0.0f && u < 1.0f;
 }
+__device__ __forceinline__ void sr_set_best(SrRow& r, u64 best) {
+  r.best = best;
+  const uint32_t key = (uint32_t)(best >> 32);
+  r.m = __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+__device__ __forceinline__ int sr_best_id(u64 best) { return (int)~(uint32_t)best; }
 
-// One block per row; the order is searched by 8 bits of the key at a time over
-// the whole row (counts for top_k, masses for top_p).
-__global__ __launch_bounds__(1024) void k_sample_rows(SampleRowsArgs a) {
-  __shared__ u64 red[16], hist[256];
-  __shared__ uint32_t s_key;
-  __shared__ u64 s_above;
-  __shared__ int s_id;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const float* l = a.logits + (int64_t)b * a.stride;
-  const int V = a.V;
-  float t, p, mp, u;
-  int k;
-  if (!sr_params(a, b, t, k, p, mp, u)) {
-    if (tid == 0) {
-      flag_dev_err(a.err, kDevErrSampleParam);
-      a.ids[b] = -1;
-    }
-    return;
-  }
-  // the maximum, lowest index first
+__device__ __forceinline__ u64 sr_chunk_max(const float* l, int i0, int i1, u64* red) {
   u64 best = 0;
-  for (int i = tid; i < V; i += 1024) {
-    const u64 x = ((u64)sr_key(l[i]) << 32) | (uint32_t)~i;
+  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
+    const u64 x = sr_place(sr_clean(l[i]), i);
     best = x > best ? x : best;
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 x = __shfl_xor(best, o);
-    best = x > best ? x : best;
-  }
-  if ((tid & 63) == 0) red[tid >> 6] = best;
-  __syncthreads();
-  for (int w = 0; w < 16; ++w) best = red[w] > best ? red[w] : best;
-  const uint32_t top = (uint32_t)(best >> 32);
-  if (top == kSrNone || t == 0.0f) {  // nothing to choose from, or greedy
-    if (tid == 0) a.ids[b] = top == kSrNone ? -1 : (int32_t)~(uint32_t)best;
-    return;
-  }
-  SrRow r;
-  r.m = sr_logit(top);
-  r.inv_t = 1.0 / (double)t;
-  r.scale = sr_scale(V);
-  r.min_p = (double)mp;
+  return sr_block_max(best, red);
+}
 
-  // The largest key whose elements and those above it reach `goal`, in
-  // elements (by = false) or mass; `above`: what the larger keys have.
-  auto search = [&](bool by_mass, double goal, uint32_t floor_key, u64& above) {
-    uint32_t prefix = 0;
-    u64 before = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += 1024) {
-        const uint32_t x = sr_key(l[i]);
-        if (x < floor_key || (shift < 24 && (x >> (shift + 8)) != prefix)) continue;
-        const u64 w = by_mass ? sr_mass(r, x) : 1;
-        if (w) atomicAdd(&hist[(x >> shift) & 255], w);
+// counts and masses of the chunk's bins into sh.count / sh.mass
+__device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SrShared& sh) {
+  sh.mass[threadIdx.x] = 0;
+  sh.count[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
+    const float l = sr_clean(r.l[i]);
+    const int bin = sr_bin(r, l);
+    if (bin < kSrBins) {
+      atomicAdd(&sh.count[bin], 1u);
+      atomicAdd(&sh.mass[bin], sr_mass(r, l));
+    }
+  }
+  __syncthreads();
+}
+
+// The bins to look into, from the row's counts and masses (thread = bin).
+__device__ __forceinline__ void sr_scan(const SrRow& r, u64 count, u64 mass, SrShared& sh) {
+  const int bin = threadIdx.x;
+  const u64 c0 = sr_block_before(count, sh.red), m0 = sr_block_before(mass, sh.red);
+  const u64 c1 = c0 + count, m1 = m0 + mass;
+  SrFound& f = sh.found;
+  if (bin == 0) {
+    f.bin_k = kSrBins;
+    f.lo = f.hi = kSrBins;
+    f.base = f.before_k = f.need_k = 0;
+  }
+  if (bin == kSrBins - 1) f.mass_k = m1;
+  __syncthreads();
+  const u64 k = (u64)r.k;
+  if (r.k > 0 && c0 < k && c1 >= k) {
+    if (c1 == k) {  // the bins up to this one are the top_k
+      f.mass_k = m1;
+      f.lo = bin + 1;  // where top_p is off: no candidates
+      f.hi = bin;
+    } else {
+      f.bin_k = bin;
+      f.before_k = m0;
+      f.need_k = k - c0;
+      f.lo = f.hi = bin;
+      f.mass_k = m1;  // an upper bound
+    }
+  }
+  __syncthreads();
+  if (r.p < 1.0) {
+    const bool cut = f.bin_k < kSrBins;
+    const double g0 = r.p * (double)(cut ? f.before_k : f.mass_k), g1 = r.p * (double)f.mass_k;
+    __syncthreads();
+    // the first bins whose running mass reaches the goal (the last bin reaches
+    // any); with g0 = 0, no bin does better than the first
+    if ((double)m1 >= g0 && (bin == 0 || (double)m0 < g0)) f.lo = bin;
+    if ((double)m1 >= g1 && (bin == 0 || (double)m0 < g1)) f.hi = bin;
+    __syncthreads();
+    if (bin == f.lo) f.base = m0;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ bool sr_candidate(const SrFound& f, int bin) {
+  return (bin >= f.lo && bin <= f.hi && bin < kSrBins) || bin == f.bin_k;
+}
+
+// The kept mass of the chunk's sure bins; its candidates into sh.list (as many
+// as fit; sh.s_int[0] counts all).
+__device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int i0, int i1,
+                                          SrShared& sh) {
+  if (threadIdx.x == 0) sh.s_int[0] = 0;
+  __syncthreads();
+  u64 sure = 0;
+  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
+    const float l = sr_clean(r.l[i]);
+    const int bin = sr_bin(r, l);
+    if (bin < f.lo) {
+      if (bin < kSrBins) sure += sr_kept_mass(r, l);
+    } else if (bin < kSrBins && sr_candidate(f, bin)) {
+      const int at = atomicAdd(&sh.s_int[0], 1);
+      if (at < kSrCap) sh.list[at] = sr_place(l, i);
+    }
+  }
+  return sr_block_sum(sure, sh.red);
+}
+
+__device__ __forceinline__ float sr_place_logit(u64 place) {
+  const uint32_t key = (uint32_t)(place >> 32);
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+// Calls fn(place) for every candidate at or above `from` in the bins [lo, hi]:
+// of the list, or of the row where the list did not hold them all.
+template <class F>
+__device__ __forceinline__ void sr_each(const SrRow& r, const SrShared& sh, int n, int lo, int hi,
+                                        u64 from, F fn) {
+  if (n <= kSrCap) {
+    for (int j = threadIdx.x; j < n; j += kSrThreads) {
+      const u64 x = sh.list[j];
+      if (x < from) continue;
+      const int bin = sr_bin(r, sr_place_logit(x));
+      if (bin >= lo && bin <= hi) fn(x);
+    }
+  } else {
+    for (int i = threadIdx.x; i < r.V; i += kSrThreads) {
+      const float l = sr_clean(r.l[i]);
+      const int bin = sr_bin(r, l);
+      if (bin < lo || bin > hi || bin >= kSrBins) continue;
+      const u64 x = sr_place(l, i);
+      if (x >= from) fn(x);
+    }
+  }
+}
+
+// The place of the candidate at which the running count (or mass), in order and
+// starting at `base`, reaches `goal`; the last one where none does.  `upto`: the
+// running value including it.  Searched by 8 bits of the place at a time,
+// beginning at the highest bit in which the candidates differ.
+template <bool MASS>
+__device__ __forceinline__ u64 sr_select(const SrRow& r, SrShared& sh, int n, int lo, int hi, u64 from,
+                                         u64 base, double goal, u64& upto) {
+  const int tid = threadIdx.x;
+  u64 mx = 0, mn = 0;  // of the places, and of their complements
+  sr_each(r, sh, n, lo, hi, from, [&](u64 x) {
+    mx = x > mx ? x : mx;
+    mn = ~x > mn ? ~x : mn;
+  });
+  mx = sr_block_max(mx, sh.red);
+  mn = ~sr_block_max(mn, sh.red);
+  int top = mx == mn ? 0 : 64 - __builtin_clzll(mx ^ mn);  // bits to decide
+  u64 prefix = top < 64 ? mx >> top : 0;
+  u64 run = base;
+  while (true) {
+    const int shift = top > 8 ? top - 8 : 0;
+    const int digits = 1 << (top - shift);
+    __syncthreads();
+    if (tid < 256) {
+      sh.mass[tid] = 0;
+      sh.count[tid] = 0;
+    }
+    __syncthreads();
+    sr_each(r, sh, n, lo, hi, from, [&](u64 x) {
+      if (top < 64 && (x >> top) != prefix) return;
+      const int d = (int)(x >> shift) & (digits - 1);
+      if (MASS) atomicAdd(&sh.mass[d], sr_mass(r, sr_place_logit(x)));
+      atomicAdd(&sh.count[d], 1u);
+      sh.any[d] = x;
+    });
+    __syncthreads();
+    if (tid < 64) {  // four digits a lane, from the largest down
+      u64 c[4], v[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 255 - (4 * tid + j);
+        c[j] = d < digits ? sh.count[d] : 0;
+        v[j] = MASS ? (d < digits ? sh.mass[d] : 0) : c[j];
+        sum += v[j];
       }
-      __syncthreads();
-      if (tid == 0) {
-        u64 run = before;
-        int d = 255;
-        for (; d > 0; --d) {
-          if ((double)(run + hist[d]) >= goal) break;
-          run += hist[d];
+      u64 x = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = __shfl_up(x, o);
+        if (tid >= o) x += y;
+      }
+      u64 at = run + x - sum;
+      // the first digit that reaches the goal, else the last that is there
+      int hit = -1, last = -1;
+      u64 hit_at = 0, last_at = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c[j] > 0) {
+          last = 4 * tid + j;
+          last_at = at;
+          if (hit < 0 && (double)(at + v[j]) >= goal) {
+            hit = last;
+            hit_at = at;
+          }
         }
-        s_key = d;
-        s_above = run;
+        at += v[j];
       }
-      __syncthreads();
-      prefix = (prefix << 8) | s_key;
-      before = s_above;
+      const u64 hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+      const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts | 1);
+      if (tid == lane) {
+        sh.s_int[1] = 255 - (hits ? hit : last);
+        sh.s_u64[0] = hits ? hit_at : last_at;
+      }
     }
-    above = before;
-    return prefix;
-  };
-  auto total = [&](uint32_t key, bool by_mass) {  // of larger keys' elements
-    u64 n = 0;
-    for (int i = tid; i < V; i += 1024) {
-      const uint32_t x = sr_key(l[i]);
-      if (x > key) n += by_mass ? sr_mass(r, x) : 1;
+    __syncthreads();
+    const int d = sh.s_int[1];
+    run = sh.s_u64[0];
+    if (sh.count[d] == 1 || shift == 0) {
+      upto = run + (MASS ? sh.mass[d] : sh.count[d]);
+      return sh.any[d];
     }
-    return sr_block_sum(n, red);
-  };
+    prefix = (prefix << (top - shift)) | (u64)d;
+    top = shift;
+  }
+}
 
-  // kept: keys above `key`, and the first `ties` indexes with the key itself
-  uint32_t key = 0;
-  u64 ties = ~0ull;
-  if (k > 0 && k < V) {
-    u64 above;
-    key = search(false, (double)k, 0, above);
-    ties = k - above;
-  }
-  if (p < 1.0f) {
-    u64 above, kept = total(key, true);
-    if (ties != ~0ull) kept += ties * sr_mass(r, key);
-    const double goal = (double)p * (double)kept;
-    const uint32_t pk = search(true, goal, key, above);
-    const u64 w = sr_mass(r, pk);
-    const u64 cap = pk == key ? ties : ~0ull;
-    if (w > 0) {
-      u64 n = (u64)ceil((goal - (double)above) / (double)w);
-      if (n < 1) n = 1;
-      ties = n < cap ? n : cap;
-      key = pk;
+// The last place that is kept, from the row's n candidates.
+__device__ __forceinline__ u64 sr_cut(const SrRow& r, SrShared& sh, int n) {
+  const SrFound f = sh.found;
+  u64 cut = 0, mass_k = f.mass_k, upto;
+  if (f.bin_k < kSrBins) {
+    cut = sr_select<false>(r, sh, n, f.bin_k, f.bin_k, 0, 0, (double)f.need_k, upto);
+    if (r.p < 1.0) {
+      u64 in = 0;
+      sr_each(r, sh, n, f.bin_k, f.bin_k, cut, [&](u64 x) { in += sr_mass(r, sr_place_logit(x)); });
+      mass_k = f.before_k + sr_block_sum(in, sh.red);
     }
   }
-  // the draw, in index order: thread tid owns a contiguous slice
-  const int C = (V + 1023) / 1024, i0 = min(tid * C, V), i1 = min(i0 + C, V);
-  const u64 tie_mass = key != 0 && sr_weight(r, key) >= r.min_p ? sr_mass(r, key) : 0;
-  u64 gt = 0, eq = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t x = sr_key(l[i]);
-    if (x > key && sr_weight(r, x) >= r.min_p) gt += sr_mass(r, x);
-    eq += x == key;
-  }
-  const u64 eq_before = sr_block_before(eq, red);
-  const u64 eq_kept = eq_before >= ties ? 0 : (eq < ties - eq_before ? eq : ties - eq_before);
-  const u64 own = gt + eq_kept * tie_mass;
-  const u64 before = sr_block_before(own, red);
-  const double target = (double)u * (double)sr_block_sum(own, red);
-  if (tid == 0) s_id = (int)~(uint32_t)best;
+  if (r.p < 1.0 && f.lo < kSrBins)
+    cut = sr_select<true>(r, sh, n, f.lo, f.hi, cut, f.base, r.p * (double)mass_k, upto);
+  return cut;
+}
+
+// Whether the token is kept before min_p: bins before lo are, the others from
+// the cut on.
+__device__ __forceinline__ bool sr_in(const SrFound& f, u64 cut, int bin, u64 place) {
+  return bin < f.lo ? bin < kSrBins : sr_candidate(f, bin) && place >= cut;
+}
+
+// The token of tokens [i0, i1) at which the kept running mass, starting at
+// `before`, exceeds the target; the row's best where rounding leaves none.
+__device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, int i0, int i1, u64 before,
+                                       double target) {
+  const SrFound f = sh.found;
+  const int per = (i1 - i0 + kSrThreads - 1) / kSrThreads;
+  const int a0 = min(i0 + (int)threadIdx.x * per, i1), a1 = min(a0 + per, i1);
+  auto mass = [&](int i) -> u64 {
+    const float l = sr_clean(r.l[i]);
+    return sr_in(f, cut, sr_bin(r, l), sr_place(l, i)) ? sr_kept_mass(r, l) : 0;
+  };
+  u64 own = 0;
+  for (int i = a0; i < a1; ++i) own += mass(i);
+  u64 run = before + sr_block_before(own, sh.red);
+  if (threadIdx.x == 0) sh.s_int[2] = sr_best_id(r.best);
   __syncthreads();
-  if (own > 0 && (double)before <= target && (double)(before + own) > target) {
-    u64 run = before, seen = eq_before;
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t x = sr_key(l[i]);
-      if (x == key) {
-        if (seen < ties) run += tie_mass;
-        ++seen;
-      } else if (x > key && sr_weight(r, x) >= r.min_p) {
-        run += sr_mass(r, x);
-      }
+  if (own > 0 && (double)run <= target && (double)(run + own) > target) {
+    for (int i = a0; i < a1; ++i) {
+      run += mass(i);
       if ((double)run > target) {
-        s_id = i;
+        sh.s_int[2] = i;
         break;
       }
     }
   }
   __syncthreads();
-  if (tid == 0) a.ids[b] = s_id;
+  return sh.s_int[2];
 }
 
-void launch_sample_rows(const SampleRowsArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(k_sample_rows, dim3(a.B), dim3(1024), 0, st, a);
+// A row's place in the workspace: C chunks.
+struct SrSpace {
+  u64 *best, *sure, *mass, *list, *found;  // [C], [C], [C][bins], [kSrCap], [8]
+  uint32_t* count;                          // [C][bins]
+  int32_t* n;                               // arrivals of the two launches, candidates
+};
+__host__ __device__ inline size_t sr_space_bytes(int C) {
+  const size_t b = (size_t)C * (16 + kSrBins * 12) + kSrCap * 8 + 64 + 64;
+  return (b + 255) & ~(size_t)255;
+}
+__device__ __forceinline__ SrSpace sr_space(const SampleRowsArgs& a, int b) {
+  SrSpace s;
+  const int C = a.chunks;
+  u64* p = reinterpret_cast<u64*>(reinterpret_cast<char*>(a.workspace) + (size_t)b * sr_space_bytes(C));
+  s.best = p;
+  s.sure = p + C;
+  s.list = p + 2 * C;
+  s.found = s.list + kSrCap;
+  s.n = reinterpret_cast<int32_t*>(s.found + 8);
+  s.mass = s.found + 16;
+  s.count = reinterpret_cast<uint32_t*>(s.mass + (size_t)C * kSrBins);
+  return s;
+}
+
+__global__ __launch_bounds__(kSrThreads) void k_sr_max(SampleRowsArgs a) {
+  __shared__ u64 red[16];
+  const int c = blockIdx.x, b = blockIdx.y;
+  const SrSpace s = sr_space(a, b);
+  const u64 best = sr_chunk_max(a.logits + (int64_t)b * a.stride, c * a.chunk,
+                                min((c + 1) * a.chunk, a.V), red);
+  if (threadIdx.x == 0) s.best[c] = best;
+  if (c == 0 && threadIdx.x < 16) s.n[threadIdx.x] = 0;
+}
+
+// The row's parameters and maximum from the chunks'; false (the answer written
+// by the row's first block) where there is nothing to search.
+__device__ __forceinline__ bool sr_begin(const SampleRowsArgs& a, const SrSpace& s, int b, SrRow& r,
+                                         u64* red, bool answer) {
+  bool greedy;
+  const bool ok = sr_params(a, b, r, greedy);
+  u64 best = 0;
+  for (int c = threadIdx.x; c < a.chunks; c += kSrThreads) best = s.best[c] > best ? s.best[c] : best;
+  best = sr_block_max(best, red);
+  sr_set_best(r, best);
+  const bool none = (uint32_t)(best >> 32) <= kSrNone;
+  if (ok && !none && !greedy) return true;
+  if (answer && blockIdx.x == 0 && threadIdx.x == 0) {
+    a.ids[b] = ok && !none ? sr_best_id(best) : -1;
+    if (!ok) flag_dev_err(a.err, kDevErrSampleParam);
+  }
+  return false;
+}
+
+__global__ __launch_bounds__(kSrThreads) void k_sr_hist(SampleRowsArgs a) {
+  __shared__ SrShared sh;
+  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const SrSpace s = sr_space(a, b);
+  SrRow r;
+  if (!sr_begin(a, s, b, r, sh.red, false)) return;
+  if (r.k == 0 && r.p >= 1.0) return;  // every bin is kept
+  sr_chunk_hist(r, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
+  sr_put(s.mass + (size_t)c * kSrBins + tid, sh.mass[tid]);
+  __hip_atomic_store(s.count + (size_t)c * kSrBins + tid, sh.count[tid], __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
+  __syncthreads();
+  if (tid == 0)
+    sh.s_int[3] = __hip_atomic_fetch_add(s.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (sh.s_int[3] != a.chunks - 1) return;
+  u64 count = 0, mass = 0;
+#pragma unroll 8
+  for (int j = 0; j < a.chunks; ++j) {
+    mass += sr_get(s.mass + (size_t)j * kSrBins + tid);
+    count += __hip_atomic_load(s.count + (size_t)j * kSrBins + tid, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+  }
+  sr_scan(r, count, mass, sh);
+  if (tid == 0) {  // read by the next launch
+    const SrFound& f = sh.found;
+    s.found[0] = (u64)f.lo | (u64)f.hi << 16 | (u64)f.bin_k << 32;
+    s.found[1] = f.base;
+    s.found[2] = f.before_k;
+    s.found[3] = f.mass_k;
+    s.found[4] = f.need_k;
+  }
+}
+
+__global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
+  __shared__ SrShared sh;
+  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const SrSpace s = sr_space(a, b);
+  SrRow r;
+  if (!sr_begin(a, s, b, r, sh.red, true)) return;
+  if (tid == 0) {
+    SrFound f;
+    f.lo = f.hi = f.bin_k = kSrBins;
+    f.base = f.before_k = f.mass_k = f.need_k = 0;
+    if (r.k > 0 || r.p < 1.0) {
+      const u64 x = s.found[0];
+      f.lo = (int)(x & 0xFFFF);
+      f.hi = (int)(x >> 16 & 0xFFFF);
+      f.bin_k = (int)(x >> 32);
+      f.base = s.found[1];
+      f.before_k = s.found[2];
+      f.mass_k = s.found[3];
+      f.need_k = s.found[4];
+    }
+    sh.found = f;
+  }
+  __syncthreads();
+  const u64 sure = sr_collect(r, sh.found, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
+  const int mine = sh.s_int[0];
+  if (tid == 0) {
+    sr_put(s.sure + c, sure);
+    sh.s_int[1] = mine > 0 ? __hip_atomic_fetch_add(s.n + 2, mine, __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_AGENT) : 0;
+  }
+  __syncthreads();
+  const int at = sh.s_int[1];
+  for (int j = tid; j < min(mine, kSrCap) && at + j < kSrCap; j += kSrThreads)
+    sr_put(s.list + at + j, sh.list[j]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
+  __syncthreads();
+  if (tid == 0) {
+    sh.s_int[3] = __hip_atomic_fetch_add(s.n + 1, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (sh.s_int[3] != a.chunks - 1) return;
+  // the row's last block
+  const int n = __hip_atomic_load(s.n + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int j = tid; j < min(n, kSrCap); j += kSrThreads) sh.list[j] = sr_get(s.list + j);
+  __syncthreads();
+  const u64 cut = sr_cut(r, sh, n);
+  // the chunks' kept masses, 512 chunks at a time: first all, then up to the draw
+  auto kept_of = [&](int c0) {
+    __syncthreads();
+    sh.mass[tid] = c0 + tid < a.chunks ? sr_get(s.sure + c0 + tid) : 0;
+    __syncthreads();
+    const SrFound f = sh.found;
+    auto add = [&](u64 x) {
+      const float l = sr_place_logit(x);
+      const int chunk = (int)~(uint32_t)x / a.chunk - c0;
+      const int bin = sr_bin(r, l);
+      if (bin >= f.lo && chunk >= 0 && chunk < kSrThreads && sr_in(f, cut, bin, x))
+        atomicAdd(&sh.mass[chunk], sr_kept_mass(r, l));
+    };
+    sr_each(r, sh, n, f.lo, kSrBins - 1, 0, add);
+    __syncthreads();
+    return sh.mass[tid];
+  };
+  u64 total = 0;
+  for (int c0 = 0; c0 < a.chunks; c0 += kSrThreads) total += sr_block_sum(kept_of(c0), sh.red);
+  const double target = r.u * (double)total;
+  u64 before = 0;
+  for (int c0 = 0; c0 < a.chunks; c0 += kSrThreads) {
+    const u64 own = a.chunks > kSrThreads ? kept_of(c0) : sh.mass[tid];
+    const u64 run = before + sr_block_before(own, sh.red);
+    if (tid == 0) sh.s_int[3] = -1;
+    __syncthreads();
+    if (own > 0 && (double)run <= target && (double)(run + own) > target) {
+      sh.s_int[3] = c0 + tid;
+      sh.s_u64[1] = run;
+    }
+    __syncthreads();
+    if (sh.s_int[3] >= 0) break;
+    before += sr_block_sum(own, sh.red);
+  }
+  int id = sr_best_id(r.best);
+  const int hit = sh.s_int[3];
+  if (hit >= 0)
+    id = sr_walk(r, sh, cut, hit * a.chunk, min((hit + 1) * a.chunk, a.V), sh.s_u64[1], target);
+  if (tid == 0) a.ids[b] = id;
+}
+
+// A row of one chunk: the same steps in one block.
+__global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
+  __shared__ SrShared sh;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  SrRow r;
+  bool greedy;
+  const bool ok = sr_params(a, b, r, greedy);
+  const u64 best = sr_chunk_max(r.l, 0, a.V, sh.red);
+  sr_set_best(r, best);
+  const bool none = (uint32_t)(best >> 32) <= kSrNone;
+  if (!ok || none || greedy) {
+    if (tid == 0) {
+      a.ids[b] = ok && !none ? sr_best_id(best) : -1;
+      if (!ok) flag_dev_err(a.err, kDevErrSampleParam);
+    }
+    return;
+  }
+  u64 cut = 0;
+  if (tid == 0) {
+    SrFound f;
+    f.lo = f.hi = f.bin_k = kSrBins;
+    f.base = f.before_k = f.mass_k = f.need_k = 0;
+    sh.found = f;
+  }
+  __syncthreads();
+  u64 total;
+  if (r.k > 0 || r.p < 1.0) {
+    sr_chunk_hist(r, 0, a.V, sh);
+    sr_scan(r, sh.count[tid], sh.mass[tid], sh);
+    total = sr_collect(r, sh.found, 0, a.V, sh);
+    const int n = sh.s_int[0];
+    cut = sr_cut(r, sh, n);
+    const SrFound f = sh.found;
+    u64 more = 0;
+    sr_each(r, sh, n, f.lo, kSrBins - 1, 0, [&](u64 x) {
+      const float l = sr_place_logit(x);
+      if (sr_in(f, cut, sr_bin(r, l), x)) more += sr_kept_mass(r, l);
+    });
+    total += sr_block_sum(more, sh.red);
+  } else {
+    total = sr_collect(r, sh.found, 0, a.V, sh);
+  }
+  const int id = sr_walk(r, sh, cut, 0, a.V, 0, r.u * (double)total);
+  if (tid == 0) a.ids[b] = id;
+}
+
+// Tokens of a chunk: few enough for some blocks per CU, 4096 at least (a block's
+// fixed steps), so that the bins' partial sums stay a fraction of the logits.
+static int sr_chunk(int B, int V) {
+  int chunk = 4096;
+  while (chunk < 65536 && (int64_t)B * ((V + chunk - 1) / chunk) > 1024) chunk *= 2;
+  return chunk;
+}
+
+size_t sample_rows_workspace(int B, int V) {
+  const int C = (V + sr_chunk(B, V) - 1) / sr_chunk(B, V);
+  return C == 1 ? 0 : (size_t)B * sr_space_bytes(C);
+}
+
+void launch_sample_rows(SampleRowsArgs a, hipStream_t st) {
+  a.chunk = sr_chunk(a.B, a.V);
+  a.chunks = (a.V + a.chunk - 1) / a.chunk;
+  if (a.chunks == 1) {
+    hipLaunchKernelGGL(k_sr_one, dim3(a.B), dim3(kSrThreads), 0, st, a);
+    return;
+  }
+  const dim3 grid(a.chunks, a.B);
+  hipLaunchKernelGGL(k_sr_max, grid, dim3(kSrThreads), 0, st, a);
+  if (a.top_k != nullptr || a.top_p != nullptr)
+    hipLaunchKernelGGL(k_sr_hist, grid, dim3(kSrThreads), 0, st, a);
+  hipLaunchKernelGGL(k_sr_pick, grid, dim3(kSrThreads), 0, st, a);
 }
 
 }  // namespace neon
