@@ -33,8 +33,8 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 // A row is cut into chunks of one block each.  The order is searched in bins of
 // 1/16 of T below the maximum (512 of them; what lies further down has mass 0):
 //   k_sr_max    chunk maxima
-//   k_sr_hist   per chunk the count and mass of every bin; the row's last block
-//               sums them and finds the bins that the top_k-th token and the
+//   k_sr_hist   adds the chunk's count and mass of every bin to the row's; the
+//               row's last block finds the bins that the top_k-th token and the
 //               token at top_p's goal can lie in
 //   k_sr_pick   per chunk the mass of the bins above those, which is kept
 //               whatever the exact places are, and the tokens of those bins (the
@@ -75,6 +75,13 @@ __device__ __forceinline__ u64 sr_mass(const SrRow& r, float l) {
 __device__ __forceinline__ u64 sr_kept_mass(const SrRow& r, float l) {
   const double w = sr_weight(r, l);
   return w >= r.min_p ? (u64)__builtin_rint(w * r.scale) : 0;
+}
+// The first bin whose weights all lie below min_p (w <= exp(-bin / 16), the
+// 1 + 2^-10 covers the rounding of the bins and of the logarithm).
+__device__ __forceinline__ int sr_min_bin(const SrRow& r) {
+  if (!(r.min_p > 0.0)) return kSrBins;
+  return (int)fminf(-__logf((float)r.min_p) * (kSrBinsPerT * (1.0f + 0x1p-10f)) + 2.0f,
+                    (float)kSrBins);
 }
 // Falls with l, never rises: each step rounds monotonically.
 __device__ __forceinline__ int sr_bin(const SrRow& r, float l) {
@@ -149,14 +156,17 @@ struct SrFound {
   u64 need_k;     // tokens of bin_k that are among the top_k
 };
 
-struct SrShared {
+struct SrHistShared {
   u64 red[16];
-  u64 list[kSrCap];
-  u64 mass[kSrBins], any[256];
+  u64 mass[kSrBins];
   uint32_t count[kSrBins];
   SrFound found;
   u64 s_u64[2];
   int s_int[4];
+};
+struct SrShared : SrHistShared {
+  u64 any[256];
+  u64 list[kSrCap];
 };
 
 // Reads row b's parameters; false where one is out of range.
@@ -186,33 +196,54 @@ __device__ __forceinline__ void sr_set_best(SrRow& r, u64 best) {
 }
 __device__ __forceinline__ int sr_best_id(u64 best) { return (int)~(uint32_t)best; }
 
+// Tokens i0 + thread, + 512, ..: eight are requested at once (past i1 the last
+// one again, as minus infinity).  fn(logits, index of the first).
+template <class F>
+__device__ __forceinline__ void sr_tokens(const float* l, int i0, int i1, F fn) {
+  for (int i = i0 + threadIdx.x; i < i1; i += 8 * kSrThreads) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = l[min(i + j * kSrThreads, i1 - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = i + j * kSrThreads < i1 ? sr_clean(v[j]) : -INFINITY;
+    fn(v, i);
+  }
+}
+
 __device__ __forceinline__ u64 sr_chunk_max(const float* l, int i0, int i1, u64* red) {
   u64 best = 0;
-  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
-    const u64 x = sr_place(sr_clean(l[i]), i);
-    best = x > best ? x : best;
-  }
+  sr_tokens(l, i0, i1, [&](const float (&v)[8], int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const u64 x = sr_place(v[j], i + j * kSrThreads);
+      best = x > best ? x : best;
+    }
+  });
   return sr_block_max(best, red);
 }
 
 // counts and masses of the chunk's bins into sh.count / sh.mass
-__device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SrShared& sh) {
+template <class SH>
+__device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SH& sh) {
   sh.mass[threadIdx.x] = 0;
   sh.count[threadIdx.x] = 0;
   __syncthreads();
-  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
-    const float l = sr_clean(r.l[i]);
-    const int bin = sr_bin(r, l);
-    if (bin < kSrBins) {
-      atomicAdd(&sh.count[bin], 1u);
-      atomicAdd(&sh.mass[bin], sr_mass(r, l));
+  sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int bin = sr_bin(r, v[j]);
+      if (bin < kSrBins) {
+        atomicAdd(&sh.count[bin], 1u);
+        atomicAdd(&sh.mass[bin], sr_mass(r, v[j]));
+      }
     }
-  }
+  });
   __syncthreads();
 }
 
 // The bins to look into, from the row's counts and masses (thread = bin).
-__device__ __forceinline__ void sr_scan(const SrRow& r, u64 count, u64 mass, SrShared& sh) {
+template <class SH>
+__device__ __forceinline__ void sr_scan(const SrRow& r, u64 count, u64 mass, SH& sh) {
   const int bin = threadIdx.x;
   const u64 c0 = sr_block_before(count, sh.red), m0 = sr_block_before(mass, sh.red);
   const u64 c1 = c0 + count, m1 = m0 + mass;
@@ -264,16 +295,30 @@ __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int 
   if (threadIdx.x == 0) sh.s_int[0] = 0;
   __syncthreads();
   u64 sure = 0;
-  for (int i = i0 + threadIdx.x; i < i1; i += kSrThreads) {
-    const float l = sr_clean(r.l[i]);
-    const int bin = sr_bin(r, l);
-    if (bin < f.lo) {
-      if (bin < kSrBins) sure += sr_kept_mass(r, l);
-    } else if (bin < kSrBins && sr_candidate(f, bin)) {
-      const int at = atomicAdd(&sh.s_int[0], 1);
-      if (at < kSrCap) sh.list[at] = sr_place(l, i);
+  const int keep = min(min(f.lo, kSrBins), sr_min_bin(r));
+  sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int i) {
+    uint32_t todo = 0;  // a bit for each that has mass to add
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int bin = sr_bin(r, v[j]);
+      if (bin < keep) {
+        todo |= 1u << j;
+      } else if (bin >= f.lo && bin < kSrBins && sr_candidate(f, bin)) {
+        const int at = atomicAdd(&sh.s_int[0], 1);
+        if (at < kSrCap) sh.list[at] = sr_place(v[j], i + j * kSrThreads);
+      }
     }
-  }
+    // A wave pays an exponential for all its lanes if one needs it, and mostly a
+    // few of a hundred tokens do: each turn takes every lane's next one.
+    while (__any(todo != 0)) {
+      const int at = __builtin_ctz(todo | 0x80000000u);
+      float l = v[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) l = at == j ? v[j] : l;
+      if (todo != 0) sure += sr_kept_mass(r, l);
+      todo &= todo - 1;
+    }
+  });
   return sr_block_sum(sure, sh.red);
 }
 
@@ -420,18 +465,27 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
   const SrFound f = sh.found;
   const int per = (i1 - i0 + kSrThreads - 1) / kSrThreads;
   const int a0 = min(i0 + (int)threadIdx.x * per, i1), a1 = min(a0 + per, i1);
-  auto mass = [&](int i) -> u64 {
-    const float l = sr_clean(r.l[i]);
-    return sr_in(f, cut, sr_bin(r, l), sr_place(l, i)) ? sr_kept_mass(r, l) : 0;
+  const int limit = sr_min_bin(r);
+  auto mass = [&](float l, int i) -> u64 {
+    const int bin = sr_bin(r, l);
+    if (bin >= limit) return 0;
+    return sr_in(f, cut, bin, sr_place(l, i)) ? sr_kept_mass(r, l) : 0;
   };
   u64 own = 0;
-  for (int i = a0; i < a1; ++i) own += mass(i);
+  for (int i = a0; i < a1; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = r.l[min(i + j, a1 - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < a1) own += mass(sr_clean(v[j]), i + j);
+  }
   u64 run = before + sr_block_before(own, sh.red);
   if (threadIdx.x == 0) sh.s_int[2] = sr_best_id(r.best);
   __syncthreads();
   if (own > 0 && (double)run <= target && (double)(run + own) > target) {
     for (int i = a0; i < a1; ++i) {
-      run += mass(i);
+      run += mass(sr_clean(r.l[i]), i);
       if ((double)run > target) {
         sh.s_int[2] = i;
         break;
@@ -444,12 +498,12 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
 
 // A row's place in the workspace: C chunks.
 struct SrSpace {
-  u64 *best, *sure, *mass, *list, *found;  // [C], [C], [C][bins], [kSrCap], [8]
-  uint32_t* count;                          // [C][bins]
+  u64 *best, *sure, *list, *found;  // [C], [C], [kSrCap], [8]
+  u64 *mass, *count;                // [bins]
   int32_t* n;                               // arrivals of the two launches, candidates
 };
 __host__ __device__ inline size_t sr_space_bytes(int C) {
-  const size_t b = (size_t)C * (16 + kSrBins * 12) + kSrCap * 8 + 64 + 64;
+  const size_t b = (size_t)C * 16 + kSrCap * 8 + 64 + 64 + kSrBins * 16;
   return (b + 255) & ~(size_t)255;
 }
 __device__ __forceinline__ SrSpace sr_space(const SampleRowsArgs& a, int b) {
@@ -462,7 +516,7 @@ __device__ __forceinline__ SrSpace sr_space(const SampleRowsArgs& a, int b) {
   s.found = s.list + kSrCap;
   s.n = reinterpret_cast<int32_t*>(s.found + 8);
   s.mass = s.found + 16;
-  s.count = reinterpret_cast<uint32_t*>(s.mass + (size_t)C * kSrBins);
+  s.count = s.mass + kSrBins;
   return s;
 }
 
@@ -473,7 +527,11 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_max(SampleRowsArgs a) {
   const u64 best = sr_chunk_max(a.logits + (int64_t)b * a.stride, c * a.chunk,
                                 min((c + 1) * a.chunk, a.V), red);
   if (threadIdx.x == 0) s.best[c] = best;
-  if (c == 0 && threadIdx.x < 16) s.n[threadIdx.x] = 0;
+  if (c == 0) {  // for the next launches
+    if (threadIdx.x < 16) s.n[threadIdx.x] = 0;
+    s.mass[threadIdx.x] = 0;
+    s.count[threadIdx.x] = 0;
+  }
 }
 
 // The row's parameters and maximum from the chunks'; false (the answer written
@@ -496,29 +554,25 @@ __device__ __forceinline__ bool sr_begin(const SampleRowsArgs& a, const SrSpace&
 }
 
 __global__ __launch_bounds__(kSrThreads) void k_sr_hist(SampleRowsArgs a) {
-  __shared__ SrShared sh;
+  __shared__ SrHistShared sh;
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const SrSpace s = sr_space(a, b);
   SrRow r;
   if (!sr_begin(a, s, b, r, sh.red, false)) return;
   if (r.k == 0 && r.p >= 1.0) return;  // every bin is kept
   sr_chunk_hist(r, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
-  sr_put(s.mass + (size_t)c * kSrBins + tid, sh.mass[tid]);
-  __hip_atomic_store(s.count + (size_t)c * kSrBins + tid, sh.count[tid], __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
+  if (sh.count[tid] > 0) {  // integers: no order changes the sums
+    __hip_atomic_fetch_add(s.mass + tid, sh.mass[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_fetch_add(s.count + tid, (u64)sh.count[tid], __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
   __syncthreads();
   if (tid == 0)
     sh.s_int[3] = __hip_atomic_fetch_add(s.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (sh.s_int[3] != a.chunks - 1) return;
-  u64 count = 0, mass = 0;
-#pragma unroll 8
-  for (int j = 0; j < a.chunks; ++j) {
-    mass += sr_get(s.mass + (size_t)j * kSrBins + tid);
-    count += __hip_atomic_load(s.count + (size_t)j * kSrBins + tid, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-  }
+  const u64 count = sr_get(s.count + tid), mass = sr_get(s.mass + tid);
   sr_scan(r, count, mass, sh);
   if (tid == 0) {  // read by the next launch
     const SrFound& f = sh.found;
