@@ -50,6 +50,9 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 constexpr int kSrThreads = 512;
 constexpr int kSrBins = 512;   // one per thread in the scan
 constexpr int kSrCap = 8192;   // candidates of a row that are listed
+constexpr int kSrPart = 8 * kSrThreads;  // tokens whose kept mass is held apart
+constexpr int kSrMaxChunk = 65536;
+constexpr int kSrMaxParts = kSrMaxChunk / kSrPart;
 constexpr float kSrBinsPerT = 16.0f;
 
 // A row's parameters as the kernels use them.
@@ -288,13 +291,15 @@ __device__ __forceinline__ bool sr_candidate(const SrFound& f, int bin) {
   return (bin >= f.lo && bin <= f.hi && bin < kSrBins) || bin == f.bin_k;
 }
 
-// The kept mass of the chunk's sure bins; its candidates into sh.list (as many
-// as fit; sh.s_int[0] counts all).
+// The kept mass of the sure bins of each part of tokens [i0, i1) (i0 a multiple
+// of kSrPart) into sh.mass[0 ..], thread = part for the result; the candidates
+// into sh.list (as many as fit; sh.s_int[0] counts all).
 __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int i0, int i1,
                                           SrShared& sh) {
-  if (threadIdx.x == 0) sh.s_int[0] = 0;
   __syncthreads();
-  u64 sure = 0;
+  if (threadIdx.x == 0) sh.s_int[0] = 0;
+  if (threadIdx.x < kSrMaxParts) sh.mass[threadIdx.x] = 0;
+  __syncthreads();
   const int keep = min(min(f.lo, kSrBins), sr_min_bin(r));
   sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int i) {
     uint32_t todo = 0;  // a bit for each that has mass to add
@@ -310,6 +315,7 @@ __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int 
     }
     // A wave pays an exponential for all its lanes if one needs it, and mostly a
     // few of a hundred tokens do: each turn takes every lane's next one.
+    u64 sure = 0;
     while (__any(todo != 0)) {
       const int at = __builtin_ctz(todo | 0x80000000u);
       float l = v[0];
@@ -318,8 +324,10 @@ __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int 
       if (todo != 0) sure += sr_kept_mass(r, l);
       todo &= todo - 1;
     }
+    if (sure > 0) atomicAdd(&sh.mass[(i - i0) / kSrPart], sure);
   });
-  return sr_block_sum(sure, sh.red);
+  __syncthreads();
+  return threadIdx.x < kSrMaxParts ? sh.mass[threadIdx.x] : 0;
 }
 
 __device__ __forceinline__ float sr_place_logit(u64 place) {
@@ -435,8 +443,72 @@ __device__ __forceinline__ u64 sr_select(const SrRow& r, SrShared& sh, int n, in
   }
 }
 
+template <int J>
+__device__ __forceinline__ u64 sr_xor_lane(u64 x) {
+  return (u64)(uint32_t)xor_lane_i<J>((int)(uint32_t)x) |
+         (u64)(uint32_t)xor_lane_i<J>((int)(x >> 32)) << 32;
+}
+// One compare-exchange of a bitonic sort, descending: runs of K, distance J.
+template <int K, int J>
+__device__ __forceinline__ void sr_sort_step(u64& x, u64* buf) {
+  const int tid = threadIdx.x;
+  u64 y;
+  if constexpr (J < 64) {
+    y = sr_xor_lane<J>(x);
+  } else {
+    __syncthreads();
+    buf[tid] = x;
+    __syncthreads();
+    y = buf[tid ^ J];
+  }
+  const bool larger = ((tid & K) == 0) == ((tid & J) == 0);
+  x = (x > y) == larger ? x : y;
+  if constexpr (J > 1) sr_sort_step<K, J / 2>(x, buf);
+}
+template <int K>
+__device__ __forceinline__ void sr_sort(u64& x, u64* buf) {
+  sr_sort_step<K, K / 2>(x, buf);
+  if constexpr (K < kSrThreads) sr_sort<2 * K>(x, buf);
+}
+
+// sr_cut for up to one candidate per thread: sorted, the places are positions.
+// A selection by digits takes about two passes for each of the two places, each
+// with a histogram, its sum and six barriers: 10 us where this takes 4.
+__device__ __forceinline__ u64 sr_cut_sorted(const SrRow& r, SrShared& sh, int n) {
+  const int tid = threadIdx.x;
+  const SrFound f = sh.found;
+  u64 x = tid < n ? sh.list[tid] : 0;
+  sr_sort<2>(x, sh.list);
+  __syncthreads();
+  sh.list[tid] = x;
+  const bool has = tid < n;
+  const float l = sr_place_logit(x);
+  const int bin = has ? sr_bin(r, l) : kSrBins;
+  u64 mass_k = f.mass_k, cut = 0;
+  const u64 mass = has && r.p < 1.0 ? sr_mass(r, l) : 0;
+  bool in = has;  // among the top_k
+  if (f.bin_k < kSrBins) {
+    const int first = __syncthreads_count(bin < f.bin_k);
+    in = has && tid < first + (int)f.need_k;
+    cut = sh.list[min(first + (int)f.need_k, n) - 1];
+    if (r.p < 1.0) mass_k = f.before_k + sr_block_sum(in && bin == f.bin_k ? mass : 0, sh.red);
+  }
+  __syncthreads();  // the sorted list is there
+  if (r.p < 1.0 && f.lo < kSrBins) {
+    const bool mine = in && bin >= f.lo && bin <= f.hi;
+    const u64 own = mine ? mass : 0;
+    const u64 upto = f.base + sr_block_before(own, sh.red) + own;
+    // the first of them that reaches the goal, else the last of them
+    const int all = __syncthreads_count(mine);
+    const int short_of = __syncthreads_count(mine && (double)upto < r.p * (double)mass_k);
+    cut = sh.list[max(min(short_of, all - 1), 0)];
+  }
+  return cut;
+}
+
 // The last place that is kept, from the row's n candidates.
 __device__ __forceinline__ u64 sr_cut(const SrRow& r, SrShared& sh, int n) {
+  if (n <= kSrThreads) return sr_cut_sorted(r, sh, n);
   const SrFound f = sh.found;
   u64 cut = 0, mass_k = f.mass_k, upto;
   if (f.bin_k < kSrBins) {
@@ -458,61 +530,147 @@ __device__ __forceinline__ bool sr_in(const SrFound& f, u64 cut, int bin, u64 pl
   return bin < f.lo ? bin < kSrBins : sr_candidate(f, bin) && place >= cut;
 }
 
-// The token of tokens [i0, i1) at which the kept running mass, starting at
-// `before`, exceeds the target; the row's best where rounding leaves none.
+// The token of the part [i0, i1) (up to kSrPart of them) at which the kept
+// running mass, starting at `before`, exceeds the target; the row's best where
+// rounding leaves none.  A thread holds the tokens tid + 512 j, so a wave's 64
+// for one j are in order: their masses add up in a segment each.
 __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, int i0, int i1, u64 before,
                                        double target) {
+  const int tid = threadIdx.x, wave = tid >> 6;
   const SrFound f = sh.found;
-  const int per = (i1 - i0 + kSrThreads - 1) / kSrThreads;
-  const int a0 = min(i0 + (int)threadIdx.x * per, i1), a1 = min(a0 + per, i1);
   const int limit = sr_min_bin(r);
-  auto mass = [&](float l, int i) -> u64 {
-    const int bin = sr_bin(r, l);
-    if (bin >= limit) return 0;
-    return sr_in(f, cut, bin, sr_place(l, i)) ? sr_kept_mass(r, l) : 0;
-  };
-  u64 own = 0;
-  for (int i = a0; i < a1; i += 8) {
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r.l[min(i + j, a1 - 1)];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < a1) own += mass(sr_clean(v[j]), i + j);
-  }
-  u64 run = before + sr_block_before(own, sh.red);
-  if (threadIdx.x == 0) sh.s_int[2] = sr_best_id(r.best);
   __syncthreads();
-  if (own > 0 && (double)run <= target && (double)(run + own) > target) {
-    for (int i = a0; i < a1; ++i) {
-      run += mass(sr_clean(r.l[i]), i);
-      if ((double)run > target) {
-        sh.s_int[2] = i;
-        break;
-      }
+  if (tid < 64) sh.mass[tid] = 0;
+  if (tid == 0) sh.s_int[2] = sr_best_id(r.best);
+  __syncthreads();
+  u64 m[8];
+  uint32_t todo = 0;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    m[j] = 0;
+    v[j] = r.l[min(i0 + tid + j * kSrThreads, i1 - 1)];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = i0 + tid + j * kSrThreads;
+    v[j] = sr_clean(v[j]);
+    const int bin = sr_bin(r, v[j]);
+    if (i < i1 && bin < limit && sr_in(f, cut, bin, sr_place(v[j], i))) todo |= 1u << j;
+  }
+  while (__any(todo != 0)) {  // as in sr_collect
+    const int at = __builtin_ctz(todo | 0x80000000u);
+    float l = v[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) l = at == j ? v[j] : l;
+    const u64 x = todo != 0 ? sr_kept_mass(r, l) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = at == j ? x : m[j];
+    if (x > 0) atomicAdd(&sh.mass[8 * at + wave], x);
+    todo &= todo - 1;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const u64 own = sh.mass[tid];
+    u64 x = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 y = __shfl_up(x, o);
+      if (tid >= o) x += y;
     }
+    x += before;
+    const u64 hit = __ballot(own > 0 && (double)x > target);
+    if (tid == (hit ? __builtin_ctzll(hit) : 0)) {
+      sh.s_int[1] = hit ? tid : -1;
+      sh.s_u64[0] = x - own;
+    }
+  }
+  __syncthreads();
+  const int seg = sh.s_int[1];
+  if (seg >= 0 && wave == (seg & 7)) {
+    const int j = seg >> 3, lane = tid & 63;
+    u64 own = m[0];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) own = j == q ? m[q] : own;
+    u64 x = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    const u64 hit = __ballot(own > 0 && (double)(x + sh.s_u64[0]) > target);
+    if (hit && lane == __builtin_ctzll(hit)) sh.s_int[2] = i0 + tid + j * kSrThreads;
   }
   __syncthreads();
   return sh.s_int[2];
 }
 
+// The draw, from the parts' kept masses: part_mass(p0) gives the thread's of 512
+// parts from p0 on.
+template <class F>
+__device__ __forceinline__ int sr_draw(const SrRow& r, SrShared& sh, u64 cut, F part_mass) {
+  const int tid = threadIdx.x, parts = (r.V + kSrPart - 1) / kSrPart;
+  u64 total = 0, own = 0;
+  for (int p0 = 0; p0 < parts; p0 += kSrThreads) {
+    own = part_mass(p0);
+    total += sr_block_sum(own, sh.red);
+  }
+  const double target = r.u * (double)total;
+  u64 before = 0;
+  for (int p0 = 0; p0 < parts; p0 += kSrThreads) {
+    if (parts > kSrThreads) own = part_mass(p0);
+    const u64 run = before + sr_block_before(own, sh.red);
+    if (tid == 0) sh.s_int[3] = -1;
+    __syncthreads();
+    if (own > 0 && (double)run <= target && (double)(run + own) > target) {
+      sh.s_int[3] = p0 + tid;
+      sh.s_u64[1] = run;
+    }
+    __syncthreads();
+    if (sh.s_int[3] >= 0) break;
+    before += sr_block_sum(own, sh.red);
+  }
+  const int hit = sh.s_int[3];
+  const u64 run = sh.s_u64[1];
+  return hit < 0 ? sr_best_id(r.best)
+                 : sr_walk(r, sh, cut, hit * kSrPart, min((hit + 1) * kSrPart, r.V), run, target);
+}
+
+// Adds the kept candidates of 512 parts from p0 on to the thread's `sure` mass.
+__device__ __forceinline__ u64 sr_part_mass(const SrRow& r, SrShared& sh, u64 cut, int n, int p0,
+                                            u64 sure) {
+  const SrFound f = sh.found;
+  __syncthreads();
+  sh.mass[threadIdx.x] = sure;
+  __syncthreads();
+  sr_each(r, sh, n, f.lo, kSrBins - 1, 0, [&](u64 x) {
+    const float l = sr_place_logit(x);
+    const int part = (int)~(uint32_t)x / kSrPart - p0;
+    if (part >= 0 && part < kSrThreads && sr_in(f, cut, sr_bin(r, l), x))
+      atomicAdd(&sh.mass[part], sr_kept_mass(r, l));
+  });
+  __syncthreads();
+  return sh.mass[threadIdx.x];
+}
+
 // A row's place in the workspace: C chunks.
 struct SrSpace {
-  u64 *best, *sure, *list, *found;  // [C], [C], [kSrCap], [8]
+  u64 *best, *sure, *list, *found;  // [C], [parts], [kSrCap], [8]
   u64 *mass, *count;                // [bins]
   int32_t* n;                               // arrivals of the two launches, candidates
 };
-__host__ __device__ inline size_t sr_space_bytes(int C) {
-  const size_t b = (size_t)C * 16 + kSrCap * 8 + 64 + 64 + kSrBins * 16;
+__host__ __device__ inline size_t sr_space_bytes(int C, int V) {
+  const size_t b = (size_t)C * 8 + (size_t)((V + kSrPart - 1) / kSrPart) * 8 + kSrCap * 8 + 64 + 64 +
+                   kSrBins * 16;
   return (b + 255) & ~(size_t)255;
 }
 __device__ __forceinline__ SrSpace sr_space(const SampleRowsArgs& a, int b) {
   SrSpace s;
   const int C = a.chunks;
-  u64* p = reinterpret_cast<u64*>(reinterpret_cast<char*>(a.workspace) + (size_t)b * sr_space_bytes(C));
+  u64* p = reinterpret_cast<u64*>(reinterpret_cast<char*>(a.workspace) + (size_t)b * sr_space_bytes(C, a.V));
   s.best = p;
   s.sure = p + C;
-  s.list = p + 2 * C;
+  s.list = s.sure + (a.V + kSrPart - 1) / kSrPart;
   s.found = s.list + kSrCap;
   s.n = reinterpret_cast<int32_t*>(s.found + 8);
   s.mass = s.found + 16;
@@ -609,11 +767,11 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   __syncthreads();
   const u64 sure = sr_collect(r, sh.found, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
   const int mine = sh.s_int[0];
-  if (tid == 0) {
-    sr_put(s.sure + c, sure);
+  const int part = c * (a.chunk / kSrPart) + tid;
+  if (tid < a.chunk / kSrPart && (int64_t)part * kSrPart < a.V) sr_put(s.sure + part, sure);
+  if (tid == 0)
     sh.s_int[1] = mine > 0 ? __hip_atomic_fetch_add(s.n + 2, mine, __ATOMIC_RELAXED,
                                                     __HIP_MEMORY_SCOPE_AGENT) : 0;
-  }
   __syncthreads();
   const int at = sh.s_int[1];
   for (int j = tid; j < min(mine, kSrCap) && at + j < kSrCap; j += kSrThreads)
@@ -630,44 +788,10 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   for (int j = tid; j < min(n, kSrCap); j += kSrThreads) sh.list[j] = sr_get(s.list + j);
   __syncthreads();
   const u64 cut = sr_cut(r, sh, n);
-  // the chunks' kept masses, 512 chunks at a time: first all, then up to the draw
-  auto kept_of = [&](int c0) {
-    __syncthreads();
-    sh.mass[tid] = c0 + tid < a.chunks ? sr_get(s.sure + c0 + tid) : 0;
-    __syncthreads();
-    const SrFound f = sh.found;
-    auto add = [&](u64 x) {
-      const float l = sr_place_logit(x);
-      const int chunk = (int)~(uint32_t)x / a.chunk - c0;
-      const int bin = sr_bin(r, l);
-      if (bin >= f.lo && chunk >= 0 && chunk < kSrThreads && sr_in(f, cut, bin, x))
-        atomicAdd(&sh.mass[chunk], sr_kept_mass(r, l));
-    };
-    sr_each(r, sh, n, f.lo, kSrBins - 1, 0, add);
-    __syncthreads();
-    return sh.mass[tid];
-  };
-  u64 total = 0;
-  for (int c0 = 0; c0 < a.chunks; c0 += kSrThreads) total += sr_block_sum(kept_of(c0), sh.red);
-  const double target = r.u * (double)total;
-  u64 before = 0;
-  for (int c0 = 0; c0 < a.chunks; c0 += kSrThreads) {
-    const u64 own = a.chunks > kSrThreads ? kept_of(c0) : sh.mass[tid];
-    const u64 run = before + sr_block_before(own, sh.red);
-    if (tid == 0) sh.s_int[3] = -1;
-    __syncthreads();
-    if (own > 0 && (double)run <= target && (double)(run + own) > target) {
-      sh.s_int[3] = c0 + tid;
-      sh.s_u64[1] = run;
-    }
-    __syncthreads();
-    if (sh.s_int[3] >= 0) break;
-    before += sr_block_sum(own, sh.red);
-  }
-  int id = sr_best_id(r.best);
-  const int hit = sh.s_int[3];
-  if (hit >= 0)
-    id = sr_walk(r, sh, cut, hit * a.chunk, min((hit + 1) * a.chunk, a.V), sh.s_u64[1], target);
+  const int parts = (a.V + kSrPart - 1) / kSrPart;
+  const int id = sr_draw(r, sh, cut, [&](int p0) {
+    return sr_part_mass(r, sh, cut, n, p0, p0 + tid < parts ? sr_get(s.sure + p0 + tid) : 0);
+  });
   if (tid == 0) a.ids[b] = id;
 }
 
@@ -696,24 +820,14 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
     sh.found = f;
   }
   __syncthreads();
-  u64 total;
   if (r.k > 0 || r.p < 1.0) {
     sr_chunk_hist(r, 0, a.V, sh);
     sr_scan(r, sh.count[tid], sh.mass[tid], sh);
-    total = sr_collect(r, sh.found, 0, a.V, sh);
-    const int n = sh.s_int[0];
-    cut = sr_cut(r, sh, n);
-    const SrFound f = sh.found;
-    u64 more = 0;
-    sr_each(r, sh, n, f.lo, kSrBins - 1, 0, [&](u64 x) {
-      const float l = sr_place_logit(x);
-      if (sr_in(f, cut, sr_bin(r, l), x)) more += sr_kept_mass(r, l);
-    });
-    total += sr_block_sum(more, sh.red);
-  } else {
-    total = sr_collect(r, sh.found, 0, a.V, sh);
   }
-  const int id = sr_walk(r, sh, cut, 0, a.V, 0, r.u * (double)total);
+  const u64 sure = sr_collect(r, sh.found, 0, a.V, sh);
+  const int n = sh.s_int[0];
+  if (r.k > 0 || r.p < 1.0) cut = sr_cut(r, sh, n);
+  const int id = sr_draw(r, sh, cut, [&](int p0) { return sr_part_mass(r, sh, cut, n, p0, sure); });
   if (tid == 0) a.ids[b] = id;
 }
 
@@ -721,13 +835,13 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
 // fixed steps), so that the bins' partial sums stay a fraction of the logits.
 static int sr_chunk(int B, int V) {
   int chunk = 4096;
-  while (chunk < 65536 && (int64_t)B * ((V + chunk - 1) / chunk) > 1024) chunk *= 2;
+  while (chunk < kSrMaxChunk && (int64_t)B * ((V + chunk - 1) / chunk) > 1024) chunk *= 2;
   return chunk;
 }
 
 size_t sample_rows_workspace(int B, int V) {
   const int C = (V + sr_chunk(B, V) - 1) / sr_chunk(B, V);
-  return C == 1 ? 0 : (size_t)B * sr_space_bytes(C);
+  return C == 1 ? 0 : (size_t)B * sr_space_bytes(C, V);
 }
 
 void launch_sample_rows(SampleRowsArgs a, hipStream_t st) {
