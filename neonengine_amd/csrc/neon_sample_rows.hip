@@ -44,12 +44,16 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 // A row of one chunk is one launch with the same steps.  Nothing but the chunks'
 // partial results crosses launches, at agent scope, so that the last block reads
 // what the others wrote without a launch in between.
-// Bound: three reads of the logits (the later two from the caches) and, for many
-// rows, one 64-bit exponential per token and pass.
+// Bound: for many rows three reads of the logits (64 x 201088: 10.5 us each at the
+// rate of a large copy) and k_sr_hist's 64-bit exponentials; for few rows the
+// chain of dependent steps, about 15 us of it in the last block of k_sr_pick.
+// Kernel times, us (max + hist + pick): 1 x 201088 2.8 + 9.5 + 16.5, 64 x 201088
+// 10.6 + 25.8 + 40.0, 7 x 32003 3.2 + 8.6 + 19.0; one block per row, 8 bits of the
+// key at a time, took 585, 1030 and 206.
 // ---------------------------------------------------------------------------
 constexpr int kSrThreads = 512;
 constexpr int kSrBins = 512;   // one per thread in the scan
-constexpr int kSrCap = 8192;   // candidates of a row that are listed
+constexpr int kSrCap = 4096;   // candidates of a row that are listed
 constexpr int kSrPart = 8 * kSrThreads;  // tokens whose kept mass is held apart
 constexpr int kSrMaxChunk = 65536;
 constexpr int kSrMaxParts = kSrMaxChunk / kSrPart;
@@ -61,23 +65,46 @@ struct SrRow {
   int V;
   float m;       // the maximum
   float bin_t;   // bins per unit of the logits
-  double inv_t;  // 1 / T
+  double m_d;    // the same
+  double to_t;   // 64 log2(e) / T
   double scale;  // 2^S
+  const double* table;
   double min_p, p, u;
   int k;         // 0: all
   uint64_t best; // key and ~index of the maximum
 };
+// exp((l - m) / T) by table (P.T.P. Tang's method): with t = 64 log2(e) (l - m)
+// / T and n the nearest integer, 2^(n / 64) = 2^(n >> 6) table[n & 63] and the
+// rest e^r, |r| <= ln 2 / 128, is a Taylor sum: r^6 / 720 < 2^-53.  t is below
+// 64 x 46.2 where a mass is not 0, so its rounding costs 2^-48.  About 20
+// instructions; exp() and a conversion to 64 bits are 50, which bound
+// k_sr_hist (64 x 201088: 37.6 -> 29.2 us).
+constexpr int kSrTable = 64;
+__device__ __forceinline__ void sr_table(double* table) {
+  if (threadIdx.x < kSrTable) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / kSrTable));
+}
 __device__ __forceinline__ double sr_weight(const SrRow& r, float l) {
-  if (l == r.m) return 1.0;  // also where both are infinite
-  return exp(((double)l - (double)r.m) * r.inv_t);
+  const double t = fmax(((double)l - r.m_d) * r.to_t, -64.0 * 1100.0);
+  const double n = __builtin_rint(t);
+  const double x = (t - n) * (0.69314718055994530942 / kSrTable);
+  const int i = (int)n;
+  double e = __builtin_fma(x, 1.0 / 120.0, 1.0 / 24.0);
+  e = __builtin_fma(x, e, 1.0 / 6.0);
+  e = __builtin_fma(x, e, 0.5);
+  e = __builtin_fma(x, e, 1.0);
+  e = __builtin_fma(x, e, 1.0);
+  e = __builtin_ldexp(r.table[i & (kSrTable - 1)] * e, i >> 6);
+  return l == r.m ? 1.0 : e;  // also where both are infinite
 }
-__device__ __forceinline__ u64 sr_mass(const SrRow& r, float l) {
-  return (u64)__builtin_rint(sr_weight(r, l) * r.scale);
+// round(w 2^S) for w 2^S <= 2^44: the low bits of w 2^S + 2^52
+__device__ __forceinline__ u64 sr_units(const SrRow& r, double w) {
+  return (u64)__builtin_bit_cast(int64_t, __builtin_fma(w, r.scale, 0x1p52)) & 0xFFFFFFFFFFFFFull;
 }
+__device__ __forceinline__ u64 sr_mass(const SrRow& r, float l) { return sr_units(r, sr_weight(r, l)); }
 // mass under min_p's limit: 0 below it
 __device__ __forceinline__ u64 sr_kept_mass(const SrRow& r, float l) {
   const double w = sr_weight(r, l);
-  return w >= r.min_p ? (u64)__builtin_rint(w * r.scale) : 0;
+  return w >= r.min_p ? sr_units(r, w) : 0;
 }
 // The first bin whose weights all lie below min_p (w <= exp(-bin / 16), the
 // 1 + 2^-10 covers the rounding of the bins and of the logarithm).
@@ -110,9 +137,26 @@ __device__ __forceinline__ void sr_put(u64* p, u64 v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+template <int J>
+__device__ __forceinline__ u64 sr_xor_lane(u64 x) {
+  return (u64)(uint32_t)xor_lane_i<J>((int)(uint32_t)x) |
+         (u64)(uint32_t)xor_lane_i<J>((int)(x >> 32)) << 32;
+}
+template <int J = 32>
+__device__ __forceinline__ u64 sr_wave_sum(u64 v) {
+  v += sr_xor_lane<J>(v);
+  if constexpr (J > 1) return sr_wave_sum<J / 2>(v);
+  else return v;
+}
+template <int J = 32>
+__device__ __forceinline__ u64 sr_wave_max(u64 v) {
+  const u64 x = sr_xor_lane<J>(v);
+  v = x > v ? x : v;
+  if constexpr (J > 1) return sr_wave_max<J / 2>(v);
+  else return v;
+}
 __device__ __forceinline__ u64 sr_block_sum(u64 v, u64* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  v = sr_wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -122,11 +166,7 @@ __device__ __forceinline__ u64 sr_block_sum(u64 v, u64* red) {
   return t;
 }
 __device__ __forceinline__ u64 sr_block_max(u64 v, u64* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 x = __shfl_xor(v, o);
-    v = x > v ? x : v;
-  }
+  v = sr_wave_max(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -161,6 +201,7 @@ struct SrFound {
 
 struct SrHistShared {
   u64 red[16];
+  double table[kSrTable];
   u64 mass[kSrBins];
   uint32_t count[kSrBins];
   SrFound found;
@@ -170,23 +211,28 @@ struct SrHistShared {
 struct SrShared : SrHistShared {
   u64 any[256];
   u64 list[kSrCap];
+  float queue[kSrThreads / 64][512];       // per wave: the tokens of eight that matter,
+  uint16_t queued[kSrThreads / 64][512];   // and which they are
 };
 
 // Reads row b's parameters; false where one is out of range.
-__device__ __forceinline__ bool sr_params(const SampleRowsArgs& a, int b, SrRow& r, bool& greedy) {
+__device__ __forceinline__ bool sr_params(const SampleRowsArgs& a, int b, double* table, SrRow& r,
+                                          bool& greedy) {
   const float t = a.temperature != nullptr ? a.temperature[b] : 1.0f;
   const float p = a.top_p != nullptr ? a.top_p[b] : 1.0f;
   const float mp = a.min_p != nullptr ? a.min_p[b] : 0.0f;
   const float u = a.u[b];
   const int k = a.top_k != nullptr ? a.top_k[b] : 0;
+  sr_table(table);  // a barrier follows with the row's maximum
+  r.table = table;
   r.l = a.logits + (int64_t)b * a.stride;
   r.V = a.V;
   r.k = k > 0 && k < a.V ? k : 0;
   r.p = (double)p;
   r.min_p = (double)mp;
   r.u = (double)u;
-  r.inv_t = 1.0 / (double)t;
-  r.bin_t = (float)r.inv_t * kSrBinsPerT;
+  r.to_t = 64.0 * 1.44269504088896340736 / (double)t;
+  r.bin_t = (float)(1.0 / (double)t) * kSrBinsPerT;
   r.scale = sr_scale(a.V);
   greedy = t == 0.0f;
   return t >= 0.0f && t < INFINITY && p > 0.0f && p <= 1.0f && mp >= 0.0f && mp <= 1.0f &&
@@ -196,36 +242,55 @@ __device__ __forceinline__ void sr_set_best(SrRow& r, u64 best) {
   r.best = best;
   const uint32_t key = (uint32_t)(best >> 32);
   r.m = __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  r.m_d = (double)r.m;
 }
 __device__ __forceinline__ int sr_best_id(u64 best) { return (int)~(uint32_t)best; }
 
-// Tokens i0 + thread, + 512, ..: eight are requested at once (past i1 the last
-// one again, as minus infinity).  fn(logits, index of the first).
+// fn(logits, index of the first) for tokens [i0, i1), i0 a multiple of kSrPart: a
+// thread's eight of a part are 512 apart.  The next part's are requested before
+// these are used; the last, incomplete part has minus infinity past i1.
 template <class F>
 __device__ __forceinline__ void sr_tokens(const float* l, int i0, int i1, F fn) {
-  for (int i = i0 + threadIdx.x; i < i1; i += 8 * kSrThreads) {
+  const int tid = threadIdx.x, full = i0 + (i1 - i0) / kSrPart * kSrPart;
+  if (full > i0) {
+    float next[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) next[j] = (l + i0 + j * kSrThreads)[tid];
+    for (int i = i0; i < full; i += kSrPart) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = next[j];
+      const float* p = l + min(i + kSrPart, full - kSrPart);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) next[j] = (p + j * kSrThreads)[tid];
+      fn(v, i + tid);
+    }
+  }
+  if (full < i1) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = l[min(i + j * kSrThreads, i1 - 1)];
+    for (int j = 0; j < 8; ++j) v[j] = l[min(full + tid + j * kSrThreads, i1 - 1)];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = i + j * kSrThreads < i1 ? sr_clean(v[j]) : -INFINITY;
-    fn(v, i);
+    for (int j = 0; j < 8; ++j) v[j] = full + tid + j * kSrThreads < i1 ? v[j] : -INFINITY;
+    fn(v, full + tid);
   }
 }
 
 __device__ __forceinline__ u64 sr_chunk_max(const float* l, int i0, int i1, u64* red) {
-  u64 best = 0;
+  float best = -INFINITY;  // of equal ones the first; a NaN is never larger
+  int at = i0;
   sr_tokens(l, i0, i1, [&](const float (&v)[8], int i) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const u64 x = sr_place(v[j], i + j * kSrThreads);
-      best = x > best ? x : best;
+      at = v[j] > best ? i + j * kSrThreads : at;
+      best = v[j] > best ? v[j] : best;
     }
   });
-  return sr_block_max(best, red);
+  return sr_block_max(sr_place(best, at), red);
 }
 
-// counts and masses of the chunk's bins into sh.count / sh.mass
+// counts (for top_k) and masses (for top_p) of the chunk's bins into sh.count /
+// sh.mass
 template <class SH>
 __device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SH& sh) {
   sh.mass[threadIdx.x] = 0;
@@ -236,8 +301,8 @@ __device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SH
     for (int j = 0; j < 8; ++j) {
       const int bin = sr_bin(r, v[j]);
       if (bin < kSrBins) {
-        atomicAdd(&sh.count[bin], 1u);
-        atomicAdd(&sh.mass[bin], sr_mass(r, v[j]));
+        if (r.k > 0) atomicAdd(&sh.count[bin], 1u);
+        if (r.p < 1.0) atomicAdd(&sh.mass[bin], sr_mass(r, v[j]));
       }
     }
   });
@@ -301,30 +366,50 @@ __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int 
   if (threadIdx.x < kSrMaxParts) sh.mass[threadIdx.x] = 0;
   __syncthreads();
   const int keep = min(min(f.lo, kSrBins), sr_min_bin(r));
+  // Mostly a few of a hundred tokens matter: those of the first bins, up to
+  // `keep`, and those of the candidates' bins.  Logits that bound them from outside:
+  auto edge = [&](int bin, double out) {
+    const double below = bin / (double)r.bin_t;
+    const float x = (float)(r.m_d - below + out * (fabs(r.m_d) + below) * 1e-6);
+    return x == x ? x : (float)-INFINITY;
+  };
+  const int c_lo = min(f.lo, f.bin_k), c_hi = max(f.hi < kSrBins ? f.hi : -1, f.bin_k < kSrBins ? f.bin_k : -1);
+  const float from = keep > 0 ? edge(keep, -1.0) : INFINITY;
+  const float c_from = c_hi >= 0 ? edge(c_hi + 1, -1.0) : INFINITY;
+  const float c_to = c_lo > 0 ? edge(c_lo, 1.0) : INFINITY;
   sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int i) {
-    uint32_t todo = 0;  // a bit for each that has mass to add
+    // gathered first: a wave pays an exponential for all its lanes if one needs it
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int n = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int bin = sr_bin(r, v[j]);
+      const bool in = v[j] >= from || (v[j] >= c_from && v[j] <= c_to);
+      const u64 who = __ballot(in);
+      if (in) {
+        const int to = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        sh.queue[wave][to] = v[j];
+        sh.queued[wave][to] = (uint16_t)(j * kSrThreads + lane);
+      }
+      n += __builtin_popcountll(who);
+    }
+    wave_lds_sync();
+    u64 sure = 0;
+    for (int q = lane; q < n; q += 64) {
+      const float l = sh.queue[wave][q];
+      const int bin = sr_bin(r, l);
       if (bin < keep) {
-        todo |= 1u << j;
+        sure += sr_kept_mass(r, l);
       } else if (bin >= f.lo && bin < kSrBins && sr_candidate(f, bin)) {
-        const int at = atomicAdd(&sh.s_int[0], 1);
-        if (at < kSrCap) sh.list[at] = sr_place(v[j], i + j * kSrThreads);
+        const int to = atomicAdd(&sh.s_int[0], 1);
+        if (to < kSrCap) sh.list[to] = sr_place(l, i - lane + (int)sh.queued[wave][q]);
       }
     }
-    // A wave pays an exponential for all its lanes if one needs it, and mostly a
-    // few of a hundred tokens do: each turn takes every lane's next one.
-    u64 sure = 0;
-    while (__any(todo != 0)) {
-      const int at = __builtin_ctz(todo | 0x80000000u);
-      float l = v[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) l = at == j ? v[j] : l;
-      if (todo != 0) sure += sr_kept_mass(r, l);
-      todo &= todo - 1;
+    wave_lds_sync();  // read before the next eight are written
+    if (__any(sure > 0)) {  // 64 lanes on one address would be done one by one
+      sure = sr_wave_sum(sure);
+      if ((threadIdx.x & 63) == 0) atomicAdd(&sh.mass[(i - i0) / kSrPart], sure);
     }
-    if (sure > 0) atomicAdd(&sh.mass[(i - i0) / kSrPart], sure);
   });
   __syncthreads();
   return threadIdx.x < kSrMaxParts ? sh.mass[threadIdx.x] : 0;
@@ -443,11 +528,6 @@ __device__ __forceinline__ u64 sr_select(const SrRow& r, SrShared& sh, int n, in
   }
 }
 
-template <int J>
-__device__ __forceinline__ u64 sr_xor_lane(u64 x) {
-  return (u64)(uint32_t)xor_lane_i<J>((int)(uint32_t)x) |
-         (u64)(uint32_t)xor_lane_i<J>((int)(x >> 32)) << 32;
-}
 // One compare-exchange of a bitonic sort, descending: runs of K, distance J.
 template <int K, int J>
 __device__ __forceinline__ void sr_sort_step(u64& x, u64* buf) {
@@ -558,7 +638,9 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
     const int bin = sr_bin(r, v[j]);
     if (i < i1 && bin < limit && sr_in(f, cut, bin, sr_place(v[j], i))) todo |= 1u << j;
   }
-  while (__any(todo != 0)) {  // as in sr_collect
+  // each turn takes every lane's next one: a wave pays an exponential for all its
+  // lanes if one needs it
+  while (__any(todo != 0)) {
     const int at = __builtin_ctz(todo | 0x80000000u);
     float l = v[0];
 #pragma unroll
@@ -695,12 +777,12 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_max(SampleRowsArgs a) {
 // The row's parameters and maximum from the chunks'; false (the answer written
 // by the row's first block) where there is nothing to search.
 __device__ __forceinline__ bool sr_begin(const SampleRowsArgs& a, const SrSpace& s, int b, SrRow& r,
-                                         u64* red, bool answer) {
+                                         SrHistShared& sh, bool answer) {
   bool greedy;
-  const bool ok = sr_params(a, b, r, greedy);
+  const bool ok = sr_params(a, b, sh.table, r, greedy);
   u64 best = 0;
   for (int c = threadIdx.x; c < a.chunks; c += kSrThreads) best = s.best[c] > best ? s.best[c] : best;
-  best = sr_block_max(best, red);
+  best = sr_block_max(best, sh.red);
   sr_set_best(r, best);
   const bool none = (uint32_t)(best >> 32) <= kSrNone;
   if (ok && !none && !greedy) return true;
@@ -716,14 +798,15 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_hist(SampleRowsArgs a) {
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const SrSpace s = sr_space(a, b);
   SrRow r;
-  if (!sr_begin(a, s, b, r, sh.red, false)) return;
+  if (!sr_begin(a, s, b, r, sh, false)) return;
   if (r.k == 0 && r.p >= 1.0) return;  // every bin is kept
   sr_chunk_hist(r, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
-  if (sh.count[tid] > 0) {  // integers: no order changes the sums
+  // integers: no order changes the sums
+  if (sh.mass[tid] > 0)
     __hip_atomic_fetch_add(s.mass + tid, sh.mass[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (sh.count[tid] > 0)
     __hip_atomic_fetch_add(s.count + tid, (u64)sh.count[tid], __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
-  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
   __syncthreads();
   if (tid == 0)
@@ -747,7 +830,7 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const SrSpace s = sr_space(a, b);
   SrRow r;
-  if (!sr_begin(a, s, b, r, sh.red, true)) return;
+  if (!sr_begin(a, s, b, r, sh, true)) return;
   if (tid == 0) {
     SrFound f;
     f.lo = f.hi = f.bin_k = kSrBins;
@@ -801,7 +884,7 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x;
   SrRow r;
   bool greedy;
-  const bool ok = sr_params(a, b, r, greedy);
+  const bool ok = sr_params(a, b, sh.table, r, greedy);
   const u64 best = sr_chunk_max(r.l, 0, a.V, sh.red);
   sr_set_best(r, best);
   const bool none = (uint32_t)(best >> 32) <= kSrNone;
@@ -831,12 +914,13 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
   if (tid == 0) a.ids[b] = id;
 }
 
-// Tokens of a chunk: few enough for some blocks per CU, 4096 at least (a block's
-// fixed steps), so that the bins' partial sums stay a fraction of the logits.
+// Tokens of a chunk, a multiple of kSrPart: as many chunks as k_sr_pick has places
+// on the chip at once (two blocks of a CU; a second round would double it), of a
+// part at least.
 static int sr_chunk(int B, int V) {
-  int chunk = 4096;
-  while (chunk < kSrMaxChunk && (int64_t)B * ((V + chunk - 1) / chunk) > 1024) chunk *= 2;
-  return chunk;
+  const int per_row = B < 512 ? 512 / B : 1;
+  const int64_t chunk = (((int64_t)V + per_row - 1) / per_row + kSrPart - 1) / kSrPart * kSrPart;
+  return chunk < kSrMaxChunk ? (int)chunk : kSrMaxChunk;
 }
 
 size_t sample_rows_workspace(int B, int V) {
