@@ -203,20 +203,34 @@ def _nbytes(t):
     return t.numel() * t.element_size()
 
 
-_cuda = None  # torch.cuda once a device was found (a process does not lose it again)
+_current = None  # (device index, its stream's handle) functions, once a device was
+                 # found (a process does not lose it again)
+
+
+def _find_current():
+    """Functions that give torch's current device, and its current stream there:
+    torch's own shortcuts to the bare numbers where it has them
+    (torch.cuda.current_stream() makes an object for 3 us)."""
+    global _current
+    import torch
+    if not torch.cuda.is_available():
+        return None
+    torch.cuda.init()
+    try:
+        from torch._C import _cuda_getCurrentRawStream as raw, _cuda_getDevice as device
+        raw(device())
+        _current = (device, raw)
+    except Exception:
+        _current = (torch.cuda.current_device, lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _current
 
 
 def _stream(stream):
     """Stream handle (None -> torch's current stream, or the default one)."""
-    global _cuda
     if stream is None:
         try:
-            if _cuda is None:
-                import torch
-                if not torch.cuda.is_available():
-                    return None
-                _cuda = torch.cuda
-            return _cuda.current_stream().cuda_stream
+            c = _current or _find_current()
+            return c[1](c[0]()) if c else None
         except Exception:
             return None
     if hasattr(stream, "cuda_stream"):
@@ -410,7 +424,9 @@ class PagedKV:
         if any(t.element_size() != (1 if mx else 2) for t in pools):
             raise ValueError("PagedKV: bf16 pools have 2-byte elements, MXFP4 codes and scales 1")
         self.pools = pools  # keeps them alive
-        self.device = k.device
+        self.device = k.get_device()
+        if any(t.get_device() != self.device for t in pools):
+            raise ValueError("PagedKV: pools on one device")
         self.format = KV_MXFP4 if mx else KV_BF16
         self.n_kv_heads, self.head_dim = heads, dim
         self.struct = PagedKVStruct(*(_ptr(t) for t in pools), *(() if mx else (None, None)),
@@ -422,85 +438,87 @@ def paged_kv(k, v, k_scales=None, v_scales=None) -> PagedKV:
     return PagedKV(k, v, k_scales, v_scales)
 
 
-def _sized(t, dtype_bytes, n, name, device):
-    """t as this many elements of this size on this device, or ValueError: the
-    library trusts the sizes that the paged calls derive from other tensors."""
-    if t.element_size() != dtype_bytes or t.numel() < n or t.device != device:
-        raise ValueError(f"{name}: needs {n} elements of {dtype_bytes} bytes on {device}, has "
-                         f"{t.numel()} of {t.element_size()} on {t.device}")
+def _arg(t, size, n, name, device):
+    """Device pointer of a contiguous tensor of at least n elements of this size
+    on this device (its index), or ValueError: the library trusts the sizes that
+    the paged calls derive from other tensors."""
+    if t.element_size() != size or t.numel() < n or t.get_device() != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{name}: needs {n} contiguous elements of {size} bytes on device "
+                         f"{device}, has {tuple(t.shape)} of {t.element_size()} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(x, size, width, name, device):
+    """(device pointer, rows, elements between them) of rows of at least `width`
+    elements: contiguous ones, or a slice of wider rows."""
+    if x.element_size() != size or x.get_device() != device or x.dim() not in (2, 3):
+        raise ValueError(f"{name}: rows of elements of {size} bytes on device {device}")
+    n = x.shape[0]
+    has = x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]
+    stride = has
+    if not x.is_contiguous():
+        inner = (1,) if x.dim() == 2 else (x.shape[2], 1)
+        if any(s != w and k > 1 for s, w, k in zip(x.stride()[1:], inner, x.shape[1:])):
+            raise ValueError(f"{name}: each row must be contiguous")
+        if n > 1:
+            stride = x.stride(0)
+    if n and has < width:
+        raise ValueError(f"{name}: rows of {width} elements, has {has}")
+    return x.data_ptr(), n, max(stride, width)
 
 
 def _on_current(device):
     """The calls go to the current device: tensors elsewhere are refused."""
-    if device.type != "cuda" or device.index != _torch_cuda().current_device():
-        raise ValueError(f"tensors on {device}: the call runs on the current HIP device")
+    c = _current or _find_current()
+    if device < 0 or c is None or device != c[0]():
+        raise ValueError(f"tensors on device {device}: the call runs on the current HIP device")
 
 
-def _torch_cuda():
-    import torch
-    return torch.cuda
-
-
-def _row_stride(x, name):
-    """Rows of a 2-D or dense 3-D tensor, and the elements between them (a
-    slice of wider rows is fine)."""
-    inner = x.stride()[1:] if x.dim() > 1 else ()
-    want = {2: (1,), 3: (x.shape[2] if x.dim() == 3 else 0, 1)}.get(x.dim())
-    if want is None or any(s != w and n > 1 for s, w, n in zip(inner, want, x.shape[1:])):
-        raise ValueError(f"{name}: rows of contiguous elements, [n_rows][width] or "
-                         "[n_rows][heads][head_dim]")
-    width = x.numel() // x.shape[0] if x.shape[0] else 0
-    return x.shape[0], (x.stride(0) if x.shape[0] > 1 else width), width
-
-
-def _paged_rows(kv, q_start, kv_len, page_table, n_rows):
-    _on_current(kv.device)
-    B = kv_len.shape[0]
+def _batch(kv, q_start, kv_len, page_table, n_rows):
+    """(q_start, kv_len, page_table, max_pages, B) of a paged call."""
+    device = kv.device
+    _on_current(device)
     if page_table.dim() != 2:
         raise ValueError("page_table: [B][max_pages]")
-    _sized(kv_len, 4, B, "kv_len", kv.device)
-    _sized(page_table, 4, B * page_table.shape[1], "page_table", kv.device)
-    if page_table.shape[0] != B:
+    B, max_pages = page_table.shape
+    if kv_len.numel() != B:
         raise ValueError("page_table: one row per sequence of kv_len")
     if q_start is not None:
-        _sized(q_start, 4, B + 1, "q_start", kv.device)
+        q_start = _arg(q_start, 4, B + 1, "q_start", device)
     elif n_rows != B:
         raise ValueError("without q_start there is one row per sequence")
-    return B, page_table.shape[1]
+    return (q_start, _arg(kv_len, 4, B, "kv_len", device),
+            _arg(page_table, 4, 1, "page_table", device), max_pages, B)
 
 
 def paged_append(kv, qkv, table, q_start, kv_len, page_table, q_out, Hq, stream=None):
     """Rotates q and k of the rows qkv [n_rows][(Hq + 2 n_kv_heads) head_dim]
     and appends k and v to the pages (neon_paged_append).  table: from
     rope_table, fp32 [2][n_pos][head_dim / 2], or None (no rotation)."""
-    n, stride, width = _row_stride(qkv, "qkv")
-    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
-    D = kv.head_dim
-    _sized(qkv, 2, n * (Hq + 2 * kv.n_kv_heads) * D, "qkv", kv.device)
-    if n and width < (Hq + 2 * kv.n_kv_heads) * D:
-        raise ValueError("qkv: rows of (Hq + 2 n_kv_heads) head_dim")
-    if Hq:
-        _sized(q_out, 2, n * Hq * D, "q_out", kv.device)
+    D, device = kv.head_dim, kv.device
+    rows, n, stride = _rows(qkv, 2, (Hq + 2 * kv.n_kv_heads) * D, "qkv", device)
+    q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
+    q_out = _arg(q_out, 2, n * Hq * D, "q_out", device) if Hq else None
     n_pos = 0
     if table is not None:
         if table.dim() != 3 or table.shape[0] != 2 or table.shape[2] != D // 2:
             raise ValueError("table: [2][n_pos][head_dim / 2]")
         n_pos = table.shape[1]
-        _sized(table, 4, n_pos * D, "table", kv.device)
-    _check(lib().neon_paged_append(kv.ref, qkv.data_ptr(), stride, _ptr(table), n_pos,
-                                   _ptr(q_start), _ptr(kv_len), _ptr(page_table), max_pages,
-                                   _ptr(q_out), n, B, Hq, _stream(stream)))
+        table = _arg(table, 4, n_pos * D, "table", device)
+    _check(lib().neon_paged_append(kv.ref, rows, stride, table, n_pos, q_start, kv_len, page_table,
+                                   max_pages, q_out, n, B, Hq, _stream(stream)))
 
 
 def paged_gather(kv, q_start, kv_len, page_table, k_out, v_out, stream=None):
     """The rows that paged_append writes for the same arguments, as bf16, into
     k_out and v_out [n_rows][n_kv_heads][head_dim] (neon_paged_gather)."""
-    n = k_out.shape[0]
-    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        _sized(t, 2, n * kv.n_kv_heads * kv.head_dim, name, kv.device)
-    _check(lib().neon_paged_gather(kv.ref, _ptr(q_start), _ptr(kv_len), _ptr(page_table),
-                                   max_pages, _ptr(k_out), _ptr(v_out), n, B, _stream(stream)))
+    n, width, device = k_out.shape[0], kv.n_kv_heads * kv.head_dim, kv.device
+    q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
+    _check(lib().neon_paged_gather(kv.ref, q_start, kv_len, page_table, max_pages,
+                                   _arg(k_out, 2, n * width, "k_out", device),
+                                   _arg(v_out, 2, n * width, "v_out", device), n, B,
+                                   _stream(stream)))
 
 
 def paged_attn_workspace(n_rows, B, Hq, Hkv, D):
@@ -515,25 +533,23 @@ def paged_attn(kv, q, sinks, q_start, kv_len, page_table, out, Hq, window=0, str
     """Attention of the rows q [n_rows][Hq head_dim] over the pages
     (neon_paged_attn).  counters: zero-filled once by the caller (each call
     leaves it zero)."""
-    n, stride, width = _row_stride(q, "q")
-    B, max_pages = _paged_rows(kv, q_start, kv_len, page_table, n)
-    D = kv.head_dim
-    _sized(q, 2, n * Hq * D, "q", kv.device)
-    if n and width < Hq * D:
-        raise ValueError("q: rows of Hq head_dim")
-    _sized(out, 2, n * Hq * D, "out", kv.device)
+    D, device = kv.head_dim, kv.device
+    rows, n, stride = _rows(q, 2, Hq * D, "q", device)
+    q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
     if sinks is not None:
-        _sized(sinks, 2, Hq, "sinks", kv.device)
+        sinks = _arg(sinks, 2, Hq, "sinks", device)
     if workspace is None or counters is None:
         wb, cb = paged_attn_workspace(n, B, Hq, kv.n_kv_heads, D)
         if workspace is None:
             workspace = _workspace(wb)
         if counters is None:
             counters = _workspace(cb, zero=True)
-    _check(lib().neon_paged_attn(kv.ref, q.data_ptr(), stride, _ptr(sinks), _ptr(q_start),
-                                 _ptr(kv_len), _ptr(page_table), max_pages, _ptr(out), n, B, Hq,
-                                 window, _ptr(workspace), _nbytes(workspace), _ptr(counters),
-                                 _nbytes(counters), _stream(stream)))
+    _check(lib().neon_paged_attn(kv.ref, rows, stride, sinks, q_start, kv_len, page_table,
+                                 max_pages, _arg(out, 2, n * Hq * D, "out", device), n, B, Hq,
+                                 window, _arg(workspace, workspace.element_size(), 0, "workspace",
+                                              device), workspace.nbytes,
+                                 _arg(counters, counters.element_size(), 0, "counters", device),
+                                 counters.nbytes, _stream(stream)))
 
 
 def sample_rows_workspace(B, V):
@@ -547,19 +563,21 @@ def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, mi
     None (neon_sample_rows)."""
     if logits.dim() != 2:
         raise ValueError("logits: [B][V]")
-    _on_current(logits.device)
-    B, V = logits.shape
-    _, stride, _ = _row_stride(logits, "logits")
-    _sized(logits, 4, B * V, "logits", logits.device)
-    for t, name in ((u, "u"), (out_ids, "out_ids"), (temperature, "temperature"),
-                    (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p")):
-        if t is not None:
-            _sized(t, 4, B, name, logits.device)
+    device = logits.get_device()
+    _on_current(device)
+    V = logits.shape[1]
+    rows, B, stride = _rows(logits, 4, V, "logits", device)
     if workspace is None:
         workspace = _workspace(sample_rows_workspace(B, V))
-    _check(lib().neon_sample_rows(logits.data_ptr(), stride, B, V, _ptr(temperature), _ptr(top_k),
-                                  _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(out_ids),
-                                  _ptr(workspace), _nbytes(workspace), _stream(stream)))
+
+    def opt(t, name):
+        return None if t is None else _arg(t, 4, B, name, device)
+
+    _check(lib().neon_sample_rows(rows, stride, B, V, opt(temperature, "temperature"),
+                                  opt(top_k, "top_k"), opt(top_p, "top_p"), opt(min_p, "min_p"),
+                                  _arg(u, 4, B, "u", device), _arg(out_ids, 4, B, "out_ids", device),
+                                  _arg(workspace, workspace.element_size(), 0, "workspace", device),
+                                  workspace.nbytes, _stream(stream)))
 
 
 PREFILL_BATCHED, PREFILL_STEPWISE, PREFILL_CHUNKED, PREFILL_MX8 = 0, 1, 2, 3
