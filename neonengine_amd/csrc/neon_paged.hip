@@ -569,7 +569,7 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers and one step ahead of the products.
 template <int D, bool F4>
-__global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAttnArgs a) {
   constexpr int R = 16, E = D / 16;
   __shared__ __align__(16) float so[4][R][D + 4];
   __shared__ float sm[4][R], sl[4][R];
@@ -637,6 +637,8 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
   };
   auto step = [&](const PaTile<D, F4>& t, int it, const int (&id)[2]) {
     const int kb = w.k0 + 32 * (wave + 4 * it);
+    // every row sees all 32 keys (else the masks: two blocks of selects under a
+    // branch of the whole wave)
     const bool full = kb >= all_lo && kb + 32 <= all_hi && (id[0] | id[1]) >= 0;
     float sv[2][4];
 #pragma unroll
@@ -645,13 +647,17 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
 #pragma unroll
       for (int n = 0; n < D / 32; ++n) acc = pa_mfma(pa_key<D>(t, s, n), q[n], acc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sv[s][i] = acc[i];
-        if (!full) {
+      for (int i = 0; i < 4; ++i) sv[s][i] = acc[i];
+    }
+    if (!full) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           const int key = kb + 16 * s + 4 * g + i;
-          if (key < k_lo || key >= k_hi || id[s] < 0) sv[s][i] = -INFINITY;
+          const bool seen = (key >= k_lo) & (key < k_hi) & (id[s] >= 0);
+          sv[s][i] = seen ? sv[s][i] : -INFINITY;
         }
-      }
     }
     float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
                      fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3]))) * c2;
@@ -683,15 +689,18 @@ __global__ __launch_bounds__(256) void k_paged_attn_few(PagedAttnArgs a) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pa_value<D>(t, s, i, c, v[s][i]);
-        if (!full) {  // rows that hold no key of the sequence may hold anything
+      for (int i = 0; i < 4; ++i) pa_value<D>(t, s, i, c, v[s][i]);
+    if (!full) {  // rows that hold no key of the sequence may hold anything
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           const int key = kb + 16 * s + 4 * g + i;
-          const bool none = key >= w.k1 || key < w.lo || id[s] < 0;
+          const bool none = (key >= w.k1) | (key < w.lo) | (id[s] < 0);
 #pragma unroll
           for (int n = 0; n < D / 32; ++n) v[s][i][n] = none ? 0u : v[s][i][n];
         }
-      }
+    }
     const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
@@ -985,7 +994,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = kb + 16 * k + 4 * g + i;
-            if (key < k_lo[t] || key >= k_hi[t] || (dead >> k & 1)) s[t][k][i] = -INFINITY;
+            const bool seen = (key >= k_lo[t]) & (key < k_hi[t]) & !(dead >> k & 1);
+            s[t][k][i] = seen ? s[t][k][i] : -INFINITY;
           }
     }
     uint4 p[2][2];
