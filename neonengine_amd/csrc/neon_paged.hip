@@ -333,9 +333,15 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   const int per = (a.r.B + 63) >> 6;  // consecutive sequences of a lane
   const int b0 = lane * per, b1 = min(b0 + per, a.r.B);
   float work = 0.0f;
+  int start0 = 0, n0 = 0, len0 = 0;  // the lane's first
   for (int b = b0; b < b1; ++b) {
     int start, len;
     const int n = pa_seq<FEW>(a, b, start, len, flag);
+    if (b == b0) {
+      start0 = start;
+      n0 = n;
+      len0 = len;
+    }
     work += (float)((n * G + R - 1) / R) * (float)pa_span<R, ALIGN>(a, G, len);
   }
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
@@ -347,8 +353,8 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   // has: the clamp lies above every grid and keeps the sums of 64 lanes in an int.
   int blocks = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
-    int start, len;
-    const int n = pa_seq<FEW>(a, b, start, len, false);
+    int start, len = len0, n = n0;
+    if (b > b0) n = pa_seq<FEW>(a, b, start, len, false);
     const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
     const int nb = (n * G + R - 1) / R * nc;
     blocks = min(blocks + nb, kPaMaxBlocks);
@@ -368,11 +374,9 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   // the owner lane's sequences, one by one
   int at = __builtin_amdgcn_readlane(blocks_to - blocks, owner);
   int slot = __builtin_amdgcn_readlane(slots_to - slots, owner);
-  for (int b = owner * per; b < min(owner * per + per, a.r.B); ++b) {
-    int start, len;
-    const int n = uni(pa_seq<FEW>(a, b, start, len, false));
-    start = uni(start);
-    len = uni(len);
+  int n = __builtin_amdgcn_readlane(n0, owner), len = __builtin_amdgcn_readlane(len0, owner);
+  int start = __builtin_amdgcn_readlane(start0, owner);  // of its first one
+  for (int b = owner * per;; ++b) {
     const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
     const int nb = (n * G + R - 1) / R * nc;
     if (idx < at + nb) {
@@ -393,8 +397,11 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
     }
     at += nb;
     slot += nc > 1 ? nb : 0;
+    if (b + 1 >= min(owner * per + per, a.r.B)) return false;
+    n = uni(pa_seq<FEW>(a, b + 1, start, len, false));
+    start = uni(start);
+    len = uni(len);
   }
-  return false;
 }
 
 // How the kernels take a 16-key step of a wave: S^T = K Q^T with
@@ -533,28 +540,90 @@ __device__ __forceinline__ float2 pa_load_agent(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// Joins the E values of a row that the chunks' blocks left (of the same launch:
-// agent-scope loads), with its (m, l) pairs.
-template <int E>
-__device__ __forceinline__ void pa_join(const float* po, const float* pml, int64_t step, int chunks,
-                                        float& M, float& L, float (&x)[E]) {
-  M = -INFINITY;
-  L = 0.0f;
+// Joins what the chunks' blocks left of a tile's R rows (in the same launch:
+// agent-scope loads), `used` of them: o at part + chunk * step + row D, (m, l)
+// behind the R rows.  256 threads: 16 for a row's D values; where fewer than 16
+// rows are used, the others take a share of the chunks.  fn(row, E values, m, l)
+// by 16 threads per row, thread t with the values (t & 15) E ..
+// Without the shares and with one chunk's loads at a time a tile of 92 chunks took
+// 25 us of a launch of 56.
+constexpr int kPaJoin = 64;  // chunks whose factors are in LDS at once
+template <int D, int R, class F>
+__device__ __forceinline__ void pa_join(const float* part, int64_t step, int chunks, int used,
+                                        float (*sf)[kPaJoin], float (*sx)[D + 4], F fn) {
+  constexpr int E = D / 16;
+  const int tid = threadIdx.x, lane16 = tid & 15, row16 = tid >> 4;
+  const int rows2 = used > 8 ? 16 : used > 4 ? 8 : used > 2 ? 4 : used > 1 ? 2 : 1;
+  const int shares = 16 / rows2, share = row16 / rows2, row = row16 & (rows2 - 1);
+  for (int r0 = 0; r0 < used; r0 += 16) {
+    float M = -INFINITY, L = 0.0f, x[E];  // M, L of row row16
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = 0.0f;
-  for (int j = 0; j < chunks; ++j) {
-    const float2 ml = pa_load_agent(pml + j * step);
-    const float mn = fmaxf(M, ml.x);
-    const float fo = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
-    const float fn = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-    L = L * fo + ml.y * fn;
+    for (int e = 0; e < E; ++e) x[e] = 0.0f;
+    const float* pml = part + R * D + 2 * (r0 + row16);
+    for (int c0 = 0; c0 < chunks; c0 += kPaJoin) {
+      // the factors of these chunks for row row16, 16 lanes of it
+      float2 ml[kPaJoin / 16];
+      float mx = M;
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 y = pa_load_agent(po + j * step + e);
-      x[e] = x[e] * fo + y.x * fn;
-      x[e + 1] = x[e + 1] * fo + y.y * fn;
+      for (int i = 0; i < kPaJoin / 16; ++i) {
+        const int j = c0 + lane16 + 16 * i;
+        ml[i] = pa_load_agent(pml + min(j, chunks - 1) * step);
+        if (j >= chunks) ml[i] = make_float2(-INFINITY, 0.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < kPaJoin / 16; ++i) mx = fmaxf(mx, ml[i].x);
+      mx = fmaxf(mx, xor_lane<1>(mx));
+      mx = fmaxf(mx, xor_lane<2>(mx));
+      mx = fmaxf(mx, xor_lane<4>(mx));
+      mx = fmaxf(mx, xor_lane<8>(mx));
+      const float me = mx == -INFINITY ? 0.0f : mx;
+      const float old = __builtin_amdgcn_exp2f(M - me);
+      float sum = 0.0f;
+      __syncthreads();  // sf is free
+#pragma unroll
+      for (int i = 0; i < kPaJoin / 16; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - me);
+        sf[row16][lane16 + 16 * i] = f;
+        sum = __builtin_fmaf(ml[i].y, f, sum);
+      }
+      sum += xor_lane<1>(sum);
+      sum += xor_lane<2>(sum);
+      sum += xor_lane<4>(sum);
+      sum += xor_lane<8>(sum);
+      L = __builtin_fmaf(L, old, sum);
+      M = mx;
+      if (c0 > 0) {  // the values so far, of row `row`
+        if (lane16 == 0) sx[row16][0] = old;
+        __syncthreads();
+        const float f = sx[row][0];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] *= f;
+      }
+      __syncthreads();
+      const int n = min(kPaJoin, chunks - c0);
+      const float* po = part + c0 * step + (r0 + row) * D + lane16 * E;
+#pragma unroll 4
+      for (int j = share; j < n; j += shares) {
+        const float f = sf[row][j];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 y = pa_load_agent(po + j * step + e);
+          x[e] = __builtin_fmaf(y.x, f, x[e]);
+          x[e + 1] = __builtin_fmaf(y.y, f, x[e + 1]);
+        }
+      }
     }
-    M = mn;
+    // the shares of a row; sx row: share * rows2 + row
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) sx[row16][lane16 * E + e] = x[e];
+    __syncthreads();
+    if (row16 < rows2) {
+      for (int k = 1; k < shares; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] += sx[k * rows2 + row16][lane16 * E + e];
+      if (r0 + row16 < used) fn(r0 + row16, x, M, L);
+    }
   }
 }
 template <int E>
@@ -567,12 +636,14 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 
 // Few rows: 16 per unit, four waves that share nothing but the result, each
 // with every fourth 32 keys of the chunk, straight from memory into the
-// operands' registers and one step ahead of the products.
+// operands' registers, some steps ahead of the products.
 template <int D, bool F4>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAttnArgs a) {
   constexpr int R = 16, E = D / 16;
+  constexpr int NT = F4 ? 4 : 2;  // steps in registers: one in use, the others on their way
   __shared__ __align__(16) float so[4][R][D + 4];
   __shared__ float sm[4][R], sl[4][R];
+  __shared__ float sf[16][kPaJoin];
   __shared__ int merge_here;
   const int h = blockIdx.x % a.kv.Hkv;
   PaWork w;
@@ -716,21 +787,22 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
     }
   };
   if (n_it > 0) {
-    PaTile<D, F4> ta, tb;
-    int ida[2], idb[2];
+    PaTile<D, F4> t[NT];
+    int id[NT][2];
     int ids = load_ids(0);
-    load_tile(ta, 0, ids, ida);
-    for (int it = 0; it < n_it; it += 2) {
-      // unconditional loads (past the last step, that one again): a load under
-      // a condition is waited for where the paths join
-      int nx = min(it + 1, n_it - 1);
-      load_tile(tb, nx, ids, idb);
-      step(ta, it, ida);
-      if (it + 1 >= n_it) break;
-      nx = min(it + 2, n_it - 1);
-      if ((nx & 31) == 0) ids = load_ids(nx);  // 32 is even: only here
-      load_tile(ta, nx, ids, ida);
-      step(tb, it + 1, idb);
+    // unconditional loads (past the last step, that one again): a load under a
+    // condition is waited for where the paths join
+#pragma unroll
+    for (int u = 0; u < NT - 1; ++u) load_tile(t[u], min(u, n_it - 1), ids, id[u]);
+    for (int it0 = 0; it0 < n_it; it0 += NT) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int it = it0 + u, nx = min(it + NT - 1, n_it - 1);
+        if (it >= n_it) break;
+        if ((nx & 31) == 0 && nx == it + NT - 1) ids = load_ids(nx);
+        load_tile(t[(u + NT - 1) % NT], nx, ids, id[(u + NT - 1) % NT]);
+        step(t[u], it, id[u]);
+      }
     }
   }
   l += xor_lane<16>(l);
@@ -776,9 +848,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
     __syncthreads();
     if (!merge_here) return;
     if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float* p0 = a.part + first * R * (D + 2);
-    pa_join<E>(p0 + tr * D + td, p0 + R * D + 2 * tr, (int64_t)a.kv.Hkv * R * (D + 2), w.chunks, M, L,
-               x);
+    pa_join<D, R>(a.part + first * R * (D + 2), (int64_t)a.kv.Hkv * R * (D + 2), w.chunks,
+                  min(R, rows - w.row0), sf, so[0], [&](int tr_, const float (&y)[E], float m_, float l_) {
+                    const int row_ = w.row0 + tr_, head = h * G + row_ % G;
+                    pa_write<E>(a.out + ((int64_t)(w.start + row_ / G) * a.Hq + head) * D + td, y,
+                                pa_finish(a, head, m_, l_));
+                  });
+    return;
   }
   if (row >= rows) return;
   const int head = h * G + row % G;
@@ -1105,15 +1181,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   __syncthreads();
   if (!merge_here) return;
   if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int r0 = tid >> 4; r0 < R; r0 += 16) {  // 16 threads of a row, E dims each
-    const int r = w.row0 + r0, td = (tid & 15) * E;
-    if (r >= rows) break;
-    float M, L, x[E];
-    pa_join<E>(p0 + r0 * D + td, p0 + R * D + 2 * r0, step_c, w.chunks, M, L, x);
-    const int head = h * G + r % G;
-    pa_write<E>(a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + td, x,
-                pa_finish(a, head, M, L));
-  }
+  // the tiles' memory is free: every wave is past its last one
+  float (*sf)[kPaJoin] = reinterpret_cast<float (*)[kPaJoin]>(&kt[0][0]);
+  float (*sx)[D + 4] = reinterpret_cast<float (*)[D + 4]>(&vt[0][0]);
+  pa_join<D, R>(p0, step_c, w.chunks, min(R, rows - w.row0), sf, sx,
+                [&](int tr, const float (&y)[E], float m_, float l_) {
+                  const int r = w.row0 + tr, head = h * G + r % G;
+                  pa_write<E>(a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + (tid & 15) * E,
+                              y, pa_finish(a, head, m_, l_));
+                });
 }
 
 // Units of R rows that n_rows rows of up to B sequences can make (per KV head).
