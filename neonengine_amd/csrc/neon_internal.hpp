@@ -434,7 +434,7 @@ struct PagedAttnArgs {
   int Hq, window;
   float* part;            // partial results of split units (paged_attn_workspace)
   int32_t* arrive;        // their counters, 0 at launch and left at 0
-  int few;                // set by the launcher
+  int few, G;             // set by the launcher
 };
 size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D);
 size_t paged_attn_counters();

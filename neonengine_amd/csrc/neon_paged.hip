@@ -285,6 +285,10 @@ constexpr int kPaFew = 32;        // (token, head) rows per KV head of the few-r
 constexpr int kPaArrive = 16;     // ints from one arrival counter to the next
 constexpr int kPaMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
 constexpr float kLog2e = 1.4426950408889634f;
+// A row's reference m (in log2 units) may trail its maximum by this much, so that
+// most steps neither compare it across the four lanes of a row nor rescale: a
+// weight is then up to 2^8, far from any limit, and as exact as one below 1.
+constexpr float kPaLag = 8.0f;
 
 typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pbf8 __attribute__((ext_vector_type(8)));
@@ -292,6 +296,7 @@ __device__ __forceinline__ pf4 pa_mfma(const uint4& a, const uint4& b, pf4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pbf8, a),
                                                  __builtin_bit_cast(pbf8, b), c, 0, 0, 0);
 }
+#define kPaOnes make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A block's work: keys [k0, k1) of a unit, all wave-uniform.
@@ -299,8 +304,12 @@ struct PaWork {
   int b, start, n, len;  // the sequence, its rows and tokens
   int row0;              // the tile's first (token, head) row
   int lo, k0, k1;        // lo: the first key that any row of the tile sees
+  int tok0, tok1;        // the tokens of its first and last row
   int chunks, slot;      // of the unit; the slot of its chunk 0
   int c;
+  int G;                 // query heads of a KV head, and 1 / G
+  float rG;
+  __device__ explicit PaWork(const PagedAttnArgs& a) : G(a.G), rG(1.0f / (float)a.G) {}
 };
 
 // Rows and length of a sequence as a kernel takes them (0 rows: none): FEW the
@@ -312,7 +321,31 @@ __device__ __forceinline__ int pa_seq(const PagedAttnArgs& a, int b, int& start,
     if (flag && len != 0) flag_dev_err(a.r.err, kDevErrPagedRows);
     return 0;
   }
-  return len > 0 && (n * (a.Hq / a.kv.Hkv) <= a.few) == FEW ? n : 0;
+  return len > 0 && (n * a.G <= a.few) == FEW ? n : 0;
+}
+
+// n / d for 0 <= n < 2^31, d > 0, with r = 1 / d to fp32: the fp32 quotient of up
+// to 2^22 is off by at most one (an integer division is some 40 instructions, and
+// every block makes a dozen before its first load).
+__device__ __forceinline__ int pa_div(int n, int d, float r) {
+  if (n >= 1 << 22) return n / d;
+  int q = (int)((float)n * r);
+  const int rest = n - q * d;
+  q += rest >= d ? 1 : 0;
+  return q - (rest < 0 ? 1 : 0);
+}
+// inclusive sums over the wave's lanes
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int pa_add_from(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int pa_scan(int x) {
+  x = pa_add_from<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x = pa_add_from<0x112, 0xF>(x);
+  x = pa_add_from<0x114, 0xF>(x);
+  x = pa_add_from<0x118, 0xF>(x);
+  x = pa_add_from<0x142, 0xA>(x);  // a row's last lane into the next row
+  return pa_add_from<0x143, 0xC>(x);  // lane 31 into the upper half
 }
 
 // Keys that any row tile of a sequence may take, its first key rounded down to
@@ -325,11 +358,13 @@ __device__ __forceinline__ int pa_span(const PagedAttnArgs& a, int G, int len) {
 
 // The work of block `idx` (of every KV head alike); false when there is none.
 // ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
-// multiples of 128).
-template <bool FEW, int R, int ALIGN, int MINC, int TARGET>
+// multiples of 128); TARGET: blocks to aim at; PLACES: blocks that the chip holds
+// at once.
+template <bool FEW, int R, int ALIGN, int MINC, int TARGET, int PLACES, bool FIT>
 __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool flag, PaWork& w) {
   const int lane = threadIdx.x & 63;
-  const int G = a.Hq / a.kv.Hkv;
+  const int G = w.G;
+  const float rG = w.rG;
   const int per = (a.r.B + 63) >> 6;  // consecutive sequences of a lane
   const int b0 = lane * per, b1 = min(b0 + per, a.r.B);
   float work = 0.0f;
@@ -347,27 +382,33 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
-  const int chunk = max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127);
+  int chunk = uni(max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
   // blocks and slots of the sequences, in order.  Row starts that overlap (an
   // error that no single sequence shows) can sum to more blocks than the grid
   // has: the clamp lies above every grid and keeps the sums of 64 lanes in an int.
-  int blocks = 0, slots = 0;
-  for (int b = b0; b < b1; ++b) {
-    int start, len = len0, n = n0;
-    if (b > b0) n = pa_seq<FEW>(a, b, start, len, false);
-    const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
-    const int nb = (n * G + R - 1) / R * nc;
-    blocks = min(blocks + nb, kPaMaxBlocks);
-    slots += nc > 1 ? nb : 0;
-  }
-  int blocks_to = blocks, slots_to = slots;
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(blocks_to, o), y = __shfl_up(slots_to, o);
-    if (lane >= o) {
-      blocks_to += x;
-      slots_to += y;
+  int blocks, slots, blocks_to;
+  for (int turn = 0;; ++turn) {
+    const float rc = 1.0f / (float)chunk;
+    blocks = 0;
+    slots = 0;
+    for (int b = b0; b < b1; ++b) {
+      int start, len = len0, n = n0;
+      if (b > b0) n = pa_seq<FEW>(a, b, start, len, false);
+      const int nc = pa_div(pa_span<R, ALIGN>(a, G, len) + chunk - 1, chunk, rc);
+      const int nb = (n * G + R - 1) / R * nc;
+      blocks = min(blocks + nb, kPaMaxBlocks);
+      slots += nc > 1 ? nb : 0;
     }
+    blocks_to = pa_scan(blocks);
+    // FIT: a few more blocks than the chip holds cost a round of their own, so
+    // larger chunks where that makes them fit (a unit is one block at least).
+    // Four MXFP4 sequences up to 131072 tokens: 58 -> 38 us; where the reads are the
+    // bound, small chunks even out the end better (64 bf16 ones: 68 -> 73 us).
+    const float over = (float)__builtin_amdgcn_readlane(blocks_to, 63) * (float)a.kv.Hkv * (1.0f / PLACES);
+    if (!FIT || turn == 3 || per > 1 || over <= 1.0f || over > 2.0f) break;
+    chunk = uni((min((int)((float)chunk * over), (1 << 30) - 128) + 128) & ~127);
   }
+  const int slots_to = pa_scan(slots);
   const uint64_t mine = __ballot(idx < blocks_to);
   if (mine == 0) return false;
   const int owner = __builtin_ctzll(mine);
@@ -376,27 +417,31 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
   int slot = __builtin_amdgcn_readlane(slots_to - slots, owner);
   int n = __builtin_amdgcn_readlane(n0, owner), len = __builtin_amdgcn_readlane(len0, owner);
   int start = __builtin_amdgcn_readlane(start0, owner);  // of its first one
+  const float rc = 1.0f / (float)chunk;
   for (int b = owner * per;; ++b) {
-    const int nc = (pa_span<R, ALIGN>(a, G, len) + chunk - 1) / chunk;
-    const int nb = (n * G + R - 1) / R * nc;
-    if (idx < at + nb) {
+    const int nc = pa_div(pa_span<R, ALIGN>(a, G, len) + chunk - 1, chunk, rc);
+    const int tiles = (n * G + R - 1) / R;
+    if (idx < at + tiles * nc) {
+      const int before = uni((idx - at) / nc);
       // the last tiles first: they see the most keys
-      const int tile = nb / nc - 1 - (idx - at) / nc;
+      const int tile = tiles - 1 - before;
       w.b = b; w.start = start; w.n = n; w.len = len;
-      w.c = (idx - at) % nc;
-      w.row0 = tile * R;
-      w.slot = slot + tile * nc;
+      w.c = uni(idx - at - before * nc);
+      w.row0 = uni(tile * R);
+      w.slot = uni(slot + tile * nc);
       const int last = min(w.row0 + R, n * G) - 1;
-      const int pos0 = len - n + w.row0 / G, pos1 = len - n + last / G;
+      w.tok0 = uni(pa_div(w.row0, G, rG));
+      w.tok1 = uni(pa_div(last, G, rG));
+      const int pos0 = len - n + w.tok0, pos1 = len - n + w.tok1;
       w.lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
       const int from = w.lo / ALIGN * ALIGN;
-      w.chunks = (pos1 + 1 - from + chunk - 1) / chunk;
-      w.k0 = from + w.c * chunk;
+      w.chunks = uni(pa_div(pos1 + 1 - from + chunk - 1, chunk, rc));
+      w.k0 = uni(from + w.c * chunk);
       w.k1 = min(w.k0 + chunk, pos1 + 1);
       return w.c < w.chunks;
     }
-    at += nb;
-    slot += nc > 1 ? nb : 0;
+    at += tiles * nc;
+    slot += nc > 1 ? tiles * nc : 0;
     if (b + 1 >= min(owner * per + per, a.r.B)) return false;
     n = uni(pa_seq<FEW>(a, b + 1, start, len, false));
     start = uni(start);
@@ -484,6 +529,20 @@ __device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, i
   }
 }
 
+// clears key i's values: rows that hold no key of the sequence may hold anything
+template <int D>
+__device__ __forceinline__ void pa_clear(PaTile<D, false>& t, int s, int i, bool none) {
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n) t.v[s][i][n] = none ? 0u : t.v[s][i][n];
+}
+template <int D>
+__device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, bool none) {
+  const uint32_t keep = D == 128 ? 0u : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;  // of its scales' word
+  uint32_t& word = t.vs[s][i * (D / 32) >> 2];
+  t.v[s][i] = none ? 0u : t.v[s][i];
+  word = none ? word & keep : word;
+}
+
 // operand n of a 16-key step's keys: the dims that pa_query gives B
 template <int D>
 __device__ __forceinline__ uint4 pa_key(const PaTile<D, false>& t, int s, int n) { return t.k[s][n]; }
@@ -505,10 +564,12 @@ __device__ __forceinline__ void pa_value(const PaTile<D, false>& t, int s, int i
 template <int D>
 __device__ __forceinline__ void pa_value(const PaTile<D, true>& t, int s, int i, int c,
                                          uint32_t (&v)[D / 32]) {
-  // scale byte i (D/32) + (block of the dims) of the four keys' bytes
-  const int at = i * (D / 32);
-  const uint32_t b = (t.vs[s][at >> 2] >> (8 * (at & 3))) >> (8 * (D == 64 ? c >> 3 : c >> 2));
-  const float sc = __uint_as_float((b & 0xFFu) << 23);
+  // The key's scale byte is byte (i & 1) 2 + c / 8 of word i / 2 (D = 64), byte
+  // c / 4 of word i (D = 128).  The conversion reads the exponent field of its
+  // scale alone (sign and fraction set at will change no result for the 256 scales
+  // x 256 code bytes, on an MI355X), so the bytes beside it need no mask.
+  const uint32_t b = D == 64 ? t.vs[s][i >> 1] >> (c & 8) : t.vs[s][i] >> (2 * (c & 12));
+  const float sc = __uint_as_float(b << (D == 64 && (i & 1) ? 7 : 23));
   v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 0));
   v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 1));
   if constexpr (D == 128) {
@@ -637,31 +698,32 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // Few rows: 16 per unit, four waves that share nothing but the result, each
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers, some steps ahead of the products.
+constexpr int pa_few_waves(int D) { return D == 64 ? 3 : 2; }  // of a SIMD (and blocks of a CU)
 template <int D, bool F4>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, pa_few_waves(D)) void k_paged_attn_few(PagedAttnArgs a) {
   constexpr int R = 16, E = D / 16;
-  constexpr int NT = F4 ? 4 : 2;  // steps in registers: one in use, the others on their way
+  constexpr int NT = 2;  // steps in registers: one in use, the others on their way
+  constexpr int kPlaces = 256 * pa_few_waves(D);
   __shared__ __align__(16) float so[4][R][D + 4];
   __shared__ float sm[4][R], sl[4][R];
   __shared__ float sf[16][kPaJoin];
   __shared__ int merge_here;
   const int h = blockIdx.x % a.kv.Hkv;
-  PaWork w;
-  if (!pa_work<true, R, 32, 256, kPaTarget>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
+  PaWork w(a);
+  if (!pa_work<true, R, 32, 256, kPaTarget, kPlaces, F4>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int G = a.Hq / a.kv.Hkv;
+  const int G = w.G;
   // the lane's query row
   const int r = w.row0 + c, rows = w.n * G;
   const bool has = r < rows;
-  const int tok = has ? r / G : 0, hq = h * G + (has ? r % G : 0);
+  const int tok = has ? pa_div(r, G, w.rG) : 0, hq = h * G + (has ? r - tok * G : 0);
   const int pos = w.len - w.n + tok;
   const int k_hi = has ? pos + 1 : 0;
   const int k_lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
   // keys that every row of the tile sees
-  const int t_last = (min(w.row0 + R, rows) - 1) / G;
-  const int all_hi = w.len - w.n + w.row0 / G + 1;
-  const int all_lo = a.window > 0 ? max(0, w.len - w.n + t_last - a.window + 1) : 0;
+  const int all_hi = w.len - w.n + w.tok0 + 1;
+  const int all_lo = a.window > 0 ? max(0, w.len - w.n + w.tok1 - a.window + 1) : 0;
   uint4 q[D / 32];
   {
     const uint16_t* qp = a.q + (int64_t)(w.start + tok) * a.q_stride + (int64_t)hq * D;
@@ -675,7 +737,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
   pf4 o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY;
+  pf4 l = pf4{0.0f, 0.0f, 0.0f, 0.0f};  // [0]: of the lane's keys (MXFP4: of all)
 
   const int tiles = (w.k1 - w.k0 + 31) >> 5;
   const int n_it = (tiles - wave + 3) >> 2;  // this wave's
@@ -706,7 +769,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
     }
     pa_load<D>(t, a.kv, g, c, at);
   };
-  auto step = [&](const PaTile<D, F4>& t, int it, const int (&id)[2]) {
+  auto step = [&](PaTile<D, F4>& t, int it, const int (&id)[2]) {
     const int kb = w.k0 + 32 * (wave + 4 * it);
     // every row sees all 32 keys (else the masks: two blocks of selects under a
     // branch of the whole wave)
@@ -728,13 +791,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
           const int key = kb + 16 * s + 4 * g + i;
           const bool seen = (key >= k_lo) & (key < k_hi) & (id[s] >= 0);
           sv[s][i] = seen ? sv[s][i] : -INFINITY;
+          pa_clear<D>(t, s, i, (key >= w.k1) | (key < w.lo) | (id[s] < 0));
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
                      fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3]))) * c2;
-    mx = fmaxf(mx, xor_lane<16>(mx));
-    mx = fmaxf(mx, xor_lane<32>(mx));
-    if (__any(mx > m)) {  // rarely, once a row has seen some keys
+    if (__any(mx > m + kPaLag)) {  // rarely, once a row has seen some keys
+      mx = fmaxf(mx, xor_lane<16>(mx));
+      mx = fmaxf(mx, xor_lane<32>(mx));
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
@@ -743,37 +807,31 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
       m = mn;
     }
     const float me = m == -INFINITY ? 0.0f : m;
-    uint32_t hi[4], lo[4];  // P in two bf16 terms
+    // P in two bf16 terms.  Over MXFP4 pages, where the vector instructions are the
+    // bound, in one, with the row's sum taken from the rounded values by a product.
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[s][i], c2, -me));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[s][i + 1], c2, -me));
-        l += p0;
-        l += p1;
         const uint32_t x = pack_bf2(p0, p1);
         hi[2 * s + i / 2] = x;
-        lo[2 * s + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
+        if constexpr (!F4) {
+          l[0] += p0;
+          l[0] += p1;
+          lo[2 * s + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
+        }
       }
     uint32_t v[2][4][D / 32];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) pa_value<D>(t, s, i, c, v[s][i]);
-    if (!full) {  // rows that hold no key of the sequence may hold anything
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = kb + 16 * s + 4 * g + i;
-          const bool none = (key >= w.k1) | (key < w.lo) | (id[s] < 0);
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) v[s][i][n] = none ? 0u : v[s][i][n];
-        }
-    }
     const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    const uint4 pl = F4 ? ph : make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if constexpr (F4) l = pa_mfma(kPaOnes, ph, l);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       uint32_t f[4];
@@ -783,7 +841,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
                                      e & 1 ? 0x07060302u : 0x05040100u);
       const uint4 vf = make_uint4(f[0], f[1], f[2], f[3]);
       o[e] = pa_mfma(vf, ph, o[e]);
-      o[e] = pa_mfma(vf, pl, o[e]);
+      if constexpr (!F4) o[e] = pa_mfma(vf, pl, o[e]);
     }
   };
   if (n_it > 0) {
@@ -805,8 +863,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
       }
     }
   }
-  l += xor_lane<16>(l);
-  l += xor_lane<32>(l);
+  if constexpr (!F4) {
+    l[0] += xor_lane<16>(l[0]);
+    l[0] += xor_lane<32>(l[0]);
+  }
   // the four waves' states
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -816,7 +876,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
           make_float4(o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]);
   if (g == 0) {
     sm[wave][c] = m;
-    sl[wave][c] = l;
+    sl[wave][c] = l[0];
   }
   __syncthreads();
   // thread: row tr, dims td .. td + E - 1
@@ -850,15 +910,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_few(PagedAt
     if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     pa_join<D, R>(a.part + first * R * (D + 2), (int64_t)a.kv.Hkv * R * (D + 2), w.chunks,
                   min(R, rows - w.row0), sf, so[0], [&](int tr_, const float (&y)[E], float m_, float l_) {
-                    const int row_ = w.row0 + tr_, head = h * G + row_ % G;
-                    pa_write<E>(a.out + ((int64_t)(w.start + row_ / G) * a.Hq + head) * D + td, y,
+                    const int tok_ = pa_div(w.row0 + tr_, G, w.rG);
+                    const int head = h * G + w.row0 + tr_ - tok_ * G;
+                    pa_write<E>(a.out + ((int64_t)(w.start + tok_) * a.Hq + head) * D + td, y,
                                 pa_finish(a, head, m_, l_));
                   });
     return;
   }
   if (row >= rows) return;
-  const int head = h * G + row % G;
-  pa_write<E>(a.out + ((int64_t)(w.start + row / G) * a.Hq + head) * D + td, x,
+  const int out_tok = pa_div(row, G, w.rG), head = h * G + row - out_tok * G;
+  pa_write<E>(a.out + ((int64_t)(w.start + out_tok) * a.Hq + head) * D + td, x,
               pa_finish(a, head, M, L));
 }
 
@@ -884,11 +945,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   __shared__ __align__(16) uint32_t vt[2][32 * D];
   __shared__ int merge_here;
   const int h = blockIdx.x % a.kv.Hkv;
-  PaWork w;
-  if (!pa_work<false, R, 64, 512, kPmTarget>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
+  PaWork w(a);
+  if (!pa_work<false, R, 64, 512, kPmTarget, 512, false>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int G = a.Hq / a.kv.Hkv, rows = w.n * G, pos0 = w.len - w.n;
+  const int G = w.G, rows = w.n * G, pos0 = w.len - w.n;
   const float c2 = (D == 64 ? 0.125f : 0.08838834764831845f) * kLog2e;
   uint4 q[2][D / 32];
   int k_hi[2], k_lo[2];
@@ -1043,8 +1104,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     l[t] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
     m[t] = -INFINITY;
   }
-  const uint4 ones = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
-
   auto compute = [&](int it, uint32_t dead) {
     const int kb = w.k0 + 64 * it, buf = it & 1;
     if (kb >= any_hi || kb + 64 <= any_lo) return;
@@ -1082,9 +1141,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
       for (int k = 0; k < 4; ++k)
         mx = fmaxf(mx, fmaxf(fmaxf(s[t][k][0], s[t][k][1]), fmaxf(s[t][k][2], s[t][k][3])));
       mx *= c2;
-      mx = fmaxf(mx, xor_lane<16>(mx));
-      mx = fmaxf(mx, xor_lane<32>(mx));
-      if (__any(mx > m[t])) {
+      if (__any(mx > m[t] + kPaLag)) {
+        mx = fmaxf(mx, xor_lane<16>(mx));
+        mx = fmaxf(mx, xor_lane<32>(mx));
         const float mn = fmaxf(m[t], mx);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
 #pragma unroll
@@ -1103,8 +1162,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i + 1], c2, -me)));
       p[t][0] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
       p[t][1] = make_uint4(pw[4], pw[5], pw[6], pw[7]);
-      l[t] = pa_mfma(ones, p[t][0], l[t]);
-      l[t] = pa_mfma(ones, p[t][1], l[t]);
+      l[t] = pa_mfma(kPaOnes, p[t][0], l[t]);
+      l[t] = pa_mfma(kPaOnes, p[t][1], l[t]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -1228,6 +1287,7 @@ size_t paged_attn_counters() { return (size_t)(2 * kPaTarget) * kPaArrive * 4; }
 
 void launch_paged_attn(PagedAttnArgs a, hipStream_t st) {
   a.few = kPaFew;
+  a.G = a.Hq / a.kv.Hkv;
   const int64_t few = pa_few_blocks(a.r, a.Hq, a.kv.Hkv), many = pa_many_blocks(a.r, a.Hq, a.kv.Hkv);
 #define PA(D, F4)                                                                              \
   do {                                                                                         \
