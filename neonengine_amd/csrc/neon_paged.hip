@@ -199,9 +199,11 @@ void launch_paged_append(const PagedKv& kv, const PagedRows& r, const uint16_t* 
                        cos_t, sin_t, n_pos, q_out, Hq);
 }
 
-// 8 MXFP4 values (one dword of codes) as bf16: v_cvt_scalef32_pk_bf16_fp4
-// reads the scale's exponent field, so s << 23 serves every scale byte (255:
-// NaN), and E2M1 x 2^(s - 127) is a bf16 value
+// 8 MXFP4 values (one dword of codes) as bf16 with the scale in the low byte of s:
+// v_cvt_scalef32_pk_bf16_fp4 reads the exponent field of its scale alone (sign and
+// fraction bits change no result for the 256 scales x 256 code bytes, on an
+// MI355X), so s << 23 serves every scale byte (255: NaN) whatever lies above it,
+// and E2M1 x 2^(s - 127) is a bf16 value
 __device__ __forceinline__ uint4 mx4_to_bf16x8(uint32_t w, uint32_t s) {
   const float sc = __uint_as_float(s << 23);
   return make_uint4(
@@ -471,10 +473,13 @@ struct PaTile<D, false> {
 template <int D>
 struct PaTile<D, true> {
   uint32_t k[2][D / 32];     // codes of dims (D/4) g ..
-  uint32_t v[2][4];          // codes of keys 4 g + i, dims (D/16) c ..
-  uint32_t ks[2];            // scale of the key's block
+  uint32_t v[2][4];          // the word with the codes of keys 4 g + i, dims (D/16) c ..
+  uint32_t ks[2];            // the word with the scale of the key's block
   uint32_t vs[2][D / 32];    // scales of the keys 4 g .. 4 g + 3
 };
+// Words, though D = 64 needs two bytes of v and D / 32 of ks: a narrower load's
+// zero extension ends up behind the loop's join, where it waits for the step that
+// was only just requested.
 
 template <int D>
 __device__ __forceinline__ void pa_load(PaTile<D, false>& t, const PagedKv& kv, int g, int c,
@@ -508,7 +513,7 @@ __device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, i
     const uint8_t* vp = kv.v + at[s] * (D / 2);
     const uint8_t* ksp = kv.ks + at[s] * (D / 32);
     const uint8_t* vsp = kv.vs + at[s] * (D / 32);
-    t.ks[s] = ksp[(uint32_t)(c * (D / 32) + (D == 64 ? g >> 1 : g))];
+    t.ks[s] = *reinterpret_cast<const uint32_t*>(ksp + (uint32_t)(c * (D / 32) & ~3));
     if constexpr (D == 64) {
       const uint2 x = *reinterpret_cast<const uint2*>(kp + (uint32_t)(c * 32 + 8 * g));
       t.k[s][0] = x.x; t.k[s][1] = x.y;
@@ -516,7 +521,7 @@ __device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, i
       t.vs[s][0] = y.x; t.vs[s][1] = y.y;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        t.v[s][i] = *reinterpret_cast<const uint16_t*>(vp + (uint32_t)((4 * g + i) * 32 + 2 * c));
+        t.v[s][i] = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)((4 * g + i) * 32 + (2 * c & ~3)));
     } else {
       const uint4 x = *reinterpret_cast<const uint4*>(kp + (uint32_t)(c * 64 + 16 * g));
       t.k[s][0] = x.x; t.k[s][1] = x.y; t.k[s][2] = x.z; t.k[s][3] = x.w;
@@ -545,10 +550,13 @@ __device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, bool 
 
 // operand n of a 16-key step's keys: the dims that pa_query gives B
 template <int D>
-__device__ __forceinline__ uint4 pa_key(const PaTile<D, false>& t, int s, int n) { return t.k[s][n]; }
+__device__ __forceinline__ uint4 pa_key(const PaTile<D, false>& t, int s, int n, int, int) {
+  return t.k[s][n];
+}
 template <int D>
-__device__ __forceinline__ uint4 pa_key(const PaTile<D, true>& t, int s, int n) {
-  return mx4_to_bf16x8(t.k[s][n], t.ks[s]);
+__device__ __forceinline__ uint4 pa_key(const PaTile<D, true>& t, int s, int n, int g, int c) {
+  // byte (c & 1) 2 + g / 2 (D = 64) or g of the scales' word
+  return mx4_to_bf16x8(t.k[s][n], t.ks[s] >> (D == 64 ? 16 * (c & 1) + 8 * (g >> 1) : 8 * g));
 }
 template <int D, bool F4>
 __device__ __forceinline__ int pa_query_dim(int n, int g) {
@@ -565,16 +573,15 @@ template <int D>
 __device__ __forceinline__ void pa_value(const PaTile<D, true>& t, int s, int i, int c,
                                          uint32_t (&v)[D / 32]) {
   // The key's scale byte is byte (i & 1) 2 + c / 8 of word i / 2 (D = 64), byte
-  // c / 4 of word i (D = 128).  The conversion reads the exponent field of its
-  // scale alone (sign and fraction set at will change no result for the 256 scales
-  // x 256 code bytes, on an MI355X), so the bytes beside it need no mask.
+  // c / 4 of word i (D = 128); the bytes beside it need no mask.
   const uint32_t b = D == 64 ? t.vs[s][i >> 1] >> (c & 8) : t.vs[s][i] >> (2 * (c & 12));
   const float sc = __uint_as_float(b << (D == 64 && (i & 1) ? 7 : 23));
-  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 0));
-  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 1));
+  const uint32_t w = D == 64 ? t.v[s][i] >> (16 * (c & 1)) : t.v[s][i];
+  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
   if constexpr (D == 128) {
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 2));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[s][i], sc, 3));
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
   }
 }
 
@@ -779,7 +786,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D)) void k_paged_attn_few(PagedAt
     for (int s = 0; s < 2; ++s) {
       pf4 acc = pf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < D / 32; ++n) acc = pa_mfma(pa_key<D>(t, s, n), q[n], acc);
+      for (int n = 0; n < D / 32; ++n) acc = pa_mfma(pa_key<D>(t, s, n, g, c), q[n], acc);
 #pragma unroll
       for (int i = 0; i < 4; ++i) sv[s][i] = acc[i];
     }
@@ -1007,7 +1014,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   // A tile's loads.  bf16: K word tid % W of keys tid / W + (256 / W) j; V
   // words tid % 8 (+ 8 j) of the keys 2 m, 2 m + 1, m = tid / 8.  MXFP4: K codes
   // of D/4 dims of key tid / 4 in k[0] and their scale in k[1].x; V codes of 8
-  // dims of the keys 2 m, 2 m + 1 (D = 128: of 16) and the two scales.
+  // dims of the keys 2 m, 2 m + 1 (D = 128: of 16) and their scales in k[1].y, .z.
   auto load_tile = [&](PmStage<D>& t, int it, int ids) {
     const int m2 = (tid >> 3 & 7) * 2;  // the pair's first key within its group (= wave)
     const int64_t va = group_at(it, ids, wave);
@@ -1015,11 +1022,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
       const int kk = tid >> 2 & 15, part = tid & 3;
       const uint8_t* kp = a.kv.k + va * (D / 2);
       const uint8_t* vp = a.kv.v + va * (D / 2);
-      t.k[1].x = (a.kv.ks + va * (D / 32))[(uint32_t)(kk * (D / 32) + (D == 64 ? part >> 1 : part))];
-      const uint8_t* vs = a.kv.vs + va * (D / 32);
-      const uint32_t sat = (uint32_t)(m2 * (D / 32) + (D == 64 ? (tid & 7) >> 2 : (tid & 7) >> 1));
-      t.k[1].y = vs[sat];
-      t.k[1].z = vs[sat + D / 32];
+      // words with the scales (see PaTile)
+      t.k[1].x = *reinterpret_cast<const uint32_t*>(a.kv.ks + va * (D / 32) + (uint32_t)(kk * (D / 32) & ~3));
+      const uint8_t* vs = a.kv.vs + va * (D / 32) + (uint32_t)(m2 * (D / 32));
+      t.k[1].y = *reinterpret_cast<const uint32_t*>(vs);  // D = 64: of both keys
+      t.k[1].z = D == 64 ? 0u : *reinterpret_cast<const uint32_t*>(vs + D / 32);
       if constexpr (D == 64) {
         const uint2 x = *reinterpret_cast<const uint2*>(kp + (uint32_t)(kk * 32 + 8 * part));
         t.k[0].x = x.x; t.k[0].y = x.y;
@@ -1078,12 +1085,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     if constexpr (F4) {
       const int key = tid >> 2, part = tid & 3;
       const uint32_t kc[4] = {t.k[0].x, t.k[0].y, t.k[0].z, t.k[0].w};
+      const uint32_t ks = t.k[1].x >> (D == 64 ? 16 * (key & 1) + 8 * (part >> 1) : 8 * part);
+      const int blk = D == 64 ? (tid & 7) >> 2 : (tid & 7) >> 1;  // of the values' dims
+      const uint32_t vs0 = t.k[1].y >> (8 * blk);
+      const uint32_t vs1 = D == 64 ? t.k[1].y >> (16 + 8 * blk) : t.k[1].z >> (8 * blk);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) put_k(buf, key, part * (D / 32) + j, mx4_to_bf16x8(kc[j], t.k[1].x));
+      for (int j = 0; j < D / 32; ++j) put_k(buf, key, part * (D / 32) + j, mx4_to_bf16x8(kc[j], ks));
 #pragma unroll
       for (int j = 0; j < D / 64; ++j) {
-        const uint4 x = mx4_to_bf16x8(j == 0 ? t.v[0][0].x : t.v[0][0].y, t.k[1].y);
-        const uint4 y = mx4_to_bf16x8(j == 0 ? t.v[1][0].x : t.v[1][0].y, t.k[1].z);
+        const uint4 x = mx4_to_bf16x8(j == 0 ? t.v[0][0].x : t.v[0][0].y, vs0);
+        const uint4 y = mx4_to_bf16x8(j == 0 ? t.v[1][0].x : t.v[1][0].y, vs1);
         put_pairs(buf, m, 8 * ((tid & 7) * (D / 64) + j), none[0] ? zero : x, none[1] ? zero : y);
       }
     } else {
