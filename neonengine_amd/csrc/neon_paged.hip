@@ -7,6 +7,8 @@
 // along D, so a token is written alone, whatever its neighbours hold.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "neon_common.hpp"
 #include "neon_internal.hpp"
 
@@ -404,8 +406,9 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool fl
     blocks_to = pa_scan(blocks);
     // FIT: a few more blocks than the chip holds cost a round of their own, so
     // larger chunks where that makes them fit (a unit is one block at least).
-    // Four MXFP4 sequences up to 131072 tokens: 58 -> 38 us; where the reads are the
-    // bound, small chunks even out the end better (64 bf16 ones: 68 -> 73 us).
+    // MXFP4, 4 sequences up to 131072 tokens 30.4 -> 29.3 us, 48 of heads of 128 25.8
+    // -> 24.6; where the reads are the bound, small chunks even out the end better
+    // (64 bf16 ones: 68 -> 73 us).
     const float over = (float)__builtin_amdgcn_readlane(blocks_to, 63) * (float)a.kv.Hkv * (1.0f / PLACES);
     if (!FIT || turn == 3 || per > 1 || over <= 1.0f || over > 2.0f) break;
     chunk = uni((min((int)((float)chunk * over), (1 << 30) - 128) + 128) & ~127);
@@ -670,15 +673,33 @@ __device__ __forceinline__ void pa_join(const float* part, int64_t step, int chu
       __syncthreads();
       const int n = min(kPaJoin, chunks - c0);
       const float* po = part + c0 * step + (r0 + row) * D + lane16 * E;
-#pragma unroll 4
-      for (int j = share; j < n; j += shares) {
-        const float f = sf[row][j];
+      // U chunks' loads at a time
+      auto take = [&](auto u_t, int j0) {
+        constexpr int U = decltype(u_t)::value;
+        float2 y[U][E / 2];
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 y = pa_load_agent(po + j * step + e);
-          x[e] = __builtin_fmaf(y.x, f, x[e]);
-          x[e + 1] = __builtin_fmaf(y.y, f, x[e + 1]);
+        for (int u = 0; u < U; ++u) {
+          const float* p = po + min(j0 + u * shares, n - 1) * step;
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) y[u][e] = pa_load_agent(p + 2 * e);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (j0 + u * shares >= n) break;
+          const float f = sf[row][j0 + u * shares];
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) {
+            x[2 * e] = __builtin_fmaf(y[u][e].x, f, x[2 * e]);
+            x[2 * e + 1] = __builtin_fmaf(y[u][e].y, f, x[2 * e + 1]);
+          }
+        }
+      };
+      if (n <= 2 * shares) {
+        take(std::integral_constant<int, 2>{}, share);
+      } else if (n <= 4 * shares) {
+        take(std::integral_constant<int, 4>{}, share);
+      } else {
+        for (int j0 = share; j0 < n; j0 += 8 * shares) take(std::integral_constant<int, 8>{}, j0);
       }
     }
     // the shares of a row; sx row: share * rows2 + row
@@ -705,12 +726,13 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // Few rows: 16 per unit, four waves that share nothing but the result, each
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers, some steps ahead of the products.
-constexpr int pa_few_waves(int D) { return D == 64 ? 3 : 2; }  // of a SIMD (and blocks of a CU)
+// waves of a SIMD, and blocks of a CU (four of D = 64 spill)
+constexpr int pa_few_waves(int D, bool f4) { return D == 64 || f4 ? 3 : 2; }
 template <int D, bool F4>
-__global__ __launch_bounds__(256, pa_few_waves(D)) void k_paged_attn_few(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(PagedAttnArgs a) {
   constexpr int R = 16, E = D / 16;
   constexpr int NT = 2;  // steps in registers: one in use, the others on their way
-  constexpr int kPlaces = 256 * pa_few_waves(D);
+  constexpr int kPlaces = 256 * pa_few_waves(D, F4);
   __shared__ __align__(16) float so[4][R][D + 4];
   __shared__ float sm[4][R], sl[4][R];
   __shared__ float sf[16][kPaJoin];
