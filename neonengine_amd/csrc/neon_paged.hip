@@ -953,25 +953,29 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 }
 
 // Many rows: 128 per unit, 32 of each wave (two tiles of 16), 64 keys at a time
-// through LDS, where the four waves share them.  K rows lie as they are, their
-// 16-byte words exchanged by the key's low bits, so the 16 lanes that read one
-// word of 16 keys touch every bank once.  V lies as pairs: dword (m, d) holds
-// the values of the keys 2 m and 2 m + 1, paired once when a tile is written
-// instead of by every wave, so a lane's four 16-byte reads are its A operands.
-// MXFP4 pages are expanded when a tile is written.  The next tile's loads are
-// on their way while a tile is used, and LDS holds two.
+// through LDS, where the four waves share them.  K and V rows lie as they are,
+// their words exchanged by the key's low bits so that a read touches every bank
+// evenly: K by 16 bytes (16 lanes read one word of 16 keys), V by 32 (16 lanes
+// read 32 bytes of 4 keys, and ds_read_b64_tr_b16 gives each lane one dim's four
+// values, which are half of its A operand).  MXFP4 pages are expanded when a tile
+// is written.  The next tile's loads are on their way while a tile is used, and
+// LDS holds two.
 // P is rounded to bf16, and the row sums come from the same rounded values (a
 // product with ones), so the rounding cancels where a row's weights share it.
+typedef short ps4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 pa_read_tr(const void* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) ps4*)p));
+}
 template <int D>
 struct PmStage {  // a thread's part of a tile on its way
-  uint4 k[D / 32], v[2][D / 64];
+  uint4 k[D / 32], v[D / 32];
 };
 
 template <int D, bool F4>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
-  __shared__ __align__(16) uint4 kt[2][64 * W];
-  __shared__ __align__(16) uint32_t vt[2][32 * D];
+  __shared__ __align__(16) uint4 kt[2][64 * W], vt[2][64 * W];
   __shared__ int merge_here;
   const int h = blockIdx.x % a.kv.Hkv;
   PaWork w(a);
@@ -1033,98 +1037,61 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
       dead |= (uint32_t)(__builtin_amdgcn_readlane(ids, 4 * (it & 15) + grp) < 0) << grp;
     return dead;
   };
-  // A tile's loads.  bf16: K word tid % W of keys tid / W + (256 / W) j; V
-  // words tid % 8 (+ 8 j) of the keys 2 m, 2 m + 1, m = tid / 8.  MXFP4: K codes
-  // of D/4 dims of key tid / 4 in k[0] and their scale in k[1].x; V codes of 8
-  // dims of the keys 2 m, 2 m + 1 (D = 128: of 16) and their scales in k[1].y, .z.
+  // A tile's loads.  bf16: word tid % W of the keys tid / W + (256 / W) j.  MXFP4:
+  // the codes of D/4 dims of key tid / 4 in [0], and the word with their scale in
+  // [1].x (see PaTile).
   auto load_tile = [&](PmStage<D>& t, int it, int ids) {
-    const int m2 = (tid >> 3 & 7) * 2;  // the pair's first key within its group (= wave)
-    const int64_t va = group_at(it, ids, wave);
     if constexpr (F4) {
+      const int64_t at = group_at(it, ids, wave);
       const int kk = tid >> 2 & 15, part = tid & 3;
-      const uint8_t* kp = a.kv.k + va * (D / 2);
-      const uint8_t* vp = a.kv.v + va * (D / 2);
-      // words with the scales (see PaTile)
-      t.k[1].x = *reinterpret_cast<const uint32_t*>(a.kv.ks + va * (D / 32) + (uint32_t)(kk * (D / 32) & ~3));
-      const uint8_t* vs = a.kv.vs + va * (D / 32) + (uint32_t)(m2 * (D / 32));
-      t.k[1].y = *reinterpret_cast<const uint32_t*>(vs);  // D = 64: of both keys
-      t.k[1].z = D == 64 ? 0u : *reinterpret_cast<const uint32_t*>(vs + D / 32);
+      const uint32_t sc = (uint32_t)(kk * (D / 32) & ~3), cd = (uint32_t)(kk * (D / 2) + (D / 8) * part);
+      t.k[1].x = *reinterpret_cast<const uint32_t*>(a.kv.ks + at * (D / 32) + sc);
+      t.v[1].x = *reinterpret_cast<const uint32_t*>(a.kv.vs + at * (D / 32) + sc);
       if constexpr (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp + (uint32_t)(kk * 32 + 8 * part));
+        const uint2 x = *reinterpret_cast<const uint2*>(a.kv.k + at * (D / 2) + cd);
+        const uint2 y = *reinterpret_cast<const uint2*>(a.kv.v + at * (D / 2) + cd);
         t.k[0].x = x.x; t.k[0].y = x.y;
-        t.v[0][0].x = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)(m2 * 32 + 4 * (tid & 7)));
-        t.v[1][0].x = *reinterpret_cast<const uint32_t*>(vp + (uint32_t)(m2 * 32 + 32 + 4 * (tid & 7)));
+        t.v[0].x = y.x; t.v[0].y = y.y;
       } else {
-        t.k[0] = *reinterpret_cast<const uint4*>(kp + (uint32_t)(kk * 64 + 16 * part));
-        const uint2 x = *reinterpret_cast<const uint2*>(vp + (uint32_t)(m2 * 64 + 8 * (tid & 7)));
-        const uint2 y = *reinterpret_cast<const uint2*>(vp + (uint32_t)(m2 * 64 + 64 + 8 * (tid & 7)));
-        t.v[0][0].x = x.x; t.v[0][0].y = x.y;
-        t.v[1][0].x = y.x; t.v[1][0].y = y.y;
+        t.k[0] = *reinterpret_cast<const uint4*>(a.kv.k + at * (D / 2) + cd);
+        t.v[0] = *reinterpret_cast<const uint4*>(a.kv.v + at * (D / 2) + cd);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
         const int key = tid / W + (256 / W) * j;  // its group is the wave's
-        const int64_t ka = group_at(it, ids, uni(key >> 4));
-        t.k[j] = *reinterpret_cast<const uint4*>(a.kv.k + ka * (2 * D) +
-                                                 (uint32_t)((key & 15) * 2 * D + 16 * (tid % W)));
+        const int64_t at = group_at(it, ids, uni(key >> 4)) * (2 * D);
+        const uint32_t off = (uint32_t)((key & 15) * 2 * D + 16 * (tid % W));
+        t.k[j] = *reinterpret_cast<const uint4*>(a.kv.k + at + off);
+        t.v[j] = *reinterpret_cast<const uint4*>(a.kv.v + at + off);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-          t.v[i][j] = *reinterpret_cast<const uint4*>(
-              a.kv.v + va * (2 * D) + (uint32_t)((m2 + i) * 2 * D + 16 * ((tid & 7) + 8 * j)));
     }
   };
-  auto put_k = [&](int buf, int key, int word, const uint4& x) {
-    kt[buf][key * W + (word ^ (key & 7))] = x;
-  };
-  auto put_pairs = [&](int buf, int m, int d0, const uint4& x, const uint4& y) {
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-    uint32_t z[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      z[2 * i] = __builtin_amdgcn_perm(ys[i], xs[i], 0x05040100u);
-      z[2 * i + 1] = __builtin_amdgcn_perm(ys[i], xs[i], 0x07060302u);
-    }
-    uint4* dst = reinterpret_cast<uint4*>(&vt[buf][m * D + d0]);
-    dst[0] = make_uint4(z[0], z[1], z[2], z[3]);
-    dst[1] = make_uint4(z[4], z[5], z[6], z[7]);
+  auto v_word = [&](int key, int word) {
+    return key * W + (word ^ (D == 64 ? (key & 6) : (key & 7) << 1));
   };
   auto write_tile = [&](const PmStage<D>& t, int it, int ids) {
-    const int buf = it & 1, m = tid >> 3, kb = w.k0 + 64 * it;
+    const int buf = it & 1, kb = w.k0 + 64 * it;
     // values of rows that hold no key of the sequence may be anything
-    const bool edge = kb < w.lo || kb + 64 > w.k1;
-    const bool dead = __builtin_amdgcn_readlane(ids, 4 * (it & 15) + wave) < 0;
-    bool none[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = kb + 2 * m + i;
-      none[i] = dead || (edge && (key < w.lo || key >= w.k1));
-    }
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    auto put = [&](int key, int word, const uint4& x, const uint4& y) {
+      const bool none = (kb + key < w.lo) | (kb + key >= w.k1) |
+                        (__builtin_amdgcn_readlane(ids, 4 * (it & 15) + uni(key >> 4)) < 0);
+      kt[buf][key * W + (word ^ (key & 7))] = x;
+      vt[buf][v_word(key, word)] = make_uint4(none ? 0u : y.x, none ? 0u : y.y, none ? 0u : y.z,
+                                              none ? 0u : y.w);
+    };
     if constexpr (F4) {
       const int key = tid >> 2, part = tid & 3;
+      const int sh = D == 64 ? 16 * (key & 1) + 8 * (part >> 1) : 8 * part;
       const uint32_t kc[4] = {t.k[0].x, t.k[0].y, t.k[0].z, t.k[0].w};
-      const uint32_t ks = t.k[1].x >> (D == 64 ? 16 * (key & 1) + 8 * (part >> 1) : 8 * part);
-      const int blk = D == 64 ? (tid & 7) >> 2 : (tid & 7) >> 1;  // of the values' dims
-      const uint32_t vs0 = t.k[1].y >> (8 * blk);
-      const uint32_t vs1 = D == 64 ? t.k[1].y >> (16 + 8 * blk) : t.k[1].z >> (8 * blk);
+      const uint32_t vc[4] = {t.v[0].x, t.v[0].y, t.v[0].z, t.v[0].w};
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) put_k(buf, key, part * (D / 32) + j, mx4_to_bf16x8(kc[j], ks));
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        const uint4 x = mx4_to_bf16x8(j == 0 ? t.v[0][0].x : t.v[0][0].y, vs0);
-        const uint4 y = mx4_to_bf16x8(j == 0 ? t.v[1][0].x : t.v[1][0].y, vs1);
-        put_pairs(buf, m, 8 * ((tid & 7) * (D / 64) + j), none[0] ? zero : x, none[1] ? zero : y);
-      }
+      for (int j = 0; j < D / 32; ++j)
+        put(key, part * (D / 32) + j, mx4_to_bf16x8(kc[j], t.k[1].x >> sh),
+            mx4_to_bf16x8(vc[j], t.v[1].x >> sh));
     } else {
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) put_k(buf, tid / W + (256 / W) * j, tid % W, t.k[j]);
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j)
-        put_pairs(buf, m, 8 * ((tid & 7) + 8 * j), none[0] ? zero : t.v[0][j], none[1] ? zero : t.v[1][j]);
+      for (int j = 0; j < D / 32; ++j) put(tid / W + (256 / W) * j, tid % W, t.k[j], t.v[j]);
     }
   };
 
@@ -1166,7 +1133,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
             s[t][k][i] = seen ? s[t][k][i] : -INFINITY;
           }
     }
-    uint4 p[2][2];
+    uint4 p_[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float mx = -INFINITY;
@@ -1193,29 +1160,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
           pw[2 * k + i / 2] =
               pack_bf2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i], c2, -me)),
                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i + 1], c2, -me)));
-      p[t][0] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
-      p[t][1] = make_uint4(pw[4], pw[5], pw[6], pw[7]);
-      l[t] = pa_mfma(kPaOnes, p[t][0], l[t]);
-      l[t] = pa_mfma(kPaOnes, p[t][1], l[t]);
+      p_[t][0] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+      p_[t][1] = make_uint4(pw[4], pw[5], pw[6], pw[7]);
+      l[t] = pa_mfma(kPaOnes, p_[t][0], l[t]);
+      l[t] = pa_mfma(kPaOnes, p_[t][1], l[t]);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
+      // lane (g, c) reads dims 4 (c & 3) .. of key 4 g + c / 4 of each 16, for each
+      // 16 dims, and gets dim c of the keys 4 g ..
+      const int key = 32 * k + 4 * g + (c >> 2);  // (the second 16 exchange alike)
+      const char* base = reinterpret_cast<const char*>(&vt[buf][0]) + 8 * (c & 1);
 #pragma unroll
-      for (int e0 = 0; e0 < E; e0 += 4) {
-        uint4 x[4];  // pair j of the lane's keys, dims E c + e0 ..
+      for (int e = 0; e < E; ++e) {
+        const char* p = base + 16 * v_word(key, 2 * e + (c >> 1 & 1));
+        const uint2 x = pa_read_tr(p), y = pa_read_tr(p + 16 * 16 * W);
+        const uint4 f = make_uint4(x.x, x.y, y.x, y.y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[j] = *reinterpret_cast<const uint4*>(
-              &vt[buf][(16 * k + 8 * (j >> 1) + 2 * g + (j & 1)) * D + E * c + e0]);
-        const uint4 f[4] = {make_uint4(x[0].x, x[1].x, x[2].x, x[3].x),
-                            make_uint4(x[0].y, x[1].y, x[2].y, x[3].y),
-                            make_uint4(x[0].z, x[1].z, x[2].z, x[3].z),
-                            make_uint4(x[0].w, x[1].w, x[2].w, x[3].w)};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int t = 0; t < 2; ++t) o[t][e0 + e] = pa_mfma(f[e], p[t][k], o[t][e0 + e]);
+        for (int t = 0; t < 2; ++t) o[t][e] = pa_mfma(f, p_[t][k], o[t][e]);
       }
+    }
   };
 
   PmStage<D> st;
@@ -1231,7 +1195,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
     compute(it, dead);
   }
 
-  // lane (g, c): row c of each tile, dims (D/4) g ..
+  // lane (g, c): row c of each tile, dims 16 e + 4 g ..
   if (w.chunks == 1) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -1239,14 +1203,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
       if (r >= rows) continue;
       const int head = h * G + r % G;
       const float fin = pa_finish(a, head, m[t], l[t][0]);
-      uint16_t* dst = a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + (D / 4) * g;
+      uint16_t* dst = a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + 4 * g;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<uint2*>(dst + E * i + e) =
-              make_uint2(pack_bf2(o[t][e][i] * fin, o[t][e + 1][i] * fin),
-                         pack_bf2(o[t][e + 2][i] * fin, o[t][e + 3][i] * fin));
+      for (int e = 0; e < E; ++e)
+        *reinterpret_cast<uint2*>(dst + 16 * e) =
+            make_uint2(pack_bf2(o[t][e][0] * fin, o[t][e][1] * fin),
+                       pack_bf2(o[t][e][2] * fin, o[t][e][3] * fin));
     }
     return;
   }
@@ -1258,10 +1220,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   for (int t = 0; t < 2; ++t) {
     const int r = 32 * wave + 16 * t + c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < E; e += 2)
-        pa_store_agent(po + r * D + (D / 4) * g + E * i + e, o[t][e][i], o[t][e + 1][i]);
+    for (int e = 0; e < E; ++e) {
+      pa_store_agent(po + r * D + 16 * e + 4 * g, o[t][e][0], o[t][e][1]);
+      pa_store_agent(po + r * D + 16 * e + 4 * g + 2, o[t][e][2], o[t][e][3]);
+    }
     if (g == 0) pa_store_agent(po + R * D + 2 * r, m[t], l[t][0]);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
