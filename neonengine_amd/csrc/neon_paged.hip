@@ -1073,10 +1073,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   auto write_tile = [&](const PmStage<D>& t, int it, int ids) {
     const int buf = it & 1, kb = w.k0 + 64 * it;
     // values of rows that hold no key of the sequence may be anything
+    // (words one by one: a copy of the struct would put the stage in private memory)
     auto put = [&](int key, int word, const uint4& x, const uint4& y) {
       const bool none = (kb + key < w.lo) | (kb + key >= w.k1) |
                         (__builtin_amdgcn_readlane(ids, 4 * (it & 15) + uni(key >> 4)) < 0);
-      kt[buf][key * W + (word ^ (key & 7))] = x;
+      kt[buf][key * W + (word ^ (key & 7))] = make_uint4(x.x, x.y, x.z, x.w);
       vt[buf][v_word(key, word)] = make_uint4(none ? 0u : y.x, none ? 0u : y.y, none ? 0u : y.z,
                                               none ? 0u : y.w);
     };
