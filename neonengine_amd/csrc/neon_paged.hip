@@ -557,18 +557,54 @@ __device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, i
   }
 }
 
-// clears key i's values: rows that hold no key of the sequence may hold anything
+// Steps at the edge: keys that some rows see and others do not, and rows of a page
+// that hold no key of the sequence and may hold anything.  A weight of 0 would turn
+// an infinity or a NaN among their values into a NaN of a row that does not see
+// it, so such values are cleared on the way, and where a key of the sequence had
+// one (`odd`), pa_odd_values adds it to the rows that see it after the last step.
+__device__ __forceinline__ uint32_t pa_odd_halves(uint32_t w) {  // 0xFFFF in each
+  return ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
+         ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+}
+// clears key i's values: all (none), or the odd ones
 template <int D>
-__device__ __forceinline__ void pa_clear(PaTile<D, false>& t, int s, int i, bool none) {
+__device__ __forceinline__ void pa_clear(PaTile<D, false>& t, int s, int i, int, bool none, bool& odd) {
 #pragma unroll
-  for (int n = 0; n < D / 32; ++n) t.v[s][i][n] = none ? 0u : t.v[s][i][n];
+  for (int n = 0; n < D / 32; ++n) {
+    const uint32_t m = pa_odd_halves(t.v[s][i][n]);
+    odd = odd || (m != 0 && !none);
+    t.v[s][i][n] = none ? 0u : t.v[s][i][n] & ~m;
+  }
 }
 template <int D>
-__device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, bool none) {
-  const uint32_t keep = D == 128 ? 0u : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;  // of its scales' word
+__device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, int c, bool none, bool& odd) {
+  // its scales' word, the bytes of the others there, and the scale of the lane's dims
   uint32_t& word = t.vs[s][i * (D / 32) >> 2];
-  t.v[s][i] = none ? 0u : t.v[s][i];
-  word = none ? word & keep : word;
+  const uint32_t keep = D == 128 ? 0u : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  const uint32_t byte = D == 64 ? word >> (16 * (i & 1) + (c & 8)) : word >> (2 * (c & 12));
+  const bool nan = (byte & 0xFFu) == 0xFFu;
+  const bool clear = none || nan;
+  odd = odd || (nan && !none);
+  t.v[s][i] = clear ? 0u : t.v[s][i];
+  word = clear ? word & keep : word;
+}
+// Adds the infinities and NaNs of keys [kb, kb + n) to the rows of the lane that
+// see them, fn(key, value of dim d0 + ..): the values again from the pages.
+template <int D, bool F4, class F>
+__device__ __forceinline__ void pa_odd_values(const PagedAttnArgs& a, const PaWork& w, int h, int kb,
+                                              int n, F fn) {
+  const int32_t* table = a.r.table + (int64_t)w.b * a.r.max_pages;
+  for (int key = max(kb, w.lo); key < min(kb + n, w.k1); ++key) {
+    const int id = table[key >> a.kv.page_log2];
+    if ((unsigned)id >= (unsigned)a.kv.n_pages) continue;
+    const int64_t at = paged_row_at(a.kv, id, h, key);
+    fn(key, [&](int d) {
+      const uint4 x = paged_load8<F4>(a.kv.v, a.kv.vs, at, D, d & ~7);
+      const uint32_t u = d & 4 ? (d & 2 ? x.w : x.z) : (d & 2 ? x.y : x.x);
+      const float v = d & 1 ? bf_hi(u) : bf_lo(u);
+      return fabsf(v) < INFINITY ? 0.0f : v;
+    });
+  }
 }
 
 // operand n of a 16-key step's keys: the dims that pa_query gives B
@@ -613,6 +649,7 @@ __device__ __forceinline__ void pa_value(const PaTile<D, true>& t, int s, int i,
 __device__ __forceinline__ float pa_finish(const PagedAttnArgs& a, int h, float m, float l) {
   if (a.sinks == nullptr) return l == 0.0f ? 0.0f : 1.0f / l;
   const float sk = bf2f(a.sinks[h]) * kLog2e, M = fmaxf(m, sk);
+  if (M == -INFINITY) return 0.0f;
   const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
   const float den = l * f + __builtin_amdgcn_exp2f(sk - M);
   return den == 0.0f ? 0.0f : f / den;
@@ -818,11 +855,23 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
     }
     pa_load<D>(t, a.kv, g, c, at);
   };
+  // whether one of the step's two pages is none (its whole step is masked)
+  auto edge_page = [&](int kb) {
+    bool none = false;
+    for (int s = 0; s < 2; ++s) {
+      const int key = kb + 16 * s;
+      none |= key < w.k1 && key + 16 > w.lo &&
+              (unsigned)table[key >> a.kv.page_log2] >= (unsigned)a.kv.n_pages;
+    }
+    return none;
+  };
+  auto inside = [&](int kb) { return kb >= all_lo && kb + 32 <= all_hi; };
+  bool odd = false;
   auto step = [&](PaTile<D, F4>& t, int it, const int (&id)[2]) {
     const int kb = w.k0 + 32 * (wave + 4 * it);
     // every row sees all 32 keys (else the masks: two blocks of selects under a
     // branch of the whole wave)
-    const bool full = kb >= all_lo && kb + 32 <= all_hi && (id[0] | id[1]) >= 0;
+    const bool full = inside(kb) && (id[0] | id[1]) >= 0;
     float sv[2][4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -840,7 +889,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
           const int key = kb + 16 * s + 4 * g + i;
           const bool seen = (key >= k_lo) & (key < k_hi) & (id[s] >= 0);
           sv[s][i] = seen ? sv[s][i] : -INFINITY;
-          pa_clear<D>(t, s, i, (key >= w.k1) | (key < w.lo) | (id[s] < 0));
+          pa_clear<D>(t, s, i, c, (key >= w.k1) | (key < w.lo) | (id[s] < 0), odd);
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
@@ -910,6 +959,23 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
         load_tile(t[(u + NT - 1) % NT], nx, ids, id[(u + NT - 1) % NT]);
         step(t[u], it, id[u]);
       }
+    }
+  }
+  if (__any(odd)) {  // lane (g, c): row c, dims (D/4) g + E i + e
+    for (int it = 0; it < n_it; ++it) {
+      const int kb = w.k0 + 32 * (wave + 4 * it);
+      // (every step with a bad page too: its other keys were cleared as well)
+      pa_odd_values<D, F4>(a, w, h, kb, 32, [&](int key, auto value) {
+        if (inside(kb) && !edge_page(kb)) return;
+        const bool seen = (key >= k_lo) & (key < k_hi);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = value((D / 4) * g + E * i + e);
+            if (seen && v != 0.0f) o[e][i] += v;
+          }
+      });
     }
   }
   if constexpr (!F4) {
@@ -996,7 +1062,7 @@ template <int D, bool F4>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
   __shared__ __align__(16) uint4 kt[2][64 * W], vt[2][64 * W];
-  __shared__ int merge_here;
+  __shared__ int merge_here, odd;
   const int h = blockIdx.x % a.kv.Hkv;
   PaWork w(a);
   if (!pa_work<false, R, 64, 512, kPmTarget, 512, false>(a, blockIdx.x / a.kv.Hkv, blockIdx.x == 0, w)) return;
@@ -1027,6 +1093,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   const int any_hi = idle ? 0 : pos0 + r_last / G + 1;
   const int all_lo = a.window > 0 && !idle ? max(0, pos0 + r_last / G - a.window + 1) : 0;
   const int any_lo = a.window > 0 && !idle ? max(0, pos0 + r_first / G - a.window + 1) : 0;
+
+  // the keys that every row of the block sees
+  const int block_hi = pos0 + w.tok0 + 1;
+  const int block_lo = a.window > 0 ? max(0, pos0 + w.tok1 - a.window + 1) : 0;
+  if (tid == 0) odd = 0;
+  __syncthreads();
 
   const int n_it = (w.k1 - w.k0 + 63) >> 6;
   const int32_t* table = a.r.table + (int64_t)w.b * a.r.max_pages;
@@ -1087,19 +1159,31 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
       }
     }
   };
+  // whether some row of the block does not see all of the tile's keys
+  auto at_edge = [&](int kb) { return kb < block_lo || kb + 64 > block_hi; };
   auto v_word = [&](int key, int word) {
     return key * W + (word ^ (D == 64 ? (key & 6) : (key & 7) << 1));
   };
   auto write_tile = [&](const PmStage<D>& t, int it, int ids) {
     const int buf = it & 1, kb = w.k0 + 64 * it;
-    // values of rows that hold no key of the sequence may be anything
+    const bool edge = at_edge(kb);
     // (words one by one: a copy of the struct would put the stage in private memory)
     auto put = [&](int key, int word, const uint4& x, const uint4& y) {
-      const bool none = (kb + key < w.lo) | (kb + key >= w.k1) |
-                        (__builtin_amdgcn_readlane(ids, 4 * (it & 15) + uni(key >> 4)) < 0);
       kt[buf][key * W + (word ^ (key & 7))] = make_uint4(x.x, x.y, x.z, x.w);
-      vt[buf][v_word(key, word)] = make_uint4(none ? 0u : y.x, none ? 0u : y.y, none ? 0u : y.z,
-                                              none ? 0u : y.w);
+      uint32_t v[4] = {y.x, y.y, y.z, y.w};
+      const bool dead = __builtin_amdgcn_readlane(ids, 4 * (it & 15) + uni(key >> 4)) < 0;
+      if (edge || dead) {
+        const bool none = (kb + key < w.lo) | (kb + key >= w.k1) | dead;
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t m = pa_odd_halves(v[i]);
+          any |= m;
+          v[i] = none ? 0u : v[i] & ~m;
+        }
+        if (!none && any != 0) odd = 1;
+      }
+      vt[buf][v_word(key, word)] = make_uint4(v[0], v[1], v[2], v[3]);
     };
     if constexpr (F4) {
       const int key = tid >> 2, part = tid & 3;
@@ -1217,6 +1301,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   }
 
   // lane (g, c): row c of each tile, dims 16 e + 4 g ..
+  __syncthreads();
+  if (odd != 0) {
+    for (int it = 0; it < n_it; ++it) {
+      const int kb = w.k0 + 64 * it;
+      if (!at_edge(kb)) continue;
+      pa_odd_values<D, F4>(a, w, h, kb, 64, [&](int key, auto value) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = value(16 * e + 4 * g + i);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (key >= k_lo[t] && key < k_hi[t] && v != 0.0f) o[t][e][i] += v;
+          }
+      });
+    }
+  }
   if (w.chunks == 1) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {

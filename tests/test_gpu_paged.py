@@ -309,6 +309,78 @@ def test_pages_behind_the_window_may_be_gone():
         check(got, ref, mag, 0x1357)
 
 
+def test_attention_odd_values_stay_with_the_rows_that_see_them():
+    """NaNs and infinities among the keys and values of tokens that some rows of a
+    tile see and others do not: before a window, and after a row's position."""
+    torch_cuda()
+    inf, nan = np.inf, np.nan
+    for mx, D, Hq, Hkv, lens, window in (
+            (False, 64, 16, 2, [(5, 70)], 0), (False, 64, 16, 2, [(6, 200)], 40),
+            (False, 128, 12, 4, [(4, 33), (3, 300)], 0), (False, 64, 64, 8, [(90, 150)], 0),
+            (False, 128, 16, 2, [(70, 260)], 30), (True, 64, 16, 2, [(5, 70)], 9),
+            (True, 128, 8, 1, [(60, 100)], 0)):
+        say(f"odd values mx={mx} D={D} lens={lens} window={window}")
+        rng = np.random.default_rng(D + window)
+        bt = Batch(rng, lens, 16, Hkv, D, mx).fill(rng)
+        for b, (n, t) in enumerate(lens):
+            at = [t - 1, t - 2, t - n + 1]
+            if window:
+                at += [t - n - window + 1, t - n - window + 2]
+            pg, rows = bt.places(b)
+            k, v = bt.get("k", b).astype(np.float32), bt.get("v", b).astype(np.float32)
+            k[t - 1, 0, 2] = nan
+            for i, a in enumerate(at):
+                v[a, 0, i] = (nan, inf, -inf, inf, nan)[i]
+                v[a, -1, 33 + i] = (inf, inf, nan, -inf, inf)[i]
+            for x, w in (("k", k), ("v", v)):
+                if mx:
+                    bt.put(x, pg, rows, w)
+                else:  # every value is a bf16 one
+                    getattr(bt, x)[pg, :, rows] = (w.view(np.uint32) >> 16).astype(np.uint16)
+        q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32))
+        got = f32(run_attn(bt, q, None, window)).astype(np.float64)
+        ne.device_check()
+        some = 0
+        for b, (n, t) in enumerate(lens):
+            k, v = bt.get("k", b), bt.get("v", b)
+            for i in range(n):
+                p = t - n + i
+                lo = max(0, p - window + 1) if window else 0
+                for h in range(Hq):
+                    row, kv = int(bt.starts[b]) + i, h // (Hq // Hkv)
+                    with np.errstate(invalid="ignore"):
+                        s = k[lo:p + 1, kv] @ f32(q[row, h]).astype(np.float64) / np.sqrt(D)
+                        e = np.exp(s - s.max()) if np.isfinite(s).all() else np.full_like(s, nan)
+                        e = (e / e.sum())[:, None]
+                        want = (e * v[lo:p + 1, kv]).sum(0)
+                        mag = (e * np.abs(v[lo:p + 1, kv])).sum(0)
+                    fine = np.isfinite(want)
+                    some += int((~fine).sum())
+                    g = got[row, h]
+                    assert np.array_equal(np.isnan(g), np.isnan(want)), (b, i, h)
+                    odd = ~fine & ~np.isnan(want)
+                    assert np.array_equal(g[odd], want[odd])
+                    bound = 2.0 ** -8 * np.abs(want[fine]) + (2.0 ** -8 + 2.0 ** -12) * mag[fine]
+                    assert (np.abs(g[fine] - want[fine]) <= bound + 1e-30).all(), (b, i, h)
+        assert some > 0
+
+
+def test_sinks_of_minus_infinity_are_none():
+    torch_cuda()
+    bt, q, sk = attn_case(False, 64, 8, 2, 16, [(1, 40), (2, 9)], seed=16)
+    d = bt.dev()
+    none = to_dev((np.full(8, -np.inf, np.float32).view(np.uint32) >> 16).astype(np.uint16))
+    out = to_dev(np.full(q.shape, 0x1357, np.uint16))
+    ne.paged_attn(d["kv"], to_dev(q), none, d["q_start"], d["kv_len"], d["table"], out, 8)
+    ref, mag = attention(bt, f32(q), None, 0)
+    check(to_host(out), ref, mag, 0x1357)
+    d["table"] = to_dev(np.full_like(bt.table, -1))
+    ne.paged_attn(d["kv"], to_dev(q), none, d["q_start"], d["kv_len"], d["table"], out, 8)
+    assert not to_host(out).any()
+    with pytest.raises(ne.NeonError):
+        ne.device_check()
+
+
 def test_attention_nothing_visible_gives_zero():
     """Every page of a sequence hidden, with and without sinks."""
     torch_cuda()
