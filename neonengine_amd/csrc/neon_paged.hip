@@ -336,16 +336,18 @@ struct PaWork {
   __device__ explicit PaWork(const PagedAttnArgs& a) : G(a.G), rG(1.0f / (float)a.G) {}
 };
 
-// Rows and length of a sequence as a kernel takes them (0 rows: none): FEW the
-// ones of up to a.few (token, head) rows per KV head, otherwise the longer ones.
+// A sequence as a kernel takes it: FEW the ones of up to a.few (token, head) rows
+// per KV head, otherwise the longer ones; n = 0: none.
+struct PaSeq {
+  int start, n, len;
+};
 template <bool FEW>
-__device__ __forceinline__ int pa_seq(const PagedAttnArgs& a, int b, int& start, int& len, bool flag) {
-  int n;
-  if (!paged_seq(a.r, a.kv.page_log2, b, start, n, len)) {
-    if (flag && len != 0) flag_dev_err(a.r.err, kDevErrPagedRows);
-    return 0;
-  }
-  return len > 0 && (n * a.G <= a.few) == FEW ? n : 0;
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
+  PaSeq q;
+  const int at = min(b, a.r.B - 1);
+  const bool ok = paged_seq(a.r, a.kv.page_log2, at, q.start, q.n, q.len);
+  q.n = ok && b < a.r.B && q.len > 0 && (q.n * a.G <= a.few) == FEW ? q.n : 0;
+  return q;
 }
 
 // n / d for 0 <= n < 2^31, d > 0, with r = 1 / d to fp32: the fp32 quotient of up
@@ -380,98 +382,110 @@ __device__ __forceinline__ int pa_span(const PagedAttnArgs& a, int G, int len) {
   return min(len, a.window + (R - 1) / G + ALIGN);
 }
 
+// Row tiles of a sequence, and its blocks in chunks of `chunk` (rc = 1 / chunk).
+template <int R>
+__device__ __forceinline__ int pa_tiles(const PaWork& w, const PaSeq& q) {
+  return (int)((unsigned)(q.n * w.G + R - 1) / R);
+}
+template <int R, int ALIGN>
+__device__ __forceinline__ int pa_chunks(const PagedAttnArgs& a, const PaWork& w, const PaSeq& q,
+                                         int chunk, float rc) {
+  return pa_div(pa_span<R, ALIGN>(a, w.G, q.len) + chunk - 1, chunk, rc);
+}
+
 // The work of block `idx` (of every KV head alike); false when there is none.
 // ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
 // multiples of 128); TARGET: blocks to aim at; PLACES: blocks that the chip holds
-// at once.
+// at once.  Lane = sequence, 64 at a time.
 template <bool FEW, int R, int ALIGN, int MINC, int TARGET, int PLACES, bool FIT>
-__device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool flag, PaWork& w) {
+__device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, bool report, PaWork& w) {
   const int lane = threadIdx.x & 63;
-  const int G = w.G;
-  const float rG = w.rG;
-  const int per = (a.r.B + 63) >> 6;  // consecutive sequences of a lane
-  const int b0 = lane * per, b1 = min(b0 + per, a.r.B);
-  float work = 0.0f;
-  int start0 = 0, n0 = 0, len0 = 0;  // the lane's first
-  for (int b = b0; b < b1; ++b) {
-    int start, len;
-    const int n = pa_seq<FEW>(a, b, start, len, flag);
-    if (b == b0) {
-      start0 = start;
-      n0 = n;
-      len0 = len;
+  const int turns = (a.r.B + 63) >> 6;
+  if (report)  // one block of the launch: the sequences that do not fit
+    for (int b = lane; b < a.r.B; b += 64) {
+      int start, n, len;
+      if (!paged_seq(a.r, a.kv.page_log2, b, start, n, len) && len != 0)
+        flag_dev_err(a.r.err, kDevErrPagedRows);
     }
-    work += (float)((n * G + R - 1) / R) * (float)pa_span<R, ALIGN>(a, G, len);
+  PaSeq q = pa_seq<FEW>(a, lane);  // the only ones of up to 64
+  float work = (float)pa_tiles<R>(w, q) * (float)pa_span<R, ALIGN>(a, w.G, q.len);
+#pragma unroll 4
+  for (int j = 1; j < turns; ++j) {
+    const PaSeq p = pa_seq<FEW>(a, 64 * j + lane);
+    work += (float)pa_tiles<R>(w, p) * (float)pa_span<R, ALIGN>(a, w.G, p.len);
   }
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
   int chunk = uni(max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
-  // blocks and slots of the sequences, in order.  Row starts that overlap (an
-  // error that no single sequence shows) can sum to more blocks than the grid
-  // has: the clamp lies above every grid and keeps the sums of 64 lanes in an int.
-  int blocks, slots, blocks_to;
-  for (int turn = 0;; ++turn) {
-    const float rc = 1.0f / (float)chunk;
-    blocks = 0;
-    slots = 0;
-    for (int b = b0; b < b1; ++b) {
-      int start, len = len0, n = n0;
-      if (b > b0) n = pa_seq<FEW>(a, b, start, len, false);
-      const int nc = pa_div(pa_span<R, ALIGN>(a, G, len) + chunk - 1, chunk, rc);
-      const int nb = (n * G + R - 1) / R * nc;
-      blocks = min(blocks + nb, kPaMaxBlocks);
-      slots += nc > 1 ? nb : 0;
-    }
-    blocks_to = pa_scan(blocks);
+  // The blocks of the sequences, in order, up to the one that idx lies in.  Row
+  // starts that overlap (an error that no single sequence shows) can sum to more
+  // blocks than the grid has: the clamp lies above every grid and keeps the sums
+  // in an int.
+  int at = 0, slot = 0, nc = 0;  // blocks and slots of the sequences before
+  float rc = 0.0f;
+  uint64_t mine = 0;
+  int j = 0;
+  for (int fit = 0;; ++fit) {
+    rc = 1.0f / (float)chunk;
+    nc = pa_chunks<R, ALIGN>(a, w, q, chunk, rc);
+    const int nb = min(pa_tiles<R>(w, q) * nc, kPaMaxBlocks);
+    const int to = pa_scan(nb), all = __builtin_amdgcn_readlane(to, 63);
     // FIT: a few more blocks than the chip holds cost a round of their own, so
     // larger chunks where that makes them fit (a unit is one block at least).
     // MXFP4, 4 sequences up to 131072 tokens 30.4 -> 29.3 us, 48 of heads of 128 25.8
     // -> 24.6; where the reads are the bound, small chunks even out the end better
     // (64 bf16 ones: 68 -> 73 us).
-    const float over = (float)__builtin_amdgcn_readlane(blocks_to, 63) * (float)a.kv.Hkv * (1.0f / PLACES);
-    if (!FIT || turn == 3 || per > 1 || over <= 1.0f || over > 2.0f) break;
-    chunk = uni((min((int)((float)chunk * over), (1 << 30) - 128) + 128) & ~127);
+    const float over = (float)all * (float)a.kv.Hkv * (1.0f / PLACES);
+    if (FIT && fit < 3 && turns == 1 && over > 1.0f && over <= 2.0f) {
+      chunk = uni((min((int)((float)chunk * over), (1 << 30) - 128) + 128) & ~127);
+      continue;
+    }
+    const int slots = nc > 1 ? nb : 0, slots_to = pa_scan(slots);
+    mine = __ballot(idx < to);
+    at = to - nb;
+    slot = slots_to - slots;
+    if (mine != 0) break;
+    const int all_slots = __builtin_amdgcn_readlane(slots_to, 63);
+    int before = all, slots_before = all_slots;
+    for (j = 1; j < turns; ++j) {
+      q = pa_seq<FEW>(a, 64 * j + lane);
+      nc = pa_chunks<R, ALIGN>(a, w, q, chunk, rc);
+      const int nb2 = min(pa_tiles<R>(w, q) * nc, kPaMaxBlocks), s2 = nc > 1 ? nb2 : 0;
+      const int to2 = pa_scan(nb2), st2 = pa_scan(s2);
+      mine = __ballot(idx - before < to2);
+      at = before + to2 - nb2;
+      slot = slots_before + st2 - s2;
+      if (mine != 0) break;
+      before += __builtin_amdgcn_readlane(to2, 63);
+      slots_before += __builtin_amdgcn_readlane(st2, 63);
+    }
+    break;
   }
-  const int slots_to = pa_scan(slots);
-  const uint64_t mine = __ballot(idx < blocks_to);
   if (mine == 0) return false;
   const int owner = __builtin_ctzll(mine);
-  // the owner lane's sequences, one by one
-  int at = __builtin_amdgcn_readlane(blocks_to - blocks, owner);
-  int slot = __builtin_amdgcn_readlane(slots_to - slots, owner);
-  int n = __builtin_amdgcn_readlane(n0, owner), len = __builtin_amdgcn_readlane(len0, owner);
-  int start = __builtin_amdgcn_readlane(start0, owner);  // of its first one
-  const float rc = 1.0f / (float)chunk;
-  for (int b = owner * per;; ++b) {
-    const int nc = pa_div(pa_span<R, ALIGN>(a, G, len) + chunk - 1, chunk, rc);
-    const int tiles = (n * G + R - 1) / R;
-    if (idx < at + tiles * nc) {
-      const int before = uni((idx - at) / nc);
-      // the last tiles first: they see the most keys
-      const int tile = tiles - 1 - before;
-      w.b = b; w.start = start; w.n = n; w.len = len;
-      w.c = uni(idx - at - before * nc);
-      w.row0 = uni(tile * R);
-      w.slot = uni(slot + tile * nc);
-      const int last = min(w.row0 + R, n * G) - 1;
-      w.tok0 = uni(pa_div(w.row0, G, rG));
-      w.tok1 = uni(pa_div(last, G, rG));
-      const int pos0 = len - n + w.tok0, pos1 = len - n + w.tok1;
-      w.lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
-      const int from = w.lo / ALIGN * ALIGN;
-      w.chunks = uni(pa_div(pos1 + 1 - from + chunk - 1, chunk, rc));
-      w.k0 = uni(from + w.c * chunk);
-      w.k1 = min(w.k0 + chunk, pos1 + 1);
-      return w.c < w.chunks;
-    }
-    at += tiles * nc;
-    slot += nc > 1 ? tiles * nc : 0;
-    if (b + 1 >= min(owner * per + per, a.r.B)) return false;
-    n = uni(pa_seq<FEW>(a, b + 1, start, len, false));
-    start = uni(start);
-    len = uni(len);
-  }
+  w.b = 64 * j + owner;
+  w.start = __builtin_amdgcn_readlane(q.start, owner);
+  w.n = __builtin_amdgcn_readlane(q.n, owner);
+  w.len = __builtin_amdgcn_readlane(q.len, owner);
+  nc = __builtin_amdgcn_readlane(nc, owner);
+  const int rel = idx - __builtin_amdgcn_readlane(at, owner);
+  const int tiles = (int)((unsigned)(w.n * w.G + R - 1) / R);
+  const int before = uni(rel / nc);
+  const int tile = tiles - 1 - before;  // the last tiles first: they see the most keys
+  w.c = rel - before * nc;
+  w.row0 = tile * R;
+  w.slot = __builtin_amdgcn_readlane(slot, owner) + tile * nc;
+  const int last = min(w.row0 + R, w.n * w.G) - 1;
+  w.tok0 = uni(pa_div(w.row0, w.G, w.rG));
+  w.tok1 = uni(pa_div(last, w.G, w.rG));
+  const int pos0 = w.len - w.n + w.tok0, pos1 = w.len - w.n + w.tok1;
+  w.lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  const int from = w.lo / ALIGN * ALIGN;
+  w.chunks = uni(pa_div(pos1 + 1 - from + chunk - 1, chunk, rc));
+  w.k0 = from + w.c * chunk;
+  w.k1 = min(w.k0 + chunk, pos1 + 1);
+  return w.c < w.chunks;
 }
 
 // How the kernels take a 16-key step of a wave: S^T = K Q^T with
