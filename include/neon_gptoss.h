@@ -471,11 +471,14 @@ typedef struct neon_paged_kv {
  *                    pages, and before those that a window reaches, are not
  *                    read.
  * Rows from q_start[B] to n_rows - 1 (padding) and the rows of a sequence with
- * kv_len 0 (a free place of the batch) are left as they are.  A sequence whose numbers do not fit (rows outside [0, n_rows], kv_len below its
- * rows or above max_pages * page_size or 2^30, a position >= n_pos) is left out, a page
- * id outside [0, n_pages) drops what it would hold (append, gather) or hides
- * its keys (attention), and neon_device_check then returns NEON_EINVAL.  (The
- * reference has no counterpart: it has no model code.) */
+ * kv_len 0 (a free place of the batch) are left as they are; n_rows 0 is no
+ * work, and the rows' buffers may then be NULL.  A sequence whose numbers do
+ * not fit (rows outside [0, n_rows], kv_len below its rows or above
+ * max_pages * page_size or 2^30, a position >= n_pos) is left out, a page id
+ * outside [0, n_pages) drops what it would hold (append, gather) or hides its
+ * keys (attention), and neon_device_check then returns NEON_EINVAL.  Outputs
+ * overlap no input and no pool.  (The reference has no counterpart: it has no
+ * model code.) */
 
 /* Rotates and appends: qkv rows [n_rows] of (Hq + 2 n_kv_heads) head_dim bf16,
  * `qkv_stride` elements apart (a multiple of 8; 16-byte aligned), hold the q,

@@ -169,7 +169,8 @@ def _check(status: int, ctx=None):
 
 def device_check(stream=None):
     """Synchronise and raise NeonError(NEON_EINVAL) if a kernel-level call on
-    the current device saw an expert id outside [0, E) since the last check."""
+    the current device saw an input out of range (an expert id outside [0, E); row
+    starts, lengths, page ids or sampling parameters) since the last check."""
     _check(lib().neon_device_check(stream))
 
 
@@ -438,15 +439,30 @@ def paged_kv(k, v, k_scales=None, v_scales=None) -> PagedKV:
     return PagedKV(k, v, k_scales, v_scales)
 
 
-def _arg(t, size, n, name, device):
+def _arg(t, size, n, name, device, real=None):
     """Device pointer of a contiguous tensor of at least n elements of this size
     on this device (its index), or ValueError: the library trusts the sizes that
-    the paged calls derive from other tensors."""
+    the paged calls derive from other tensors.  real: floating point or not."""
     if t.element_size() != size or t.numel() < n or t.get_device() != device or \
-            not t.is_contiguous():
-        raise ValueError(f"{name}: needs {n} contiguous elements of {size} bytes on device "
-                         f"{device}, has {tuple(t.shape)} of {t.element_size()} on {t.device}")
+            not t.is_contiguous() or (real is not None and t.is_floating_point() is not real):
+        raise ValueError(f"{name}: needs {n} contiguous elements of {size} bytes"
+                         f"{'' if real is None else ' (floats)' if real else ' (integers)'} on "
+                         f"device {device}, has {tuple(t.shape)} of {t.dtype} on {t.device}")
     return t.data_ptr()
+
+
+def _scratch(nbytes, stream, zero=False):
+    """_workspace, allocated (and zeroed) on the stream that the call runs on:
+    memory of another one could be in use there still, or handed out again
+    before the call is done."""
+    if stream is None:
+        return _workspace(nbytes, zero)
+    import torch
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream)) if int(stream) else \
+            torch.cuda.default_stream()
+    with torch.cuda.stream(stream):
+        return _workspace(nbytes, zero)
 
 
 def _rows(x, size, width, name, device):
@@ -456,16 +472,17 @@ def _rows(x, size, width, name, device):
         raise ValueError(f"{name}: rows of elements of {size} bytes on device {device}")
     n = x.shape[0]
     has = x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]
-    stride = has
+    stride = max(has, width)
     if not x.is_contiguous():
         inner = (1,) if x.dim() == 2 else (x.shape[2], 1)
         if any(s != w and k > 1 for s, w, k in zip(x.stride()[1:], inner, x.shape[1:])):
             raise ValueError(f"{name}: each row must be contiguous")
         if n > 1:
             stride = x.stride(0)
-    if n and has < width:
-        raise ValueError(f"{name}: rows of {width} elements, has {has}")
-    return x.data_ptr(), n, max(stride, width)
+    if n and (has < width or stride < width):
+        raise ValueError(f"{name}: rows of {width} elements that do not overlap, has {has}, "
+                         f"{stride} apart")
+    return x.data_ptr(), n, stride
 
 
 def _on_current(device):
@@ -485,11 +502,11 @@ def _batch(kv, q_start, kv_len, page_table, n_rows):
     if kv_len.numel() != B:
         raise ValueError("page_table: one row per sequence of kv_len")
     if q_start is not None:
-        q_start = _arg(q_start, 4, B + 1, "q_start", device)
+        q_start = _arg(q_start, 4, B + 1, "q_start", device, False)
     elif n_rows != B:
         raise ValueError("without q_start there is one row per sequence")
-    return (q_start, _arg(kv_len, 4, B, "kv_len", device),
-            _arg(page_table, 4, 1, "page_table", device), max_pages, B)
+    return (q_start, _arg(kv_len, 4, B, "kv_len", device, False),
+            _arg(page_table, 4, 1, "page_table", device, False), max_pages, B)
 
 
 def paged_append(kv, qkv, table, q_start, kv_len, page_table, q_out, Hq, stream=None):
@@ -505,7 +522,7 @@ def paged_append(kv, qkv, table, q_start, kv_len, page_table, q_out, Hq, stream=
         if table.dim() != 3 or table.shape[0] != 2 or table.shape[2] != D // 2:
             raise ValueError("table: [2][n_pos][head_dim / 2]")
         n_pos = table.shape[1]
-        table = _arg(table, 4, n_pos * D, "table", device)
+        table = _arg(table, 4, n_pos * D, "table", device, True)
     _check(lib().neon_paged_append(kv.ref, rows, stride, table, n_pos, q_start, kv_len, page_table,
                                    max_pages, q_out, n, B, Hq, _stream(stream)))
 
@@ -541,9 +558,9 @@ def paged_attn(kv, q, sinks, q_start, kv_len, page_table, out, Hq, window=0, str
     if workspace is None or counters is None:
         wb, cb = paged_attn_workspace(n, B, Hq, kv.n_kv_heads, D)
         if workspace is None:
-            workspace = _workspace(wb)
+            workspace = _scratch(wb, stream)
         if counters is None:
-            counters = _workspace(cb, zero=True)
+            counters = _scratch(cb, stream, zero=True)
     _check(lib().neon_paged_attn(kv.ref, rows, stride, sinks, q_start, kv_len, page_table,
                                  max_pages, _arg(out, 2, n * Hq * D, "out", device), n, B, Hq,
                                  window, _arg(workspace, workspace.element_size(), 0, "workspace",
@@ -568,14 +585,14 @@ def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, mi
     V = logits.shape[1]
     rows, B, stride = _rows(logits, 4, V, "logits", device)
     if workspace is None:
-        workspace = _workspace(sample_rows_workspace(B, V))
+        workspace = _scratch(sample_rows_workspace(B, V), stream)
 
-    def opt(t, name):
-        return None if t is None else _arg(t, 4, B, name, device)
+    def opt(t, name, real=True):
+        return None if t is None else _arg(t, 4, B, name, device, real)
 
     _check(lib().neon_sample_rows(rows, stride, B, V, opt(temperature, "temperature"),
-                                  opt(top_k, "top_k"), opt(top_p, "top_p"), opt(min_p, "min_p"),
-                                  _arg(u, 4, B, "u", device), _arg(out_ids, 4, B, "out_ids", device),
+                                  opt(top_k, "top_k", False), opt(top_p, "top_p"), opt(min_p, "min_p"),
+                                  opt(u, "u"), opt(out_ids, "out_ids", False),
                                   _arg(workspace, workspace.element_size(), 0, "workspace", device),
                                   workspace.nbytes, _stream(stream)))
 

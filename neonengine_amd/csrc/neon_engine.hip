@@ -2288,6 +2288,7 @@ extern "C" neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t
   const char* why;
   if (!paged_args(kv, q_start, kv_len, page_table, max_pages, n_rows, B, c, r, why))
     KFAIL(NEON_EINVAL, "neon_paged_append: %s", why);
+  if (n_rows == 0) return NEON_OK;  // its buffers may be NULL
   if (!qkv || Hq < 0 || Hq > 65535 || (Hq > 0 && !q_out))
     KFAIL(NEON_EINVAL, "neon_paged_append: null pointer or Hq=%d", Hq);
   if (qkv_stride < (int64_t)(Hq + 2 * c.Hkv) * c.D || qkv_stride % 8 || !aligned16(qkv) ||
@@ -2295,7 +2296,6 @@ extern "C" neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t
     KFAIL(NEON_EINVAL, "neon_paged_append: rows must be 16-byte aligned, a multiple of 8 elements "
           "and at least (Hq + 2 n_kv_heads) head_dim apart");
   if (table && n_pos < 1) KFAIL(NEON_EINVAL, "neon_paged_append: n_pos=%d", n_pos);
-  if (n_rows == 0) return NEON_OK;
   r.err = device_status_word();
   launch_paged_append(c, r, qkv, qkv_stride, table,
                       table ? table + (size_t)n_pos * (c.D / 2) : nullptr, n_pos, q_out, Hq,
@@ -2312,9 +2312,9 @@ extern "C" neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t*
   const char* why;
   if (!paged_args(kv, q_start, kv_len, page_table, max_pages, n_rows, B, c, r, why))
     KFAIL(NEON_EINVAL, "neon_paged_gather: %s", why);
+  if (n_rows == 0) return NEON_OK;
   if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
     KFAIL(NEON_EINVAL, "neon_paged_gather: k_out and v_out must be given, 16-byte aligned");
-  if (n_rows == 0) return NEON_OK;
   r.err = device_status_word();
   launch_paged_gather(c, r, k_out, v_out, S(stream));
   KLAUNCHED();
@@ -2352,6 +2352,7 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
   if (!paged_attn_shape_ok(n_rows, B, Hq, a.kv.Hkv, a.kv.D))
     KFAIL(NEON_EINVAL, "neon_paged_attn: Hq=%d must be a multiple of n_kv_heads=%d, at most 64 "
           "per KV head, and n_rows=%d fit a launch", Hq, a.kv.Hkv, n_rows);
+  if (n_rows == 0) return NEON_OK;
   if (!q || !out || !aligned16(q) || !aligned16(out) || q_stride % 8 ||
       q_stride < (int64_t)Hq * a.kv.D || window < 0)
     KFAIL(NEON_EINVAL, "neon_paged_attn: q and out must be given, 16-byte aligned, q rows a "
@@ -2364,7 +2365,6 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
   if (needc > 0 && (!counters || counter_bytes < needc || !aligned16(counters)))
     KFAIL(NEON_EINVAL, "neon_paged_attn: counters of %zu bytes, %zu needed (16-byte aligned)",
           counter_bytes, needc);
-  if (n_rows == 0) return NEON_OK;
   a.r.err = device_status_word();
   a.q = q; a.q_stride = q_stride; a.sinks = sinks; a.out = out; a.Hq = Hq; a.window = window;
   a.part = (float*)workspace; a.arrive = counters;

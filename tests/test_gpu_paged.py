@@ -645,3 +645,68 @@ def test_wrapper_refusals():
         with pytest.raises(ne.NeonError):
             ne.paged_attn(d["kv"], q, None, None, *args, out, 4,
                           workspace=torch.empty(1, dtype=torch.uint8, device="cuda"))
+
+
+def test_wrapper_takes_no_rows():
+    rng = np.random.default_rng(2)
+    bt = Batch(rng, [(0, 5), (0, 0)], 16, 2, 64, False, q_start=True).fill(rng)
+    d = bt.dev()
+    args = (d["q_start"], d["kv_len"], d["table"])
+    qkv, q, kv = (empty_dev((0, h, 64), np.uint16) for h in (8, 4, 2))
+    ne.paged_append(d["kv"], qkv, None, *args, q, 4)
+    ne.paged_gather(d["kv"], *args, kv, kv)
+    ne.paged_attn(d["kv"], q, None, *args, q, 4)
+    ne.device_check()
+
+
+def test_wrapper_refuses_overlapping_rows_and_other_kinds():
+    torch = torch_cuda()
+    rng = np.random.default_rng(1)
+    bt = Batch(rng, [(1, 5), (1, 5)], 16, 2, 64, False, q_start=False).fill(rng)
+    d = bt.dev()
+    q = empty_dev((2, 4, 64), np.uint16)
+    args = (d["kv_len"], d["table"])
+    logits, u = torch.zeros((2, 99), device="cuda"), torch.zeros(2, device="cuda")
+    ids = torch.zeros(2, dtype=torch.int32, device="cuda")
+    ne.sample_rows(logits, u, ids)
+    for call in (
+        lambda: ne.paged_attn(d["kv"], q[:1].expand(2, 4, 64), None, None, *args, q, 4),
+        lambda: ne.paged_attn(d["kv"], q, None, None, d["kv_len"].float(), d["table"], q, 4),
+        lambda: ne.paged_attn(d["kv"], q, None, None, d["kv_len"], d["table"].float(), q, 4),
+        lambda: ne.sample_rows(logits[:1].expand(2, 99), u, ids),
+        lambda: ne.sample_rows(logits, u, u),
+        lambda: ne.sample_rows(logits, ids, ids),
+        lambda: ne.sample_rows(logits, u, ids, temperature=ids),
+        lambda: ne.sample_rows(logits, u, ids, top_k=u),
+        lambda: ne.sample_rows(logits, u[0].expand(2), ids),
+    ):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_own_scratch_belongs_to_the_stream_of_the_call(handle):
+    """Calls without a workspace, on a stream that is behind, while the current
+    stream takes and writes memory of the same size: what a call allocates must
+    not be that memory."""
+    torch = torch_cuda()
+    bt, q, sk = attn_case(False, 64, 64, 8, 64, [(1, 3000), (1, 100)], seed=30)
+    d, qd, skd = bt.dev(), to_dev(q), to_dev(bf16(sk))
+    outs = [empty_dev(q.shape, np.uint16) for _ in range(8)]
+    side = torch.cuda.Stream()
+    big = torch.randn((4096, 4096), device="cuda")
+    wb, cb = ne.paged_attn_workspace(2, 2, 64, 8, 64)
+    ne.paged_attn(d["kv"], qd, skd, None, d["kv_len"], d["table"], outs[0], 64)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            big = big @ big * 1e-3
+    for out in outs:
+        ne.paged_attn(d["kv"], qd, skd, None, d["kv_len"], d["table"], out, 64,
+                      stream=side.cuda_stream if handle else side)
+        junk = [torch.full((max(n, 1),), 0x7F, dtype=torch.uint8, device="cuda") for n in (wb, cb)]
+    torch.cuda.synchronize()
+    del junk
+    ref, mag = attention(bt, f32(q), sk, 0)
+    for out in outs:
+        check(to_host(out), ref, mag, 0)

@@ -168,3 +168,11 @@ def test_plain_quantiser_is_nearest():
 def test_bf16_rounding_helper():
     x = np.array([1.0, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, -2.5], np.float32)
     assert f32(bf16(x)).tolist() == [1.0, 1.0, 1 + 2.0 ** -6, -2.5]
+
+
+def test_no_rows_need_no_buffers():
+    """A tensor of no rows has no memory."""
+    assert append(n_rows=0, qkv=None, q_out=None) == ne.NEON_OK
+    assert gather(n_rows=0, k_out=None, v_out=None) == ne.NEON_OK
+    assert attn(n_rows=0, q=None, out=None, ws=None, wb=0, cnt=None, cb=0) == ne.NEON_OK
+    assert attn(n_rows=0, page_size=24) == ne.NEON_EINVAL
