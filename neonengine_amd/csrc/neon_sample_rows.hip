@@ -155,6 +155,22 @@ __device__ __forceinline__ u64 sr_wave_max(u64 v) {
   if constexpr (J > 1) return sr_wave_max<J / 2>(v);
   else return v;
 }
+// v plus that of the lane that CTRL names, where ROWS has the lane's row (DPP)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 sr_add_from(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return v + ((u64)hi << 32 | lo);
+}
+// sum of the lanes up to this one
+__device__ __forceinline__ u64 sr_wave_scan(u64 v) {
+  v = sr_add_from<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = sr_add_from<0x112, 0xF>(v);
+  v = sr_add_from<0x114, 0xF>(v);
+  v = sr_add_from<0x118, 0xF>(v);
+  v = sr_add_from<0x142, 0xA>(v);  // a row's last lane into the next row
+  return sr_add_from<0x143, 0xC>(v);  // lane 31 into the upper half
+}
 __device__ __forceinline__ u64 sr_block_sum(u64 v, u64* red) {
   v = sr_wave_sum(v);
   __syncthreads();
@@ -176,12 +192,7 @@ __device__ __forceinline__ u64 sr_block_max(u64 v, u64* red) {
 }
 // sum of the threads before this one
 __device__ __forceinline__ u64 sr_block_before(u64 v, u64* red) {
-  u64 x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 y = __shfl_up(x, o);
-    if ((int)(threadIdx.x & 63) >= o) x += y;
-  }
+  u64 x = sr_wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = x;
   __syncthreads();
@@ -249,37 +260,34 @@ __device__ __forceinline__ int sr_best_id(u64 best) { return (int)~(uint32_t)bes
 // fn(logits, index of the first) for tokens [i0, i1), i0 a multiple of kSrPart: a
 // thread's eight of a part are 512 apart.  The next part's are requested before
 // these are used; the last, incomplete part has minus infinity past i1.
+// The first part (`first`) may be requested before work that its use waits for.
+struct SrPart {
+  float v[8];
+};
+__device__ __forceinline__ SrPart sr_part(const float* l, int i, int i1) {
+  SrPart p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p.v[j] = l[min(i + (int)threadIdx.x + j * kSrThreads, i1 - 1)];
+  return p;
+}
 template <class F>
-__device__ __forceinline__ void sr_tokens(const float* l, int i0, int i1, F fn) {
-  const int tid = threadIdx.x, full = i0 + (i1 - i0) / kSrPart * kSrPart;
-  if (full > i0) {
-    float next[8];
+__device__ __forceinline__ void sr_tokens(const float* l, int i0, int i1, SrPart next, F fn) {
+  const int tid = threadIdx.x;
+  for (int i = i0; i < i1; i += kSrPart) {
+    SrPart p = next;
+    if (i + kSrPart < i1) next = sr_part(l, i + kSrPart, i1);
+    if (i + kSrPart > i1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) next[j] = (l + i0 + j * kSrThreads)[tid];
-    for (int i = i0; i < full; i += kSrPart) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = next[j];
-      const float* p = l + min(i + kSrPart, full - kSrPart);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) next[j] = (p + j * kSrThreads)[tid];
-      fn(v, i + tid);
+      for (int j = 0; j < 8; ++j) p.v[j] = i + tid + j * kSrThreads < i1 ? p.v[j] : -INFINITY;
     }
-  }
-  if (full < i1) {
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = l[min(full + tid + j * kSrThreads, i1 - 1)];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = full + tid + j * kSrThreads < i1 ? v[j] : -INFINITY;
-    fn(v, full + tid);
+    fn(p.v, i + tid);
   }
 }
 
 __device__ __forceinline__ u64 sr_chunk_max(const float* l, int i0, int i1, u64* red) {
   float best = -INFINITY;  // of equal ones the first; a NaN is never larger
   int at = i0;
-  sr_tokens(l, i0, i1, [&](const float (&v)[8], int i) {
+  sr_tokens(l, i0, i1, sr_part(l, i0, i1), [&](const float (&v)[8], int i) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       at = v[j] > best ? i + j * kSrThreads : at;
@@ -292,11 +300,11 @@ __device__ __forceinline__ u64 sr_chunk_max(const float* l, int i0, int i1, u64*
 // counts (for top_k) and masses (for top_p) of the chunk's bins into sh.count /
 // sh.mass
 template <class SH>
-__device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, SH& sh) {
+__device__ __forceinline__ void sr_chunk_hist(const SrRow& r, int i0, int i1, const SrPart& first, SH& sh) {
   sh.mass[threadIdx.x] = 0;
   sh.count[threadIdx.x] = 0;
   __syncthreads();
-  sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int) {
+  sr_tokens(r.l, i0, i1, first, [&](const float (&v)[8], int) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int bin = sr_bin(r, v[j]);
@@ -360,7 +368,7 @@ __device__ __forceinline__ bool sr_candidate(const SrFound& f, int bin) {
 // of kSrPart) into sh.mass[0 ..], thread = part for the result; the candidates
 // into sh.list (as many as fit; sh.s_int[0] counts all).
 __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int i0, int i1,
-                                          SrShared& sh) {
+                                          const SrPart& first, SrShared& sh) {
   __syncthreads();
   if (threadIdx.x == 0) sh.s_int[0] = 0;
   if (threadIdx.x < kSrMaxParts) sh.mass[threadIdx.x] = 0;
@@ -377,7 +385,7 @@ __device__ __forceinline__ u64 sr_collect(const SrRow& r, const SrFound& f, int 
   const float from = keep > 0 ? edge(keep, -1.0) : INFINITY;
   const float c_from = c_hi >= 0 ? edge(c_hi + 1, -1.0) : INFINITY;
   const float c_to = c_lo > 0 ? edge(c_lo, 1.0) : INFINITY;
-  sr_tokens(r.l, i0, i1, [&](const float (&v)[8], int i) {
+  sr_tokens(r.l, i0, i1, first, [&](const float (&v)[8], int i) {
     // gathered first: a wave pays an exponential for all its lanes if one needs it
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int n = 0;
@@ -487,12 +495,7 @@ __device__ __forceinline__ u64 sr_select(const SrRow& r, SrShared& sh, int n, in
         v[j] = MASS ? (d < digits ? sh.mass[d] : 0) : c[j];
         sum += v[j];
       }
-      u64 x = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(x, o);
-        if (tid >= o) x += y;
-      }
+      const u64 x = sr_wave_scan(sum);
       u64 at = run + x - sum;
       // the first digit that reaches the goal, else the last that is there
       int hit = -1, last = -1;
@@ -528,27 +531,34 @@ __device__ __forceinline__ u64 sr_select(const SrRow& r, SrShared& sh, int n, in
   }
 }
 
-// One compare-exchange of a bitonic sort, descending: runs of K, distance J.
-template <int K, int J>
-__device__ __forceinline__ void sr_sort_step(u64& x, u64* buf) {
-  const int tid = threadIdx.x;
-  u64 y;
-  if constexpr (J < 64) {
-    y = sr_xor_lane<J>(x);
-  } else {
-    __syncthreads();
-    buf[tid] = x;
-    __syncthreads();
-    y = buf[tid ^ J];
+// Bitonic sort, descending, of the threads' x; those from n on hold 0.  Loops:
+// unrolled, the 45 steps are fetched once each, which takes longer than they do.
+template <int J>
+__device__ __forceinline__ u64 sr_sort_lanes(u64 x, int K) {
+  if (J < K) {
+    const u64 y = sr_xor_lane<J>(x);
+    const bool larger = ((threadIdx.x & K) == 0) == ((threadIdx.x & J) == 0);
+    x = (x > y) == larger ? x : y;
   }
-  const bool larger = ((tid & K) == 0) == ((tid & J) == 0);
-  x = (x > y) == larger ? x : y;
-  if constexpr (J > 1) sr_sort_step<K, J / 2>(x, buf);
+  if constexpr (J > 1) return sr_sort_lanes<J / 2>(x, K);
+  else return x;
 }
-template <int K>
-__device__ __forceinline__ void sr_sort(u64& x, u64* buf) {
-  sr_sort_step<K, K / 2>(x, buf);
-  if constexpr (K < kSrThreads) sr_sort<2 * K>(x, buf);
+__device__ __forceinline__ u64 sr_sort(u64 x, u64* buf, int n) {
+  const int tid = threadIdx.x;
+#pragma unroll 1
+  for (int K = 2; K < 2 * n && K <= kSrThreads; K *= 2) {  // runs of K, distance J
+#pragma unroll 1
+    for (int J = K / 2; J >= 64; J /= 2) {
+      __syncthreads();
+      buf[tid] = x;
+      __syncthreads();
+      const u64 y = buf[tid ^ J];
+      const bool larger = ((tid & K) == 0) == ((tid & J) == 0);
+      x = (x > y) == larger ? x : y;
+    }
+    x = sr_sort_lanes<32>(x, K);
+  }
+  return x;
 }
 
 // sr_cut for up to one candidate per thread: sorted, the places are positions.
@@ -558,7 +568,7 @@ __device__ __forceinline__ u64 sr_cut_sorted(const SrRow& r, SrShared& sh, int n
   const int tid = threadIdx.x;
   const SrFound f = sh.found;
   u64 x = tid < n ? sh.list[tid] : 0;
-  sr_sort<2>(x, sh.list);
+  x = sr_sort(x, sh.list, n);
   __syncthreads();
   sh.list[tid] = x;
   const bool has = tid < n;
@@ -654,13 +664,7 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
   __syncthreads();
   if (tid < 64) {
     const u64 own = sh.mass[tid];
-    u64 x = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 y = __shfl_up(x, o);
-      if (tid >= o) x += y;
-    }
-    x += before;
+    const u64 x = sr_wave_scan(own) + before;
     const u64 hit = __ballot(own > 0 && (double)x > target);
     if (tid == (hit ? __builtin_ctzll(hit) : 0)) {
       sh.s_int[1] = hit ? tid : -1;
@@ -674,12 +678,7 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
     u64 own = m[0];
 #pragma unroll
     for (int q = 1; q < 8; ++q) own = j == q ? m[q] : own;
-    u64 x = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
+    const u64 x = sr_wave_scan(own);
     const u64 hit = __ballot(own > 0 && (double)(x + sh.s_u64[0]) > target);
     if (hit && lane == __builtin_ctzll(hit)) sh.s_int[2] = i0 + tid + j * kSrThreads;
   }
@@ -737,12 +736,12 @@ __device__ __forceinline__ u64 sr_part_mass(const SrRow& r, SrShared& sh, u64 cu
 
 // A row's place in the workspace: C chunks.
 struct SrSpace {
-  u64 *best, *sure, *list, *found;  // [C], [parts], [kSrCap], [8]
-  u64 *mass, *count;                // [bins]
-  int32_t* n;                               // arrivals of the two launches, candidates
+  u64 *best, *sure, *list;  // [C], [parts], [kSrCap]
+  u64 *mass, *count;        // [kSrBins]
+  int32_t* n;               // candidates, arrivals
 };
 __host__ __device__ inline size_t sr_space_bytes(int C, int V) {
-  const size_t b = (size_t)C * 8 + (size_t)((V + kSrPart - 1) / kSrPart) * 8 + kSrCap * 8 + 64 + 64 +
+  const size_t b = (size_t)C * 8 + (size_t)((V + kSrPart - 1) / kSrPart) * 8 + kSrCap * 8 + 64 +
                    kSrBins * 16;
   return (b + 255) & ~(size_t)255;
 }
@@ -753,9 +752,8 @@ __device__ __forceinline__ SrSpace sr_space(const SampleRowsArgs& a, int b) {
   s.best = p;
   s.sure = p + C;
   s.list = s.sure + (a.V + kSrPart - 1) / kSrPart;
-  s.found = s.list + kSrCap;
-  s.n = reinterpret_cast<int32_t*>(s.found + 8);
-  s.mass = s.found + 16;
+  s.n = reinterpret_cast<int32_t*>(s.list + kSrCap);
+  s.mass = s.list + kSrCap + 8;
   s.count = s.mass + kSrBins;
   return s;
 }
@@ -768,7 +766,7 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_max(SampleRowsArgs a) {
                                 min((c + 1) * a.chunk, a.V), red);
   if (threadIdx.x == 0) s.best[c] = best;
   if (c == 0) {  // for the next launches
-    if (threadIdx.x < 16) s.n[threadIdx.x] = 0;
+    if (threadIdx.x < 2) s.n[threadIdx.x] = 0;
     s.mass[threadIdx.x] = 0;
     s.count[threadIdx.x] = 0;
   }
@@ -796,64 +794,48 @@ __device__ __forceinline__ bool sr_begin(const SampleRowsArgs& a, const SrSpace&
 __global__ __launch_bounds__(kSrThreads) void k_sr_hist(SampleRowsArgs a) {
   __shared__ SrHistShared sh;
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int i0 = c * a.chunk, i1 = min(i0 + a.chunk, a.V);
   const SrSpace s = sr_space(a, b);
+  const SrPart first = sr_part(a.logits + (int64_t)b * a.stride, i0, i1);
   SrRow r;
   if (!sr_begin(a, s, b, r, sh, false)) return;
   if (r.k == 0 && r.p >= 1.0) return;  // every bin is kept
-  sr_chunk_hist(r, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
+  sr_chunk_hist(r, i0, i1, first, sh);
   // integers: no order changes the sums
   if (sh.mass[tid] > 0)
     __hip_atomic_fetch_add(s.mass + tid, sh.mass[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (sh.count[tid] > 0)
     __hip_atomic_fetch_add(s.count + tid, (u64)sh.count[tid], __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
-  __syncthreads();
-  if (tid == 0)
-    sh.s_int[3] = __hip_atomic_fetch_add(s.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (sh.s_int[3] != a.chunks - 1) return;
-  const u64 count = sr_get(s.count + tid), mass = sr_get(s.mass + tid);
-  sr_scan(r, count, mass, sh);
-  if (tid == 0) {  // read by the next launch
-    const SrFound& f = sh.found;
-    s.found[0] = (u64)f.lo | (u64)f.hi << 16 | (u64)f.bin_k << 32;
-    s.found[1] = f.base;
-    s.found[2] = f.before_k;
-    s.found[3] = f.mass_k;
-    s.found[4] = f.need_k;
+}
+
+__device__ __forceinline__ void sr_no_cut(SrFound& f) {
+  if (threadIdx.x == 0) {
+    f.lo = f.hi = f.bin_k = kSrBins;
+    f.base = f.before_k = f.mass_k = f.need_k = 0;
   }
+  __syncthreads();
 }
 
 __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   __shared__ SrShared sh;
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int i0 = c * a.chunk, i1 = min(i0 + a.chunk, a.V);
   const SrSpace s = sr_space(a, b);
+  const SrPart first = sr_part(a.logits + (int64_t)b * a.stride, i0, i1);
+  const u64 count = s.count[tid], mass = s.mass[tid];
   SrRow r;
   if (!sr_begin(a, s, b, r, sh, true)) return;
-  if (tid == 0) {
-    SrFound f;
-    f.lo = f.hi = f.bin_k = kSrBins;
-    f.base = f.before_k = f.mass_k = f.need_k = 0;
-    if (r.k > 0 || r.p < 1.0) {
-      const u64 x = s.found[0];
-      f.lo = (int)(x & 0xFFFF);
-      f.hi = (int)(x >> 16 & 0xFFFF);
-      f.bin_k = (int)(x >> 32);
-      f.base = s.found[1];
-      f.before_k = s.found[2];
-      f.mass_k = s.found[3];
-      f.need_k = s.found[4];
-    }
-    sh.found = f;
-  }
-  __syncthreads();
-  const u64 sure = sr_collect(r, sh.found, c * a.chunk, min((c + 1) * a.chunk, a.V), sh);
+  // every block for itself: an arrival in k_sr_hist and a scan by the row's last
+  // block there take 3 us more
+  if (r.k > 0 || r.p < 1.0) sr_scan(r, count, mass, sh);
+  else sr_no_cut(sh.found);
+  const u64 sure = sr_collect(r, sh.found, i0, i1, first, sh);
   const int mine = sh.s_int[0];
   const int part = c * (a.chunk / kSrPart) + tid;
   if (tid < a.chunk / kSrPart && (int64_t)part * kSrPart < a.V) sr_put(s.sure + part, sure);
   if (tid == 0)
-    sh.s_int[1] = mine > 0 ? __hip_atomic_fetch_add(s.n + 2, mine, __ATOMIC_RELAXED,
+    sh.s_int[1] = mine > 0 ? __hip_atomic_fetch_add(s.n, mine, __ATOMIC_RELAXED,
                                                     __HIP_MEMORY_SCOPE_AGENT) : 0;
   __syncthreads();
   const int at = sh.s_int[1];
@@ -866,14 +848,17 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   }
   __syncthreads();
   if (sh.s_int[3] != a.chunks - 1) return;
-  // the row's last block
-  const int n = __hip_atomic_load(s.n + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int j = tid; j < min(n, kSrCap); j += kSrThreads) sh.list[j] = sr_get(s.list + j);
+  // the row's last block; what it reads is requested together
+  const int parts = (a.V + kSrPart - 1) / kSrPart;
+  const int n = __hip_atomic_load(s.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const u64 place = sr_get(s.list + tid), part_sure = tid < parts ? sr_get(s.sure + tid) : 0;
+  if (tid < n) sh.list[tid] = place;
+  for (int j = tid + kSrThreads; j < min(n, kSrCap); j += kSrThreads) sh.list[j] = sr_get(s.list + j);
   __syncthreads();
   const u64 cut = sr_cut(r, sh, n);
-  const int parts = (a.V + kSrPart - 1) / kSrPart;
   const int id = sr_draw(r, sh, cut, [&](int p0) {
-    return sr_part_mass(r, sh, cut, n, p0, p0 + tid < parts ? sr_get(s.sure + p0 + tid) : 0);
+    const u64 own = p0 == 0 ? part_sure : p0 + tid < parts ? sr_get(s.sure + p0 + tid) : 0;
+    return sr_part_mass(r, sh, cut, n, p0, own);
   });
   if (tid == 0) a.ids[b] = id;
 }
@@ -896,18 +881,13 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_one(SampleRowsArgs a) {
     return;
   }
   u64 cut = 0;
-  if (tid == 0) {
-    SrFound f;
-    f.lo = f.hi = f.bin_k = kSrBins;
-    f.base = f.before_k = f.mass_k = f.need_k = 0;
-    sh.found = f;
-  }
-  __syncthreads();
   if (r.k > 0 || r.p < 1.0) {
-    sr_chunk_hist(r, 0, a.V, sh);
+    sr_chunk_hist(r, 0, a.V, sr_part(r.l, 0, a.V), sh);
     sr_scan(r, sh.count[tid], sh.mass[tid], sh);
+  } else {
+    sr_no_cut(sh.found);
   }
-  const u64 sure = sr_collect(r, sh.found, 0, a.V, sh);
+  const u64 sure = sr_collect(r, sh.found, 0, a.V, sr_part(r.l, 0, a.V), sh);
   const int n = sh.s_int[0];
   if (r.k > 0 || r.p < 1.0) cut = sr_cut(r, sh, n);
   const int id = sr_draw(r, sh, cut, [&](int p0) { return sr_part_mass(r, sh, cut, n, p0, sure); });

@@ -1,9 +1,8 @@
 """CPU check of the arrivals of the paged attention kernels and of the per-row
-sampling kernels in their compiled gfx950 assembly: what a block leaves for the
+sampling kernel in their compiled gfx950 assembly: what a block leaves for the
 last one has completed, for every wave of it, before its arrival is counted.  The
-attention kernels store partials at agent scope; the sampling kernels add to a
-histogram (k_sr_hist) and list candidates (k_sr_pick) with agent-scope atomics and
-stores."""
+attention kernels store partials at agent scope; k_sr_pick lists candidates and
+masses with agent-scope stores."""
 import os
 import re
 import shutil
@@ -81,7 +80,6 @@ def test_paged_attention_arrival_order(asm_of, kernel, form):
     assert problems == [], problems[:4]
 
 
-@pytest.mark.parametrize("kernel", ["k_sr_hist", "k_sr_pick"])
-def test_sample_rows_arrival_order(asm_of, kernel):
-    problems = order_problems(kernel_asm(asm_of("neon_sample_rows"), kernel))
+def test_sample_rows_arrival_order(asm_of):
+    problems = order_problems(kernel_asm(asm_of("neon_sample_rows"), "k_sr_pick"))
     assert problems == [], problems
