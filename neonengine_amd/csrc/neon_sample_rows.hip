@@ -190,14 +190,24 @@ __device__ __forceinline__ u64 sr_block_max(u64 v, u64* red) {
   for (int w = 0; w < kSrThreads / 64; ++w) v = red[w] > v ? red[w] : v;
   return v;
 }
-// sum of the threads before this one
-__device__ __forceinline__ u64 sr_block_before(u64 v, u64* red) {
+// sum of the threads before this one; `all`: of the block's
+__device__ __forceinline__ u64 sr_block_before(u64 v, u64* red, u64& all) {
   u64 x = sr_wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = x;
   __syncthreads();
-  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) x += red[w];
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kSrThreads / 64; ++w) {
+    const u64 y = red[w];
+    all += y;
+    if (w < (int)(threadIdx.x >> 6)) x += y;
+  }
   return x - v;
+}
+__device__ __forceinline__ u64 sr_block_before(u64 v, u64* red) {
+  u64 all;
+  return sr_block_before(v, red, all);
 }
 
 // What the scan of the bins finds.
@@ -545,6 +555,7 @@ __device__ __forceinline__ u64 sr_sort_lanes(u64 x, int K) {
 }
 __device__ __forceinline__ u64 sr_sort(u64 x, u64* buf, int n) {
   const int tid = threadIdx.x;
+  const bool in = (tid & ~63) < 1 << (32 - __builtin_clz(max(n - 1, 1)));
 #pragma unroll 1
   for (int K = 2; K < 2 * n && K <= kSrThreads; K *= 2) {  // runs of K, distance J
 #pragma unroll 1
@@ -556,7 +567,7 @@ __device__ __forceinline__ u64 sr_sort(u64 x, u64* buf, int n) {
       const bool larger = ((tid & K) == 0) == ((tid & J) == 0);
       x = (x > y) == larger ? x : y;
     }
-    x = sr_sort_lanes<32>(x, K);
+    if (in) x = sr_sort_lanes<32>(x, K);  // the other waves hold zeros only
   }
   return x;
 }
@@ -691,16 +702,20 @@ __device__ __forceinline__ int sr_walk(const SrRow& r, SrShared& sh, u64 cut, in
 template <class F>
 __device__ __forceinline__ int sr_draw(const SrRow& r, SrShared& sh, u64 cut, F part_mass) {
   const int tid = threadIdx.x, parts = (r.V + kSrPart - 1) / kSrPart;
-  u64 total = 0, own = 0;
+  u64 total = 0, own = 0, run = 0, all = 0;
   for (int p0 = 0; p0 < parts; p0 += kSrThreads) {
     own = part_mass(p0);
-    total += sr_block_sum(own, sh.red);
+    run = sr_block_before(own, sh.red, all);
+    total += all;
   }
   const double target = r.u * (double)total;
   u64 before = 0;
   for (int p0 = 0; p0 < parts; p0 += kSrThreads) {
-    if (parts > kSrThreads) own = part_mass(p0);
-    const u64 run = before + sr_block_before(own, sh.red);
+    if (parts > kSrThreads) {
+      own = part_mass(p0);
+      run = before + sr_block_before(own, sh.red, all);
+      before += all;
+    }
     if (tid == 0) sh.s_int[3] = -1;
     __syncthreads();
     if (own > 0 && (double)run <= target && (double)(run + own) > target) {
@@ -709,12 +724,11 @@ __device__ __forceinline__ int sr_draw(const SrRow& r, SrShared& sh, u64 cut, F 
     }
     __syncthreads();
     if (sh.s_int[3] >= 0) break;
-    before += sr_block_sum(own, sh.red);
   }
   const int hit = sh.s_int[3];
-  const u64 run = sh.s_u64[1];
+  const u64 start = sh.s_u64[1];
   return hit < 0 ? sr_best_id(r.best)
-                 : sr_walk(r, sh, cut, hit * kSrPart, min((hit + 1) * kSrPart, r.V), run, target);
+                 : sr_walk(r, sh, cut, hit * kSrPart, min((hit + 1) * kSrPart, r.V), start, target);
 }
 
 // Adds the kept candidates of 512 parts from p0 on to the thread's `sure` mass.
