@@ -75,26 +75,26 @@ struct SrRow {
 };
 // exp((l - m) / T) by table (P.T.P. Tang's method): with t = 64 log2(e) (l - m)
 // / T and n the nearest integer, 2^(n / 64) = 2^(n >> 6) table[n & 63] and the
-// rest e^r, |r| <= ln 2 / 128, is a Taylor sum: r^6 / 720 < 2^-53.  t is below
-// 64 x 46.2 where a mass is not 0, so its rounding costs 2^-48.  About 20
-// instructions; exp() and a conversion to 64 bits are 50, which bound
-// k_sr_hist (64 x 201088: 37.6 -> 29.2 us).
+// rest 2^(x / 64), |x| <= 1/2, is a Taylor sum in x: with y = x ln 2 / 64 its
+// next term y^6 / 720 < 2^-53.  t is below 64 x 46.2 where a mass is not 0, so
+// its rounding costs 2^-48.  About 20 instructions; exp() and a conversion to
+// 64 bits are 50, which bound k_sr_hist (64 x 201088: 37.6 -> 29.2 us).  For
+// tokens in a bin only: no overflow; both infinite give t = NaN, which is 0 here.
 constexpr int kSrTable = 64;
 __device__ __forceinline__ void sr_table(double* table) {
   if (threadIdx.x < kSrTable) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / kSrTable));
 }
 __device__ __forceinline__ double sr_weight(const SrRow& r, float l) {
-  const double t = fmax(((double)l - r.m_d) * r.to_t, -64.0 * 1100.0);
-  const double n = __builtin_rint(t);
-  const double x = (t - n) * (0.69314718055994530942 / kSrTable);
+  constexpr double L = 0.69314718055994530942 / kSrTable;
+  const double t = fmin(((double)l - r.m_d) * r.to_t, 0.0);
+  const double n = __builtin_rint(t), x = t - n;
   const int i = (int)n;
-  double e = __builtin_fma(x, 1.0 / 120.0, 1.0 / 24.0);
-  e = __builtin_fma(x, e, 1.0 / 6.0);
-  e = __builtin_fma(x, e, 0.5);
+  double e = __builtin_fma(x, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+  e = __builtin_fma(x, e, L * L * L / 6.0);
+  e = __builtin_fma(x, e, L * L / 2.0);
+  e = __builtin_fma(x, e, L);
   e = __builtin_fma(x, e, 1.0);
-  e = __builtin_fma(x, e, 1.0);
-  e = __builtin_ldexp(r.table[i & (kSrTable - 1)] * e, i >> 6);
-  return l == r.m ? 1.0 : e;  // also where both are infinite
+  return __builtin_ldexp(r.table[i & (kSrTable - 1)] * e, i >> 6);
 }
 // round(w 2^S) for w 2^S <= 2^44: the low bits of w 2^S + 2^52
 __device__ __forceinline__ u64 sr_units(const SrRow& r, double w) {
@@ -276,8 +276,13 @@ struct SrPart {
 };
 __device__ __forceinline__ SrPart sr_part(const float* l, int i, int i1) {
   SrPart p;
+  if (i + kSrPart <= i1) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p.v[j] = l[min(i + (int)threadIdx.x + j * kSrThreads, i1 - 1)];
+    for (int j = 0; j < 8; ++j) p.v[j] = (l + i + j * kSrThreads)[threadIdx.x];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p.v[j] = l[min(i + (int)threadIdx.x + j * kSrThreads, i1 - 1)];
+  }
   return p;
 }
 template <class F>
