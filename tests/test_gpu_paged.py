@@ -710,3 +710,33 @@ def test_own_scratch_belongs_to_the_stream_of_the_call(handle):
     ref, mag = attention(bt, f32(q), sk, 0)
     for out in outs:
         check(to_host(out), ref, mag, 0)
+
+
+def test_overlapping_row_starts_leave_the_counters_zero():
+    """Starts 0, 1280, 0, 1280, ...: every second sequence is one that fits, and
+    all of them together make more units than the grid has blocks, with the long
+    one's chunks across its end.  The call reports it, and the next one is right."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(9)
+    n, B, long_at = 1280, 119, 60
+    bt = Batch(rng, [(n, n)], 4096, 1, 64, False).fill(rng)
+    d = bt.dev()
+    q = bf16(rng.normal(size=(n, 1, 64)).astype(np.float32))
+    qd, out = to_dev(q), empty_dev(q.shape, np.uint16)
+    starts = to_dev(np.array([0, n] * ((B + 1) // 2), np.int32))
+    lens = np.full(B, n, np.int32)
+    lens[long_at] = 200000
+    table = np.full((B, 49), int(bt.table[0, 0]), np.int32)
+    wb, cb = ne.paged_attn_workspace(n, B, 1, 1, 64)
+    ws = torch.empty(wb, dtype=torch.uint8, device="cuda")
+    counters = torch.zeros(cb, dtype=torch.uint8, device="cuda")
+    ne.paged_attn(d["kv"], qd, None, starts, to_dev(lens), to_dev(table), out, 1, workspace=ws,
+                  counters=counters)
+    with pytest.raises(ne.NeonError):
+        ne.device_check()
+    assert not counters.any().item()
+    ne.paged_attn(d["kv"], qd, None, d["q_start"], d["kv_len"], d["table"], out, 1, workspace=ws,
+                  counters=counters)
+    ref, mag = attention(bt, f32(q), None, 0)
+    check(to_host(out), ref, mag, 0)
+    ne.device_check()
