@@ -1400,7 +1400,8 @@ static int64_t pa_units(int n_rows, int B, int G, int R) {
 // both unless all rows together are few.
 static int64_t pa_few_blocks(const PagedRows& r, int Hq, int Hkv) {
   if (r.q_start == nullptr && Hq / Hkv > kPaFew) return 0;
-  return (kPaTarget / Hkv + 1 + pa_units(r.n_rows, r.B, Hq / Hkv, 16)) * Hkv;
+  const int64_t units = pa_units(r.n_rows, r.B, Hq / Hkv, 16), most = r.B * (int64_t)(kPaFew / 16);
+  return (kPaTarget / Hkv + 1 + (units < most ? units : most)) * Hkv;
 }
 static int64_t pa_many_blocks(const PagedRows& r, int Hq, int Hkv) {
   const int64_t G = Hq / Hkv;
