@@ -1391,33 +1391,45 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
                 });
 }
 
-// Units of R rows that n_rows rows of up to B sequences can make (per KV head).
-static int64_t pa_units(int n_rows, int B, int G, int R) {
-  return (int64_t)n_rows * G / R + B;
+// Blocks per KV head for `units` units: target / Hkv of equal work and one more per
+// unit, or as many chunks of at least minc keys as the longest sequence that the
+// table holds can have.  Blocks without work are not free: a launch of 17000 of
+// them before a prompt chunk's took 14 us.
+static int64_t pa_blocks(const PagedAttnArgs& a, int64_t units, int R, int align, int minc,
+                         int target) {
+  const int64_t holds = (int64_t)a.r.max_pages << a.kv.page_log2, longest = 1 << 30;
+  int64_t keys = holds < longest ? holds : longest;
+  const int64_t seen = (int64_t)a.window + (R - 1) / a.G + align;
+  if (a.window > 0 && seen < keys) keys = seen;
+  const int64_t even = target / a.kv.Hkv + 1 + units, all = units * ((keys + minc - 1) / minc);
+  return (even < all ? even : all) * a.kv.Hkv;
 }
 // Blocks of the two launches (0: no row can be of that kind).  One row per
 // sequence has G rows; with row starts the host does not know, and launches
-// both unless all rows together are few.
-static int64_t pa_few_blocks(const PagedRows& r, int Hq, int Hkv) {
-  if (r.q_start == nullptr && Hq / Hkv > kPaFew) return 0;
-  const int64_t units = pa_units(r.n_rows, r.B, Hq / Hkv, 16), most = r.B * (int64_t)(kPaFew / 16);
-  return (kPaTarget / Hkv + 1 + (units < most ? units : most)) * Hkv;
+// both unless all rows together are few.  Units are at most one per R rows and
+// one per sequence.
+static int64_t pa_few_blocks(const PagedAttnArgs& a) {
+  if (a.r.q_start == nullptr && a.G > kPaFew) return 0;
+  const int64_t units = (int64_t)a.r.n_rows * a.G / 16 + a.r.B, most = a.r.B * (int64_t)(kPaFew / 16);
+  return pa_blocks(a, units < most ? units : most, 16, 32, 256, kPaTarget);
 }
-static int64_t pa_many_blocks(const PagedRows& r, int Hq, int Hkv) {
-  const int64_t G = Hq / Hkv;
-  if (r.q_start == nullptr ? G <= kPaFew : r.n_rows * G <= kPaFew) return 0;
-  const int64_t most = r.n_rows * G / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
-  return (kPmTarget / Hkv + 1 + pa_units(r.n_rows, (int)(most < r.B ? most : r.B), (int)G, 128)) *
-         Hkv;
+static int64_t pa_many_blocks(const PagedAttnArgs& a) {
+  const int64_t rows = (int64_t)a.r.n_rows * a.G;
+  if (a.r.q_start == nullptr ? a.G <= kPaFew : rows <= kPaFew) return 0;
+  const int64_t most = rows / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
+  return pa_blocks(a, rows / 128 + (most < a.r.B ? most : a.r.B), 128, 64, 512, kPmTarget);
 }
 
 bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {
-  PagedRows r{};
+  PagedAttnArgs a{};
   static const int32_t given = 0;
-  r.q_start = &given;
-  r.n_rows = n_rows;
-  r.B = B;
-  return pa_few_blocks(r, Hq, Hkv) < kPaMaxBlocks && pa_many_blocks(r, Hq, Hkv) < kPaMaxBlocks;
+  a.r.q_start = &given;
+  a.r.n_rows = n_rows;
+  a.r.B = B;
+  a.r.max_pages = 1 << 30;
+  a.kv.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  return pa_few_blocks(a) < kPaMaxBlocks && pa_many_blocks(a) < kPaMaxBlocks;
 }
 // The two launches use the same places, one after the other.
 size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D) {
@@ -1429,7 +1441,7 @@ size_t paged_attn_counters() { return (size_t)(2 * kPaTarget) * kPaArrive * 4; }
 void launch_paged_attn(PagedAttnArgs a, hipStream_t st) {
   a.few = kPaFew;
   a.G = a.Hq / a.kv.Hkv;
-  const int64_t few = pa_few_blocks(a.r, a.Hq, a.kv.Hkv), many = pa_many_blocks(a.r, a.Hq, a.kv.Hkv);
+  const int64_t few = pa_few_blocks(a), many = pa_many_blocks(a);
 #define PA(D, F4)                                                                              \
   do {                                                                                         \
     if (few)                                                                                   \

@@ -86,7 +86,7 @@ def test_gather_refusals(bad):
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(q=P + 4), dict(out=None), dict(out=P + 8), dict(stride=248),
     dict(stride=260), dict(Hq=3), dict(Hq=1), dict(Hq=0), dict(Hq=130, stride=1 << 20),
-    dict(window=-1), dict(n_rows=1 << 22, Hq=64, n_kv_heads=64, stride=4096)], ids=str)
+    dict(window=-1), dict(n_rows=1 << 17, B=65535, Hq=1024, n_kv_heads=1024, stride=1 << 16)], ids=str)
 def test_attn_refusals(bad):
     assert attn(**bad) == ne.NEON_EINVAL
 
