@@ -423,16 +423,29 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
         flag_dev_err(a.r.err, kDevErrPagedRows);
     }
   PaSeq q = pa_seq<FEW>(a, lane);  // the only ones of up to 64
-  float work = (float)pa_tiles<R>(w, q) * (float)pa_span<R, ALIGN>(a, w.G, q.len);
+  float work = 0.0f, most = 0.0f;
+  auto add = [&](const PaSeq& p) {
+    const float span = (float)pa_span<R, ALIGN>(a, w.G, p.len), tiles = (float)pa_tiles<R>(w, p);
+    work += tiles * span;
+    most = fmaxf(most, tiles > 0.0f ? span : 0.0f);
+  };
+  add(q);
 #pragma unroll 4
-  for (int j = 1; j < turns; ++j) {
-    const PaSeq p = pa_seq<FEW>(a, 64 * j + lane);
-    work += (float)pa_tiles<R>(w, p) * (float)pa_span<R, ALIGN>(a, w.G, p.len);
-  }
+  for (int j = 1; j < turns; ++j) add(pa_seq<FEW>(a, 64 * j + lane));
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
-  int chunk = uni(max(MINC, (min((int)min(share, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
+  // The tiles of the many-row kernel are joined at some 0.6 us a chunk, and cutting
+  // one at all costs what 4 or 5 of its 64-key steps do: none of up to 512 keys, and
+  // chunks of at least sqrt(25 n) of n (319 rows of 583 tokens, 1 head of 128:
+  // 37 -> 28 us against chunks of 512; 40 of 60000 129 -> 90; 230 tokens cut in two
+  // 17 -> 27).
+  float least = share;
+  if (!FEW) {
+    most = wave_max(most);
+    least = fmaxf(share, most <= 512.0f ? 511.0f : __builtin_sqrtf(25.0f * most));
+  }
+  int chunk = uni(max(MINC, (min((int)min(least, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
   // The blocks of the sequences, in order, up to the one that idx lies in.  Row
   // starts that overlap (an error that no single sequence shows) can sum to more
   // blocks than the grid has: the clamp lies above every grid and keeps the sums
@@ -699,108 +712,106 @@ __device__ __forceinline__ float2 pa_load_agent(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// Joins what the chunks' blocks left of a tile's R rows (in the same launch:
+// Joins what the chunks' blocks left of a tile's 16 rows (in the same launch:
 // agent-scope loads), `used` of them: o at part + chunk * step + row D, (m, l)
-// behind the R rows.  256 threads: 16 for a row's D values; where fewer than 16
+// behind the rows.  256 threads: 16 for a row's D values; where fewer than 16
 // rows are used, the others take a share of the chunks.  fn(row, E values, m, l)
 // by 16 threads per row, thread t with the values (t & 15) E ..
 // Without the shares and with one chunk's loads at a time the join of a tile of 92
 // chunks took 25 us; the whole call for one sequence of 30000 tokens takes 26.
 constexpr int kPaJoin = 64;  // chunks whose factors are in LDS at once
-template <int D, int R, class F>
+template <int D, class F>
 __device__ __forceinline__ void pa_join(const float* part, int64_t step, int chunks, int used,
                                         float (*sf)[kPaJoin], float (*sx)[D + 4], F fn) {
-  constexpr int E = D / 16;
+  constexpr int R = 16, E = D / 16;
   const int tid = threadIdx.x, lane16 = tid & 15, row16 = tid >> 4;
   const int rows2 = used > 8 ? 16 : used > 4 ? 8 : used > 2 ? 4 : used > 1 ? 2 : 1;
   const int shares = 16 / rows2, share = row16 / rows2, row = row16 & (rows2 - 1);
-  for (int r0 = 0; r0 < used; r0 += 16) {
-    float M = -INFINITY, L = 0.0f, x[E];  // M, L of row row16
+  float M = -INFINITY, L = 0.0f, x[E];  // M, L of row row16
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.0f;
-    const float* pml = part + R * D + 2 * (r0 + row16);
-    for (int c0 = 0; c0 < chunks; c0 += kPaJoin) {
-      // the factors of these chunks for row row16, 16 lanes of it
-      float2 ml[kPaJoin / 16];
-      float mx = M;
+  for (int e = 0; e < E; ++e) x[e] = 0.0f;
+  const float* pml = part + R * D + 2 * row16;
+  for (int c0 = 0; c0 < chunks; c0 += kPaJoin) {
+    // the factors of these chunks for row row16, 16 lanes of it
+    float2 ml[kPaJoin / 16];
+    float mx = M;
 #pragma unroll
-      for (int i = 0; i < kPaJoin / 16; ++i) {
-        const int j = c0 + lane16 + 16 * i;
-        ml[i] = pa_load_agent(pml + min(j, chunks - 1) * step);
-        if (j >= chunks) ml[i] = make_float2(-INFINITY, 0.0f);
-      }
+    for (int i = 0; i < kPaJoin / 16; ++i) {
+      const int j = c0 + lane16 + 16 * i;
+      ml[i] = pa_load_agent(pml + min(j, chunks - 1) * step);
+      if (j >= chunks) ml[i] = make_float2(-INFINITY, 0.0f);
+    }
 #pragma unroll
-      for (int i = 0; i < kPaJoin / 16; ++i) mx = fmaxf(mx, ml[i].x);
-      mx = fmaxf(mx, xor_lane<1>(mx));
-      mx = fmaxf(mx, xor_lane<2>(mx));
-      mx = fmaxf(mx, xor_lane<4>(mx));
-      mx = fmaxf(mx, xor_lane<8>(mx));
-      const float me = mx == -INFINITY ? 0.0f : mx;
-      const float old = __builtin_amdgcn_exp2f(M - me);
-      float sum = 0.0f;
-      __syncthreads();  // sf is free
+    for (int i = 0; i < kPaJoin / 16; ++i) mx = fmaxf(mx, ml[i].x);
+    mx = fmaxf(mx, xor_lane<1>(mx));
+    mx = fmaxf(mx, xor_lane<2>(mx));
+    mx = fmaxf(mx, xor_lane<4>(mx));
+    mx = fmaxf(mx, xor_lane<8>(mx));
+    const float me = mx == -INFINITY ? 0.0f : mx;
+    const float old = __builtin_amdgcn_exp2f(M - me);
+    float sum = 0.0f;
+    __syncthreads();  // sf is free
 #pragma unroll
-      for (int i = 0; i < kPaJoin / 16; ++i) {
-        const float f = __builtin_amdgcn_exp2f(ml[i].x - me);
-        sf[row16][lane16 + 16 * i] = f;
-        sum = __builtin_fmaf(ml[i].y, f, sum);
-      }
-      sum += xor_lane<1>(sum);
-      sum += xor_lane<2>(sum);
-      sum += xor_lane<4>(sum);
-      sum += xor_lane<8>(sum);
-      L = __builtin_fmaf(L, old, sum);
-      M = mx;
-      if (c0 > 0) {  // the values so far, of row `row`
-        if (lane16 == 0) sx[row16][0] = old;
-        __syncthreads();
-        const float f = sx[row][0];
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] *= f;
-      }
+    for (int i = 0; i < kPaJoin / 16; ++i) {
+      const float f = __builtin_amdgcn_exp2f(ml[i].x - me);
+      sf[row16][lane16 + 16 * i] = f;
+      sum = __builtin_fmaf(ml[i].y, f, sum);
+    }
+    sum += xor_lane<1>(sum);
+    sum += xor_lane<2>(sum);
+    sum += xor_lane<4>(sum);
+    sum += xor_lane<8>(sum);
+    L = __builtin_fmaf(L, old, sum);
+    M = mx;
+    if (c0 > 0) {  // the values so far, of row `row`
+      if (lane16 == 0) sx[row16][0] = old;
       __syncthreads();
-      const int n = min(kPaJoin, chunks - c0);
-      const float* po = part + c0 * step + (r0 + row) * D + lane16 * E;
-      // U chunks' loads at a time
-      auto take = [&](auto u_t, int j0) {
-        constexpr int U = decltype(u_t)::value;
-        float2 y[U][E / 2];
+      const float f = sx[row][0];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float* p = po + min(j0 + u * shares, n - 1) * step;
+      for (int e = 0; e < E; ++e) x[e] *= f;
+    }
+    __syncthreads();
+    const int n = min(kPaJoin, chunks - c0);
+    const float* po = part + c0 * step + row * D + lane16 * E;
+    // U chunks' loads at a time
+    auto take = [&](auto u_t, int j0) {
+      constexpr int U = decltype(u_t)::value;
+      float2 y[U][E / 2];
 #pragma unroll
-          for (int e = 0; e < E / 2; ++e) y[u][e] = pa_load_agent(p + 2 * e);
-        }
+      for (int u = 0; u < U; ++u) {
+        const float* p = po + min(j0 + u * shares, n - 1) * step;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (j0 + u * shares >= n) break;
-          const float f = sf[row][j0 + u * shares];
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) {
-            x[2 * e] = __builtin_fmaf(y[u][e].x, f, x[2 * e]);
-            x[2 * e + 1] = __builtin_fmaf(y[u][e].y, f, x[2 * e + 1]);
-          }
-        }
-      };
-      if (n <= 2 * shares) {
-        take(std::integral_constant<int, 2>{}, share);
-      } else if (n <= 4 * shares) {
-        take(std::integral_constant<int, 4>{}, share);
-      } else {
-        for (int j0 = share; j0 < n; j0 += 8 * shares) take(std::integral_constant<int, 8>{}, j0);
+        for (int e = 0; e < E / 2; ++e) y[u][e] = pa_load_agent(p + 2 * e);
       }
-    }
-    // the shares of a row; sx row: share * rows2 + row
-    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e) sx[row16][lane16 * E + e] = x[e];
-    __syncthreads();
-    if (row16 < rows2) {
-      for (int k = 1; k < shares; ++k)
+      for (int u = 0; u < U; ++u) {
+        if (j0 + u * shares >= n) break;
+        const float f = sf[row][j0 + u * shares];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] += sx[k * rows2 + row16][lane16 * E + e];
-      if (r0 + row16 < used) fn(r0 + row16, x, M, L);
+        for (int e = 0; e < E / 2; ++e) {
+          x[2 * e] = __builtin_fmaf(y[u][e].x, f, x[2 * e]);
+          x[2 * e + 1] = __builtin_fmaf(y[u][e].y, f, x[2 * e + 1]);
+        }
+      }
+    };
+    if (n <= 2 * shares) {
+      take(std::integral_constant<int, 2>{}, share);
+    } else if (n <= 4 * shares) {
+      take(std::integral_constant<int, 4>{}, share);
+    } else {
+      for (int j0 = share; j0 < n; j0 += 8 * shares) take(std::integral_constant<int, 8>{}, j0);
     }
+  }
+  // the shares of a row; sx row: share * rows2 + row
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) sx[row16][lane16 * E + e] = x[e];
+  __syncthreads();
+  if (row16 < rows2) {
+    for (int k = 1; k < shares; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += sx[k * rows2 + row16][lane16 * E + e];
+    if (row16 < used) fn(row16, x, M, L);
   }
 }
 template <int E>
@@ -1061,7 +1072,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
     __syncthreads();
     if (!merge_here) return;
     if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    pa_join<D, R>(a.part + first * R * (D + 2), (int64_t)a.kv.Hkv * R * (D + 2), w.chunks,
+    pa_join<D>(a.part + first * R * (D + 2), (int64_t)a.kv.Hkv * R * (D + 2), w.chunks,
                   min(R, rows - w.row0), sf, so[0], [&](int tr_, const float (&y)[E], float m_, float l_) {
                     const int tok_ = pa_div(w.row0 + tr_, G, w.rG);
                     const int head = h * G + w.row0 + tr_ - tok_ * G;
@@ -1099,6 +1110,135 @@ struct PmStage {  // a thread's part of a tile on its way
   uint4 k[D / 32], v[D / 32];
 };
 
+// pa_join for a tile of 128 rows: two threads a row for its maximum, sum and the
+// chunks' factors sf; then groups of four values, NG of a thread at a time, with U
+// chunks' loads on their way: all rows and two (or one) of up to 8 chunks, else
+// 4096 / D rows and four (64 rows of 8000 tokens 31.3 -> 27.3 us; 256 of 4000 the
+// other way round, 48.8 -> 45.9).  By 16 rows at a time, every step for each, two
+// chunks of 128 rows of 128 took 13 us.
+constexpr int kPmJoin = 32;  // chunks whose factors are in LDS at once
+template <int D>
+__device__ __forceinline__ void pm_join(const PagedAttnArgs& a, const PaWork& w, int h,
+                                        const float* part, int64_t step, float (*sf)[kPmJoin],
+                                        float* fin) {
+  constexpr int R = 128, Q = D / 4;  // Q groups of a row
+  const int tid = threadIdx.x, row = tid >> 1, side = tid & 1;
+  const int used = min(R, w.n * w.G - w.row0);
+  const float* pml = part + R * D + 2 * row;
+  // (m, l) of the chunks from c0 on, every second one of U each
+  auto load = [&](auto& ml, int c0) {
+    const int n = w.chunks - c0;
+#pragma unroll
+    for (int u = 0; u < (int)(sizeof(ml) / sizeof(ml[0])); ++u) {
+      ml[u] = pa_load_agent(pml + (c0 + min(side + 2 * u, n - 1)) * step);
+      if (side + 2 * u >= n) ml[u] = make_float2(-INFINITY, 0.0f);
+    }
+  };
+  float M = -INFINITY, L = 0.0f;
+  auto put = [&](const auto& ml) {
+    const float me = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int u = 0; u < (int)(sizeof(ml) / sizeof(ml[0])); ++u)
+      sf[row][side + 2 * u] = __builtin_amdgcn_exp2f(ml[u].x - me);
+  };
+  auto totals = [&](auto u_t) {
+    constexpr int U = decltype(u_t)::value;
+    float2 ml[U];
+    for (int c0 = 0; c0 < w.chunks; c0 += 2 * U) {
+      load(ml, c0);
+      float mx = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, ml[u].x);
+      mx = fmaxf(mx, xor_lane<1>(mx));
+      const float me = mx == -INFINITY ? 0.0f : mx;
+      float sum = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        sum = __builtin_fmaf(ml[u].y, __builtin_amdgcn_exp2f(ml[u].x - me), sum);
+      sum += xor_lane<1>(sum);
+      L = __builtin_fmaf(L, __builtin_amdgcn_exp2f(M - me), sum);
+      M = mx;
+    }
+    if (w.chunks <= kPmJoin) put(ml);
+  };
+  if (w.chunks <= 4) totals(std::integral_constant<int, 2>{});
+  else if (w.chunks <= 8) totals(std::integral_constant<int, 4>{});
+  else totals(std::integral_constant<int, kPmJoin / 2>{});
+  auto place = [&](int r, int& tok, int& head) {
+    tok = pa_div(w.row0 + r, w.G, w.rG);
+    head = h * w.G + w.row0 + r - tok * w.G;
+  };
+  __syncthreads();
+  auto join = [&](auto ng_t, auto u_t) {
+    constexpr int NG = decltype(ng_t)::value, U = decltype(u_t)::value, RB = 1024 * NG / D;
+    const uint32_t lane4 = 4 * tid;
+#pragma unroll 1
+    for (int r0 = 0; r0 < used; r0 += RB) {
+      float4 x[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+      for (int c0 = 0; c0 < w.chunks; c0 += kPmJoin) {
+        if (w.chunks > kPmJoin) {
+          float2 ml[kPmJoin / 2];
+          load(ml, c0);
+          __syncthreads();
+          put(ml);
+          __syncthreads();
+        }
+        const int n = min(kPmJoin, w.chunks - c0);
+        for (int j0 = 0; j0 < n; j0 += U) {
+          float2 y[U][NG][2];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const float* p = part + (c0 + min(j0 + u, n - 1)) * step + r0 * D;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              y[u][i][0] = pa_load_agent(p + 1024 * i + lane4);
+              y[u][i][1] = pa_load_agent(p + 1024 * i + 2 + lane4);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (j0 + u >= n) break;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              const float f = sf[r0 + (tid + 256 * i) / Q][j0 + u];
+              x[i].x = __builtin_fmaf(y[u][i][0].x, f, x[i].x);
+              x[i].y = __builtin_fmaf(y[u][i][0].y, f, x[i].y);
+              x[i].z = __builtin_fmaf(y[u][i][1].x, f, x[i].z);
+              x[i].w = __builtin_fmaf(y[u][i][1].y, f, x[i].w);
+            }
+          }
+        }
+      }
+      if (r0 == 0) {
+        if (side == 0 && row < used) {
+          int tok, head;
+          place(row, tok, head);
+          fin[row] = pa_finish(a, head, M, L);
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int r = r0 + (tid + 256 * i) / Q;
+        if (r >= used) break;
+        int tok, head;
+        place(r, tok, head);
+        const float f = fin[r];
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(w.start + tok) * a.Hq + head) * D +
+                                  4 * (tid % Q)) =
+            make_uint2(pack_bf2(x[i].x * f, x[i].y * f), pack_bf2(x[i].z * f, x[i].w * f));
+      }
+    }
+  };
+  if (used > 64 && w.chunks <= 8)
+    join(std::integral_constant<int, D / 8>{}, std::integral_constant<int, 128 / D>{});
+  else
+    join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+}
+
 template <int D, bool F4>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
@@ -1106,7 +1246,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   __shared__ int merge_here, odd;
   const int h = blockIdx.x % a.kv.Hkv;
   PaWork w(a);
-  if (!pa_work<false, R, 64, 512, kPmTarget, 512, false>(
+  if (!pa_work<false, R, 64, 256, kPmTarget, 512, false>(
           a, blockIdx.x / a.kv.Hkv, gridDim.x / a.kv.Hkv, blockIdx.x == 0, w))
     return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
@@ -1402,14 +1542,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
   if (!merge_here) return;
   if (tid == 0) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // the tiles' memory is free: every wave is past its last one
-  float (*sf)[kPaJoin] = reinterpret_cast<float (*)[kPaJoin]>(&kt[0][0]);
-  float (*sx)[D + 4] = reinterpret_cast<float (*)[D + 4]>(&vt[0][0]);
-  pa_join<D, R>(p0, step_c, w.chunks, min(R, rows - w.row0), sf, sx,
-                [&](int tr, const float (&y)[E], float m_, float l_) {
-                  const int r = w.row0 + tr, head = h * G + r % G;
-                  pa_write<E>(a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + (tid & 15) * E,
-                              y, pa_finish(a, head, m_, l_));
-                });
+  pm_join<D>(a, w, h, p0, step_c, reinterpret_cast<float (*)[kPmJoin]>(&kt[0][0]),
+             reinterpret_cast<float*>(&vt[0][0]));
 }
 
 // Blocks per KV head for `units` units: target / Hkv of equal work and one more per
@@ -1438,7 +1572,7 @@ static int64_t pa_many_blocks(const PagedAttnArgs& a) {
   const int64_t rows = (int64_t)a.r.n_rows * a.G;
   if (a.r.q_start == nullptr ? a.G <= kPaFew : rows <= kPaFew) return 0;
   const int64_t most = rows / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
-  return pa_blocks(a, rows / 128 + (most < a.r.B ? most : a.r.B), 128, 64, 512, kPmTarget);
+  return pa_blocks(a, rows / 128 + (most < a.r.B ? most : a.r.B), 128, 64, 256, kPmTarget);
 }
 
 bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {

@@ -740,3 +740,24 @@ def test_overlapping_row_starts_leave_the_counters_zero():
     ref, mag = attention(bt, f32(q), None, 0)
     check(to_host(out), ref, mag, 0)
     ne.device_check()
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,rows,length", [
+    (False, 64, 1, 1, 128, 1000),   # few chunks of a whole tile, of more than 64 rows
+    (False, 128, 1, 1, 100, 1000),
+    (True, 64, 1, 1, 70, 2000),
+    (True, 128, 2, 2, 200, 2000),   # the second tile of 72
+    (False, 64, 1, 1, 40, 1000),    # of up to 64
+    (False, 128, 3, 1, 11, 1500),
+    (False, 64, 1, 1, 130, 6000),   # more than 8 chunks
+    (True, 128, 1, 1, 130, 6000),
+    (False, 64, 1, 1, 40, 40000),   # more than 32
+    (False, 128, 1, 1, 128, 40000),
+    (False, 64, 1, 1, 128, 512),    # one
+    (False, 64, 1, 1, 128, 513),
+])
+def test_attention_joins_of_many_rows(mx, D, Hq, Hkv, rows, length):
+    torch_cuda()
+    bt, q, sk = attn_case(mx, D, Hq, Hkv, 64, [(rows, length)], seed=rows + length)
+    ref, mag = attention(bt, f32(q), sk, 0)
+    check(run_attn(bt, q, sk, 0), ref, mag, 0x1357)
