@@ -317,7 +317,8 @@ void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out,
 // arrive joins them (stores and loads at agent scope, as in k_attn_split).
 // ---------------------------------------------------------------------------
 constexpr int kPaTarget = 1024;   // blocks of equal work to aim at: 4 per CU
-constexpr int kPmTarget = 512;    // of the many-row kernel: 2 per CU
+constexpr int kPmTarget = 512;    // of the many-row kernel: 2 per CU (640 to 1024: 256
+                                  // rows of 4000 tokens 45 -> 52 to 60 us, for the joins)
 constexpr int kPaFew = 32;        // (token, head) rows per KV head of the few-row kernel
 constexpr int kPaArrive = 16;     // ints from one arrival counter to the next
 constexpr int kPaMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
@@ -1239,8 +1240,10 @@ __device__ __forceinline__ void pm_join(const PagedAttnArgs& a, const PaWork& w,
     join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
 }
 
+// Three blocks of a CU at D = 64 (168 registers; 169, and so two of them, made the
+// prompt chunk 298 us), two at 128.
 template <int D, bool F4>
-__global__ __launch_bounds__(256, 2) void k_paged_attn_many(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedAttnArgs a) {
   constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
   __shared__ __align__(16) uint4 kt[2][64 * W], vt[2][64 * W];
   __shared__ int merge_here, odd;
