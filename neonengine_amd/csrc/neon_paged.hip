@@ -436,16 +436,15 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
-  // The tiles of the many-row kernel are joined at some 0.6 us a chunk, and cutting
-  // one at all costs what 4 or 5 of its 64-key steps do: none of up to 512 keys, and
-  // chunks of at least sqrt(25 n) of n (319 rows of 583 tokens, 1 head of 128:
-  // 37 -> 28 us against chunks of 512; 40 of 60000 129 -> 90; 230 tokens cut in two
-  // 17 -> 27).
-  float least = share;
-  if (!FEW) {
-    most = wave_max(most);
-    least = fmaxf(share, most <= 512.0f ? 511.0f : __builtin_sqrtf(25.0f * most));
-  }
+  // Few blocks: the last one of a unit joins its chunks one after another, so of n
+  // keys chunks of sqrt(cost n) at least, the cost of joining one against that of a
+  // key.  Few rows (256 or more keys): one sequence of 16000 tokens 15.1 -> 12.5 us,
+  // of 30000 26.1 -> 19.9.  Tiles of 128 rows: 40 rows of 60000 129 -> 90, 319 of 583
+  // (1 head of 128) 37 -> 28; and a unit of up to 512 keys is not cut, which costs
+  // what 4 or 5 of its 64-key steps do (230 tokens in two 17 -> 27).
+  most = wave_max(most);
+  const float cost = __builtin_sqrtf((FEW ? 10.0f : 25.0f) * most);
+  const float least = fmaxf(share, !FEW && most <= 512.0f ? 511.0f : cost);
   int chunk = uni(max(MINC, (min((int)min(least, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
   // The blocks of the sequences, in order, up to the one that idx lies in.  Row
   // starts that overlap (an error that no single sequence shows) can sum to more
@@ -719,7 +718,7 @@ __device__ __forceinline__ float2 pa_load_agent(const float* p) {
 // rows are used, the others take a share of the chunks.  fn(row, E values, m, l)
 // by 16 threads per row, thread t with the values (t & 15) E ..
 // Without the shares and with one chunk's loads at a time the join of a tile of 92
-// chunks took 25 us; the whole call for one sequence of 30000 tokens takes 26.
+// chunks took 25 us; the whole call for one sequence of 30000 tokens takes 20.
 constexpr int kPaJoin = 64;  // chunks whose factors are in LDS at once
 template <int D, class F>
 __device__ __forceinline__ void pa_join(const float* part, int64_t step, int chunks, int used,
@@ -831,7 +830,8 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // MXFP4 at 3 to 3.6 TB/s by the vector units as well, which expand the codes
 // (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, half busy); few short
 // sequences by the chain of lookups, loads and the join (5 us for one of 64 tokens).
-// Waves of a SIMD, and blocks of a CU (four of D = 64 spill)
+// Waves of a SIMD, and blocks of a CU (four of D = 64: bf16 spills, MXFP4 4 sequences
+// of up to 131072 tokens 29.1 -> 30.3 us)
 constexpr int pa_few_waves(int D, bool f4) { return D == 64 || f4 ? 3 : 2; }
 template <int D, bool F4>
 __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(PagedAttnArgs a) {
@@ -1098,7 +1098,8 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 // LDS holds two.
 // Bound: the vector units (69% busy: an exponential, at a quarter of their rate, and
 // some five plain instructions a score) beside the matrix units (40%): the last 2048
-// and 819 rows of 6001 and 2925 tokens, 64 heads, in 252 us, 797 TFLOP/s.
+// and 819 rows of 6001 and 2925 tokens, 64 heads, in 250 us, 800 TFLOP/s; one
+// prompt of 8192 tokens 788, heads of 128 893.
 // P is rounded to bf16, and the row sums come from the same rounded values (a
 // product with ones), so the rounding cancels where a row's weights share it.
 typedef short ps4 __attribute__((ext_vector_type(4)));
