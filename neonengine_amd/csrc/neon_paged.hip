@@ -605,7 +605,7 @@ __device__ __forceinline__ void pa_load(PaTile<D, true>& t, const PagedKv& kv, i
 // that hold no key of the sequence and may hold anything.  A weight of 0 would turn
 // an infinity or a NaN among their values into a NaN of a row that does not see
 // it, so such values are cleared on the way, and where a key of the sequence had
-// one (`odd`), pa_odd_values adds it to the rows that see it after the last step.
+// one (`odd`), the rows that see it get it after the last step (pa_odd_values).
 __device__ __forceinline__ uint32_t pa_odd_halves(uint32_t w) {  // 0xFFFF in each
   return ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
          ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
@@ -632,8 +632,8 @@ __device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, int c
   t.v[s][i] = clear ? 0u : t.v[s][i];
   word = clear ? word & keep : word;
 }
-// Adds the infinities and NaNs of keys [kb, kb + n) to the rows of the lane that
-// see them, fn(key, value of dim d0 + ..): the values again from the pages.
+// fn(key, value(d)) for the keys [kb, kb + n): the infinities and NaNs of a value, 0
+// for a finite one, from the pages again.
 template <int D, bool F4, class F>
 __device__ __forceinline__ void pa_odd_values(const PagedAttnArgs& a, const PaWork& w, int h, int kb,
                                               int n, F fn) {
@@ -905,16 +905,6 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
     }
     pa_load<D>(t, a.kv, g, c, at);
   };
-  // whether one of the step's two pages is none (its whole step is masked)
-  auto edge_page = [&](int kb) {
-    bool none = false;
-    for (int s = 0; s < 2; ++s) {
-      const int key = kb + 16 * s;
-      none |= key < w.k1 && key + 16 > w.lo &&
-              (unsigned)table[key >> a.kv.page_log2] >= (unsigned)a.kv.n_pages;
-    }
-    return none;
-  };
   auto inside = [&](int kb) { return kb >= all_lo && kb + 32 <= all_hi; };
   bool odd = false;
   auto step = [&](PaTile<D, F4>& t, int it, const int (&id)[2]) {
@@ -1011,22 +1001,35 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
       }
     }
   }
+  // An infinity among the values of a step that every row sees meets both terms of P:
+  // its product with the second is the other infinity, or NaN.
+  if constexpr (!F4) {
+    float z = 0.0f;  // NaN where an element is not finite
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[e][i], 0.0f, z);
+    odd = odd || z != z;
+  }
   if (__any(odd)) {  // lane (g, c): row c, dims (D/4) g + E i + e
-    for (int it = 0; it < n_it; ++it) {
-      const int kb = w.k0 + 32 * (wave + 4 * it);
-      // (every step with a bad page too: its other keys were cleared as well)
-      pa_odd_values<D, F4>(a, w, h, kb, 32, [&](int key, auto value) {
-        if (inside(kb) && !edge_page(kb)) return;
+    pf4 sum[E];      // of the infinities and NaNs alone
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int it = 0; it < n_it; ++it)
+      pa_odd_values<D, F4>(a, w, h, w.k0 + 32 * (wave + 4 * it), 32, [&](int key, auto value) {
         const bool seen = (key >= k_lo) & (key < k_hi);
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = value((D / 4) * g + E * i + e);
-            if (seen && v != 0.0f) o[e][i] += v;
+            if (seen) sum[e][i] += v;
           }
       });
-    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[e][i] = sum[e][i] != 0.0f ? sum[e][i] : o[e][i];
   }
   if constexpr (!F4) {
     l[0] += xor_lane<16>(l[0]);

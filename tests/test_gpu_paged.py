@@ -761,3 +761,30 @@ def test_attention_joins_of_many_rows(mx, D, Hq, Hkv, rows, length):
     bt, q, sk = attn_case(mx, D, Hq, Hkv, 64, [(rows, length)], seed=rows + length)
     ref, mag = attention(bt, f32(q), sk, 0)
     check(run_attn(bt, q, sk, 0), ref, mag, 0x1357)
+
+
+@pytest.mark.parametrize("D,lens", [(64, [(1, 70)]), (64, [(3, 300)]), (128, [(1, 700)]),
+                                    (128, [(60, 300)]), (64, [(200, 600)])])
+def test_infinities_that_every_row_sees(D, lens):
+    """A row that sees one infinity among the values of a dim gets it; both, or a NaN:
+    NaN.  Weights here are above 2^-40, so no product underflows."""
+    torch_cuda()
+    rng = np.random.default_rng(5)
+    bt = Batch(rng, lens, 16, 2, D, False).fill(rng)
+    odd = {0: np.inf, 1: -np.inf, 2: np.nan, 40: np.inf}
+    for b, (n, t) in enumerate(lens):
+        pg, rows = bt.places(b)
+        v = bt.get("v", b).astype(np.float32)
+        for d, x in odd.items():
+            v[7, :, d] = x
+        v[3, 1, 40] = -np.inf
+        bt.v[pg, :, rows] = (v.view(np.uint32) >> 16).astype(np.uint16)
+    q = bf16(rng.normal(size=(bt.n_rows, 4, D)).astype(np.float32))
+    got = f32(run_attn(bt, q, None, 0))
+    assert (got[:, :, 0] == np.inf).all() and (got[:, :, 1] == -np.inf).all()
+    assert np.isnan(got[:, :, 2]).all()
+    assert (got[:, :2, 40] == np.inf).all() and np.isnan(got[:, 2:, 40]).all()
+    rest = [d for d in range(D) if d not in odd]
+    ref, mag = attention(bt, f32(q), None, 0)
+    off = np.abs(got[..., rest] - ref[..., rest])
+    assert (off <= 2.0 ** -8 * np.abs(ref[..., rest]) + (2.0 ** -8 + 2.0 ** -12) * mag[..., rest]).all()
