@@ -2357,8 +2357,8 @@ extern "C" neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* 
       q_stride < (int64_t)Hq * a.kv.D || window < 0)
     KFAIL(NEON_EINVAL, "neon_paged_attn: q and out must be given, 16-byte aligned, q rows a "
           "multiple of 8 elements and at least Hq head_dim apart, window >= 0");
-  const size_t need = neon_paged_attn_workspace(n_rows, B, Hq, a.kv.Hkv, a.kv.D);
-  const size_t needc = neon_paged_attn_counters(n_rows, B, Hq, a.kv.Hkv, a.kv.D);
+  const size_t need = paged_attn_workspace(n_rows, Hq, a.kv.Hkv, a.kv.D);
+  const size_t needc = paged_attn_counters();
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     KFAIL(NEON_EINVAL, "neon_paged_attn: workspace of %zu bytes, %zu needed (16-byte aligned)",
           workspace_bytes, need);

@@ -434,7 +434,8 @@ struct PagedAttnArgs {
   int Hq, window;
   float* part;            // partial results of split units (paged_attn_workspace)
   int32_t* arrive;        // their counters, 0 at launch and left at 0
-  int few, G;             // set by the launcher
+  int G;                  // set by the launcher, as
+  bool small;             // whether all rows may be the few-row kernel's
 };
 size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D);
 size_t paged_attn_counters();

@@ -350,17 +350,22 @@ struct PaWork {
   __device__ explicit PaWork(const PagedAttnArgs& a) : G(a.G), rG(1.0f / (float)a.G) {}
 };
 
-// A sequence as a kernel takes it: FEW the ones of up to a.few (token, head) rows
-// per KV head, otherwise the longer ones; n = 0: none.
+// A sequence's rows (n = 0: none) and length.
 struct PaSeq {
   int start, n, len;
 };
-template <bool FEW>
 __device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
   PaSeq q;
   const int at = min(b, a.r.B - 1);
   const bool ok = paged_seq(a.r, a.kv.page_log2, at, q.start, q.n, q.len);
-  q.n = ok && b < a.r.B && q.len > 0 && (q.n * a.G <= a.few) == FEW ? q.n : 0;
+  q.n = ok && b < a.r.B && q.len > 0 ? q.n : 0;
+  return q;
+}
+// The same where it is the kernel's: FEW the ones of up to `few` (token, head) rows
+// per KV head, otherwise the longer ones.
+template <bool FEW>
+__device__ __forceinline__ PaSeq pa_of(const PagedAttnArgs& a, int few, PaSeq q) {
+  q.n = (q.n * a.G <= few) == FEW ? q.n : 0;
   return q;
 }
 
@@ -407,6 +412,25 @@ __device__ __forceinline__ int pa_chunks(const PagedAttnArgs& a, const PaWork& w
   return pa_div(pa_span<R, ALIGN>(a, w.G, q.len) + chunk - 1, chunk, rc);
 }
 
+// The most rows of a sequence that the few-row kernel takes.  All, where the whole
+// call is kPaSmall 16-row tiles x keys x KV heads at most: with so little work the
+// length of a block's chain counts, and 16 rows have a short one (8 heads for 1, 250
+// rows of 254 tokens 13.5 -> 8.9 us; 319 rows of 583 of 2 heads of 128 27.7 -> 13;
+// from 200000 on 128 rows at a time are the faster: 100 rows of 500, 64 heads for 8,
+// 17.6 against 20).  Both kernels compute it from the same numbers.
+constexpr int kPaSmall = 131072;
+__device__ __forceinline__ int pa_few_rows(const PagedAttnArgs& a, const PaWork& w,
+                                           const PaSeq& first, int turns) {
+  if (!a.small) return kPaFew;
+  float work = 0.0f;
+  auto add = [&](const PaSeq& q) {
+    work += (float)pa_tiles<16>(w, q) * (float)pa_span<16, 32>(a, w.G, q.len);
+  };
+  add(first);
+  for (int j = 1; j < turns; ++j) add(pa_seq(a, 64 * j + (threadIdx.x & 63)));
+  return uni(wave_sum(work) * (float)a.kv.Hkv <= kPaSmall * 1.001f ? 1 << 30 : kPaFew);
+}
+
 // The work of block `idx` of `blocks` (of every KV head alike); false when there is
 // none.
 // ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
@@ -423,7 +447,9 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
       if (!paged_seq(a.r, a.kv.page_log2, b, start, n, len) && len != 0)
         flag_dev_err(a.r.err, kDevErrPagedRows);
     }
-  PaSeq q = pa_seq<FEW>(a, lane);  // the only ones of up to 64
+  const PaSeq first = pa_seq(a, lane);  // the only ones of up to 64
+  const int few = pa_few_rows(a, w, first, turns);
+  PaSeq q = pa_of<FEW>(a, few, first);
   float work = 0.0f, most = 0.0f;
   auto add = [&](const PaSeq& p) {
     const float span = (float)pa_span<R, ALIGN>(a, w.G, p.len), tiles = (float)pa_tiles<R>(w, p);
@@ -432,7 +458,7 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
   };
   add(q);
 #pragma unroll 4
-  for (int j = 1; j < turns; ++j) add(pa_seq<FEW>(a, 64 * j + lane));
+  for (int j = 1; j < turns; ++j) add(pa_of<FEW>(a, few, pa_seq(a, 64 * j + lane)));
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
@@ -477,7 +503,7 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
     const int all_slots = __builtin_amdgcn_readlane(slots_to, 63);
     int before = all, slots_before = all_slots;
     for (j = 1; j < turns; ++j) {
-      q = pa_seq<FEW>(a, 64 * j + lane);
+      q = pa_of<FEW>(a, few, pa_seq(a, 64 * j + lane));
       nc = pa_chunks<R, ALIGN>(a, w, q, chunk, rc);
       const int nb2 = min(pa_tiles<R>(w, q) * nc, kPaMaxBlocks), s2 = nc > 1 ? nb2 : 0;
       const int to2 = pa_scan(nb2), st2 = pa_scan(s2);
@@ -1553,33 +1579,46 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
              reinterpret_cast<float*>(&vt[0][0]));
 }
 
-// Blocks per KV head for `units` units: target / Hkv of equal work and one more per
+// Most keys that a row tile of R rows can see.
+static int64_t pa_keys(const PagedAttnArgs& a, int R, int align) {
+  const int64_t holds = (int64_t)a.r.max_pages << a.kv.page_log2, longest = 1 << 30;
+  const int64_t keys = holds < longest ? holds : longest;
+  const int64_t seen = (int64_t)a.window + (R - 1) / a.G + align;
+  return a.window > 0 && seen < keys ? seen : keys;
+}
+// Blocks for `units` units per KV head: target / Hkv of equal work and one more per
 // unit, or as many chunks of at least minc keys as the longest sequence that the
 // table holds can have.  Blocks without work are not free: a launch of 17000 of
 // them before a prompt chunk's took 14 us.
-static int64_t pa_blocks(const PagedAttnArgs& a, int64_t units, int R, int align, int minc,
-                         int target) {
-  const int64_t holds = (int64_t)a.r.max_pages << a.kv.page_log2, longest = 1 << 30;
-  int64_t keys = holds < longest ? holds : longest;
-  const int64_t seen = (int64_t)a.window + (R - 1) / a.G + align;
-  if (a.window > 0 && seen < keys) keys = seen;
+static int64_t pa_blocks(const PagedAttnArgs& a, int64_t units, int64_t keys, int minc, int target) {
   const int64_t even = target / a.kv.Hkv + 1 + units, all = units * ((keys + minc - 1) / minc);
   return (even < all ? even : all) * a.kv.Hkv;
 }
-// Blocks of the two launches (0: no row can be of that kind).  One row per
-// sequence has G rows; with row starts the host does not know, and launches
-// both unless all rows together are few.  Units are at most one per R rows and
-// one per sequence.
-static int64_t pa_few_blocks(const PagedAttnArgs& a) {
-  if (a.r.q_start == nullptr && a.G > kPaFew) return 0;
-  const int64_t units = (int64_t)a.r.n_rows * a.G / 16 + a.r.B, most = a.r.B * (int64_t)(kPaFew / 16);
-  return pa_blocks(a, units < most ? units : most, 16, 32, 256, kPaTarget);
-}
-static int64_t pa_many_blocks(const PagedAttnArgs& a) {
+struct PaGrid {
+  int64_t few, many;  // blocks of the two launches (0: no row can be of that kind)
+  bool small;         // the few-row one has room for all rows of a small call
+};
+// One row per sequence has G rows; with row starts the host does not know, and
+// launches both unless all rows together are few, or surely a small call.  Units are
+// at most one per R rows and one per sequence; of up to kPaFew rows two a sequence.
+static PaGrid pa_grid(const PagedAttnArgs& a) {
   const int64_t rows = (int64_t)a.r.n_rows * a.G;
-  if (a.r.q_start == nullptr ? a.G <= kPaFew : rows <= kPaFew) return 0;
-  const int64_t most = rows / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
-  return pa_blocks(a, rows / 128 + (most < a.r.B ? most : a.r.B), 128, 64, 256, kPmTarget);
+  const bool none_few = a.r.q_start == nullptr && a.G > kPaFew;
+  const bool all_few = a.r.q_start == nullptr ? a.G <= kPaFew : rows <= kPaFew;
+  const int64_t units = rows / 16 + a.r.B, two = a.r.B * (int64_t)(kPaFew / 16);
+  const int64_t keys = pa_keys(a, 16, 32);
+  PaGrid g;
+  g.few = none_few ? 0 : pa_blocks(a, units < two ? units : two, keys, 256, kPaTarget);
+  if (all_few) return g.many = 0, g.small = false, g;
+  const int64_t longer = rows / (kPaFew + 1) + 1;  // sequences of more rows than kPaFew
+  g.many = pa_blocks(a, rows / 128 + (longer < a.r.B ? longer : a.r.B), pa_keys(a, 128, 64), 256,
+                     kPmTarget);
+  // of a small call, sum of tiles x keys / 256 and one more per unit
+  const int64_t small = units * a.kv.Hkv + kPaSmall / 256 + 2;
+  g.small = small <= (g.few > 1024 ? g.few : 1024);
+  if (g.small && g.few < small) g.few = small;
+  if (g.small && units * a.kv.Hkv * keys <= kPaSmall) g.many = 0;
+  return g;
 }
 
 bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {
@@ -1591,7 +1630,8 @@ bool paged_attn_fits(int n_rows, int B, int Hq, int Hkv) {
   a.r.max_pages = 1 << 30;
   a.kv.Hkv = Hkv;
   a.G = Hq / Hkv;
-  return pa_few_blocks(a) < kPaMaxBlocks && pa_many_blocks(a) < kPaMaxBlocks;
+  const PaGrid g = pa_grid(a);
+  return g.few < kPaMaxBlocks && g.many < kPaMaxBlocks;
 }
 // The two launches use the same places, one after the other.
 size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D) {
@@ -1601,15 +1641,15 @@ size_t paged_attn_workspace(int n_rows, int Hq, int Hkv, int D) {
 size_t paged_attn_counters() { return (size_t)(2 * kPaTarget) * kPaArrive * 4; }
 
 void launch_paged_attn(PagedAttnArgs a, hipStream_t st) {
-  a.few = kPaFew;
   a.G = a.Hq / a.kv.Hkv;
-  const int64_t few = pa_few_blocks(a), many = pa_many_blocks(a);
+  const PaGrid g = pa_grid(a);
+  a.small = g.small;
 #define PA(D, F4)                                                                              \
   do {                                                                                         \
-    if (few)                                                                                   \
-      hipLaunchKernelGGL((k_paged_attn_few<D, F4>), dim3((unsigned)few), dim3(256), 0, st, a); \
-    if (many)                                                                                  \
-      hipLaunchKernelGGL((k_paged_attn_many<D, F4>), dim3((unsigned)many), dim3(256), 0, st, a); \
+    if (g.few)                                                                                   \
+      hipLaunchKernelGGL((k_paged_attn_few<D, F4>), dim3((unsigned)g.few), dim3(256), 0, st, a); \
+    if (g.many)                                                                                  \
+      hipLaunchKernelGGL((k_paged_attn_many<D, F4>), dim3((unsigned)g.many), dim3(256), 0, st, a); \
   } while (0)
   if (a.kv.D == 64) {
     if (a.kv.ks != nullptr) PA(64, true); else PA(64, false);

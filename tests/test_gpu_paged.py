@@ -788,3 +788,25 @@ def test_infinities_that_every_row_sees(D, lens):
     ref, mag = attention(bt, f32(q), None, 0)
     off = np.abs(got[..., rest] - ref[..., rest])
     assert (off <= 2.0 ** -8 * np.abs(ref[..., rest]) + (2.0 ** -8 + 2.0 ** -12) * mag[..., rest]).all()
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,width,window,q_start", [
+    (False, 64, 8, 1, [(250, 254)], None, 0, True),
+    (False, 64, 8, 1, [(250, 254)], 900, 0, True),  # the host cannot tell that it is small
+    (True, 128, 2, 2, [(319, 583), (85, 227), (221, 418)], 100, 0, True),
+    (False, 128, 12, 2, [(150, 254), (149, 149), (1, 90), (0, 0)], 300, 33, True),
+    (True, 64, 1, 1, [(40, 60)] * 70, 90, 0, True),  # more than 64 sequences
+    (False, 64, 8, 1, [(256, 1024)], 900, 0, True),  # 128 tiles of 16 rows x 1024: the border
+    (False, 64, 8, 1, [(256, 1026)], 900, 0, True),
+    (False, 64, 64, 1, [(1, 500), (1, 30), (1, 1)], None, 0, False),  # 64 rows of one token
+    (False, 64, 64, 1, [(1, 500), (1, 30), (1, 1)], 2000, 0, False),
+])
+def test_attention_of_small_calls(mx, D, Hq, Hkv, lens, width, window, q_start):
+    torch_cuda()
+    rng = np.random.default_rng(len(lens) + D)
+    bt = Batch(rng, lens, 16, Hkv, D, mx, q_start=q_start, width=width).fill(rng)
+    q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32) * 2)
+    sk = f32(bf16(rng.normal(size=Hq).astype(np.float32)))
+    ref, mag = attention(bt, f32(q), sk, window)
+    check(run_attn(bt, q, sk, window), ref, mag, 0x1357)
+    ne.device_check()
