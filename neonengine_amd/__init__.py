@@ -465,17 +465,25 @@ def _scratch(nbytes, stream, zero=False):
         return _workspace(nbytes, zero)
 
 
+def _buffer(t, name, device):
+    """Device pointer of a contiguous tensor on this device."""
+    if t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous memory on device {device}")
+    return t.data_ptr()
+
+
 def _rows(x, size, width, name, device):
     """(device pointer, rows, elements between them) of rows of at least `width`
     elements: contiguous ones, or a slice of wider rows."""
-    if x.element_size() != size or x.get_device() != device or x.dim() not in (2, 3):
+    shape = x.shape
+    if x.element_size() != size or x.get_device() != device or len(shape) not in (2, 3):
         raise ValueError(f"{name}: rows of elements of {size} bytes on device {device}")
-    n = x.shape[0]
-    has = x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]
-    stride = max(has, width)
+    n = shape[0]
+    has = shape[1] if len(shape) == 2 else shape[1] * shape[2]
+    stride = has if has > width else width
     if not x.is_contiguous():
-        inner = (1,) if x.dim() == 2 else (x.shape[2], 1)
-        if any(s != w and k > 1 for s, w, k in zip(x.stride()[1:], inner, x.shape[1:])):
+        inner = (1,) if len(shape) == 2 else (shape[2], 1)
+        if any(s != w and k > 1 for s, w, k in zip(x.stride()[1:], inner, shape[1:])):
             raise ValueError(f"{name}: each row must be contiguous")
         if n > 1:
             stride = x.stride(0)
@@ -485,20 +493,22 @@ def _rows(x, size, width, name, device):
     return x.data_ptr(), n, stride
 
 
-def _on_current(device):
-    """The calls go to the current device: tensors elsewhere are refused."""
+def _on_current(device, stream):
+    """The stream's handle (None: the current one); the calls go to the current
+    device: tensors elsewhere are refused."""
     c = _current or _find_current()
     if device < 0 or c is None or device != c[0]():
         raise ValueError(f"tensors on device {device}: the call runs on the current HIP device")
+    return c[1](device) if stream is None else _stream(stream)
 
 
 def _batch(kv, q_start, kv_len, page_table, n_rows):
     """(q_start, kv_len, page_table, max_pages, B) of a paged call."""
     device = kv.device
-    _on_current(device)
-    if page_table.dim() != 2:
+    shape = page_table.shape
+    if len(shape) != 2:
         raise ValueError("page_table: [B][max_pages]")
-    B, max_pages = page_table.shape
+    B, max_pages = shape
     if kv_len.numel() != B:
         raise ValueError("page_table: one row per sequence of kv_len")
     if q_start is not None:
@@ -514,28 +524,30 @@ def paged_append(kv, qkv, table, q_start, kv_len, page_table, q_out, Hq, stream=
     and appends k and v to the pages (neon_paged_append).  table: from
     rope_table, fp32 [2][n_pos][head_dim / 2], or None (no rotation)."""
     D, device = kv.head_dim, kv.device
+    on = _on_current(device, stream)
     rows, n, stride = _rows(qkv, 2, (Hq + 2 * kv.n_kv_heads) * D, "qkv", device)
     q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
     q_out = _arg(q_out, 2, n * Hq * D, "q_out", device) if Hq else None
     n_pos = 0
     if table is not None:
-        if table.dim() != 3 or table.shape[0] != 2 or table.shape[2] != D // 2:
+        shape = table.shape
+        if len(shape) != 3 or shape[0] != 2 or shape[2] != D // 2:
             raise ValueError("table: [2][n_pos][head_dim / 2]")
-        n_pos = table.shape[1]
+        n_pos = shape[1]
         table = _arg(table, 4, n_pos * D, "table", device, True)
     _check(lib().neon_paged_append(kv.ref, rows, stride, table, n_pos, q_start, kv_len, page_table,
-                                   max_pages, q_out, n, B, Hq, _stream(stream)))
+                                   max_pages, q_out, n, B, Hq, on))
 
 
 def paged_gather(kv, q_start, kv_len, page_table, k_out, v_out, stream=None):
     """The rows that paged_append writes for the same arguments, as bf16, into
     k_out and v_out [n_rows][n_kv_heads][head_dim] (neon_paged_gather)."""
     n, width, device = k_out.shape[0], kv.n_kv_heads * kv.head_dim, kv.device
+    on = _on_current(device, stream)
     q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
     _check(lib().neon_paged_gather(kv.ref, q_start, kv_len, page_table, max_pages,
                                    _arg(k_out, 2, n * width, "k_out", device),
-                                   _arg(v_out, 2, n * width, "v_out", device), n, B,
-                                   _stream(stream)))
+                                   _arg(v_out, 2, n * width, "v_out", device), n, B, on))
 
 
 def paged_attn_workspace(n_rows, B, Hq, Hkv, D):
@@ -551,6 +563,7 @@ def paged_attn(kv, q, sinks, q_start, kv_len, page_table, out, Hq, window=0, str
     (neon_paged_attn).  counters: zero-filled once by the caller (each call
     leaves it zero)."""
     D, device = kv.head_dim, kv.device
+    on = _on_current(device, stream)
     rows, n, stride = _rows(q, 2, Hq * D, "q", device)
     q_start, kv_len, page_table, max_pages, B = _batch(kv, q_start, kv_len, page_table, n)
     if sinks is not None:
@@ -561,12 +574,11 @@ def paged_attn(kv, q, sinks, q_start, kv_len, page_table, out, Hq, window=0, str
             workspace = _scratch(wb, stream)
         if counters is None:
             counters = _scratch(cb, stream, zero=True)
+    wb, cb = workspace.nbytes, counters.nbytes
     _check(lib().neon_paged_attn(kv.ref, rows, stride, sinks, q_start, kv_len, page_table,
                                  max_pages, _arg(out, 2, n * Hq * D, "out", device), n, B, Hq,
-                                 window, _arg(workspace, workspace.element_size(), 0, "workspace",
-                                              device), workspace.nbytes,
-                                 _arg(counters, counters.element_size(), 0, "counters", device),
-                                 counters.nbytes, _stream(stream)))
+                                 window, _buffer(workspace, "workspace", device), wb,
+                                 _buffer(counters, "counters", device), cb, on))
 
 
 def sample_rows_workspace(B, V):
@@ -581,7 +593,7 @@ def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, mi
     if logits.dim() != 2:
         raise ValueError("logits: [B][V]")
     device = logits.get_device()
-    _on_current(device)
+    on = _on_current(device, stream)
     V = logits.shape[1]
     rows, B, stride = _rows(logits, 4, V, "logits", device)
     if workspace is None:
@@ -593,8 +605,7 @@ def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, mi
     _check(lib().neon_sample_rows(rows, stride, B, V, opt(temperature, "temperature"),
                                   opt(top_k, "top_k", False), opt(top_p, "top_p"), opt(min_p, "min_p"),
                                   opt(u, "u"), opt(out_ids, "out_ids", False),
-                                  _arg(workspace, workspace.element_size(), 0, "workspace", device),
-                                  workspace.nbytes, _stream(stream)))
+                                  _buffer(workspace, "workspace", device), workspace.nbytes, on))
 
 
 PREFILL_BATCHED, PREFILL_STEPWISE, PREFILL_CHUNKED, PREFILL_MX8 = 0, 1, 2, 3
