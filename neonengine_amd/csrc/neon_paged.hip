@@ -435,7 +435,7 @@ __device__ __forceinline__ int pa_few_rows(const PagedAttnArgs& a, const PaWork&
 // none.
 // ALIGN: units start at a multiple of it; MINC: the least chunk (chunks are
 // multiples of 128); TARGET: blocks to aim at; PLACES: blocks that the chip holds
-// at once.  Lane = sequence, 64 at a time.
+// at once; FIT: MXFP4.  Lane = sequence, 64 at a time.
 template <bool FEW, int R, int ALIGN, int MINC, int TARGET, int PLACES, bool FIT>
 __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blocks, bool report,
                                         PaWork& w) {
@@ -450,10 +450,11 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
   const PaSeq first = pa_seq(a, lane);  // the only ones of up to 64
   const int few = pa_few_rows(a, w, first, turns);
   PaSeq q = pa_of<FEW>(a, few, first);
-  float work = 0.0f, most = 0.0f;
+  float work = 0.0f, most = 0.0f, units = 0.0f;
   auto add = [&](const PaSeq& p) {
     const float span = (float)pa_span<R, ALIGN>(a, w.G, p.len), tiles = (float)pa_tiles<R>(w, p);
     work += tiles * span;
+    units += tiles;
     most = fmaxf(most, tiles > 0.0f ? span : 0.0f);
   };
   add(q);
@@ -462,15 +463,23 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
   // 1.001: the fp32 sum and this product are each off by a few 2^-24.  From
   // 2^30 on no sequence is longer than a chunk.
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
-  // Few blocks: the last one of a unit joins its chunks one after another, so of n
-  // keys chunks of sqrt(cost n) at least, the cost of joining one against that of a
-  // key.  Few rows (256 or more keys): one sequence of 16000 tokens 15.1 -> 12.5 us,
-  // of 30000 26.1 -> 19.9.  Tiles of 128 rows: 40 rows of 60000 129 -> 90, 319 of 583
-  // (1 head of 128) 37 -> 28; and a unit of up to 512 keys is not cut, which costs
-  // what 4 or 5 of its 64-key steps do (230 tokens in two 17 -> 27).
+  // Cutting costs the partial results and the join, by the last block of a unit, one
+  // chunk after another:
+  // - up to 512 keys are not cut (64 sequences of 500 tokens 24.7 -> 15.2 us, one of
+  //   301 8.2 -> 7.3; 230 rows of 230 tokens in two 17 -> 27);
+  // - nor are few rows whose blocks run all at once and none of which is much longer
+  //   than a CU's share of the work (of 256; a block alone reads about as fast): 64
+  //   sequences of 1000 tokens 31.4 -> 24.0, of 50 to 1500 28.8 -> 25.8; MXFP4 blocks
+  //   are slower (32 of 50 to 2000 12.7 -> 13.4), so two thirds of it there;
+  // - chunks of n keys are sqrt(cost n) at least, the cost of joining one against that
+  //   of a key (one sequence of 16000 tokens 15.1 -> 12.5, of 30000 26.1 -> 19.9; tiles
+  //   of 128 rows: 40 rows of 60000 129 -> 90, 319 of 583, 1 head of 128, 37 -> 28).
   most = wave_max(most);
   const float cost = __builtin_sqrtf((FEW ? 10.0f : 25.0f) * most);
-  const float least = fmaxf(share, !FEW && most <= 512.0f ? 511.0f : cost);
+  float least = fmaxf(share, most <= 512.0f ? 511.0f : cost);
+  if (FEW && most <= share * (TARGET / (FIT ? 384.0f : 256.0f)) + 512.0f &&
+      wave_sum(units) * (float)a.kv.Hkv <= (float)PLACES)
+    least = fmaxf(least, most);
   int chunk = uni(max(MINC, (min((int)min(least, 0x1p30f), (1 << 30) - 128) + 128) & ~127));
   // The blocks of the sequences, in order, up to the one that idx lies in.  Row
   // starts that overlap (an error that no single sequence shows) can sum to more
