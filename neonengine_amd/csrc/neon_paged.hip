@@ -1134,12 +1134,12 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 // values, which are half of its A operand).  MXFP4 pages are expanded when a tile
 // is written.  The next tile's loads are on their way while a tile is used, and
 // LDS holds two.
-// Bound: the vector units (69% busy: an exponential, at a quarter of their rate, and
-// some five plain instructions a score) beside the matrix units (40%): the last 2048
-// and 819 rows of 6001 and 2925 tokens, 64 heads, in 250 us, 800 TFLOP/s; one
-// prompt of 8192 tokens 788, heads of 128 893.
-// P is rounded to bf16, and the row sums come from the same rounded values (a
-// product with ones), so the rounding cancels where a row's weights share it.
+// P is kept in two bf16 terms (2^-16 of a weight), as over the contiguous cache: with
+// one, 2^-9 of a weight, the prompt chunk below took 253 us.
+// Bound: the vector units (76% busy: an exponential and some eight plain instructions
+// a score) beside the matrix units (39%): the last 2048 and 819 rows of 6001 and 2925
+// tokens, 64 heads, in 341 us, 590 TFLOP/s; one prompt of 8192 tokens 609, heads of
+// 128 690.
 typedef short ps4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 pa_read_tr(const void* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -1280,7 +1280,7 @@ __device__ __forceinline__ void pm_join(const PagedAttnArgs& a, const PaWork& w,
 }
 
 // Three blocks of a CU at D = 64 (168 registers; 169, and so two of them, made the
-// prompt chunk 298 us), two at 128.
+// prompt chunk 393 us), two at 128.
 template <int D, bool F4>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedAttnArgs a) {
   constexpr int R = 128, E = D / 16, W = D / 8;  // W: 16-byte words of a row
@@ -1425,13 +1425,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
     }
   };
 
-  pf4 o[2][E], l[2];
-  float m[2];
+  pf4 o[2][E];
+  float m[2], l[2];  // l: of the lane's keys
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int e = 0; e < E; ++e) o[t][e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-    l[t] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    l[t] = 0.0f;
     m[t] = -INFINITY;
   }
   auto compute = [&](int it, uint32_t dead) {
@@ -1463,7 +1463,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
             s[t][k][i] = seen ? s[t][k][i] : -INFINITY;
           }
     }
-    uint4 p_[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float mx = -INFINITY;
@@ -1481,22 +1480,28 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
         l[t] *= f;
         m[t] = mn;
       }
-      const float me = m[t] == -INFINITY ? 0.0f : m[t];
-      uint32_t pw[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2)
-          pw[2 * k + i / 2] =
-              pack_bf2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i], c2, -me)),
-                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i + 1], c2, -me)));
-      p_[t][0] = make_uint4(pw[0], pw[1], pw[2], pw[3]);
-      p_[t][1] = make_uint4(pw[4], pw[5], pw[6], pw[7]);
-      l[t] = pa_mfma(kPaOnes, p_[t][0], l[t]);
-      l[t] = pa_mfma(kPaOnes, p_[t][1], l[t]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+      uint4 ph[2], pl[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float me = m[t] == -INFINITY ? 0.0f : m[t];
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * k + j][i], c2, -me));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * k + j][i + 1], c2, -me));
+            const uint32_t x = pack_bf2(p0, p1);
+            l[t] += p0 + p1;
+            hi[2 * j + i / 2] = x;
+            lo[2 * j + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
+          }
+        ph[t] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        pl[t] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
       // lane (g, c) reads dims 4 (c & 3) .. of key 4 g + c / 4 of each 16, for each
       // 16 dims, and gets dim c of the keys 4 g ..
       const int key = 32 * k + 4 * g + (c >> 2);  // (the second 16 exchange alike)
@@ -1507,7 +1512,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
         const uint2 x = pa_read_tr(p), y = pa_read_tr(p + 16 * 16 * W);
         const uint4 f = make_uint4(x.x, x.y, y.x, y.y);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) o[t][e] = pa_mfma(f, p_[t][k], o[t][e]);
+        for (int t = 0; t < 2; ++t) {
+          o[t][e] = pa_mfma(f, ph[t], o[t][e]);
+          o[t][e] = pa_mfma(f, pl[t], o[t][e]);
+        }
       }
     }
   };
@@ -1527,22 +1535,43 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
 
   // lane (g, c): row c of each tile, dims 16 e + 4 g ..
   __syncthreads();
-  if (odd != 0) {
-    for (int it = 0; it < n_it; ++it) {
-      const int kb = w.k0 + 64 * it;
-      if (!at_edge(kb)) continue;
-      pa_odd_values<D, F4>(a, w, h, kb, 64, [&](int key, auto value) {
+  // as in the other kernel: infinities and NaNs cleared at an edge, and infinities
+  // that met both terms of P
+  float z = 0.0f;  // NaN where an element is not finite
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = value(16 * e + 4 * g + i);
+    for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-              if (key >= k_lo[t] && key < k_hi[t] && v != 0.0f) o[t][e][i] += v;
-          }
-      });
-    }
+      for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[t][e][i], 0.0f, z);
+  if (odd != 0 || __any(z != z)) {
+    pf4 sum[2][E];  // of the infinities and NaNs alone
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[t][e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    pa_odd_values<D, F4>(a, w, h, w.k0, w.k1 - w.k0, [&](int key, auto value) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = value(16 * e + 4 * g + i);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (key >= k_lo[t] && key < k_hi[t]) sum[t][e][i] += v;
+        }
+    });
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][e][i] = sum[t][e][i] != 0.0f ? sum[t][e][i] : o[t][e][i];
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    l[t] += xor_lane<16>(l[t]);
+    l[t] += xor_lane<32>(l[t]);
   }
   if (w.chunks == 1) {
 #pragma unroll
@@ -1550,7 +1579,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
       const int r = r_first + 16 * t + c;
       if (r >= rows) continue;
       const int head = h * G + r % G;
-      const float fin = pa_finish(a, head, m[t], l[t][0]);
+      const float fin = pa_finish(a, head, m[t], l[t]);
       uint16_t* dst = a.out + ((int64_t)(w.start + r / G) * a.Hq + head) * D + 4 * g;
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -1572,7 +1601,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
       pa_store_agent(po + r * D + 16 * e + 4 * g, o[t][e][0], o[t][e][1]);
       pa_store_agent(po + r * D + 16 * e + 4 * g + 2, o[t][e][2], o[t][e][3]);
     }
-    if (g == 0) pa_store_agent(po + R * D + 2 * r, m[t], l[t][0]);
+    if (g == 0) pa_store_agent(po + R * D + 2 * r, m[t], l[t]);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have completed
   __syncthreads();

@@ -141,3 +141,72 @@ def attention(batch, q, sinks, window, hidden=lambda b, t: None):
             out[r0:r0 + n, h] = p @ vg
             mag[r0:r0 + n, h] = p @ np.abs(vg)
     return out, mag
+
+
+class Route:
+    """How neon_paged_attn takes a batch (the rules of its launch and of its block
+    finder), so that a test can say which kernel and which split it reaches.
+    many[b]: sequence b's rows are the many-row kernel's; of each kernel ("few",
+    "many") chunk, its keys, and why: "share" (equal work for every block), "cost"
+    (of the join) or "uncut"; fitted: chunks made larger to fit the chip at once."""
+
+    def __init__(self, batch, Hq, window):
+        lens, page, Hkv, B = batch.lens, batch.page, batch.Hkv, len(batch.lens)
+        self.G = G = Hq // Hkv
+        self.batch, self.Hkv, self.window = batch, Hkv, window
+        holds = min(batch.table.shape[1] * page, 1 << 30)
+
+        def keys(R, align):
+            return min(holds, window + (R - 1) // G + align) if window > 0 else holds
+
+        def blocks(units, most, target):
+            return min(target // Hkv + 1 + units, units * -(-most // 256)) * Hkv
+
+        rows, starts = batch.n_rows * G, batch.q_start is not None
+        units = rows // 16 + B
+        few = 0 if not starts and G > 32 else blocks(min(units, 2 * B), keys(16, 32), 1024)
+        small = units * Hkv + 131072 // 256 + 2
+        can = (rows > 32 if starts else G > 32) and small <= max(few, 1024)
+        work = sum(-(-n * G // 16) * self.span(t, 16, 32) for n, t in lens) * Hkv
+        self.small = can and work <= 131072
+        self.near = can and abs(work / 131072 - 1) < 0.01  # the kernel's fp32 sum may differ
+        self.many = [t > 0 and n * G > 32 and not self.small for n, t in lens]
+        self.chunk, self.why, self.fitted = {}, {}, {}
+        for kind, R, align, target, places in (
+                ("few", 16, 32, 1024, 256 * (3 if batch.D == 64 or batch.mx else 2)),
+                ("many", 128, 64, 512, 512)):
+            self._cut(kind, R, align, target, places)
+
+    def span(self, t, R, align):
+        return t if self.window <= 0 or self.window >= t else \
+            min(t, self.window + (R - 1) // self.G + align)
+
+    def _cut(self, kind, R, align, target, places):
+        mine = [(n, t) for (n, t), m in zip(self.batch.lens, self.many)
+                if n and t and m == (kind == "many")]
+        if not mine:
+            return
+        tiles = [-(-n * self.G // R) for n, _ in mine]
+        span = [self.span(t, R, align) for _, t in mine]
+        share = sum(a * s for a, s in zip(tiles, span)) * self.Hkv * 1.001 / target
+        most, fit = max(span), kind == "few" and self.batch.mx
+        cost = ((10 if kind == "few" else 25) * most) ** 0.5
+        least, why = max((share, "share"), (511, "uncut") if most <= 512 else (cost, "cost"))
+        if kind == "few" and sum(tiles) * self.Hkv <= places and \
+                most <= share * (target / (384 if fit else 256)) + 512 and most > least:
+            least, why = most, "uncut"
+        chunk = max(256, (int(least) + 128) & ~127)
+        n = 0
+        while fit and n < 3 and len(self.batch.lens) <= 64:
+            over = sum(a * -(-s // chunk) for a, s in zip(tiles, span)) * self.Hkv / places
+            if not 1 < over <= 2:
+                break
+            chunk, n = (int(chunk * over) + 128) & ~127, n + 1
+        self.chunk[kind], self.why[kind], self.fitted[kind] = chunk, why, n
+
+    def chunks(self, b):
+        """Chunks of sequence b's longest tile."""
+        n, t = self.batch.lens[b]
+        kind = "many" if self.many[b] else "few"
+        span = self.span(t, *((128, 64) if self.many[b] else (16, 32)))
+        return -(-span // self.chunk[kind]) if n and t else 0

@@ -1,0 +1,176 @@
+"""GPU tests of the paged calls form by form: which kernel and which split a case
+reaches is asserted from the launch's own rules (paged_util.Route).
+
+Bounds are computed from the inputs.  With S = max_j sum_d |q_d k_d| / sqrt(D) over
+the keys that a row sees, n of them, and A = sum_j p_j |v_j| in 64 bits:
+  a score is a sum of D exact products in fp32, each addition off by at most 2^-23
+  of S (truncated or rounded), then scaled, shifted by the maximum and raised to a
+  power by instructions good to 2^-22 of S and 2^-22: (D + 4) 2^-23 S + 2^-22;
+  a weight p_j is off by that relative to itself, and by as much again from the
+  normalising sum;
+  P is kept in two bf16 terms: 2^-16;
+  sums of n terms in fp32: n 2^-23, and again in the normalising sum;
+  the output is rounded to bf16: 2^-8 of itself.
+So |got - ref| <= 2^-8 |ref| + 1.01 A (2 ((D + 4) 2^-23 S + 2^-22) + 2^-16 + n 2^-22)."""
+import sys
+
+import numpy as np
+import pytest
+
+import neonengine_amd as ne
+from tests.gpu_util import empty_dev, to_dev, to_host, torch_cuda
+from tests.paged_util import Batch, Route, attention, bf16, f32
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+def limits(bt, q, ref, mag, window):
+    """The bound above, per row, head and dim (rows of no sequence: 0)."""
+    n_rows, Hq, D = q.shape
+    S, seen = np.zeros((n_rows, Hq)), np.zeros(n_rows)
+    for b, (n, t) in enumerate(bt.lens):
+        if n == 0 or t == 0:
+            continue
+        k, r0 = np.abs(bt.get("k", b)), int(bt.starts[b])
+        pos = np.arange(t - n, t)
+        lo = np.maximum(0, pos - window + 1) if window else np.zeros(n, int)
+        vis = (np.arange(t) <= pos[:, None]) & (np.arange(t) >= lo[:, None])
+        seen[r0:r0 + n] = vis.sum(1)
+        for h in range(Hq):
+            s = np.abs(q[r0:r0 + n, h]).astype(np.float64) @ k[:, h // (Hq // bt.Hkv)].T
+            S[r0:r0 + n, h] = np.where(vis, s, 0).max(1) / np.sqrt(D)
+    rel = 2 * ((D + 4) * 2.0 ** -23 * S + 2.0 ** -22) + 2.0 ** -16 + seen[:, None] * 2.0 ** -22
+    return 2.0 ** -8 * np.abs(ref) + 1.01 * rel[..., None] * mag + 1e-30
+
+
+def attend(bt, q, sk, window, left=0x1357, **kw):
+    d = bt.dev()
+    out = to_dev(np.full(q.shape, left, np.uint16))
+    ne.paged_attn(d["kv"], to_dev(q), None if sk is None else to_dev(bf16(sk)), d["q_start"],
+                  d["kv_len"], d["table"], out, q.shape[1], window=window, **kw)
+    return to_host(out)
+
+
+def compare(bt, q, sk, window, got=None, left=0x1357):
+    if got is None:
+        got = attend(bt, q, sk, window, left)
+    ref, mag = attention(bt, f32(q), sk, window)
+    none = np.isnan(mag)
+    assert np.array_equal(got[none], np.full(none.sum(), left, np.uint16))
+    bound = limits(bt, f32(q), np.where(none, 0, ref), np.where(none, 0, mag), window)
+    g = f32(got).astype(np.float64)
+    off = np.where(none, 0, np.abs(g - np.where(none, 0, ref)) / bound)
+    say(f"  worst error / bound = {off.max():.3f}")
+    assert off.max() <= 1.0, (off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+def make(mx, D, Hq, Hkv, page, lens, window, seed, scale=0.5, sinks=True, **kw):
+    rng = np.random.default_rng(seed)
+    bt = Batch(rng, lens, page, Hkv, D, mx, **kw).fill(rng)
+    q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32) * scale)
+    sk = f32(bf16(rng.normal(size=Hq).astype(np.float32))) if sinks else None
+    return bt, q, sk
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,window,many", [
+    (False, 64, 64, 8, [(1200, 1200)], 4, True),
+    (False, 128, 32, 8, [(1100, 1300), (900, 900)], 3, True),
+    (True, 64, 64, 8, [(1200, 1200)], 4, True),
+    (True, 128, 32, 8, [(1100, 1300), (900, 900)], 3, True),
+    (False, 64, 64, 8, [(n, n) for n in (5, 6, 3, 8, 2, 1, 4)] + [(500, 500)], 0, True),
+    (False, 64, 64, 8, [(1, n) for n in (1, 2, 3, 4, 5, 6, 7, 8)], 0, False),
+    (False, 128, 32, 8, [(2, n) for n in (2, 3, 4, 5, 6, 7, 8)], 4, False),
+])
+def test_weights_keep_sixteen_bits(mx, D, Hq, Hkv, lens, window, many):
+    """Rows that see few keys, where a weight's own rounding shows."""
+    torch_cuda()
+    say(f"weights mx={mx} D={D} Hq={Hq} Hkv={Hkv} lens={lens} window={window}")
+    bt, q, sk = make(mx, D, Hq, Hkv, 16, lens, window, seed=D + window + mx)
+    r = Route(bt, Hq, window)
+    assert not r.near and any(r.many) is many
+    compare(bt, q, sk, window)
+    ne.device_check()
+
+
+def odd_attention(bt, q, window):
+    """attention() without sinks where keys and values hold NaNs and infinities: a
+    row has those of the tokens that it sees, whatever their weight; and mag."""
+    n_rows, Hq, D = q.shape
+    out, mag = np.full((n_rows, Hq, D), np.nan), np.full((n_rows, Hq, D), np.nan)
+    for b, (n, t) in enumerate(bt.lens):
+        k, v, r0 = bt.get("k", b), bt.get("v", b), int(bt.starts[b])
+        pos, key = np.arange(t - n, t), np.arange(t)
+        seen = key[None] <= pos[:, None]
+        if window:
+            seen &= key[None] > pos[:, None] - window
+        for h in range(Hq):
+            g = h // (Hq // bt.Hkv)
+            bad = ~np.isfinite(k[:, g]).all(1)
+            kg = np.where(bad[:, None], 0, k[:, g])
+            s = np.where(seen, q[r0:r0 + n, h].astype(np.float64) @ kg.T / np.sqrt(D), -np.inf)
+            e = np.exp(s - s.max(1, keepdims=True))
+            p = e / e.sum(1, keepdims=True)
+            vg = np.where(np.isfinite(v[:, g]), v[:, g], 0)
+            o = p @ vg
+            up, down, nan = (seen.astype(np.float64) @ x > 0 for x in
+                             (v[:, g] == np.inf, v[:, g] == -np.inf, np.isnan(v[:, g])))
+            o = np.where(up, np.inf, np.where(down, -np.inf, o))
+            o = np.where(nan | (up & down) | (seen & bad).any(1)[:, None], np.nan, o)
+            out[r0:r0 + n, h], mag[r0:r0 + n, h] = o, p @ np.abs(vg)
+    return out, mag
+
+
+def put_odd(bt, x, b, tok, head, dim, value):
+    """One element of a token's key or value (MXFP4: its whole block is NaN then)."""
+    pg, at = (int(i[0]) for i in bt.places(b, tok, tok + 1))
+    if bt.mx:
+        getattr(bt, x + "s")[pg, head, at, dim // 32] = 255
+    else:
+        getattr(bt, x)[pg, head, at, dim] = np.float32(value).view(np.uint32) >> 16
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,window", [
+    (False, 64, 64, 8, [(400, 450), (1, 30)], 0),
+    (False, 64, 64, 8, [(500, 900)], 100),
+    (False, 128, 32, 8, [(300, 700)], 0),
+    (False, 128, 32, 8, [(900, 1000)], 70),
+    (True, 128, 32, 8, [(900, 1000)], 70),
+])
+def test_odd_values_in_tiles_of_many_rows(mx, D, Hq, Hkv, lens, window):
+    """NaNs and infinities in tokens that all rows of a tile see (both terms of a
+    weight meet them), that some see, and behind a window."""
+    torch_cuda()
+    say(f"odd values mx={mx} D={D} lens={lens} window={window}")
+    bt, q, _ = make(mx, D, Hq, Hkv, 16, lens, window, seed=D + window + 7, sinks=False)
+    r = Route(bt, Hq, window)
+    assert not r.near and r.many[0]
+    inf, nan = np.inf, np.nan
+    n, t = lens[0]
+    for i, tok in enumerate((t - n, t - n + 1, t - n + 66, t - 70, t - 2, t - 1)):
+        put_odd(bt, "v", 0, tok, 0, i, (inf, nan, -inf, inf, nan, -inf)[i])
+        put_odd(bt, "v", 0, tok, Hkv - 1, D - 10 + i % 2, (inf, inf, -inf, inf, inf, -inf)[i])
+    if t > n:
+        put_odd(bt, "v", 0, 0, 1, 5, inf)
+        put_odd(bt, "v", 0, 1, 2, 6, nan)
+    put_odd(bt, "k", 0, t - 1, 3, 2, nan)
+    got = f32(attend(bt, q, None, window)).astype(np.float64)
+    ne.device_check()
+    want, mag = odd_attention(bt, f32(q), window)
+    fine = np.isfinite(want)
+    assert 0 < (~fine).sum() < fine.size
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    odd = ~fine & ~np.isnan(want)
+    assert mx or odd.any()
+    assert np.array_equal(got[odd], want[odd])
+    k = getattr(bt, "ks" if mx else "k")  # for the bound: the NaN key counts as a zero
+    pg, at = (int(i[0]) for i in bt.places(0, t - 1, t))
+    k[pg, 3, at] = 0
+    bound = limits(bt, f32(q), np.where(fine, want, 0), mag, window)
+    off = np.where(fine, np.abs(np.where(fine, got - np.where(fine, want, 0), 0)) / bound, 0)
+    say(f"  worst error / bound = {off.max():.3f}")
+    assert off.max() <= 1.0
