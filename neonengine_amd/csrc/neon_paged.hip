@@ -334,7 +334,6 @@ __device__ __forceinline__ pf4 pa_mfma(const uint4& a, const uint4& b, pf4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pbf8, a),
                                                  __builtin_bit_cast(pbf8, b), c, 0, 0, 0);
 }
-#define kPaOnes make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A block's work: keys [k0, k1) of a unit, all wave-uniform.
@@ -862,8 +861,8 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // operands' registers, some steps ahead of the products.
 // Bound: the bytes of the visible keys, read once (64 sequences of up to 8192
 // tokens, 8 heads of 64 for 64: 285 MB in 65 us, 4.4 TB/s; 256 of 2000: 5.4 TB/s);
-// MXFP4 at 3 to 3.6 TB/s by the vector units as well, which expand the codes
-// (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, half busy); few short
+// MXFP4 at 2.9 to 3.6 TB/s by the vector units as well, which expand the codes
+// (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, 54% busy); few short
 // sequences by the chain of lookups, loads and the join (5 us for one of 64 tokens).
 // Waves of a SIMD, and blocks of a CU (four of D = 64: bf16 spills, MXFP4 4 sequences
 // of up to 131072 tokens 29.1 -> 30.3 us)
@@ -909,7 +908,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY;
-  pf4 l = pf4{0.0f, 0.0f, 0.0f, 0.0f};  // [0]: of the lane's keys (MXFP4: of all)
+  float l = 0.0f;  // of the lane's keys
 
   const int tiles = (w.k1 - w.k0 + 31) >> 5;
   const int n_it = (tiles - wave + 3) >> 2;  // this wave's
@@ -980,8 +979,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
       m = mn;
     }
     const float me = m == -INFINITY ? 0.0f : m;
-    // P in two bf16 terms.  Over MXFP4 pages, where the vector instructions are the
-    // bound, in one, with the row's sum taken from the rounded values by a product.
+    // P in two bf16 terms (2^-16 of a weight)
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -991,11 +989,9 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[s][i + 1], c2, -me));
         const uint32_t x = pack_bf2(p0, p1);
         hi[2 * s + i / 2] = x;
-        if constexpr (!F4) {
-          l[0] += p0;
-          l[0] += p1;
-          lo[2 * s + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
-        }
+        l += p0;
+        l += p1;
+        lo[2 * s + i / 2] = pack_bf2(p0 - bf_lo(x), p1 - bf_hi(x));
       }
     uint32_t v[2][4][D / 32];
 #pragma unroll
@@ -1003,8 +999,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 #pragma unroll
       for (int i = 0; i < 4; ++i) pa_value<D>(t, s, i, c, v[s][i]);
     const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    const uint4 pl = F4 ? ph : make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    if constexpr (F4) l = pa_mfma(kPaOnes, ph, l);
+    const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       uint32_t f[4];
@@ -1014,7 +1009,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
                                      e & 1 ? 0x07060302u : 0x05040100u);
       const uint4 vf = make_uint4(f[0], f[1], f[2], f[3]);
       o[e] = pa_mfma(vf, ph, o[e]);
-      if constexpr (!F4) o[e] = pa_mfma(vf, pl, o[e]);
+      o[e] = pa_mfma(vf, pl, o[e]);
     }
   };
   if (n_it > 0) {
@@ -1038,14 +1033,12 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
   }
   // An infinity among the values of a step that every row sees meets both terms of P:
   // its product with the second is the other infinity, or NaN.
-  if constexpr (!F4) {
-    float z = 0.0f;  // NaN where an element is not finite
+  float z = 0.0f;  // NaN where an element is not finite
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+  for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[e][i], 0.0f, z);
-    odd = odd || z != z;
-  }
+    for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[e][i], 0.0f, z);
+  odd = odd || z != z;
   if (__any(odd)) {  // lane (g, c): row c, dims (D/4) g + E i + e
     pf4 sum[E];      // of the infinities and NaNs alone
 #pragma unroll
@@ -1066,10 +1059,8 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[e][i] = sum[e][i] != 0.0f ? sum[e][i] : o[e][i];
   }
-  if constexpr (!F4) {
-    l[0] += xor_lane<16>(l[0]);
-    l[0] += xor_lane<32>(l[0]);
-  }
+  l += xor_lane<16>(l);
+  l += xor_lane<32>(l);
   // the four waves' states
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -1079,7 +1070,7 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
           make_float4(o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]);
   if (g == 0) {
     sm[wave][c] = m;
-    sl[wave][c] = l[0];
+    sl[wave][c] = l;
   }
   __syncthreads();
   // thread: row tr, dims td .. td + E - 1

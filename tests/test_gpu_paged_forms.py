@@ -85,6 +85,8 @@ def make(mx, D, Hq, Hkv, page, lens, window, seed, scale=0.5, sinks=True, **kw):
     (False, 64, 64, 8, [(n, n) for n in (5, 6, 3, 8, 2, 1, 4)] + [(500, 500)], 0, True),
     (False, 64, 64, 8, [(1, n) for n in (1, 2, 3, 4, 5, 6, 7, 8)], 0, False),
     (False, 128, 32, 8, [(2, n) for n in (2, 3, 4, 5, 6, 7, 8)], 4, False),
+    (True, 64, 64, 8, [(1, n) for n in (1, 2, 3, 4, 5, 6, 7, 8)], 0, False),
+    (True, 128, 32, 8, [(2, n) for n in (2, 3, 4, 5, 6, 7, 8)], 4, False),
 ])
 def test_weights_keep_sixteen_bits(mx, D, Hq, Hkv, lens, window, many):
     """Rows that see few keys, where a weight's own rounding shows."""
@@ -139,6 +141,7 @@ def put_odd(bt, x, b, tok, head, dim, value):
     (False, 64, 64, 8, [(500, 900)], 100),
     (False, 128, 32, 8, [(300, 700)], 0),
     (False, 128, 32, 8, [(900, 1000)], 70),
+    (True, 64, 64, 8, [(400, 450), (1, 30)], 0),
     (True, 128, 32, 8, [(900, 1000)], 70),
 ])
 def test_odd_values_in_tiles_of_many_rows(mx, D, Hq, Hkv, lens, window):
