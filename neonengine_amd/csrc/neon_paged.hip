@@ -662,8 +662,13 @@ __device__ __forceinline__ void pa_clear(PaTile<D, true>& t, int s, int i, int c
   const uint32_t byte = D == 64 ? word >> (16 * (i & 1) + (c & 8)) : word >> (2 * (c & 12));
   const bool nan = (byte & 0xFFu) == 0xFFu;
   const bool clear = none || nan;
-  odd = odd || (nan && !none);
-  t.v[s][i] = clear ? 0u : t.v[s][i];
+  // 4 and 6 times 2^126, and from 2 on times 2^127, read as infinities: those codes
+  // (the word's other lanes' too, which this lane does not use)
+  const uint32_t two = t.v[s][i] & 0x44444444u, four = two & t.v[s][i] << 1;
+  uint32_t inf = (byte & 0xFFu) == 254u ? two : (byte & 0xFFu) == 253u ? four : 0u;
+  inf |= inf << 1 | inf >> 1 | inf >> 2;
+  odd = odd || ((nan || inf != 0) && !none);
+  t.v[s][i] = clear ? 0u : t.v[s][i] & ~inf;
   word = clear ? word & keep : word;
 }
 // fn(key, value(d)) for the keys [kb, kb + n): the infinities and NaNs of a value, 0

@@ -106,6 +106,7 @@ def odd_attention(bt, q, window):
     out, mag = np.full((n_rows, Hq, D), np.nan), np.full((n_rows, Hq, D), np.nan)
     for b, (n, t) in enumerate(bt.lens):
         k, v, r0 = bt.get("k", b), bt.get("v", b), int(bt.starts[b])
+        v = np.where(np.abs(v) >= 2.0 ** 128, np.copysign(np.inf, v), v)  # as bf16 reads them
         pos, key = np.arange(t - n, t), np.arange(t)
         seen = key[None] <= pos[:, None]
         if window:
@@ -173,6 +174,52 @@ def test_odd_values_in_tiles_of_many_rows(mx, D, Hq, Hkv, lens, window):
     k = getattr(bt, "ks" if mx else "k")  # for the bound: the NaN key counts as a zero
     pg, at = (int(i[0]) for i in bt.places(0, t - 1, t))
     k[pg, 3, at] = 0
+    bound = limits(bt, f32(q), np.where(fine, want, 0), mag, window)
+    off = np.where(fine, np.abs(np.where(fine, got - np.where(fine, want, 0), 0)) / bound, 0)
+    say(f"  worst error / bound = {off.max():.3f}")
+    assert off.max() <= 1.0
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,lens,window,many", [
+    (64, 16, 2, [(2, 70), (2, 40)], 0, False),
+    (64, 16, 2, [(4, 300)], 40, False),
+    (128, 8, 2, [(6, 90)], 0, False),
+    (128, 8, 2, [(5, 300)], 17, False),
+    (64, 64, 8, [(400, 450)], 0, True),
+    (128, 32, 8, [(900, 1000)], 70, True),
+])
+def test_mxfp4_values_past_bf16(D, Hq, Hkv, lens, window, many):
+    """Scales of 2^126 and 2^127 make infinities of the larger codes: theirs are the
+    rows that see them, and the finite values beside them stay."""
+    torch_cuda()
+    say(f"mxfp4 past bf16 D={D} lens={lens} window={window}")
+    bt, q, _ = make(True, D, Hq, Hkv, 16, lens, window, seed=D + window, sinks=False)
+    r = Route(bt, Hq, window)
+    assert not r.near and r.many[0] is many
+
+    def put(b, tok, head, block, scale, codes):  # codes: {dim of the block: code}
+        pg, at = (int(i[0]) for i in bt.places(b, tok, tok + 1))
+        bt.vs[pg, head, at, block] = scale
+        row = bt.v[pg, head, at, 16 * block:16 * block + 16]
+        row[:] = 0
+        for d, code in codes.items():
+            row[d // 2] |= code << 4 * (d % 2)
+
+    n, t = lens[0]
+    for i, tok in enumerate((t - 1, t - 2, t - n + 1)):
+        put(0, tok, i % 2, 0, 254, {i: 7, 5 + i: 12})          # 6 and -2 times 2^127
+        put(0, tok, i % 2, 1, 253, {i: 6, 9 + i: 15, 20: 0})   # 4 and -6 times 2^126
+    put(0, t - 1, 1, 0, 253, {30: 5})                          # 3 times 2^126: finite
+    if window:
+        put(0, t - n - window + 1, 0, 1, 254, {31: 4})
+    got = f32(attend(bt, q, None, window)).astype(np.float64)
+    ne.device_check()
+    want, mag = odd_attention(bt, f32(q), window)
+    fine = np.isfinite(want)
+    assert 0 < (~fine).sum() < fine.size
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+    assert (np.abs(want[fine]) > 2.0 ** 100).any()
     bound = limits(bt, f32(q), np.where(fine, want, 0), mag, window)
     off = np.where(fine, np.abs(np.where(fine, got - np.where(fine, want, 0), 0)) / bound, 0)
     say(f"  worst error / bound = {off.max():.3f}")
