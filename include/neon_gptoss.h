@@ -539,7 +539,8 @@ neon_status neon_paged_attn(const neon_paged_kv* kv, const uint16_t* q, int64_t 
  * parameter outside its range (temperature < 0 or infinite, top_p outside
  * (0, 1], min_p outside [0, 1], u outside [0, 1), a NaN) gives -1 and
  * neon_device_check NEON_EINVAL.  V up to 2^24.  workspace:
- * neon_sample_rows_workspace(B, V) bytes, 16-byte aligned, any contents. */
+ * neon_sample_rows_workspace(B, V) bytes, 16-byte aligned, any contents; they
+ * serve every call of up to B rows of V tokens. */
 size_t neon_sample_rows_workspace(int B, int V);
 neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
                              const float* temperature, const int32_t* top_k, const float* top_p,

@@ -2386,7 +2386,7 @@ extern "C" neon_status neon_sample_rows(const float* logits, int64_t stride, int
   if (B < 1 || B > 65535 || V < 1 || V > (1 << 24) || stride < V)
     KFAIL(NEON_EINVAL, "neon_sample_rows: bad shape B=%d V=%d stride=%lld", B, V,
           (long long)stride);
-  const size_t need = neon_sample_rows_workspace(B, V);
+  const size_t need = sample_rows_needs(B, V);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     KFAIL(NEON_EINVAL, "neon_sample_rows: workspace of %zu bytes, %zu needed (16-byte aligned)",
           workspace_bytes, need);

@@ -457,7 +457,8 @@ struct SampleRowsArgs {
   void* workspace;
   int chunk, chunks;  // set by the launcher
 };
-size_t sample_rows_workspace(int B, int V);
+size_t sample_rows_needs(int B, int V);      // bytes that a launch uses
+size_t sample_rows_workspace(int B, int V);  // the most of those of up to B rows
 void launch_sample_rows(SampleRowsArgs a, hipStream_t st);
 
 }  // namespace neon

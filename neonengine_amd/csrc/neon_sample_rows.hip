@@ -922,9 +922,20 @@ static int sr_chunk(int B, int V) {
   return chunk < kSrMaxChunk ? (int)chunk : kSrMaxChunk;
 }
 
-size_t sample_rows_workspace(int B, int V) {
+size_t sample_rows_needs(int B, int V) {
   const int C = (V + sr_chunk(B, V) - 1) / sr_chunk(B, V);
   return C == 1 ? 0 : (size_t)B * sr_space_bytes(C, V);
+}
+// The most that a batch of up to B rows needs: fewer rows are cut into more chunks
+// each.  A chunk depends on 512 / B alone, so of the batches with the same quotient
+// the largest needs the most.
+size_t sample_rows_workspace(int B, int V) {
+  size_t most = sample_rows_needs(B, V);
+  for (int b = B < 512 ? B : 511; b >= 1; b = 512 / (512 / b + 1)) {
+    const size_t n = sample_rows_needs(b, V);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 void launch_sample_rows(SampleRowsArgs a, hipStream_t st) {
