@@ -17,6 +17,7 @@ namespace neon {
 // ---------------------------------------------------------------------------
 // Rows of the batch
 // ---------------------------------------------------------------------------
+constexpr int kPagedLongest = 1 << 30;
 // Whether a sequence's rows and length are ones that the buffers hold (device
 // data: checked before anything is addressed with it).  A sequence of length 0
 // is a free place of the batch: it has no rows to take.  Lengths up to 2^30
@@ -24,7 +25,7 @@ namespace neon {
 __device__ __forceinline__ bool paged_fits(const PagedRows& r, int page_log2, int start, int end,
                                            int len) {
   return (start >= 0) & (end >= start) & (end <= r.n_rows) & (len >= end - start) &
-         (len <= (1 << 30)) & ((int64_t)len <= ((int64_t)r.max_pages << page_log2));
+         (len <= kPagedLongest) & ((int64_t)len <= ((int64_t)r.max_pages << page_log2));
 }
 __device__ __forceinline__ bool paged_seq(const PagedRows& r, int page_log2, int b, int& start,
                                           int& n, int& len) {
@@ -38,16 +39,17 @@ __device__ __forceinline__ bool paged_seq(const PagedRows& r, int page_log2, int
 // The sequence and position of a row, found by the wave (every lane calls it with
 // the same row); false when the row belongs to no sequence.  A lane looks at a
 // sequence with loads that depend on nothing, so a row costs one round trip
-// (reading the found one's numbers again made it three).  The wave that asks for
+// (reading the found one's numbers again made it three).  A sequence that has rows
+// fits up to `most` tokens (the positions that have angles).  The wave that asks for
 // row 0 with `report` reports the sequences that do not fit.
-__device__ __forceinline__ bool paged_row(const PagedRows& r, int page_log2, int row, bool report,
-                                          int& b, int& pos) {
+__device__ __forceinline__ bool paged_row(const PagedRows& r, int page_log2, int most, int row,
+                                          bool report, int& b, int& pos) {
   const int lane = threadIdx.x & 63;
   if (r.q_start == nullptr) {
     b = row;
     const int len = r.kv_len[row];
     pos = len - 1;
-    const bool ok = paged_fits(r, page_log2, row, row + 1, len);
+    const bool ok = paged_fits(r, page_log2, row, row + 1, len) & (len <= most);
     if (!ok && len != 0 && report && lane == 0) flag_dev_err(r.err, kDevErrPagedRows);
     return ok;
   }
@@ -55,7 +57,7 @@ __device__ __forceinline__ bool paged_row(const PagedRows& r, int page_log2, int
   for (int i0 = 0; i0 < r.B; i0 += 64) {
     const int i = min(i0 + lane, r.B - 1);  // (past the end: the last one again)
     const int start = r.q_start[i], end = r.q_start[i + 1], len = r.kv_len[i];
-    const bool ok = paged_fits(r, page_log2, start, end, len);
+    const bool ok = paged_fits(r, page_log2, start, end, len) & ((len <= most) | (start == end));
     if (row == 0 && report && !ok && len != 0) flag_dev_err(r.err, kDevErrPagedRows);
     const uint64_t in = __ballot(ok & (start <= row) & (row < end));
     if (b < 0 && in != 0) {
@@ -154,11 +156,9 @@ __global__ __launch_bounds__(512) void k_paged_append(
   const uint16_t* src0 = row_src + (int64_t)(it0 / per) * kv.D + (it0 % per) * 8;
   uint4 w1 = *reinterpret_cast<const uint4*>(src0), w2 = *reinterpret_cast<const uint4*>(src0 + half);
   int b, pos;
-  if (!paged_row(r, kv.page_log2, row, threadIdx.x < 64, b, pos)) return;
-  if (cos_t != nullptr && pos >= n_pos) {
-    if (threadIdx.x == 0) flag_dev_err(r.err, kDevErrPagedRows);
+  if (!paged_row(r, kv.page_log2, cos_t != nullptr ? n_pos : kPagedLongest, row,
+                 threadIdx.x < 64, b, pos))
     return;
-  }
   // the first elements' angles with the page id, in one round trip
   const int id = r.table[(int64_t)b * r.max_pages + (pos >> kv.page_log2)];
   float4 cs[4];
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void k_paged_gather(PagedKv kv, PagedRows r,
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= r.n_rows) return;
   int b, pos;
-  if (!paged_row(r, kv.page_log2, row, true, b, pos)) return;
+  if (!paged_row(r, kv.page_log2, kPagedLongest, row, true, b, pos)) return;
   const int id = r.table[(int64_t)b * r.max_pages + (pos >> kv.page_log2)];
   if ((unsigned)id >= (unsigned)kv.n_pages) {
     if (lane == 0) flag_dev_err(r.err, kDevErrPageId);

@@ -224,3 +224,37 @@ def test_mxfp4_values_past_bf16(D, Hq, Hkv, lens, window, many):
     off = np.where(fine, np.abs(np.where(fine, got - np.where(fine, want, 0), 0)) / bound, 0)
     say(f"  worst error / bound = {off.max():.3f}")
     assert off.max() <= 1.0
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_append_leaves_out_a_sequence_that_crosses_the_angles(mx):
+    """Positions 6 .. 11 and a table of 8: none of the rows is written; the others
+    are, and a sequence without rows may be longer than the table."""
+    torch_cuda()
+    rng = np.random.default_rng(31)
+    Hq, Hkv, D, lens = 2, 1, 64, [(2, 8), (6, 12), (0, 30), (3, 5)]
+    bt = Batch(rng, lens, 16, Hkv, D, mx).fill(rng)
+    x = to_dev(bf16(rng.normal(size=(bt.n_rows, Hq + 2 * Hkv, D)).astype(np.float32)))
+    table = rng.normal(size=(2, 12, D // 2)).astype(np.float32)
+
+    def append(n_pos, starts, kv_len):
+        d = bt.dev()
+        q_out = to_dev(np.full((bt.n_rows, Hq, D), 0x2468, np.uint16))
+        ne.paged_append(d["kv"], x, to_dev(np.ascontiguousarray(table[:, :n_pos])), to_dev(starts),
+                        to_dev(kv_len), d["table"], q_out, Hq)
+        return [to_host(q_out)] + [to_host(d[c]) for c in ("k", "v") + (("ks", "vs") if mx else ())]
+
+    got = append(8, bt.q_start, bt.kv_len)
+    with pytest.raises(ne.NeonError) as e:
+        ne.device_check()
+    assert e.value.status == ne.NEON_EINVAL
+    gone = bt.kv_len.copy()
+    gone[1] = 0  # a free place: its rows are left as they are
+    want = append(12, bt.q_start, gone)
+    ne.device_check()
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    assert (got[0][2:8] == 0x2468).all() and (got[0][[0, 1, 8, 9, 10]] != 0x2468).any((1, 2)).all()
+    fits = bt.kv_len.copy()
+    fits[1] = 8  # 6 rows, the last at position 7
+    append(8, bt.q_start, fits)
+    ne.device_check()
