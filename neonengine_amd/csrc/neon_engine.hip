@@ -2296,6 +2296,9 @@ extern "C" neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t
     KFAIL(NEON_EINVAL, "neon_paged_append: rows must be 16-byte aligned, a multiple of 8 elements "
           "and at least (Hq + 2 n_kv_heads) head_dim apart");
   if (table && n_pos < 1) KFAIL(NEON_EINVAL, "neon_paged_append: n_pos=%d", n_pos);
+  if (!paged_append_fits(n_rows, c.Hkv, Hq, c.D))
+    KFAIL(NEON_EINVAL, "neon_paged_append: %d rows of %d heads are more than a launch holds", n_rows,
+          Hq + 2 * c.Hkv);
   r.err = device_status_word();
   launch_paged_append(c, r, qkv, qkv_stride, table,
                       table ? table + (size_t)n_pos * (c.D / 2) : nullptr, n_pos, q_out, Hq,

@@ -421,6 +421,7 @@ struct PagedRows {
 void launch_paged_append(const PagedKv& kv, const PagedRows& r, const uint16_t* qkv, int64_t stride,
                          const float* cos_t, const float* sin_t, int n_pos, uint16_t* q_out, int Hq,
                          hipStream_t st);
+bool paged_append_fits(int n_rows, int Hkv, int Hq, int D);  // the launch holds them
 // the rows of the batch as the cache holds them, [n_rows][Hkv][D] bf16
 void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out, uint16_t* v_out,
                          hipStream_t st);

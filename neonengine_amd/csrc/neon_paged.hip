@@ -219,11 +219,19 @@ __global__ __launch_bounds__(512) void k_paged_append(
   }
 }
 
+static int append_threads(int Hkv, int Hq, int D) {
+  const int items = (Hq + 2 * Hkv) * (D >> 4);
+  return items >= 512 ? 512 : (items + 63) & ~63;
+}
+// a launch holds fewer than 2^32 threads
+bool paged_append_fits(int n_rows, int Hkv, int Hq, int D) {
+  return (int64_t)n_rows * append_threads(Hkv, Hq, D) < (int64_t)1 << 32;
+}
+
 void launch_paged_append(const PagedKv& kv, const PagedRows& r, const uint16_t* qkv, int64_t stride,
                          const float* cos_t, const float* sin_t, int n_pos, uint16_t* q_out, int Hq,
                          hipStream_t st) {
-  const int items = (Hq + 2 * kv.Hkv) * (kv.D >> 4);
-  const dim3 grid(r.n_rows), block(items >= 512 ? 512 : (items + 63) & ~63);
+  const dim3 grid(r.n_rows), block(append_threads(kv.Hkv, Hq, kv.D));
 #define PAPP(F4)                                                                               \
   hipLaunchKernelGGL(k_paged_append<F4>, grid, block, 0, st, kv, r, qkv, stride, cos_t, sin_t, \
                      n_pos, q_out, Hq)

@@ -14,3 +14,13 @@ def test_sampling_workspace_never_falls(V):
 def test_attention_workspace_never_falls():
     sizes = [ne.paged_attn_workspace(n, 64, 64, 8, 64) for n in (*range(1, 100), 4096, 100000)]
     assert sizes == sorted(sizes)
+
+
+def test_append_refuses_more_threads_than_a_launch_holds():
+    """2^23 rows of 512 threads are 2^32, one more than a launch has."""
+    import ctypes as C
+    P = 4096  # an aligned address, never dereferenced: the call is refused first
+    kv = ne.PagedKVStruct(P, P, None, None, ne.KV_BF16, 8, 16, 8, 64)
+    status = ne.lib().neon_paged_append(C.addressof(kv), P, 144 * 64, P, 9, P, P, P, 1 << 20, P,
+                                        1 << 23, 2, 128, None)
+    assert status == ne.NEON_EINVAL
