@@ -206,14 +206,16 @@ def _nbytes(t):
 
 _current = None  # (device index, its stream's handle) functions, once a device was
                  # found (a process does not lose it again)
+_fp16 = None     # torch.float16 from then on: it has the size of bf16
 
 
 def _find_current():
     """Functions that give torch's current device, and its current stream there:
     torch's own shortcuts to the bare numbers where it has them
     (torch.cuda.current_stream() makes an object for 3 us)."""
-    global _current
+    global _current, _fp16
     import torch
+    _fp16 = torch.float16
     if not torch.cuda.is_available():
         return None
     torch.cuda.init()
@@ -422,7 +424,8 @@ class PagedKV:
         if tuple(v.shape) != tuple(k.shape) or \
                 any(tuple(t.shape) != (n_pages, heads, page, dim // 32) for t in pools[2:]):
             raise ValueError("PagedKV: k, v (and their scales) must have matching shapes")
-        if any(t.element_size() != (1 if mx else 2) for t in pools):
+        import torch
+        if any(t.element_size() != (1 if mx else 2) or t.dtype is torch.float16 for t in pools):
             raise ValueError("PagedKV: bf16 pools have 2-byte elements, MXFP4 codes and scales 1")
         self.pools = pools  # keeps them alive
         self.device = k.get_device()
@@ -442,11 +445,13 @@ def paged_kv(k, v, k_scales=None, v_scales=None) -> PagedKV:
 def _arg(t, size, n, name, device, real=None):
     """Device pointer of a contiguous tensor of at least n elements of this size
     on this device (its index), or ValueError: the library trusts the sizes that
-    the paged calls derive from other tensors.  real: floating point or not."""
+    the paged calls derive from other tensors.  real: floating point or not (None:
+    bf16, or integers that hold its bits)."""
     if t.element_size() != size or t.numel() < n or t.get_device() != device or \
-            not t.is_contiguous() or (real is not None and t.is_floating_point() is not real):
+            not t.is_contiguous() or t.dtype is _fp16 or \
+            (real is not None and t.is_floating_point() is not real):
         raise ValueError(f"{name}: needs {n} contiguous elements of {size} bytes"
-                         f"{'' if real is None else ' (floats)' if real else ' (integers)'} on "
+                         f"{' (bf16)' if real is None else ' (floats)' if real else ' (integers)'} on "
                          f"device {device}, has {tuple(t.shape)} of {t.dtype} on {t.device}")
     return t.data_ptr()
 
@@ -476,8 +481,9 @@ def _rows(x, size, width, name, device):
     """(device pointer, rows, elements between them) of rows of at least `width`
     elements: contiguous ones, or a slice of wider rows."""
     shape = x.shape
-    if x.element_size() != size or x.get_device() != device or len(shape) not in (2, 3):
-        raise ValueError(f"{name}: rows of elements of {size} bytes on device {device}")
+    if x.element_size() != size or x.get_device() != device or len(shape) not in (2, 3) or \
+            (x.dtype is _fp16 if size == 2 else not x.is_floating_point()):
+        raise ValueError(f"{name}: rows of {'bf16' if size == 2 else 'fp32'} on device {device}")
     n = shape[0]
     has = shape[1] if len(shape) == 2 else shape[1] * shape[2]
     stride = has if has > width else width

@@ -258,3 +258,39 @@ def test_append_leaves_out_a_sequence_that_crosses_the_angles(mx):
     fits[1] = 8  # 6 rows, the last at position 7
     append(8, bt.q_start, fits)
     ne.device_check()
+
+
+def test_wrappers_refuse_other_number_types():
+    """fp16 has the size of bf16, int32 that of fp32."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(1)
+    bt = Batch(rng, [(1, 5), (1, 5)], 16, 2, 64, False, q_start=False).fill(rng)
+    d = bt.dev()
+    args = (None, d["kv_len"], d["table"])
+
+    def rows(heads, dtype):
+        return torch.zeros((2, heads, 64), dtype=dtype, device="cuda")
+
+    b, h = torch.bfloat16, torch.float16
+    sinks = torch.zeros(4, dtype=b, device="cuda")
+    logits, ids = torch.zeros((2, 99), device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    u = torch.zeros(2, device="cuda")
+    ne.paged_attn(d["kv"], rows(4, b), sinks, *args, rows(4, b), 4)
+    ne.paged_append(d["kv"], rows(8, b), None, *args, rows(4, b), 4)
+    ne.paged_append(d["kv"], rows(8, torch.int16), None, *args, rows(4, torch.int16), 4)  # bf16 bits
+    ne.paged_gather(d["kv"], *args, rows(2, b), rows(2, b))
+    ne.sample_rows(logits, u, ids)
+    ne.device_check()
+    for call in (
+        lambda: ne.paged_attn(d["kv"], rows(4, h), sinks, *args, rows(4, b), 4),
+        lambda: ne.paged_attn(d["kv"], rows(4, b), sinks.half(), *args, rows(4, b), 4),
+        lambda: ne.paged_attn(d["kv"], rows(4, b), sinks, *args, rows(4, h), 4),
+        lambda: ne.paged_append(d["kv"], rows(8, h), None, *args, rows(4, b), 4),
+        lambda: ne.paged_append(d["kv"], rows(8, b), None, *args, rows(4, h), 4),
+        lambda: ne.paged_gather(d["kv"], *args, rows(2, h), rows(2, b)),
+        lambda: ne.paged_gather(d["kv"], *args, rows(2, b), rows(2, h)),
+        lambda: ne.paged_kv(d["k"].view(h), d["v"].view(h)),
+        lambda: ne.sample_rows(logits.int(), u, ids),
+    ):
+        with pytest.raises(ValueError):
+            call()

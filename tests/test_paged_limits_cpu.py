@@ -24,3 +24,14 @@ def test_append_refuses_more_threads_than_a_launch_holds():
     status = ne.lib().neon_paged_append(C.addressof(kv), P, 144 * 64, P, 9, P, P, P, 1 << 20, P,
                                         1 << 23, 2, 128, None)
     assert status == ne.NEON_EINVAL
+
+
+def test_paged_kv_refuses_other_number_types():
+    torch = pytest.importorskip("torch")
+    shape = (2, 1, 16, 64)
+    for dtype in (torch.bfloat16, torch.int16):
+        ne.paged_kv(torch.zeros(shape, dtype=dtype), torch.zeros(shape, dtype=dtype))
+    half, whole = (torch.zeros(shape, dtype=t) for t in (torch.float16, torch.bfloat16))
+    for k, v in ((half, half), (whole, half), (half, whole)):
+        with pytest.raises(ValueError):
+            ne.paged_kv(k, v)
