@@ -210,3 +210,7 @@ class Route:
         kind = "many" if self.many[b] else "few"
         span = self.span(t, *((128, 64) if self.many[b] else (16, 32)))
         return -(-span // self.chunk[kind]) if n and t else 0
+
+    def run(self, b):
+        """The most terms that follow one another in a sum: a chunk's, then chunks."""
+        return self.chunk["many" if self.many[b] else "few"] + self.chunks(b)

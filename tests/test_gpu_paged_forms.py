@@ -9,7 +9,8 @@ the keys that a row sees, n of them, and A = sum_j p_j |v_j| in 64 bits:
   a weight p_j is off by that relative to itself, and by as much again from the
   normalising sum;
   P is kept in two bf16 terms: 2^-16;
-  sums of n terms in fp32: n 2^-23, and again in the normalising sum;
+  sums of n terms in fp32: n 2^-23, and again in the normalising sum; of a cut axis a
+  chunk's keys and then the chunks;
   the output is rounded to bf16: 2^-8 of itself.
 So |got - ref| <= 2^-8 |ref| + 1.01 A (2 ((D + 4) 2^-23 S + 2^-22) + 2^-16 + n 2^-22)."""
 import sys
@@ -29,7 +30,7 @@ def say(*a):
     sys.stdout.flush()
 
 
-def limits(bt, q, ref, mag, window):
+def limits(bt, q, ref, mag, window, route=None):
     """The bound above, per row, head and dim (rows of no sequence: 0)."""
     n_rows, Hq, D = q.shape
     S, seen = np.zeros((n_rows, Hq)), np.zeros(n_rows)
@@ -44,6 +45,8 @@ def limits(bt, q, ref, mag, window):
         for h in range(Hq):
             s = np.abs(q[r0:r0 + n, h]).astype(np.float64) @ k[:, h // (Hq // bt.Hkv)].T
             S[r0:r0 + n, h] = np.where(vis, s, 0).max(1) / np.sqrt(D)
+        if route is not None:
+            seen[r0:r0 + n] = np.minimum(seen[r0:r0 + n], route.run(b))
     rel = 2 * ((D + 4) * 2.0 ** -23 * S + 2.0 ** -22) + 2.0 ** -16 + seen[:, None] * 2.0 ** -22
     return 2.0 ** -8 * np.abs(ref) + 1.01 * rel[..., None] * mag + 1e-30
 
@@ -62,7 +65,8 @@ def compare(bt, q, sk, window, got=None, left=0x1357):
     ref, mag = attention(bt, f32(q), sk, window)
     none = np.isnan(mag)
     assert np.array_equal(got[none], np.full(none.sum(), left, np.uint16))
-    bound = limits(bt, f32(q), np.where(none, 0, ref), np.where(none, 0, mag), window)
+    bound = limits(bt, f32(q), np.where(none, 0, ref), np.where(none, 0, mag), window,
+                   Route(bt, q.shape[1], window))
     g = f32(got).astype(np.float64)
     off = np.where(none, 0, np.abs(g - np.where(none, 0, ref)) / bound)
     say(f"  worst error / bound = {off.max():.3f}")
@@ -294,3 +298,208 @@ def test_wrappers_refuse_other_number_types():
     ):
         with pytest.raises(ValueError):
             call()
+
+
+def make_codes(D, Hq, Hkv, page, lens, seed, **kw):
+    """As make() over MXFP4 pages, of codes and scales that are random themselves
+    (quantising long caches on the host takes longer than the rest)."""
+    rng = np.random.default_rng(seed)
+    bt = Batch(rng, lens, page, Hkv, D, True, **kw)
+    for b, (_, t) in enumerate(lens):
+        pg, at = bt.places(b)
+        for x in "kv":
+            getattr(bt, x)[pg, :, at] = rng.integers(0, 256, (t, Hkv, D // 2), dtype=np.uint8)
+            getattr(bt, x + "s")[pg, :, at] = rng.integers(124, 128, (t, Hkv, D // 32), dtype=np.uint8)
+    q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32) * 0.3)
+    return bt, q, f32(bf16(rng.normal(size=Hq).astype(np.float32)))
+
+
+def build(mx, D, Hq, Hkv, page, lens, seed, **kw):
+    if mx:
+        return make_codes(D, Hq, Hkv, page, lens, seed, **kw)
+    return make(False, D, Hq, Hkv, page, lens, 0, seed, **kw)
+
+
+JOINS = [
+    # (rows, length, Hkv, chunks): of the longest tile
+    (330, 800, 8, (2, 4)),      # every tile has more than 64 rows
+    (300, 900, 8, (2, 4)),      # the last one 44
+    (200, 1500, 8, (5, 8)),
+    (70, 2000, 16, (5, 8)),
+    (60, 1900, 32, (5, 8)),     # no tile of more than 64
+    (100, 4000, 8, (9, 32)),
+    (40, 60000, 2, (33, 64)),
+    (100, 60000, 2, (33, 64)),
+]
+
+
+@pytest.mark.parametrize("rows,length,Hkv,chunks", JOINS)
+@pytest.mark.parametrize("mx,D", [(False, 64), (False, 128), (True, 64), (True, 128)])
+def test_joins_in_the_many_row_kernel(rows, length, Hkv, chunks, mx, D):
+    torch_cuda()
+    say(f"join mx={mx} D={D} rows={rows} length={length} Hkv={Hkv}")
+    bt, q, sk = build(mx, D, Hkv, Hkv, 64, [(rows, length)], rows + D)
+    r = Route(bt, Hkv, 0)
+    assert not r.near and r.many[0] and chunks[0] <= r.chunks(0) <= chunks[1], r.__dict__
+    compare(bt, q, sk, 0)
+    ne.device_check()
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,window,why", [
+    (False, 64, 64, 8, [(500, 1100)], 0, "share"),           # equal work for every block
+    (False, 128, 32, 8, [(900, 1700), (1, 50)], 0, "share"),
+    (True, 64, 64, 8, [(500, 1100), (3, 700)], 0, "share"),
+    (True, 128, 32, 8, [(900, 1700)], 0, "share"),
+    (False, 64, 8, 8, [(300, 5000), (200, 2100)], 1500, "cost"),  # windows and chunks
+    (False, 128, 8, 8, [(300, 5000)], 2000, "cost"),
+    (True, 64, 16, 8, [(300, 5000), (2, 40)], 1500, "cost"),
+    (True, 128, 8, 8, [(300, 3000)], 1999, "cost"),
+    (False, 64, 32, 8, [(700, 1900), (600, 1800)], 900, "share"),
+])
+def test_splits_of_the_many_row_kernel(mx, D, Hq, Hkv, lens, window, why):
+    torch_cuda()
+    say(f"split mx={mx} D={D} lens={lens} window={window}")
+    bt, q, sk = build(mx, D, Hq, Hkv, 32, lens, D + window + len(lens))
+    r = Route(bt, Hq, window)
+    assert not r.near and r.many[0] and r.why["many"] == why and r.chunks(0) > 1, r.__dict__
+    compare(bt, q, sk, window)
+    ne.device_check()
+
+
+def spread(B, short, long, at):
+    """One row each: lengths around `short`, those of the places `at` around `long`."""
+    return [(1, (long if b in at else short) + (b * 37) % 101) for b in range(B)]
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens", [
+    (False, 64, 16, 8, spread(100, 400, 4000, (3, 10, 64, 66, 70, 95, 99))),
+    (False, 128, 16, 8, spread(100, 400, 4000, (3, 10, 64, 66, 70, 95, 99))),
+    (True, 64, 16, 8, spread(100, 400, 4000, (3, 10, 64, 66, 70, 95, 99))),
+    (True, 128, 16, 8, spread(100, 400, 4000, (3, 10, 64, 66, 70, 95, 99))),
+    (False, 64, 16, 4, spread(200, 500, 3000, (0, 63, 64, 127, 128, 130, 191, 192, 199))),
+    (True, 64, 8, 4, spread(200, 500, 3000, (0, 63, 64, 127, 128, 130, 191, 192, 199))),
+])
+def test_split_sequences_past_the_first_64(mx, D, Hq, Hkv, lens):
+    """The chunk is a block's share of the work, and sequences of every turn of the
+    block finder are cut."""
+    torch_cuda()
+    say(f"past 64 mx={mx} D={D} B={len(lens)}")
+    bt, q, sk = build(mx, D, Hq, Hkv, 64, lens, len(lens) + D, q_start=False)
+    r = Route(bt, Hq, 0)
+    assert r.why["few"] == "share" and not any(r.many), r.__dict__
+    cut = [b for b in range(len(lens)) if r.chunks(b) > 1]
+    assert cut[0] < 64 and len([b for b in cut if b >= 64]) >= 3
+    compare(bt, q, sk, 0)
+    ne.device_check()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_mixed_rows_past_the_first_64(mx):
+    """Decode steps, drafts and prompt chunks of 150 sequences; both kernels."""
+    torch_cuda()
+    lens = [((1, 3, 0, 60 + b % 30)[b % 4], 90 + (b * 53) % 200 + (3000 if b in (5, 67, 70, 131, 133)
+                                                               else 0)) for b in range(150)]
+    bt, q, sk = build(mx, 64, 16, 4, 32, lens, 9, pad=2)
+    r = Route(bt, 16, 0)
+    assert not r.near and sum(r.many) > 30
+    for kind in (True, False):
+        cut = [b for b in range(150) if r.many[b] is kind and lens[b][0] and r.chunks(b) > 1]
+        assert cut and cut[-1] >= 64, (kind, cut)
+    compare(bt, q, sk, 0)
+    ne.device_check()
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,lens,window", [
+    (64, 64, 8, [(1, 500 + 110 * b) for b in range(40)], 0),
+    (128, 16, 8, [(1, 300 + (b * 701) % 5000) for b in range(48)], 0),
+    (64, 16, 8, [(2, 4000 - 50 * b) for b in range(30)], 3000),
+])
+def test_mxfp4_chunks_that_fit_the_chip_at_once(D, Hq, Hkv, lens, window):
+    torch_cuda()
+    say(f"fit D={D} B={len(lens)} window={window}")
+    bt, q, sk = make_codes(D, Hq, Hkv, 64, lens, D + len(lens))
+    r = Route(bt, Hq, window)
+    assert r.fitted["few"] > 0 and max(map(r.chunks, range(len(lens)))) > 1, r.__dict__
+    compare(bt, q, sk, window)
+    ne.device_check()
+
+
+def free_page_0(bt):
+    """Page 0, which a block reads where a page id is no page, is nobody's: poison."""
+    spare = np.setdiff1d(np.arange(bt.n_pages), bt.table)
+    if 0 not in spare:
+        bt.table[bt.table == 0] = spare[0]
+    return bt
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens", [
+    (False, 64, 64, 8, [(400, 450), (200, 333)]),
+    (False, 128, 32, 8, [(500, 700)]),
+    (True, 64, 64, 8, [(400, 450), (200, 333)]),
+    (True, 128, 32, 8, [(500, 700)]),
+])
+def test_hidden_pages_in_tiles_of_many_rows(mx, D, Hq, Hkv, lens):
+    torch_cuda()
+    say(f"hidden mx={mx} D={D} lens={lens}")
+    rng = np.random.default_rng(D)
+    bt = free_page_0(Batch(rng, lens, 16, Hkv, D, mx)).fill(rng)
+    q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32) * 0.5)
+    r = Route(bt, Hq, 0)
+    assert not r.near and all(r.many)
+    good, t = bt.table, bt.table.copy()
+    dead = {0: (0, 1, 5, 20, 27), 1: (2, 20)}  # groups of a tile, at its edges, a whole tile
+    if len(lens) > 1:
+        dead[1] = (4, 5, 6, 7)
+    for b in range(len(lens)):
+        for i, j in enumerate(dead[b]):
+            t[b, j] = (bt.n_pages, -1, 1 << 30)[i % 3]
+    bt.table = t
+    got = attend(bt, q, None, 0)
+    with pytest.raises(ne.NeonError):
+        ne.device_check()
+    bt.table = good
+    ref, mag = attention(bt, f32(q), None, 0,
+                         hidden=lambda b, n: np.isin(np.arange(n) // 16, dead[b]))
+    off = np.abs(f32(got) - ref) / limits(bt, f32(q), ref, mag, 0)
+    say(f"  worst error / bound = {off.max():.3f}")
+    assert off.max() <= 1.0
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,window", [
+    (False, 64, 64, 8, [(600, 1500)], 200),
+    (True, 128, 32, 8, [(900, 1600)], 100),
+])
+def test_many_rows_and_pages_behind_the_window(mx, D, Hq, Hkv, lens, window):
+    """Their table entries are not looked at, their memory is poison."""
+    torch_cuda()
+    rng = np.random.default_rng(D)
+    bt = free_page_0(Batch(rng, lens, 16, Hkv, D, mx)).fill(rng)
+    q = bf16(rng.normal(size=(bt.n_rows, Hq, D)).astype(np.float32) * 0.5)
+    r = Route(bt, Hq, window)
+    assert not r.near and all(r.many)
+    ref, mag = attention(bt, f32(q), None, window)
+    bound = limits(bt, f32(q), ref, mag, window)
+    n, t = lens[0]
+    gone = (t - n - window + 1) // 16
+    ids = bt.table[0, :gone].copy()
+    bt.k[ids], bt.v[ids] = (0x77, 0x77) if mx else (0x7FC1, 0x7FC1)
+    if mx:
+        bt.ks[ids] = bt.vs[ids] = 255
+    bt.table[0, :gone] = -1
+    off = np.abs(f32(attend(bt, q, None, window)) - ref) / bound
+    ne.device_check()
+    assert off.max() <= 1.0
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_many_rows_over_shared_and_repeated_pages(mx):
+    torch_cuda()
+    rng = np.random.default_rng(6)
+    bt = Batch(rng, [(400, 900), (300, 500)], 16, 8, 64, mx).fill(rng)
+    bt.table[1, :10] = bt.table[0, :10]
+    bt.table[0, 30] = bt.table[0, 2]
+    q = bf16(rng.normal(size=(bt.n_rows, 64, 64)).astype(np.float32) * 0.5)
+    r = Route(bt, 64, 0)
+    assert not r.near and all(r.many)
+    compare(bt, q, None, 0)
+    ne.device_check()
