@@ -8,9 +8,10 @@
 // in index order, exceeds u times the kept mass.
 //
 // Masses are integers, round(w 2^S) with V 2^S <= 2^62: sums are exact, so no
-// order of threads or atomics changes a draw.  A token more than 31 below the
-// maximum (in units of T) has mass 0 and cannot be drawn; its share is under
-// 2^-44 of the most probable token's, below the 2^-24 steps of u.
+// order of threads or atomics changes a draw.  A token more than 31.2 below the
+// maximum (in units of T; 45 ln 2, less past 2^18 tokens, where S is smaller) has
+// mass 0 and cannot be drawn; its share is under 2^-45 of the most probable token's,
+// below the 2^-24 steps of u.
 #include <hip/hip_runtime.h>
 
 #include "neon_common.hpp"
