@@ -421,11 +421,13 @@ __device__ __forceinline__ int pa_chunks(const PagedAttnArgs& a, const PaWork& w
 
 // The most rows of a sequence that the few-row kernel takes.  All, where the whole
 // call is kPaSmall 16-row tiles x keys x KV heads at most: with so little work the
-// length of a block's chain counts, and 16 rows have a short one (8 heads for 1, 250
-// rows of 254 tokens 13.5 -> 8.9 us; 319 rows of 583 of 2 heads of 128 27.7 -> 13;
-// from 200000 on 128 rows at a time are the faster: 100 rows of 500, 64 heads for 8,
-// 17.6 against 20).  Both kernels compute it from the same numbers.
-constexpr int kPaSmall = 131072;
+// length of a block's chain counts, and 16 rows have a short one.  128 rows at a time
+// against 16, heads of 64, 8 KV heads for 8 unless given: 200 rows of 300 tokens (31000)
+// 16.7 -> 7.7 us, 300 of 1000 (152000) 22.6 -> 11.2, 64 heads, 100 of 500 (200000) 21.5
+// -> 12.1 and 200 of 300 (240000) 17.2 -> 13.8 (heads of 128 23.5 -> 22.2).  Further up
+// the two cross: 64 heads, 400 of 400 (640000) 22.7 and 24.1, heads of 128 32 and 41.
+// Both kernels compute it from the same numbers.
+constexpr int kPaSmall = 262144;
 __device__ __forceinline__ int pa_few_rows(const PagedAttnArgs& a, const PaWork& w,
                                            const PaSeq& first, int turns) {
   if (!a.small) return kPaFew;
@@ -1657,7 +1659,7 @@ static PaGrid pa_grid(const PagedAttnArgs& a) {
                      kPmTarget);
   // of a small call, sum of tiles x keys / 256 and one more per unit
   const int64_t small = units * a.kv.Hkv + kPaSmall / 256 + 2;
-  g.small = small <= (g.few > 1024 ? g.few : 1024);
+  g.small = small <= (g.few > 2048 ? g.few : 2048);
   if (g.small && g.few < small) g.few = small;
   if (g.small && units * a.kv.Hkv * keys <= kPaSmall) g.many = 0;
   return g;

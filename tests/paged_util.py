@@ -143,6 +143,9 @@ def attention(batch, q, sinks, window, hidden=lambda b, t: None):
     return out, mag
 
 
+SMALL = 262144  # 16-row tiles x keys x KV heads of a call that takes 16 rows at a time
+
+
 class Route:
     """How neon_paged_attn takes a batch (the rules of its launch and of its block
     finder), so that a test can say which kernel and which split it reaches.
@@ -165,11 +168,11 @@ class Route:
         rows, starts = batch.n_rows * G, batch.q_start is not None
         units = rows // 16 + B
         few = 0 if not starts and G > 32 else blocks(min(units, 2 * B), keys(16, 32), 1024)
-        small = units * Hkv + 131072 // 256 + 2
-        can = (rows > 32 if starts else G > 32) and small <= max(few, 1024)
+        small = units * Hkv + SMALL // 256 + 2
+        can = (rows > 32 if starts else G > 32) and small <= max(few, 2048)
         work = sum(-(-n * G // 16) * self.span(t, 16, 32) for n, t in lens) * Hkv
-        self.small = can and work <= 131072
-        self.near = can and abs(work / 131072 - 1) < 0.01  # the kernel's fp32 sum may differ
+        self.small = can and work <= SMALL
+        self.near = can and abs(work / SMALL - 1) < 0.01  # the kernel's fp32 sum may differ
         self.many = [t > 0 and n * G > 32 and not self.small for n, t in lens]
         self.chunk, self.why, self.fitted = {}, {}, {}
         for kind, R, align, target, places in (

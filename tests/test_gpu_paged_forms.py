@@ -322,12 +322,12 @@ def build(mx, D, Hq, Hkv, page, lens, seed, **kw):
 
 JOINS = [
     # (rows, length, Hkv, chunks): of the longest tile
-    (330, 800, 8, (2, 4)),      # every tile has more than 64 rows
-    (300, 900, 8, (2, 4)),      # the last one 44
-    (200, 1500, 8, (5, 8)),
-    (70, 2000, 16, (5, 8)),
-    (60, 1900, 32, (5, 8)),     # no tile of more than 64
-    (100, 4000, 8, (9, 32)),
+    (330, 800, 24, (2, 4)),     # every tile has more than 64 rows
+    (300, 900, 24, (2, 4)),     # the last one 44
+    (200, 1500, 16, (5, 8)),
+    (70, 2000, 32, (5, 8)),
+    (60, 1900, 48, (5, 8)),     # no tile of more than 64
+    (100, 4000, 16, (9, 32)),
     (40, 60000, 2, (33, 64)),
     (100, 60000, 2, (33, 64)),
 ]
@@ -502,4 +502,24 @@ def test_many_rows_over_shared_and_repeated_pages(mx):
     r = Route(bt, 64, 0)
     assert not r.near and all(r.many)
     compare(bt, q, None, 0)
+    ne.device_check()
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,rows,length,small", [
+    (False, 64, 64, 8, 100, 500, True),    # 200000
+    (True, 64, 64, 8, 100, 500, True),
+    (False, 128, 8, 8, 300, 1000, True),   # 152000
+    (True, 128, 8, 1, 300, 1000, True),
+    (False, 128, 1, 1, 40, 60000, True),   # 180000, cut into many chunks
+    (True, 64, 2, 2, 34, 40000, True),     # 240000
+    (False, 64, 64, 8, 100, 700, False),   # 280000
+    (False, 64, 8, 1, 512, 1050, False),   # 268800
+])
+def test_small_calls_on_both_sides_of_the_border(mx, D, Hq, Hkv, rows, length, small):
+    torch_cuda()
+    say(f"border mx={mx} D={D} rows={rows} length={length}")
+    bt, q, sk = build(mx, D, Hq, Hkv, 32, [(rows, length)], rows + length)
+    r = Route(bt, Hq, 0)
+    assert not r.near and r.small is small
+    compare(bt, q, sk, 0)
     ne.device_check()
