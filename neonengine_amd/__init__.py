@@ -448,8 +448,8 @@ def _arg(t, size, n, name, device, real=None):
     the paged calls derive from other tensors.  real: floating point or not (None:
     bf16, or integers that hold its bits)."""
     if t.element_size() != size or t.numel() < n or t.get_device() != device or \
-            not t.is_contiguous() or t.dtype is _fp16 or \
-            (real is not None and t.is_floating_point() is not real):
+            not t.is_contiguous() or \
+            (t.dtype is _fp16 if real is None else t.is_floating_point() is not real):
         raise ValueError(f"{name}: needs {n} contiguous elements of {size} bytes"
                          f"{' (bf16)' if real is None else ' (floats)' if real else ' (integers)'} on "
                          f"device {device}, has {tuple(t.shape)} of {t.dtype} on {t.device}")
