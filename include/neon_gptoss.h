@@ -477,8 +477,9 @@ typedef struct neon_paged_kv {
  * max_pages * page_size or 2^30, a position >= n_pos) is left out, a page id
  * outside [0, n_pages) drops what it would hold (append, gather) or hides its
  * keys (attention), and neon_device_check then returns NEON_EINVAL.  Outputs
- * overlap no input and no pool.  (The reference has no counterpart: it has no
- * model code.) */
+ * overlap no input and no pool.  B is 1 to 65535, n_rows up to 2^23
+ * (neon_paged_append: below 2^23 where a row has more than 448 runs of 16
+ * elements).  (The reference has no counterpart: it has no model code.) */
 
 /* Rotates and appends: qkv rows [n_rows] of (Hq + 2 n_kv_heads) head_dim bf16,
  * `qkv_stride` elements apart (a multiple of 8; 16-byte aligned), hold the q,
@@ -498,7 +499,8 @@ neon_status neon_paged_append(const neon_paged_kv* kv, const uint16_t* qkv, int6
 /* Reads rows back: the positions that neon_paged_append writes for the same
  * arguments, as bf16 (MXFP4: exact), into k_out, v_out
  * [n_rows][n_kv_heads][head_dim].  With q_start the running sum of kv_len, the
- * whole sequences. */
+ * whole sequences.  (Codes of 4 and 6 at the scale byte 253, and from 2 on at 254,
+ * lie past bf16 and read as infinities, here and in neon_paged_attn.) */
 neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t* q_start,
                               const int32_t* kv_len, const int32_t* page_table, int max_pages,
                               uint16_t* k_out, uint16_t* v_out, int n_rows, int B, void* stream);
@@ -510,6 +512,12 @@ neon_status neon_paged_gather(const neon_paged_kv* kv, const int32_t* q_start,
  * [n_rows][Hq head_dim] bf16, 16-byte aligned; a row that sees no key gets 0.
  * Hq a multiple of n_kv_heads, at most 64 query heads per KV head.  Any number
  * of rows per sequence: decode steps, drafts and prompt chunks in one call.
+ * Weights are kept in two bf16 terms (2^-16 of each), maxima and sums in fp32,
+ * whatever the format and the rows.  Sums are divided once, at the end: values
+ * from about 2^100 on can overflow on the way.  A NaN or an infinity among the
+ * values belongs to the rows that see its token.  How a sequence is cut depends on
+ * the whole batch: the same batch gives the same bits, another one may give a
+ * sequence other last bits.
  *   workspace, counters  as neon_attn_decode: neon_paged_attn_workspace(...)
  *                        bytes of any contents and
  *                        neon_paged_attn_counters(...) bytes, zero before

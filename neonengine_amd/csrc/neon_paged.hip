@@ -266,7 +266,9 @@ __device__ __forceinline__ uint4 paged_load8(const uint8_t* pool, const uint8_t*
 
 // ---------------------------------------------------------------------------
 // Gather: the batch's rows as the cache holds them, a wave per row, 8 elements a
-// lane.  Bound: the bytes read and written (7.6k rows from MXFP4 pages 6.5 us).
+// lane.  Bound: the bytes read and written (74k rows of 8 heads of 64 from bf16 pages
+// 50 us, 6.1 TB/s, from MXFP4 35 us, 5.5); a short call by a wave's chain of lookup,
+// page id and loads (36 rows 2.5 us; 6.8k 5.3 and 5.4, MXFP4 at 3.3 TB/s).
 // ---------------------------------------------------------------------------
 template <bool F4>
 __global__ __launch_bounds__(256) void k_paged_gather(PagedKv kv, PagedRows r,
@@ -325,8 +327,8 @@ void launch_paged_gather(const PagedKv& kv, const PagedRows& r, uint16_t* k_out,
 // arrive joins them (stores and loads at agent scope, as in k_attn_split).
 // ---------------------------------------------------------------------------
 constexpr int kPaTarget = 1024;   // blocks of equal work to aim at: 4 per CU
-constexpr int kPmTarget = 512;    // of the many-row kernel: 2 per CU (640 to 1024: 256
-                                  // rows of 4000 tokens 45 -> 52 to 60 us, for the joins)
+constexpr int kPmTarget = 512;    // of the many-row kernel: 2 per CU (768 and 1024: 256
+                                  // rows of 4000 tokens 55 -> 60 and 69 us, for the joins)
 constexpr int kPaFew = 32;        // (token, head) rows per KV head of the few-row kernel
 constexpr int kPaArrive = 16;     // ints from one arrival counter to the next
 constexpr int kPaMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
@@ -474,15 +476,15 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
   const float share = wave_sum(work) * (float)a.kv.Hkv * (1.001f / TARGET);
   // Cutting costs the partial results and the join, by the last block of a unit, one
   // chunk after another:
-  // - up to 512 keys are not cut (64 sequences of 500 tokens 24.7 -> 15.2 us, one of
-  //   301 8.2 -> 7.3; 230 rows of 230 tokens in two 17 -> 27);
+  // - up to 512 keys are not cut (8 sequences of 40 rows of 300 tokens 24.5 -> 16.7 us);
   // - nor are few rows whose blocks run all at once and none of which is much longer
   //   than a CU's share of the work (of 256; a block alone reads about as fast): 64
   //   sequences of 1000 tokens 31.4 -> 24.0, of 50 to 1500 28.8 -> 25.8; MXFP4 blocks
-  //   are slower (32 of 50 to 2000 12.7 -> 13.4), so two thirds of it there;
+  //   are slower (64 of 50 to 4000 28.5 -> 32), so two thirds of it there;
   // - chunks of n keys are sqrt(cost n) at least, the cost of joining one against that
-  //   of a key (one sequence of 16000 tokens 15.1 -> 12.5, of 30000 26.1 -> 19.9; tiles
-  //   of 128 rows: 40 rows of 60000 129 -> 90, 319 of 583, 1 head of 128, 37 -> 28).
+  //   of a key (one sequence of 16000 tokens 15.5 -> 12.5, of 30000 25.7 -> 20.5; tiles
+  //   of 128 rows: 32 rows of 8000, 64 heads for 8, 68 -> 40, 100 of 60000 of 2 heads
+  //   239 -> 88).
   most = wave_max(most);
   const float cost = __builtin_sqrtf((FEW ? 10.0f : 25.0f) * most);
   float least = fmaxf(share, most <= 512.0f ? 511.0f : cost);
@@ -505,9 +507,9 @@ __device__ __forceinline__ bool pa_work(const PagedAttnArgs& a, int idx, int blo
     const int to = pa_scan(nb), all = __builtin_amdgcn_readlane(to, 63);
     // FIT: a few more blocks than the chip holds cost a round of their own, so
     // larger chunks where that makes them fit (a unit is one block at least).
-    // MXFP4, 4 sequences up to 131072 tokens 30.4 -> 29.3 us, 48 of heads of 128 25.8
-    // -> 24.6; where the reads are the bound, small chunks even out the end better
-    // (64 bf16 ones: 68 -> 73 us).
+    // MXFP4, 4 sequences up to 131072 tokens 38.6 -> 37.4 us, 48 of 100 to 6000, heads
+    // of 128, 40.9 -> 36.9; where the reads are the bound, small chunks even out the end
+    // better (64 bf16 ones: 68 -> 73 us).
     const float over = (float)all * (float)a.kv.Hkv * (1.0f / PLACES);
     if (FIT && fit < 3 && turns == 1 && over > 1.0f && over <= 2.0f) {
       chunk = uni((min((int)((float)chunk * over), (1 << 30) - 128) + 128) & ~127);
@@ -875,12 +877,12 @@ __device__ __forceinline__ void pa_write(uint16_t* dst, const float (&x)[E], flo
 // with every fourth 32 keys of the chunk, straight from memory into the
 // operands' registers, some steps ahead of the products.
 // Bound: the bytes of the visible keys, read once (64 sequences of up to 8192
-// tokens, 8 heads of 64 for 64: 285 MB in 65 us, 4.4 TB/s; 256 of 2000: 5.4 TB/s);
+// tokens, 8 heads of 64 for 64: 285 MB in 65 us, 4.4 TB/s; 256 of 2000: 5.2 TB/s);
 // MXFP4 at 2.9 to 3.6 TB/s by the vector units as well, which expand the codes
-// (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, 54% busy); few short
+// (48 sequences of up to 6000 tokens, heads of 128: 73 MB in 25 us, 53% busy); few short
 // sequences by the chain of lookups, loads and the join (5 us for one of 64 tokens).
-// Waves of a SIMD, and blocks of a CU (four of D = 64: bf16 spills, MXFP4 4 sequences
-// of up to 131072 tokens 29.1 -> 30.3 us)
+// Waves of a SIMD, and blocks of a CU (four of D = 64: bf16 the same, MXFP4 4 sequences
+// of up to 131072 tokens 30.7 -> 31.2 us, 64 of up to 4000 28 -> 26)
 constexpr int pa_few_waves(int D, bool f4) { return D == 64 || f4 ? 3 : 2; }
 template <int D, bool F4>
 __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(PagedAttnArgs a) {
@@ -1159,8 +1161,8 @@ struct PmStage {  // a thread's part of a tile on its way
 // pa_join for a tile of 128 rows: two threads a row for its maximum, sum and the
 // chunks' factors sf; then groups of four values, NG of a thread at a time, with U
 // chunks' loads on their way: all rows and two (or one) of up to 8 chunks, else
-// 4096 / D rows and four (64 rows of 8000 tokens 31.3 -> 27.3 us; 256 of 4000 the
-// other way round, 48.8 -> 45.9).  By 16 rows at a time, every step for each, two
+// 4096 / D rows and four (40 rows of 60000 tokens, 8 heads of 128, 146 -> 128 us; 256 of
+// 4000 the other way round, 57 -> 55).  By 16 rows at a time, every step for each, two
 // chunks of 128 rows of 128 took 13 us.
 constexpr int kPmJoin = 32;  // chunks whose factors are in LDS at once
 template <int D>

@@ -38,9 +38,9 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 //   k_sr_pick   finds the bins that the top_k-th token and the token at top_p's goal
 //               can lie in (every block for itself), then per chunk the mass of the
 //               bins above those, which is kept whatever the exact places are, and
-//               the tokens of those bins (the candidates, some hundreds of a large
-//               vocabulary); the row's last block finds the two places among the
-//               candidates, then the part that holds the draw, then the token in it
+//               the tokens of those bins (the candidates); the row's last block
+//               finds the two places among the candidates, then the part that holds
+//               the draw, then the token in it
 // A row of one chunk is one launch with the same steps.  Nothing but the chunks'
 // partial results crosses launches, at agent scope, so that the last block reads
 // what the others wrote without a launch in between.
@@ -48,6 +48,10 @@ constexpr uint32_t kSrNone = 0x007FFFFFu;  // key of minus infinity
 // rate of a large copy), k_sr_hist's 64-bit exponentials (vector units 75% busy) and
 // the last blocks; for few rows the chain of dependent steps, about 10 us of it in
 // the last block of k_sr_pick (sort 4.5, draw 3.5).
+// Candidates are some hundreds of 201088 normal logits at a deviation of 2.5 T (sorted,
+// up to 512), up to 4096 at 1.3 T (selected by digits: 34 us for one row), and more
+// where the row is flatter: then the last block reads the row again for each step, and
+// one row of deviation T takes 520 us, 64 of them 960.
 // Kernel times, us (max + hist + pick): 1 x 201088 3 + 5 + 16, 64 x 201088 10.5 +
 // 22.5 + 37, 7 x 32003 3 + 4.5 + 18; one block per row, 8 bits of the key at a time,
 // took 585, 1030 and 206.
