@@ -1050,12 +1050,14 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
   }
   // An infinity among the values of a step that every row sees meets both terms of P:
   // its product with the second is the other infinity, or NaN.
+  l += xor_lane<16>(l);
+  l += xor_lane<32>(l);
   float z = 0.0f;  // NaN where an element is not finite
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[e][i], 0.0f, z);
-  odd = odd || z != z;
+  odd = odd || (z != z && l == l);  // (a row with a NaN among its scores is all NaN)
   if (__any(odd)) {  // lane (g, c): row c, dims (D/4) g + E i + e
     pf4 sum[E];      // of the infinities and NaNs alone
 #pragma unroll
@@ -1076,8 +1078,6 @@ __global__ __launch_bounds__(256, pa_few_waves(D, F4)) void k_paged_attn_few(Pag
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[e][i] = sum[e][i] != 0.0f ? sum[e][i] : o[e][i];
   }
-  l += xor_lane<16>(l);
-  l += xor_lane<32>(l);
   // the four waves' states
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -1545,14 +1545,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
   __syncthreads();
   // as in the other kernel: infinities and NaNs cleared at an edge, and infinities
   // that met both terms of P
-  float z = 0.0f;  // NaN where an element is not finite
+  bool more = false;
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t) {
+    l[t] += xor_lane<16>(l[t]);
+    l[t] += xor_lane<32>(l[t]);
+    float z = 0.0f;  // NaN where an element is not finite
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) z = __builtin_fmaf(o[t][e][i], 0.0f, z);
-  if (odd != 0 || __any(z != z)) {
+    more = more || (z != z && l[t] == l[t]);
+  }
+  if (odd != 0 || __any(more)) {
     pf4 sum[2][E];  // of the infinities and NaNs alone
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -1575,11 +1580,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_attn_many(PagedA
       for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[t][e][i] = sum[t][e][i] != 0.0f ? sum[t][e][i] : o[t][e][i];
-  }
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    l[t] += xor_lane<16>(l[t]);
-    l[t] += xor_lane<32>(l[t]);
   }
   if (w.chunks == 1) {
 #pragma unroll

@@ -523,3 +523,44 @@ def test_small_calls_on_both_sides_of_the_border(mx, D, Hq, Hkv, rows, length, s
     assert not r.near and r.small is small
     compare(bt, q, sk, 0)
     ne.device_check()
+
+
+@pytest.mark.parametrize("mx,D,Hq,Hkv,lens,window,many", [
+    (False, 64, 16, 2, [(5, 300), (1, 40)], 0, False),
+    (True, 128, 8, 2, [(3, 200), (2, 2)], 50, False),
+    (False, 64, 64, 8, [(400, 450)], 0, True),
+    (True, 128, 32, 8, [(500, 700)], 0, True),
+])
+def test_odd_queries_stay_in_their_rows(mx, D, Hq, Hkv, lens, window, many):
+    """A NaN or an infinity in a query makes its row NaN, and no other; infinities
+    among the values are found beside it."""
+    torch_cuda()
+    say(f"odd queries mx={mx} D={D} lens={lens}")
+    bt, q, sk = make(mx, D, Hq, Hkv, 16, lens, window, seed=D + 77)
+    r = Route(bt, Hq, window)
+    assert not r.near and r.many[0] is many
+    last = bt.n_rows - 1
+    odd = [(0, 0), (1, Hq - 1), (last, 1)]
+    for (row, h), x in zip(odd, (0x7FC0, 0x7F80, 0xFFC0)):
+        q[row, h, 3] = x
+    put_odd(bt, "v", 0, lens[0][1] - lens[0][0], 0, 5, np.inf)  # the first row's last key
+    got = f32(attend(bt, q, sk, window)).astype(np.float64)
+    ne.device_check()
+    ok = np.ones(q.shape[:2], bool)
+    for row, h in odd:
+        assert np.isnan(got[row, h]).all()
+        ok[row, h] = False
+        q[row, h] = 0
+    sees = np.zeros(q.shape, bool)
+    sees[:lens[0][0], :Hq // Hkv, 0 if mx else 5:32 if mx else 6] = True
+    if window:
+        sees[window:] = False
+    assert (np.isnan(got) if mx else got == np.inf)[sees & ok[..., None]].all()
+    if mx:  # the block counts as zeros below
+        pg, at = (int(i[0]) for i in bt.places(0, lens[0][1] - lens[0][0], lens[0][1] - lens[0][0] + 1))
+        bt.vs[pg, 0, at, 0], bt.v[pg, 0, at, :16] = 127, 0
+    else:
+        put_odd(bt, "v", 0, lens[0][1] - lens[0][0], 0, 5, 0.0)
+    ref, mag = attention(bt, f32(q), sk, window)
+    off = np.abs(got - ref) / limits(bt, f32(q), ref, mag, window)
+    assert off[ok[..., None] & ~sees].max() <= 1.0
