@@ -555,6 +555,115 @@ neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
                              const float* min_p, const float* u, int32_t* out_ids,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- beam search --------------------------------------------------------- */
+/* A request b of B has W places (1 to 32); a place is row b W + w of every array
+ * and of the batch that the paged calls or neon_attn_decode take.  A place whose
+ * score is -inf holds no beam: its logits are not read.  (The reference has no
+ * counterpart: it has no model code.) */
+
+/* The next beams from logits (device fp32, rows [B W] `stride` >= V elements
+ * apart).  A candidate (place w, token t) has the value
+ *   v = score[w] + l[w][t] - log sum_u exp(l[w][u])   (64 bits, rounded once),
+ * candidates are ordered by (v descending, place ascending, token ascending), those
+ * of one place by their logit.
+ *   - The W best candidates that are no stop token (stop [n_stop], device ids, at
+ *     most 16, others than a token's are ignored; NULL with n_stop 0) go on.  The
+ *     best child of a beam takes its beam's place, the other children, in their
+ *     order, the free places in ascending order: token, parent (row of the beam that
+ *     it continues) and out_score, [B W] each; out_score may be score.  So a beam
+ *     that goes on keeps its place, and only the states of the others move.  Places
+ *     past the candidates get token -1, parent -1, score -inf.
+ *   - Stop tokens among the W best of all candidates end: end_token, end_parent,
+ *     end_score [B W], a request's in their order from its first entry on, then -1,
+ *     -1, -inf.  All three may be NULL.
+ * A first step has one beam per request: the others' scores are -inf.  Logits of
+ * -inf and NaN are never chosen.  A beam with a score of NaN or +inf or a logit of
+ * +inf, or with nothing above -inf, has no candidates (neon_device_check gives
+ * NEON_EINVAL for the first three).  B is 1 to 65535, V up to 2^24.
+ * workspace: neon_beam_select_workspace(...) bytes, 16-byte aligned, any contents. */
+size_t neon_beam_select_workspace(int B, int W, int V, int n_stop);
+neon_status neon_beam_select(const float* logits, int64_t stride, int B, int W, int V,
+                             const float* score, const int32_t* stop, int n_stop, int32_t* token,
+                             int32_t* parent, float* out_score, int32_t* end_token,
+                             int32_t* end_parent, float* end_score, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Moves the states of beams in place: row r of every state becomes what row
+ * parent[r] was (device int32 [B W], a row of the same request; -1 or r itself: left
+ * as it is).  states: host array of n_states device pointers (16-byte aligned), each
+ * [B W][slabs][T][row_bytes] (row_bytes a multiple of 4; a contiguous cache of
+ * neon_attn_decode has slabs = Hkv, T = T_max, row_bytes = 2 D).  len [B W] (device
+ * int32, or NULL for T): the first min(len[parent[r]], T) rows of each slab are moved,
+ * rows past them left.  Any parents within a request, permutations too.  A parent of
+ * another request leaves its row as it is (neon_device_check NEON_EINVAL). */
+neon_status neon_beam_reorder(void* const* states, int n_states, int B, int W, int slabs, int T,
+                              int row_bytes, const int32_t* len, const int32_t* parent,
+                              void* stream);
+
+/* ---- the pages of a cache as a whole -------------------------------------- */
+/* refs [n_pages] (device int32): how many hold each page, sequences of the batch
+ * and others (a prefix that is kept); 0: free.  A sequence of n tokens holds the
+ * pages of the first ceil(n / page_size) entries of its page table row.  One table
+ * serves the caches of all layers.  n_pages is up to 2^24, page_size a power of two
+ * from 16 to 65536, B and B_in 1 to 65535.
+ *
+ * neon_pages_fork: which pages the sequences hold next.  Sequence b < B continues the
+ * first keep[b] tokens (NULL: all) of row parent[b] of page_table (B_in rows; NULL: its
+ * own, then B == B_in; -1: of none) and has room for add[b] more (NULL: one where the
+ * parent has tokens, else none):
+ *   - len_out[b] = keep + add is the kv_len of the append that follows; the table row
+ *     gets the kept pages, then free ones (entries past them are left as they are);
+ *   - rows of page_table that no sequence continues are given up, and what a
+ *     sequence does not keep of its own; pages that nobody holds then are free;
+ *   - a kept page that is partly full and written next (add > 0), and that others
+ *     hold too, is copied: copy_src[b] -> copy_dst[b], the first copy_rows[b] tokens
+ *     (-1, -1, 0: nothing to copy), for neon_pages_copy before the append.  If all its
+ *     holders write, the first of them keeps the page.
+ * Beams and samples (parent from neon_beam_select, or the prompt's row for each), the
+ * growth of a step (parent and keep NULL), dropped drafts (keep), new sequences (parent
+ * -1) and freed ones (len 0) are all this call.  Free pages are taken in the order of
+ * their ids, by b, then by place, the copy's first.  Pages freed by the call are free
+ * in it.  refs_out may be refs, len_out may be kv_len, table_out may be page_table
+ * where parent is NULL; otherwise outputs overlap nothing.
+ * Where no page is left the entry is -1 and neon_device_check gives NEON_EKV_FULL; a
+ * sequence whose numbers do not fit (parent, keep, add, a length) is left without
+ * tokens, entries outside [0, n_pages) are passed on and not counted
+ * (neon_device_check NEON_EINVAL, also for a count that falls below 0).
+ *   workspace  neon_pages_workspace(n_pages, B) bytes, 16-byte aligned, any contents;
+ *   counters   neon_pages_counters(n_pages) bytes, zero before their first use and
+ *              left zero by every call. */
+size_t neon_pages_workspace(int n_pages, int B);
+size_t neon_pages_counters(int n_pages);
+neon_status neon_pages_fork(const int32_t* refs, const int32_t* page_table, const int32_t* kv_len,
+                            int B_in, const int32_t* parent, const int32_t* keep,
+                            const int32_t* add, int32_t* refs_out, int32_t* table_out,
+                            int32_t* len_out, int32_t* copy_src, int32_t* copy_dst,
+                            int32_t* copy_rows, int B, int n_pages, int page_size, int max_pages,
+                            void* workspace, size_t workspace_bytes, int32_t* counters,
+                            size_t counter_bytes, void* stream);
+
+/* Copies pages src[i] -> dst[i] (device int32 [n]; -1 in either: nothing), the first
+ * rows[i] tokens of each (NULL: whole pages; rows past them are left), in n_kv caches of
+ * one shape and format (host array).  No page may be written twice, or written and
+ * read.  An id outside [0, n_pages) or rows outside [0, page_size] drop the entry
+ * (neon_device_check NEON_EINVAL). */
+neon_status neon_pages_copy(const neon_paged_kv* kv, int n_kv, const int32_t* src,
+                            const int32_t* dst, const int32_t* rows, int n, void* stream);
+
+/* neon_pages_compact: with U pages in use (refs not 0), the used ones from id U on
+ * move to the free ids below U, both in ascending order: copy_src[j] -> copy_dst[j]
+ * (each [n_pages / 2], -1 past the moves) for neon_pages_copy, moved_to[p] the new id
+ * of page p (-1: it was free) for holders outside the batch.  refs_out [n_pages] and
+ * the table rows (table_out: the entries that a sequence holds) follow.  refs_out may
+ * be refs, table_out may be page_table.  A sequence whose length does not fit is left
+ * out, an entry outside [0, n_pages) passed on, an entry of a free page becomes -1
+ * (neon_device_check NEON_EINVAL).  workspace as above. */
+neon_status neon_pages_compact(const int32_t* refs, const int32_t* page_table,
+                               const int32_t* kv_len, int32_t* refs_out, int32_t* table_out,
+                               int32_t* moved_to, int32_t* copy_src, int32_t* copy_dst, int B,
+                               int n_pages, int page_size, int max_pages, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

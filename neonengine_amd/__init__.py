@@ -42,6 +42,8 @@ EXPORTS = (
     "neon_seq_add", "neon_seq_remove",
     "neon_paged_append", "neon_paged_gather", "neon_paged_attn", "neon_paged_attn_workspace",
     "neon_paged_attn_counters", "neon_sample_rows", "neon_sample_rows_workspace",
+    "neon_beam_select", "neon_beam_select_workspace", "neon_beam_reorder", "neon_pages_fork",
+    "neon_pages_workspace", "neon_pages_counters", "neon_pages_copy", "neon_pages_compact",
 )
 
 
@@ -138,6 +140,11 @@ def lib():
             "neon_paged_attn": [_P, _P, _I64, _P, _P, _P, _P, _I, _P] + [_I] * 4 +
                                [_P, _SZ, _P, _SZ, _P],
             "neon_sample_rows": [_P, _I64, _I, _I] + [_P] * 7 + [_SZ, _P],
+            "neon_beam_select": [_P, _I64, _I, _I, _I, _P, _P, _I] + [_P] * 7 + [_SZ, _P],
+            "neon_beam_reorder": [_P] + [_I] * 6 + [_P] * 3,
+            "neon_pages_fork": [_P] * 3 + [_I] + [_P] * 9 + [_I] * 4 + [_P, _SZ, _P, _SZ, _P],
+            "neon_pages_copy": [_P, _I, _P, _P, _P, _I, _P],
+            "neon_pages_compact": [_P] * 8 + [_I] * 4 + [_P, _SZ, _P],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -151,7 +158,10 @@ def lib():
                            "neon_moe_prefill_workspace": [_I] * 6,
                            "neon_paged_attn_workspace": [_I] * 5,
                            "neon_paged_attn_counters": [_I] * 5,
-                           "neon_sample_rows_workspace": [_I] * 2}.items():
+                           "neon_sample_rows_workspace": [_I] * 2,
+                           "neon_beam_select_workspace": [_I] * 4,
+                           "neon_pages_workspace": [_I] * 2,
+                           "neon_pages_counters": [_I]}.items():
             f = getattr(L, name)
             f.argtypes = args
             f.restype = _SZ
@@ -170,7 +180,8 @@ def _check(status: int, ctx=None):
 def device_check(stream=None):
     """Synchronise and raise NeonError(NEON_EINVAL) if a kernel-level call on
     the current device saw an input out of range (an expert id outside [0, E); row
-    starts, lengths, page ids or sampling parameters) since the last check."""
+    starts, lengths, page ids, sampling parameters, scores, parents or reference counts)
+    since the last check, NeonError(NEON_EKV_FULL) if pages ran out."""
     _check(lib().neon_device_check(stream))
 
 
@@ -612,6 +623,177 @@ def sample_rows(logits, u, out_ids, temperature=None, top_k=None, top_p=None, mi
                                   opt(top_k, "top_k", False), opt(top_p, "top_p"), opt(min_p, "min_p"),
                                   opt(u, "u"), opt(out_ids, "out_ids", False),
                                   _buffer(workspace, "workspace", device), workspace.nbytes, on))
+
+
+def beam_select_workspace(B, W, V, n_stop):
+    return lib().neon_beam_select_workspace(B, W, V, n_stop)
+
+
+def beam_select(logits, score, W, token, parent, out_score, stop=None, ended=None, stream=None,
+                workspace=None):
+    """The next beams of requests with W places each (neon_beam_select): logits
+    [B W][V] (fp32; rows may be a slice of wider ones), score [B W] fp32; token and
+    parent int32, out_score fp32, [B W] each.  stop: int32 ids or None.  ended:
+    (end_token, end_parent, end_score) or None."""
+    if logits.dim() != 2:
+        raise ValueError("logits: [B W][V]")
+    device = logits.get_device()
+    on = _on_current(device, stream)
+    V = logits.shape[1]
+    rows, N, stride = _rows(logits, 4, V, "logits", device)
+    if W < 1 or N % W:
+        raise ValueError(f"logits: {N} rows are not requests of {W} places")
+    n_stop = 0 if stop is None else stop.numel()
+    if workspace is None:
+        workspace = _scratch(beam_select_workspace(N // W, W, V, n_stop), stream)
+    end = (None,) * 3 if ended is None else (
+        _arg(ended[0], 4, N, "end_token", device, False),
+        _arg(ended[1], 4, N, "end_parent", device, False),
+        _arg(ended[2], 4, N, "end_score", device, True))
+    _check(lib().neon_beam_select(
+        rows, stride, N // W, W, V, _arg(score, 4, N, "score", device, True),
+        _arg(stop, 4, n_stop, "stop", device, False) if n_stop else None, n_stop,
+        _arg(token, 4, N, "token", device, False), _arg(parent, 4, N, "parent", device, False),
+        _arg(out_score, 4, N, "out_score", device, True), *end,
+        _buffer(workspace, "workspace", device), workspace.nbytes, on))
+
+
+class BeamStates:
+    """States of beams that move together (neon_beam_reorder): tensors of one shape
+    and type, [B W][slabs][T][...], [B W][T][...] or [B W][T]; rows of a multiple of 4
+    bytes."""
+
+    def __init__(self, states, W):
+        states = tuple(states)
+        if not states or W < 1:
+            raise ValueError("BeamStates: at least one state and one place")
+        shape, size = tuple(states[0].shape), states[0].element_size()
+        self.device = states[0].get_device()
+        if len(shape) < 2 or shape[0] % W or any(n < 1 for n in shape):
+            raise ValueError(f"BeamStates: [B W][slabs][T][..] or [B W][T][..], has {shape}")
+        if any(tuple(t.shape) != shape or t.element_size() != size or
+               t.get_device() != self.device for t in states):
+            raise ValueError("BeamStates: states of one shape and type, on one device")
+        self.states = states  # keeps them alive
+        self.W, self.rows = W, shape[0]
+        slabs, T, row = (1, shape[1], shape[2:]) if len(shape) < 4 else (shape[1], shape[2], shape[3:])
+        n = size
+        for k in row:
+            n *= k
+        self.ptrs = (C.c_void_p * len(states))(*(_ptr(t) for t in states))
+        self.args = (len(states), shape[0] // W, W, slabs, T, n)
+
+
+def beam_states(states, W) -> BeamStates:
+    return BeamStates(states, W)
+
+
+def beam_reorder(states, parent, length=None, stream=None):
+    """Row r of every state becomes what row parent[r] was, in place
+    (neon_beam_reorder); length int32 [B W]: the tokens of each row, or None for whole
+    rows."""
+    device = states.device
+    on = _on_current(device, stream)
+    N = states.rows
+    _check(lib().neon_beam_reorder(
+        C.addressof(states.ptrs), *states.args,
+        None if length is None else _arg(length, 4, N, "length", device, False),
+        _arg(parent, 4, N, "parent", device, False), on))
+
+
+def pages_workspace(n_pages, B):
+    """(workspace bytes, counter bytes) of neon_pages_fork; neon_pages_compact takes
+    the workspace alone."""
+    L = lib()
+    return L.neon_pages_workspace(n_pages, B), L.neon_pages_counters(n_pages)
+
+
+def _pages(refs, table, kv_len, refs_out):
+    """(device, n_pages, rows, max_pages, pointers) of the arrays of a page plan."""
+    if table.dim() != 2 or kv_len.numel() != table.shape[0]:
+        raise ValueError("table: [B][max_pages], one row per sequence of kv_len")
+    device, n = refs.get_device(), refs.numel()
+    return device, n, *table.shape, (
+        _arg(refs, 4, n, "refs", device, False), _arg(table, 4, 1, "table", device, False),
+        _arg(kv_len, 4, 1, "kv_len", device, False)), _arg(refs_out, 4, n, "refs_out", device, False)
+
+
+def pages_fork(refs, table, kv_len, page_size, refs_out, table_out, len_out, copies, parent=None,
+               keep=None, add=None, stream=None, workspace=None, counters=None):
+    """Which pages the sequences hold next (neon_pages_fork): refs int32 [n_pages],
+    table int32 [B_in][max_pages], kv_len int32 [B_in]; parent, keep, add int32 [B] or
+    None; table_out int32 [B][max_pages], len_out int32 [B], copies (src, dst, rows)
+    int32 [B] each.  counters: zero-filled once by the caller (each call leaves it
+    zero)."""
+    device, n, B_in, width, ins, refs_out = _pages(refs, table, kv_len, refs_out)
+    on = _on_current(device, stream)
+    B = table_out.shape[0]
+    if table_out.dim() != 2 or table_out.shape[1] != width:
+        raise ValueError("table_out: rows of as many entries as table")
+    if workspace is None or counters is None:
+        wb, cb = pages_workspace(n, B)
+        if workspace is None:
+            workspace = _scratch(wb, stream)
+        if counters is None:
+            counters = _scratch(cb, stream, zero=True)
+
+    def opt(t, name):
+        return None if t is None else _arg(t, 4, B, name, device, False)
+
+    _check(lib().neon_pages_fork(
+        *ins, B_in, opt(parent, "parent"), opt(keep, "keep"), opt(add, "add"), refs_out,
+        _arg(table_out, 4, B * width, "table_out", device, False), opt(len_out, "len_out"),
+        opt(copies[0], "copies[0]"), opt(copies[1], "copies[1]"), opt(copies[2], "copies[2]"), B, n,
+        page_size, width, _buffer(workspace, "workspace", device), workspace.nbytes,
+        _buffer(counters, "counters", device), counters.nbytes, on))
+
+
+class PagedLayers:
+    """Caches of one shape and format that share a page table (the layers of a model)."""
+
+    def __init__(self, caches):
+        self.caches = tuple(caches)  # keeps them alive
+        if not self.caches:
+            raise ValueError("PagedLayers: at least one cache")
+        first = self.caches[0]
+        self.device, self.format = first.device, first.format
+        if any(c.device != first.device for c in self.caches):
+            raise ValueError("PagedLayers: caches on one device")
+        self.structs = (PagedKVStruct * len(self.caches))(*(c.struct for c in self.caches))
+
+
+def paged_layers(caches) -> PagedLayers:
+    return PagedLayers(caches)
+
+
+def pages_copy(layers, src, dst, rows=None, stream=None):
+    """Copies pages src[i] -> dst[i], the first rows[i] tokens of each (None: all), in
+    every cache of `layers` (PagedLayers or one PagedKV; neon_pages_copy)."""
+    if isinstance(layers, PagedKV):
+        layers = PagedLayers([layers])
+    device = layers.device
+    on = _on_current(device, stream)
+    n = src.numel()
+    _check(lib().neon_pages_copy(
+        C.addressof(layers.structs), len(layers.caches), _arg(src, 4, n, "src", device, False),
+        _arg(dst, 4, n, "dst", device, False),
+        None if rows is None else _arg(rows, 4, n, "rows", device, False), n, on))
+
+
+def pages_compact(refs, table, kv_len, page_size, refs_out, table_out, moved_to, copies, stream=None,
+                  workspace=None):
+    """Moves the used pages of a pool to its lowest ids (neon_pages_compact): moved_to
+    int32 [n_pages], copies (src, dst) int32 [n_pages / 2] each, for pages_copy."""
+    device, n, B, width, ins, refs_out = _pages(refs, table, kv_len, refs_out)
+    on = _on_current(device, stream)
+    if workspace is None:
+        workspace = _scratch(pages_workspace(n, B)[0], stream)
+    _check(lib().neon_pages_compact(
+        *ins, refs_out, _arg(table_out, 4, B * width, "table_out", device, False),
+        _arg(moved_to, 4, n, "moved_to", device, False),
+        _arg(copies[0], 4, n // 2, "copies[0]", device, False),
+        _arg(copies[1], 4, n // 2, "copies[1]", device, False), B, n, page_size, width,
+        _buffer(workspace, "workspace", device), workspace.nbytes, on))
 
 
 PREFILL_BATCHED, PREFILL_STEPWISE, PREFILL_CHUNKED, PREFILL_MX8 = 0, 1, 2, 3

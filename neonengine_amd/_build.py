@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libneon_gptoss.so")
 SOURCES = ["neon_kernels.hip", "neon_exact.hip", "neon_exact_prompt.hip", "neon_exact_attn.hip",
            "neon_prefill.hip", "neon_mx.hip", "neon_paged.hip", "neon_sample_rows.hip",
-           "neon_engine.hip"]
+           "neon_beam.hip", "neon_pages.hip", "neon_engine.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1728,6 +1728,15 @@ extern "C" neon_status neon_device_check(void* stream) {
   if (bits & kDevErrPageId)
     KFAIL(NEON_EINVAL, "a paged call needed a page id outside [0, n_pages) (status bits 0x%x); "
           "that page's rows were dropped or hidden", bits);
+  if (bits & kDevErrPagesFull)
+    KFAIL(NEON_EKV_FULL, "neon_pages_fork needed more pages than are free (status bits 0x%x); the "
+          "entries without one are -1", bits);
+  if (bits & kDevErrPagePlan)
+    KFAIL(NEON_EINVAL, "neon_pages_fork or neon_pages_compact saw a parent, length, keep, add or "
+          "reference count out of range (status bits 0x%x); that sequence was left out", bits);
+  if (bits & kDevErrBeam)
+    KFAIL(NEON_EINVAL, "neon_beam_select saw a score or logit that is none, or neon_beam_reorder a "
+          "parent of another request (status bits 0x%x); that beam was left out", bits);
   if (bits & kDevErrSampleParam)
     KFAIL(NEON_EINVAL, "neon_sample_rows saw a row's parameter out of range (status bits 0x%x); "
           "that row's id is -1", bits);
@@ -2398,5 +2407,170 @@ extern "C" neon_status neon_sample_rows(const float* logits, int64_t stride, int
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
   a.ids = out_ids; a.workspace = workspace; a.err = device_status_word();
   launch_sample_rows(a, S(stream));
+  KLAUNCHED();
+}
+
+// ---- beam search --------------------------------------------------------------
+static bool beam_shape_ok(int B, int W, int V, int n_stop) {
+  return B >= 1 && B <= 65535 && W >= 1 && W <= kBeamMaxW && V >= 1 && V <= (1 << 24) &&
+         n_stop >= 0 && n_stop <= kBeamMaxStop && beam_select_fits(B, W, V);
+}
+
+extern "C" size_t neon_beam_select_workspace(int B, int W, int V, int n_stop) {
+  return beam_shape_ok(B, W, V, n_stop) ? beam_select_workspace(B, W, V, n_stop) : 0;
+}
+
+extern "C" neon_status neon_beam_select(const float* logits, int64_t stride, int B, int W, int V,
+                                        const float* score, const int32_t* stop, int n_stop,
+                                        int32_t* token, int32_t* parent, float* out_score,
+                                        int32_t* end_token, int32_t* end_parent, float* end_score,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (!logits || !score || !token || !parent || !out_score || (n_stop > 0 && !stop))
+    KFAIL(NEON_EINVAL, "neon_beam_select: null pointer");
+  if (!beam_shape_ok(B, W, V, n_stop) || stride < V)
+    KFAIL(NEON_EINVAL, "neon_beam_select: bad shape B=%d W=%d V=%d n_stop=%d stride=%lld", B, W, V,
+          n_stop, (long long)stride);
+  if ((end_token == nullptr) != (end_parent == nullptr) ||
+      (end_token == nullptr) != (end_score == nullptr))
+    KFAIL(NEON_EINVAL, "neon_beam_select: end_token, end_parent and end_score go together");
+  const size_t need = beam_select_workspace(B, W, V, n_stop);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    KFAIL(NEON_EINVAL, "neon_beam_select: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace_bytes, need);
+  BeamSelectArgs a;
+  a.logits = logits; a.stride = stride; a.B = B; a.W = W; a.V = V; a.n_stop = n_stop;
+  a.score = score; a.stop = stop; a.token = token; a.parent = parent; a.out_score = out_score;
+  a.end_token = end_token; a.end_parent = end_parent; a.end_score = end_score;
+  a.err = device_status_word(); a.workspace = workspace;
+  launch_beam_select(a, S(stream));
+  KLAUNCHED();
+}
+
+extern "C" neon_status neon_beam_reorder(void* const* states, int n_states, int B, int W, int slabs,
+                                         int T, int row_bytes, const int32_t* len,
+                                         const int32_t* parent, void* stream) {
+  if (!parent || n_states < 0 || (n_states > 0 && !states))
+    KFAIL(NEON_EINVAL, "neon_beam_reorder: null pointer or n_states=%d", n_states);
+  for (int x = 0; x < n_states; ++x)
+    if (!states[x] || !aligned16(states[x]))
+      KFAIL(NEON_EINVAL, "neon_beam_reorder: state %d must be given, 16-byte aligned", x);
+  BeamReorderArgs a;
+  a.parent = parent; a.len = len; a.groups = B; a.W = W; a.slabs = slabs; a.T = T;
+  a.row_bytes = row_bytes;
+  if (B < 1 || B > 65535 || W < 1 || W > kBeamMaxW || slabs < 1 || T < 1 || row_bytes < 4 ||
+      row_bytes % 4 || !beam_reorder_fits(a))
+    KFAIL(NEON_EINVAL, "neon_beam_reorder: bad shape B=%d W=%d slabs=%d T=%d row_bytes=%d (a "
+          "multiple of 4)", B, W, slabs, T, row_bytes);
+  a.err = device_status_word();
+  if (n_states > 0) launch_beam_reorder(a, states, n_states, S(stream));
+  KLAUNCHED();
+}
+
+// ---- the pages of a cache as a whole --------------------------------------------
+static bool pages_shape_ok(int n_pages, int page_size, int max_pages, int B) {
+  return n_pages >= 1 && n_pages <= kPagesMax && page_size >= 16 && page_size <= 65536 &&
+         (page_size & (page_size - 1)) == 0 && max_pages >= 1 && B >= 1 && B <= 65535 &&
+         pages_fits(B, max_pages);
+}
+
+extern "C" size_t neon_pages_workspace(int n_pages, int B) {
+  return n_pages >= 1 && n_pages <= kPagesMax && B >= 1 && B <= 65535 ? pages_workspace(n_pages, B)
+                                                                      : 0;
+}
+extern "C" size_t neon_pages_counters(int n_pages) {
+  return n_pages >= 1 && n_pages <= kPagesMax ? pages_counters(n_pages) : 0;
+}
+
+extern "C" neon_status neon_pages_fork(const int32_t* refs, const int32_t* page_table,
+                                       const int32_t* kv_len, int B_in, const int32_t* parent,
+                                       const int32_t* keep, const int32_t* add, int32_t* refs_out,
+                                       int32_t* table_out, int32_t* len_out, int32_t* copy_src,
+                                       int32_t* copy_dst, int32_t* copy_rows, int B, int n_pages,
+                                       int page_size, int max_pages, void* workspace,
+                                       size_t workspace_bytes, int32_t* counters,
+                                       size_t counter_bytes, void* stream) {
+  if (!refs || !page_table || !kv_len || !refs_out || !table_out || !len_out || !copy_src ||
+      !copy_dst || !copy_rows)
+    KFAIL(NEON_EINVAL, "neon_pages_fork: null pointer");
+  if (!pages_shape_ok(n_pages, page_size, max_pages, B) ||
+      !pages_shape_ok(n_pages, page_size, max_pages, B_in))
+    KFAIL(NEON_EINVAL, "neon_pages_fork: bad shape n_pages=%d page_size=%d max_pages=%d B_in=%d "
+          "B=%d", n_pages, page_size, max_pages, B_in, B);
+  if (!parent && B != B_in)
+    KFAIL(NEON_EINVAL, "neon_pages_fork: without parent there are as many sequences as before");
+  if (parent && table_out == page_table)
+    KFAIL(NEON_EINVAL, "neon_pages_fork: with parent, table_out is another array than page_table");
+  const size_t need = pages_workspace(n_pages, B), needc = pages_counters(n_pages);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    KFAIL(NEON_EINVAL, "neon_pages_fork: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace_bytes, need);
+  if (!counters || counter_bytes < needc || !aligned16(counters))
+    KFAIL(NEON_EINVAL, "neon_pages_fork: counters of %zu bytes, %zu needed (16-byte aligned)",
+          counter_bytes, needc);
+  PagesForkArgs a;
+  a.refs = refs; a.table = page_table; a.len = kv_len; a.parent = parent; a.keep = keep; a.add = add;
+  a.refs_out = refs_out; a.table_out = table_out; a.len_out = len_out;
+  a.copy_src = copy_src; a.copy_dst = copy_dst; a.copy_rows = copy_rows;
+  a.B_in = B_in; a.B = B; a.n_pages = n_pages; a.page_log2 = __builtin_ctz((unsigned)page_size);
+  a.max_pages = max_pages; a.err = device_status_word();
+  a.workspace = workspace; a.counters = counters;
+  launch_pages_fork(a, S(stream));
+  KLAUNCHED();
+}
+
+extern "C" neon_status neon_pages_copy(const neon_paged_kv* kv, int n_kv, const int32_t* src,
+                                       const int32_t* dst, const int32_t* rows, int n,
+                                       void* stream) {
+  if (!kv || n_kv < 1 || n < 0 || n > (1 << 24) || (n > 0 && (!src || !dst)))
+    KFAIL(NEON_EINVAL, "neon_pages_copy: null pointer, n_kv=%d or n=%d", n_kv, n);
+  std::vector<PagedKv> c;
+  try {
+    c.resize((size_t)n_kv);
+  } catch (...) {
+    KFAIL(NEON_ENOMEM, "neon_pages_copy: no memory for %d caches", n_kv);
+  }
+  for (int x = 0; x < n_kv; ++x) {
+    PagedRows r;
+    const char* why;
+    const int32_t one = 0;  // the batch's arguments, which this call has not
+    if (!paged_args(kv + x, nullptr, &one, &one, 1, 1, 1, c[x], r, why))
+      KFAIL(NEON_EINVAL, "neon_pages_copy: cache %d: %s", x, why);
+    if (kv[x].format != kv[0].format || kv[x].n_pages != kv[0].n_pages ||
+        kv[x].page_size != kv[0].page_size || kv[x].n_kv_heads != kv[0].n_kv_heads ||
+        kv[x].head_dim != kv[0].head_dim)
+      KFAIL(NEON_EINVAL, "neon_pages_copy: cache %d differs from the first in shape or format", x);
+  }
+  if (!pages_copy_fits(c[0], n))
+    KFAIL(NEON_EINVAL, "neon_pages_copy: %d pages are more than a launch holds", n);
+  if (n == 0) return NEON_OK;
+  PagesCopyArgs a;
+  a.src = src; a.dst = dst; a.rows = rows; a.n = n; a.err = device_status_word();
+  launch_pages_copy(a, c.data(), n_kv, S(stream));
+  KLAUNCHED();
+}
+
+extern "C" neon_status neon_pages_compact(const int32_t* refs, const int32_t* page_table,
+                                          const int32_t* kv_len, int32_t* refs_out,
+                                          int32_t* table_out, int32_t* moved_to, int32_t* copy_src,
+                                          int32_t* copy_dst, int B, int n_pages, int page_size,
+                                          int max_pages, void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+  // (a pool of one page has no moves to list)
+  if (!refs || !page_table || !kv_len || !refs_out || !table_out || !moved_to ||
+      (n_pages > 1 && (!copy_src || !copy_dst)))
+    KFAIL(NEON_EINVAL, "neon_pages_compact: null pointer");
+  if (!pages_shape_ok(n_pages, page_size, max_pages, B))
+    KFAIL(NEON_EINVAL, "neon_pages_compact: bad shape n_pages=%d page_size=%d max_pages=%d B=%d",
+          n_pages, page_size, max_pages, B);
+  const size_t need = pages_workspace(n_pages, B);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    KFAIL(NEON_EINVAL, "neon_pages_compact: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace_bytes, need);
+  PagesCompactArgs a;
+  a.refs = refs; a.table = page_table; a.len = kv_len; a.refs_out = refs_out;
+  a.table_out = table_out; a.moved_to = moved_to; a.copy_src = copy_src; a.copy_dst = copy_dst;
+  a.B = B; a.n_pages = n_pages; a.page_log2 = __builtin_ctz((unsigned)page_size);
+  a.max_pages = max_pages; a.err = device_status_word(); a.workspace = workspace;
+  launch_pages_compact(a, S(stream));
   KLAUNCHED();
 }

@@ -147,6 +147,9 @@ constexpr int32_t kDevErrSyncTimeout = 2;   // a grid-wide wait gave up (results
 constexpr int32_t kDevErrPagedRows = 4;     // q_start / kv_len of a paged batch out of range
 constexpr int32_t kDevErrPageId = 8;        // a page id outside [0, n_pages) where a page is needed
 constexpr int32_t kDevErrSampleParam = 16;  // a row's sampling parameter out of range
+constexpr int32_t kDevErrBeam = 32;         // a beam's score, logit or parent that is none
+constexpr int32_t kDevErrPagePlan = 64;     // parent, keep, add, a length or a reference count out of range
+constexpr int32_t kDevErrPagesFull = 128;   // more pages needed than are free
 // polls a grid-wide wait makes before it gives up (~1 s)
 constexpr int kMoeSpinLimit = 1 << 20;
 
@@ -461,5 +464,80 @@ struct SampleRowsArgs {
 size_t sample_rows_needs(int B, int V);      // bytes that a launch uses
 size_t sample_rows_workspace(int B, int V);  // the most of those of up to B rows
 void launch_sample_rows(SampleRowsArgs a, hipStream_t st);
+
+// ---- beam search (neon_beam.hip) -----------------------------------------------
+constexpr int kBeamMaxW = 32, kBeamMaxStop = 16;
+struct BmSum;
+struct BeamSelectArgs {
+  const float* logits;  // [B W][stride]
+  int64_t stride;
+  int B, W, V, n_stop;
+  const float* score;   // [B W]
+  const int32_t* stop;  // [n_stop]
+  int32_t *token, *parent;
+  float* out_score;
+  int32_t *end_token, *end_parent;  // NULL: not wanted
+  float* end_score;
+  int32_t* err;
+  void* workspace;
+  // set by the launcher
+  int K, chunks, steps;
+  BmSum* sums;               // [rows][chunks]
+  unsigned long long* keys;  // [rows][chunks][K]
+};
+bool beam_select_fits(int B, int W, int V);  // the launch's grid holds them
+size_t beam_select_workspace(int B, int W, int V, int n_stop);
+void launch_beam_select(BeamSelectArgs a, hipStream_t st);
+
+constexpr int kBeamStates = 64;  // states of a launch
+struct BeamReorderArgs {
+  const int32_t *parent, *len;
+  int groups, W, slabs, T, row_bytes;
+  int32_t* err;
+  // set by the launcher
+  void* state[kBeamStates];
+  int per, parts;         // units of a row; blocks of a slab
+  int64_t slab, seq;      // units of a slab, of a sequence
+};
+bool beam_reorder_fits(const BeamReorderArgs& a);
+void launch_beam_reorder(BeamReorderArgs a, void* const* states, int n_states, hipStream_t st);
+
+// ---- the pages of a cache as a whole (neon_pages.hip) ---------------------------
+struct PagesForkArgs {
+  const int32_t *refs, *table, *len;  // [n_pages], [B_in][max_pages], [B_in]
+  const int32_t *parent, *keep, *add;  // [B], each may be NULL
+  int32_t *refs_out, *table_out, *len_out;
+  int32_t *copy_src, *copy_dst, *copy_rows;  // [B]
+  int B_in, B, n_pages, page_log2, max_pages;
+  int32_t* err;
+  void* workspace;
+  int32_t* counters;  // zero at launch and left zero
+};
+struct PagesCompactArgs {
+  const int32_t *refs, *table, *len;  // [n_pages], [B][max_pages], [B]
+  int32_t *refs_out, *table_out, *moved_to, *copy_src, *copy_dst;
+  int B, n_pages, page_log2, max_pages;
+  int32_t* err;
+  void* workspace;
+};
+constexpr int kPagesMax = 1 << 24;
+size_t pages_workspace(int n_pages, int B);
+size_t pages_counters(int n_pages);
+bool pages_fits(int B, int max_pages);  // the launches' grids hold them
+void launch_pages_fork(const PagesForkArgs& a, hipStream_t st);
+void launch_pages_compact(const PagesCompactArgs& a, hipStream_t st);
+
+constexpr int kPagesLayers = 64;  // caches of a launch
+struct PagesCopyArgs {
+  const int32_t *src, *dst, *rows;  // [n]; rows NULL: whole pages
+  int n;
+  int32_t* err;
+  // set by the launcher
+  PagedKv kv;                      // shapes
+  uint8_t* pool[kPagesLayers][4];  // k, v and their scales (NULL)
+};
+bool pages_copy_fits(const PagedKv& kv, int n);
+// kv [n_kv]: caches of one shape and format
+void launch_pages_copy(PagesCopyArgs a, const PagedKv* kv, int n_kv, hipStream_t st);
 
 }  // namespace neon
