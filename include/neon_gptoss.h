@@ -580,7 +580,8 @@ neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
  * -inf and NaN are never chosen.  A beam with a score of NaN or +inf or a logit of
  * +inf, or with nothing above -inf, has no candidates (neon_device_check gives
  * NEON_EINVAL for the first three).  B is 1 to 65535, V up to 2^24.
- * workspace: neon_beam_select_workspace(...) bytes, 16-byte aligned, any contents. */
+ * workspace: neon_beam_select_workspace(...) bytes, 16-byte aligned, any contents;
+ * they serve every call of up to B requests of the same W, V and n_stop. */
 size_t neon_beam_select_workspace(int B, int W, int V, int n_stop);
 neon_status neon_beam_select(const float* logits, int64_t stride, int B, int W, int V,
                              const float* score, const int32_t* stop, int n_stop, int32_t* token,

@@ -2433,7 +2433,7 @@ extern "C" neon_status neon_beam_select(const float* logits, int64_t stride, int
   if ((end_token == nullptr) != (end_parent == nullptr) ||
       (end_token == nullptr) != (end_score == nullptr))
     KFAIL(NEON_EINVAL, "neon_beam_select: end_token, end_parent and end_score go together");
-  const size_t need = beam_select_workspace(B, W, V, n_stop);
+  const size_t need = beam_select_needs(B, W, V, n_stop);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     KFAIL(NEON_EINVAL, "neon_beam_select: workspace of %zu bytes, %zu needed (16-byte aligned)",
           workspace_bytes, need);

@@ -481,12 +481,13 @@ struct BeamSelectArgs {
   int32_t* err;
   void* workspace;
   // set by the launcher
-  int K, chunks, steps;
+  int K, chunks;
   BmSum* sums;               // [rows][chunks]
   unsigned long long* keys;  // [rows][chunks][K]
 };
 bool beam_select_fits(int B, int W, int V);  // the launch's grid holds them
-size_t beam_select_workspace(int B, int W, int V, int n_stop);
+size_t beam_select_needs(int B, int W, int V, int n_stop);      // bytes that a launch uses
+size_t beam_select_workspace(int B, int W, int V, int n_stop);  // the most of those of up to B
 void launch_beam_select(BeamSelectArgs a, hipStream_t st);
 
 constexpr int kBeamStates = 64;  // states of a launch

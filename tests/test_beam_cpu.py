@@ -32,8 +32,18 @@ def test_select_refusals(bad):
                                           (3, 32, 1 << 24, 1)])
 def test_select_workspace_is_checked(B, W, V, n_stop):
     n = ne.beam_select_workspace(B, W, V, n_stop)
-    assert n > 0
-    assert select(B=B, W=W, V=V, stride=V, n_stop=n_stop, wb=n - 1) == ne.NEON_EINVAL
+    assert n >= B * W * 8 * (W + n_stop)
+    assert select(B=B, W=W, V=V, stride=V, n_stop=n_stop, wb=B * W * 8 * (W + n_stop)) == ne.NEON_EINVAL
+
+
+@pytest.mark.parametrize("W,V,n_stop", [(1, 201088, 0), (4, 32003, 3), (8, 60000, 1), (32, 5, 16), (5, 1, 0)])
+def test_select_workspace_serves_smaller_batches(W, V, n_stop):
+    """The query never falls as B grows."""
+    last = 0
+    for B in list(range(1, 400)) + list(range(400, 65536, 397)):
+        n = ne.beam_select_workspace(B, W, V, n_stop)
+        assert n >= last
+        last = n
 
 
 def reorder(states=(P, P), n=None, B=2, W=4, slabs=2, T=8, row=128, length=P, parent=P):

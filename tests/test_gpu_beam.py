@@ -141,15 +141,13 @@ def test_select_stop_ids():
 
 
 def test_select_in_place_and_shared_workspace():
-    """out_score may be score; a workspace of any contents and of a larger call serves."""
+    """out_score may be score; a workspace of any contents and of a larger batch serves."""
     torch = torch_cuda()
     rng = np.random.default_rng(8)
-    ws = torch.full((ne.beam_select_workspace(9, 8, 9000, 16),), 0xFF, dtype=torch.uint8, device="cuda")
-    for B, W, V in ((9, 8, 9000), (2, 3, 4100), (9, 8, 1)):
-        l, score = case(rng, B, W, V)
-        want = beam_util.select(l, score, W, [0])
-        check(run(l, score, W, [0], alias=True, workspace=ws[:max(16, ne.beam_select_workspace(B, W, V, 1))]),
-              want)
+    ws = torch.full((ne.beam_select_workspace(40, 8, 60000, 1),), 0xFF, dtype=torch.uint8, device="cuda")
+    for B in (40, 9, 1):
+        l, score = case(rng, B, 8, 60000)
+        check(run(l, score, 8, [0], alias=True, workspace=ws), beam_util.select(l, score, 8, [0]))
 
 
 def test_select_far_offsets():
