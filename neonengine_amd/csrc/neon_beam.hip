@@ -16,24 +16,24 @@
 namespace neon {
 
 typedef unsigned long long u64;
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---------------------------------------------------------------------------
-// The K best of what a wave's lanes hold.  The K-th largest of the lanes' maxima is a
-// bound that few others reach (K lanes hold something at least as large), so what
-// reaches it is listed in LDS, and its order is found by counting.
+// The K best of what a wave sees.  The K-th largest of the lanes' maxima is a bound that
+// few others reach (K lanes hold something at least as large), so what reaches it goes
+// into a list in LDS, and its order is found by counting.
 // ---------------------------------------------------------------------------
-constexpr int kBmList = 128;  // entries of a wave's list
 __device__ __forceinline__ u64 bm_lane_key(u64 v, int lane) {
   return (u64)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
          (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
 }
-// The largest x, of the upper 18 bits, that K of the wave's values reach; 0 where fewer
+// The largest x, of the upper 16 bits, that K of the wave's values reach; 0 where fewer
 // than K lanes have a value.  Two bits at a time: the three counts of a step do not wait
 // for each other.
 __device__ __forceinline__ uint32_t bm_kth(uint32_t v, int K) {
   uint32_t x = 0;
 #pragma unroll
-  for (int bit = 30; bit >= 14; bit -= 2) {
+  for (int bit = 30; bit >= 16; bit -= 2) {
     const uint32_t y1 = x | 1u << bit, y2 = x | 2u << bit, y3 = x | 3u << bit;
     const int n1 = __builtin_popcountll(__ballot(v >= y1));
     const int n2 = __builtin_popcountll(__ballot(v >= y2));
@@ -47,33 +47,66 @@ __device__ __forceinline__ int bm_rank(u64 mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// Where more than kBmList reach the bound (rows of equal logits, orders that put
-// all large ones into few lanes): lane i holds the i-th best key, and each candidate is
-// put in its place.  Of equal keys the earlier one offered is the better.
-__device__ __forceinline__ uint32_t bm_before(uint32_t v) {  // the lane before's (lane 0: 0)
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xF, 0xF, false);  // wave_shr 1
-}
-struct BmBest {
-  u64 key = 0;       // 0: none
-  uint32_t what = 0;  // that belongs to it
-  u64 last = 0;      // the K-th best (uniform)
-  // the lane's k (0: none) and what belongs to it: first + lane
-  __device__ __forceinline__ void offer(u64 k, uint32_t first, int K) {
+// A wave's list of the best keys so far (unique; 0: none).
+constexpr int kBmFull = 128;           // with more than these it is cut down to K
+constexpr int kBmList = kBmFull + 64;  // 64 at most are added at once
+struct BmList {
+  u64* key;           // LDS, kBmList of the wave's own
+  int n = 0;
+  uint32_t least = 0x00800000u;  // upper halves below it are not among the K best (all logits
+                                 // above minus infinity reach this one)
+  u64 last = 0;        // nor are keys up to this one
+  __device__ __forceinline__ explicit BmList(u64* p) : key(p) {}
+  // a bound from the lanes' maxima of something that is added next
+  __device__ __forceinline__ void bound(uint32_t top, int K) { least = max(least, bm_kth(top, K)); }
+  // (n is at most kBmFull)
+  __device__ __forceinline__ void add(u64 k) {
+    const bool is = (uint32_t)(k >> 32) >= least && k > last;
+    const u64 in = __ballot(is);
+    if (is) key[n + bm_rank(in)] = k;
+    n += __builtin_popcountll(in);
+  }
+  // the K best, in order
+  __device__ __forceinline__ void cut(int K) {
     const int lane = threadIdx.x & 63;
-    u64 in = __ballot(k > last);
-    while (in != 0) {
-      const int from = __builtin_ctzll(in);
-      const u64 x = bm_lane_key(k, from);
-      const int at = __builtin_popcountll(__ballot(key >= x));
-      const u64 kb = (u64)bm_before((uint32_t)key) | (u64)bm_before((uint32_t)(key >> 32)) << 32;
-      const uint32_t wb = bm_before(what);
-      key = lane > at ? kb : lane == at ? x : key;
-      what = lane > at ? wb : lane == at ? first + from : what;
-      last = bm_lane_key(key, K - 1);
-      in &= (~1ull << from) & __ballot(k > last);
+    wave_lds_sync();
+    u64 k[3];
+#pragma unroll
+    for (int h = 0; h < 3; ++h) k[h] = 64 * h + lane < n ? key[64 * h + lane] : 0;
+    bound((uint32_t)(max(max(k[0], k[1]), k[2]) >> 32), K);
+    wave_lds_sync();
+#pragma unroll
+    for (int h = 0; h < 3; ++h) {
+      u64 in = __ballot((uint32_t)(k[h] >> 32) >= least);
+      while (in != 0) {
+        const int j = __builtin_ctzll(in);
+        in &= in - 1;
+        const u64 x = bm_lane_key(k[h], j);
+        const int at = __builtin_popcountll(__ballot(k[0] > x)) + __builtin_popcountll(__ballot(k[1] > x)) +
+                       __builtin_popcountll(__ballot(k[2] > x));
+        if (at < K && lane == j) key[at] = x;
+      }
     }
+    wave_lds_sync();
+    if (n >= K) last = max(last, key[K - 1]);
+    n = min(n, K);
   }
 };
+
+// Keys of a list that come before `mine`: every lane reads the same ones, so nothing goes
+// through scalar registers.  Entries from n to the next multiple of 8 are read: `pad` gives
+// them 0, by one wave, before a barrier.
+__device__ __forceinline__ void bm_pad(u64* key, int n) {
+  const int lane = threadIdx.x & 63;
+  if (lane < 8) key[n + lane] = 0;
+}
+__device__ __forceinline__ int bm_before(const u64* key, int n, u64 mine) {
+  int p = 0;
+  for (int j = 0; j < n; j += 8)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p += key[j + i] > mine;
+  return p;
+}
 
 // Order of a logit as an integer: larger logit, larger key; both zeros are one, and
 // minus infinity is 0 (no candidate).
@@ -139,310 +172,358 @@ __device__ __forceinline__ double bm_wave_sum(double v) {
 __device__ __forceinline__ bool bm_alive(float score) { return score > -INFINITY && score < INFINITY; }
 
 // ---------------------------------------------------------------------------
-// A chunk of a row: its maximum, the sum of exponentials and its K = W + n_stop best
-// tokens (of W + n_stop at least W are no stop tokens, and a stop token that is not
-// among them has W better ones in its own row).  A wave holds 1024 NB tokens, 16 NB of a
-// lane.
+// A chunk of a row: the sum of exponentials and its K = W + n_stop best tokens (of
+// W + n_stop at least W are no stop tokens, and a stop token that is not among them has W
+// better ones in its own row).  A wave requests all its tokens at once, up to kBmGroups
+// groups of 256 (4 of a lane), and takes the exponentials of a group as it comes: relative
+// to the maximum of the first one, which a later maximum replaces only where it is 64
+// above (the sum is as exact, and most groups have nothing to rescale).  Then the maxima
+// of the block's lanes give the bound of its list.
 // ---------------------------------------------------------------------------
+constexpr int kBmGroups = 8;
+constexpr float kBmAbove = 64.0f;
 struct __align__(16) BmSum {
-  double s;
-  float m;
+  double s;  // sum of exp(l - m)
+  float m;   // -inf: no token, +inf: a logit of it
   float pad;
 };
 
-// 16 logits of a lane: elements 4 k + j are the tokens t0 + 256 k + 4 lane + j.  A row
-// begins at any multiple of 4 bytes; which lane takes a token does not depend on it, so
-// equal rows have equal sums, and equal beams are ordered by their places.  Tokens past
-// the end and NaNs are minus infinity.
+// Group k of a wave: lane i has the tokens t0 + 256 k + 4 i .. + 3.  A row begins at any
+// multiple of 4 bytes; which lane takes a token does not depend on it, so equal rows have
+// equal sums, and equal beams are ordered by their places.  Tokens past the end are minus
+// infinity, groups past the wave's the last one again (a load under a condition of its own
+// is waited for where the paths join).
 typedef float bm_f4 __attribute__((ext_vector_type(4), aligned(4)));
-template <int N>
-__device__ __forceinline__ void bm_load(const float* row, int V, int t0, int lane, float (&x)[N]) {
-  if (t0 + 64 * N <= V) {  // the whole wave's
+template <int NG>
+__device__ __forceinline__ void bm_load(const float* row, int V, int t0, int groups, int lane,
+                                        float (&x)[4 * NG]) {
+  if (t0 + 256 * groups <= V) {
 #pragma unroll
-    for (int k = 0; k < N / 4; ++k) {
-      const bm_f4 v = *reinterpret_cast<const bm_f4*>(row + t0 + 256 * k + 4 * lane);
+    for (int k = 0; k < NG; ++k) {
+      const bm_f4 v = *reinterpret_cast<const bm_f4*>(row + t0 + 256 * min(k, groups - 1) + 4u * lane);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[4 * k + j] = v[j];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int t = t0 + 256 * (e >> 2) + 4 * lane + (e & 3);
-      const float v = row[min(t, V - 1)];
+    for (int e = 0; e < 4 * NG; ++e) {
+      const int t = t0 + 256 * min(e >> 2, groups - 1) + 4 * lane + (e & 3);
+      const float v = row[(uint32_t)min(t, V - 1)];
       x[e] = t < V ? v : -INFINITY;
     }
   }
-#pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = x[e] != x[e] ? -INFINITY : x[e];
 }
 
-template <int NB>
+template <int NG>
 __global__ __launch_bounds__(256) void k_beam_part(BeamSelectArgs a) {
-  constexpr int N = 16 * NB;
-  __shared__ u64 list[4][kBmList];
-  __shared__ int count[4];
+  __shared__ u64 keys[4][kBmList];
+  __shared__ double sums[4][64];
+  __shared__ float tops[4][64];
+  __shared__ u64 joint[4 * 64 + 8];
+  __shared__ int total;
   __shared__ float ms[4];
-  __shared__ double ss[4];
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   if (!bm_alive(a.score[row])) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int K = a.K;
-  const int t0 = (chunk * 4 + wave) * 64 * N;
+  const int first = (chunk * 4 + wave) * a.groups * 256;
+  const int groups = first < a.V ? min(a.groups, (a.V - first + 255) >> 8) : 0;
   const BmExp exp_of;
-  float m = -INFINITY;
-  double s = 0.0;
-  int n = 0;
-  if (t0 < a.V) {
-    float x[N], top4[N / 4], top;
-    bm_load<N>(a.logits + (int64_t)row * a.stride, a.V, t0, lane, x);
+  float x[4 * NG], top = -INFINITY, m = -INFINITY;
+  double s[2];
+  if (groups > 0) {
+    bm_load<NG>(a.logits + (int64_t)row * a.stride, a.V, first, groups, lane, x);
+    // a NaN is a quiet one from here on: maxima pass it over, comparisons fail
 #pragma unroll
-    for (int k = 0; k < N / 4; ++k) {
-      top4[k] = fmaxf(fmaxf(x[4 * k], x[4 * k + 1]), fmaxf(x[4 * k + 2], x[4 * k + 3]));
-      top = k == 0 ? top4[0] : fmaxf(top, top4[k]);
-    }
-    m = wave_max(top);
-    if (m != -INFINITY && m != INFINITY) {
-      const double md = (double)m;
-      double part[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_canonicalizef(x[j]);
+    m = wave_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), -INFINITY));
+    for (bool again = true; again;) {
+      const double md = m == -INFINITY ? 0.0 : (double)m;
+      s[0] = s[1] = 0.0;
 #pragma unroll
-      for (int e = 0; e < N; ++e) part[e & 3] += exp_of((double)x[e] - md);
-      s = bm_wave_sum((part[0] + part[1]) + (part[2] + part[3]));
-    }
-    const uint32_t bound = bm_kth(bm_ordered(top), K);
-    const float least = bound == 0 ? -3.4028234663852886e38f : bm_logit(bound);
-    auto token = [&](int e) { return t0 + 256 * (e >> 2) + 4 * lane + (e & 3); };
+      for (int k = 0; k < NG; ++k) {
+        if (k < groups) {
+          float* y = x + 4 * k;
 #pragma unroll
-    for (int k = 0; k < N / 4; ++k) {
-      if (__ballot(top4[k] >= least) == 0) continue;
+          for (int j = 0; j < 4; ++j) y[j] = __builtin_canonicalizef(y[j]);
+          top = fmaxf(top, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 in = __ballot(x[4 * k + j] >= least);
-        if (in == 0) continue;
-        const int at = n + bm_rank(in);
-        if (x[4 * k + j] >= least && at < kBmList) list[wave][at] = bm_key(x[4 * k + j], token(4 * k + j));
-        n += __builtin_popcountll(in);
+          for (int j = 0; j < 4; ++j) s[j & 1] += exp_of((double)y[j] - md);
+        }
       }
-    }
-    if (n > kBmList) {
-      BmBest best;
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (__ballot(x[e] >= least) != 0) best.offer(x[e] >= least ? bm_key(x[e], token(e)) : 0, 0, K);
-      }
-      if (lane < K) list[wave][lane] = best.key;
-      n = K;
+      again = __any((top > m + kBmAbove) | ((m == -INFINITY) & (top > m)));
+      if (again) m = wave_max(top);
     }
   }
-  if (lane == 0) {
-    count[wave] = n;
-    ms[wave] = m;
-    ss[wave] = s;
-  }
+  tops[wave][lane] = top;
+  for (int i = threadIdx.x; i < 4 * 64 + 8; i += 256) joint[i] = 0;
+  if (threadIdx.x == 0) total = 0;
   __syncthreads();
-  // the places of the four lists' keys
+  const float all4 = fmaxf(fmaxf(tops[0][lane], tops[1][lane]), fmaxf(tops[2][lane], tops[3][lane]));
+  BmList list(keys[wave]);
+  list.bound(bm_ordered(all4), K);
+  const float least = bm_logit(list.least);
+  // which of the lane's logits reach the bound: bit 4 NG - 1 - e
+  u64 reach = 0;
+  if (groups > 0) {
+#pragma unroll
+    for (int e = 0; e < 4 * NG; ++e) reach = reach << 1 | ((x[e] >= least) & (e < 4 * groups));
+  }
+  while (__any(reach != 0)) {  // every lane its next one
+    const int bit = 63 - __builtin_clzll(reach | 1), e = 4 * NG - 1 - bit;
+    float v = x[0];
+#pragma unroll
+    for (int i = 1; i < 4 * NG; ++i) v = e == i ? x[i] : v;
+    list.add(reach != 0 ? bm_key(v, first + 256 * (e >> 2) + 4 * lane + (e & 3)) : 0);
+    reach &= ~(1ull << bit);
+    if (list.n > kBmFull) list.cut(K);
+  }
+  if (list.n > 64) list.cut(K);
+  sums[wave][lane] = groups > 0 && m != -INFINITY ? s[0] + s[1] : 0.0;
+  // the waves' lists as one, in any order
+  int base = 0;
+  if (lane == 0) {
+    base = atomicAdd(&total, list.n);
+    ms[wave] = m;
+  }
+  base = uni(base);
+  if (lane < list.n) joint[base + lane] = keys[wave][lane];
+  __syncthreads();
+  const int all = total, i = threadIdx.x;
   const int64_t at = (int64_t)row * a.chunks + chunk;
-  const int all = count[0] + count[1] + count[2] + count[3];
-  for (int i = lane; i < n; i += 64) {
-    const u64 mine = list[wave][i];
-    int place = 0;
-    for (int w = 0; w < 4; ++w)
-      for (int j = 0; j < count[w]; ++j) place += list[w][j] > mine;
+  if (i < all) {
+    const u64 mine = joint[i];
+    const int place = bm_before(joint, all, mine);
     if (place < K) a.keys[at * K + place] = mine;
   }
-  if ((int)threadIdx.x < K && (int)threadIdx.x >= all) a.keys[at * K + threadIdx.x] = 0;
-  if (threadIdx.x == 0) {
+  if (i >= all && i < K) a.keys[at * K + i] = 0;
+  if (wave == 3) {
     const float M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-    double S = 0.0;
-    for (int w = 0; w < 4; ++w)
-      if (ms[w] != -INFINITY) S += ss[w] * exp_of((double)ms[w] - (double)M);
-    a.sums[at].s = S;
-    a.sums[at].m = M;
+    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const double f = ms[w] == -INFINITY ? 0.0 : exp_of((double)ms[w] - (double)M);
+      sum += sums[w][lane] * f;
+    }
+    sum = bm_wave_sum(sum);
+    if (lane == 0) {
+      a.sums[at].s = sum;
+      a.sums[at].m = M;
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
-// A request: the K best of each row, then the W best that go on and the stop tokens
-// among the W best.
+// A request: the K best of each row (a wave each), then the W best that go on and the
+// stop tokens among the W best.
 // ---------------------------------------------------------------------------
 constexpr int kBmMaxK = kBeamMaxW + kBeamMaxStop;
 constexpr int kBmJoinWaves = 16;
+constexpr int kBmAhead = 8;  // keys of a lane that are requested at once
+constexpr int kBmOpen = kBeamMaxW * kBmMaxK;
 __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs a) {
-  __shared__ u64 list[kBmJoinWaves][kBmList];
-  __shared__ u64 value[kBeamMaxW * kBmMaxK];  // of (place, rank), ordered; 0: none
-  __shared__ int token[kBeamMaxW * kBmMaxK];
+  __shared__ u64 lists[kBmJoinWaves][kBmList + 8];
+  __shared__ u64 value[kBmOpen];  // of (place, rank), ordered; 0: none
+  __shared__ int token[kBmOpen];  // | place << 24, negative: a stop token
+  __shared__ u64 key_all[kBmOpen + 8], key_live[kBmOpen + 8];
+  __shared__ int from[kBmOpen], total;
   __shared__ int stop[kBeamMaxStop];
-  const int b = blockIdx.x, W = a.W, K = a.K;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ int next[kBeamMaxW], over[kBeamMaxW], to_free[kBeamMaxW];
+  const int b = blockIdx.x, W = a.W, K = a.K, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const BmExp exp_of;
-  if (threadIdx.x < kBeamMaxStop) stop[threadIdx.x] = (int)threadIdx.x < a.n_stop ? a.stop[threadIdx.x] : -1;
-  for (int w = wave; w < W; w += kBmJoinWaves) {
-    const int row = b * W + w;
+  if ((int)threadIdx.x < a.n_stop) stop[threadIdx.x] = a.stop[threadIdx.x];
+  if (threadIdx.x < kBeamMaxW) next[threadIdx.x] = over[threadIdx.x] = -1;
+  for (int i = threadIdx.x; i < W * K + 8; i += blockDim.x) key_all[i] = key_live[i] = 0;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  for (int w = wave; w < W; w += waves) {
+    const int row = b * W + w, all = a.chunks * K;
+    const BmSum* sums = a.sums + (int64_t)row * a.chunks;
+    const u64* keys = a.keys + (int64_t)row * all;
+    // what the row's chunks left, on its way at once (a row without a beam has nothing
+    // there that is used)
     const float score = a.score[row];
+    BmSum sum = sums[min(lane, a.chunks - 1)];
+    u64 k[kBmAhead];
+#pragma unroll
+    for (int h = 0; h < kBmAhead; ++h) k[h] = keys[min(64 * h + lane, all - 1)];
     bool alive = bm_alive(score);
     if (lane == 0 && (score != score || score == INFINITY)) flag_dev_err(a.err, kDevErrBeam);
     double lse = 0.0;
+    BmList list(lists[wave]);
     if (alive) {
-      float m = -INFINITY;
-      for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, a.sums[(int64_t)row * a.chunks + c].m);
+      float m = lane < a.chunks ? sum.m : -INFINITY;
+      for (int c = 64 + lane; c < a.chunks; c += 64) m = fmaxf(m, sums[c].m);
       m = wave_max(m);
       double s = 0.0;
       for (int c = lane; c < a.chunks; c += 64) {
-        const BmSum p = a.sums[(int64_t)row * a.chunks + c];
-        if (p.m != -INFINITY) s += p.s * exp_of((double)p.m - (double)m);
+        if (c != lane) sum = sums[c];
+        if (sum.m != -INFINITY) s += sum.s * exp_of((double)sum.m - (double)m);
       }
       s = bm_wave_sum(s);
       if (lane == 0 && m == INFINITY) flag_dev_err(a.err, kDevErrBeam);
       alive = m > -INFINITY && m < INFINITY;
       lse = (double)m + log(s);
     }
-    int n = 0;
     if (alive) {
-      const int all = a.chunks * K;
-      const u64* keys = a.keys + (int64_t)row * all;
-      u64 top = 0;
-      for (int i = lane; i < all; i += 64) top = max(top, keys[i]);
-      const uint32_t least = bm_kth((uint32_t)(top >> 32), K);
-      for (int i0 = 0; i0 < all; i0 += 64) {
-        const u64 k = i0 + lane < all ? keys[i0 + lane] : 0;
-        const bool is = k != 0 && (uint32_t)(k >> 32) >= least;
-        const u64 in = __ballot(is);
-        const int at = n + bm_rank(in);
-        if (is && at < kBmList) list[wave][at] = k;
-        n += __builtin_popcountll(in);
+      for (int i0 = 0; i0 < all; i0 += 64 * kBmAhead) {
+        if (i0 > 0)
+#pragma unroll
+          for (int h = 0; h < kBmAhead; ++h) k[h] = keys[min(i0 + 64 * h + lane, all - 1)];
+        u64 top = 0;
+#pragma unroll
+        for (int h = 0; h < kBmAhead; ++h) {
+          k[h] = i0 + 64 * h + lane < all ? k[h] : 0;
+          top = max(top, k[h]);
+        }
+        list.bound((uint32_t)(top >> 32), K);
+        uint32_t reach = 0;  // bit h: the lane's k[h] does
+#pragma unroll
+        for (int h = 0; h < kBmAhead; ++h) reach |= (uint32_t)((uint32_t)(k[h] >> 32) >= list.least) << h;
+        while (__any(reach != 0)) {  // every lane its next one
+          const int h = __builtin_ctz(reach | 1u << 31);
+          u64 one = k[0];
+#pragma unroll
+          for (int i = 1; i < kBmAhead; ++i) one = h == i ? k[i] : one;
+          list.add(reach != 0 ? one : 0);
+          reach &= reach - 1;
+          if (list.n > kBmFull) list.cut(K);
+        }
       }
-      if (n > kBmList) {
-        BmBest best;
-        for (int i0 = 0; i0 < all; i0 += 64) best.offer(i0 + lane < all ? keys[i0 + lane] : 0, 0, K);
-        if (lane < K) list[wave][lane] = best.key;
-        n = K;
-      }
-      wave_lds_sync();
+      if (list.n > 64) list.cut(K);
     }
-    if (lane < K && lane >= n) value[w * K + lane] = 0;
-    for (int i = lane; i < n; i += 64) {
-      const u64 mine = list[wave][i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += list[wave][j] > mine;
-      if (place < K) {
-        const double v = (double)score + ((double)bm_logit((uint32_t)(mine >> 32)) - lse);
-        value[w * K + place] = bm_ordered64(v);
-        token[w * K + place] = (int)~(uint32_t)mine;
-      }
+    bm_pad(lists[wave], list.n);
+    wave_lds_sync();
+    const u64 mine = lane < list.n ? lists[wave][lane] : 0;
+    const int place = bm_before(lists[wave], list.n, mine);
+    if (lane < list.n && place < K) {
+      const int t = (int)~(uint32_t)mine;
+      const double v = (double)score + ((double)bm_logit((uint32_t)(mine >> 32)) - lse);
+      value[w * K + place] = bm_ordered64(v);
+      bool is = false;
+      for (int j = 0; j < a.n_stop; ++j) is |= t == stop[j];
+      token[w * K + place] = t | w << 24 | (is ? 1 << 31 : 0);
     }
+    if (lane < K && lane >= list.n) value[w * K + lane] = 0;
     wave_lds_sync();  // the list is free
   }
   __syncthreads();
-  if (wave > 1) return;
-  // wave 0: the W best of all; wave 1: of those that are no stop tokens; equal ones in
-  // the order of place and rank
-  auto is_stop = [&](int t) {
-    bool is = false;
-    for (int i = 0; i < a.n_stop; ++i) is |= t == stop[i];
-    return is;
-  };
+  // every candidate's place among all, if it is a stop token, or among those that are
+  // none: larger values before it, and equal ones of a lower index.  Of more than 64, those
+  // that cannot be among the W best are left out first.
   const int all = W * K;
-  auto value_of = [&](int i) {
-    u64 k = i < all ? value[i] : 0;
-    if (wave == 1 && k != 0 && is_stop(token[i])) k = 0;
-    return k;
-  };
-  u64 top = 0;
-  for (int i = lane; i < all; i += 64) top = max(top, value_of(i));
-  const uint32_t least = bm_kth((uint32_t)(top >> 32), W);
-  BmBest best;
-  for (int i0 = 0; i0 < all; i0 += 64) {
-    const u64 k = value_of(i0 + lane);
-    best.offer((uint32_t)(k >> 32) >= least ? k : 0, (uint32_t)i0, W);
+  u64 least = 1;
+  if (all > 64) {
+    u64 top = 0;
+    for (int i = lane; i < all; i += 64) top = max(top, token[i] < 0 ? 0 : value[i]);
+    least = max(1ull, (u64)bm_kth((uint32_t)(top >> 32), W) << 32);
   }
-  const bool has = lane < W && best.key != 0;
-  const int place = has ? (int)best.what / K : -1;
-  const int tok = has ? token[best.what] : -1;
-  const float v = has ? (float)bm_value64(best.key) : -INFINITY;
-  if (wave == 0) {
+  for (int i = threadIdx.x; i < all; i += blockDim.x) {
+    const u64 v = value[i];
+    if (v < least) continue;
+    const int at = atomicAdd(&total, 1);
+    key_all[at] = v;
+    key_live[at] = token[i] < 0 ? 0 : v;
+    from[at] = i;
+  }
+  __syncthreads();
+  const int n = total;
+  for (int c = threadIdx.x; c < n; c += blockDim.x) {
+    const u64 v = key_all[c];
+    const bool is = key_live[c] == 0;
+    const u64* among = is ? key_all : key_live;
+    int more = 0, as_much = 0;
+    for (int j = 0; j < n; j += 8)
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const u64 x = among[j + g];
+        more += x > v;
+        as_much += x >= v;
+      }
+    if (as_much - more > 1)  // (a stop token is not among its own, with equal ones it is)
+      for (int j = 0; j < n; ++j) more += among[j] == v && from[j] < from[c];
+    if (more < W) (is ? over : next)[more] = from[c];
+  }
+  __syncthreads();
+  if (wave > 1) return;
+  const int i = lane < W ? (wave == 0 ? next : over)[lane] : -1;
+  const int tok = i >= 0 ? token[i] & 0xFFFFFF : -1, place = i >= 0 ? token[i] >> 24 & 31 : -1;
+  const float v = i >= 0 ? (float)bm_value64(value[i]) : -INFINITY;
+  if (wave == 1) {  // (places between stop tokens are empty)
     if (a.end_token == nullptr) return;
-    const bool ends = has && is_stop(tok);
-    const u64 over = __ballot(ends);
-    const int at = bm_rank(over);
-    if (ends) {
-      a.end_token[b * W + at] = tok;
-      a.end_parent[b * W + at] = b * W + place;
-      a.end_score[b * W + at] = v;
-    }
-    if (lane >= __builtin_popcountll(over) && lane < W) {
-      a.end_token[b * W + lane] = -1;
-      a.end_parent[b * W + lane] = -1;
-      a.end_score[b * W + lane] = -INFINITY;
+    const u64 in = __ballot(i >= 0);
+    const int n_in = __builtin_popcountll(in);
+    if (lane < W) {
+      const int at = b * W + (i >= 0 ? bm_rank(in) : n_in + bm_rank(~in));
+      a.end_token[at] = tok;
+      a.end_parent[at] = i >= 0 ? b * W + place : -1;
+      a.end_score[at] = v;
     }
     return;
   }
-  // the first child of a beam keeps its place
-  bool keeps = false;
+  // the first child of a beam keeps its place; the others take the free ones in order
+  bool keeps = i >= 0;
   u64 taken = 0;
-  for (int w = 0; w < W; ++w) {
-    const u64 children = __ballot(place == w);
-    if (children == 0) continue;
-    taken |= 1ull << w;
-    keeps |= lane == __builtin_ctzll(children);
+  for (int j = 0; j < W; ++j) {
+    const int p = __builtin_amdgcn_readlane(place, j);
+    if (p >= 0) taken |= 1ull << p;
+    keeps &= !(j < lane && p == place);
   }
+  const u64 open = __ballot(lane < W && !(taken >> lane & 1));
+  if (open >> lane & 1) to_free[bm_rank(open)] = lane;
   const u64 movers = __ballot(lane < W && !keeps);
-  int nth = bm_rank(movers);  // the free place that a mover takes
-  u64 open = ~taken;
-  int to = place;
-  if (!keeps) {
-    for (; nth > 0; --nth) open &= open - 1;
-    to = __builtin_ctzll(open);
-  }
+  wave_lds_sync();
   if (lane < W) {
-    a.token[b * W + to] = tok;
-    a.parent[b * W + to] = has ? b * W + place : -1;
-    a.out_score[b * W + to] = v;
+    const int to = b * W + (keeps ? place : to_free[bm_rank(movers)]);
+    a.token[to] = tok;
+    a.parent[to] = i >= 0 ? b * W + place : -1;
+    a.out_score[to] = v;
   }
 }
 
-// Batches of 16 tokens of a lane: four where the chip is full several times over.
-static int beam_batches(int64_t rows, int V) {
-  const int64_t waves = rows * (((int64_t)V + 1023) / 1024);
-  return waves >= 16384 ? 4 : waves >= 4096 ? 2 : 1;
+// Groups of a wave: as many blocks as run at once, where there are enough tokens; no fewer
+// than 4 groups, since the join takes the chunks' keys one row after another.
+constexpr int64_t kBmPlaces = 1536;
+static int beam_groups(int64_t rows, int V) {
+  const int64_t chunks = std::max<int64_t>(1, kBmPlaces / rows);
+  const int64_t groups = ((int64_t)V + 1024 * chunks - 1) / (1024 * chunks);
+  return (int)std::min<int64_t>(std::max<int64_t>(groups, 4), kBmGroups);
 }
-static int beam_chunks(int V, int nb) { return (int)(((int64_t)V + 4096 * nb - 1) / (4096 * nb)); }
+static int beam_chunks(int V, int groups) {
+  const int64_t per = 1024 * (int64_t)groups;
+  return (int)(((int64_t)V + per - 1) / per);
+}
 constexpr int64_t kBmMaxBlocks = 1 << 24;  // of 256 threads: a launch holds fewer than 2^32
 bool beam_select_fits(int B, int W, int V) {
   const int64_t rows = (int64_t)B * W;
-  return rows * beam_chunks(V, beam_batches(rows, V)) < kBmMaxBlocks;
+  return rows * beam_chunks(V, beam_groups(rows, V)) < kBmMaxBlocks;
 }
 static size_t beam_chunk_bytes(int K) { return (size_t)K * 8 + sizeof(BmSum); }
 size_t beam_select_needs(int B, int W, int V, int n_stop) {
   const int64_t rows = (int64_t)B * W;
-  return (size_t)rows * beam_chunks(V, beam_batches(rows, V)) * beam_chunk_bytes(W + n_stop);
+  return (size_t)rows * beam_chunks(V, beam_groups(rows, V)) * beam_chunk_bytes(W + n_stop);
 }
-// Fewer rows may be cut into more chunks: the most that any number up to B needs is at
-// B or right before a step of beam_batches.
+// Fewer rows may be cut into more chunks, but into no more than run at once, or than
+// those of the most groups.
 size_t beam_select_workspace(int B, int W, int V, int n_stop) {
-  size_t most = beam_select_needs(B, W, V, n_stop);
-  int lo = 1, hi = B;
-  for (int nb = beam_batches((int64_t)B * W, V); nb > 1; nb >>= 1) {
-    for (lo = 1; lo < hi;) {  // the first B with as many batches as this
-      const int mid = lo + (hi - lo) / 2;
-      if (beam_batches((int64_t)mid * W, V) >= nb) hi = mid;
-      else lo = mid + 1;
-    }
-    hi = lo;
-    if (lo > 1) most = std::max(most, beam_select_needs(lo - 1, W, V, n_stop));
-  }
-  return most;
+  const int64_t rows = (int64_t)B * W;
+  const int64_t chunks = std::min(rows * beam_chunks(V, 4),
+                                  std::max(kBmPlaces + rows, rows * beam_chunks(V, kBmGroups)));
+  return (size_t)chunks * beam_chunk_bytes(W + n_stop);
 }
 void launch_beam_select(BeamSelectArgs a, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.W;
-  const int nb = beam_batches(rows, a.V);
-  a.chunks = beam_chunks(a.V, nb);
+  a.groups = beam_groups(rows, a.V);
+  a.chunks = beam_chunks(a.V, a.groups);
   a.K = a.W + a.n_stop;
   a.sums = (BmSum*)a.workspace;
   a.keys = (u64*)(a.sums + (size_t)rows * a.chunks);
   const dim3 grid((unsigned)(rows * a.chunks));
-  if (nb == 4) hipLaunchKernelGGL(k_beam_part<4>, grid, dim3(256), 0, st, a);
-  else if (nb == 2) hipLaunchKernelGGL(k_beam_part<2>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(k_beam_part<1>, grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.B), dim3(64 * kBmJoinWaves), 0, st, a);
+  if (a.groups > 4) hipLaunchKernelGGL(k_beam_part<kBmGroups>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(k_beam_part<4>, grid, dim3(256), 0, st, a);
+  const int waves = std::min(std::max(a.W, 2), kBmJoinWaves);
+  hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.B), dim3(64 * waves), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------

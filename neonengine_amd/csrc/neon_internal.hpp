@@ -481,7 +481,7 @@ struct BeamSelectArgs {
   int32_t* err;
   void* workspace;
   // set by the launcher
-  int K, chunks;
+  int K, chunks, groups;
   BmSum* sums;               // [rows][chunks]
   unsigned long long* keys;  // [rows][chunks][K]
 };
