@@ -526,48 +526,83 @@ void launch_beam_select(BeamSelectArgs a, hipStream_t st) {
   hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.B), dim3(64 * waves), 0, st, a);
 }
 
+constexpr int kReorderUnits = 4;
 // ---------------------------------------------------------------------------
-// Moving states: a thread takes one place of the W beams of a request in a state and
-// reads all that move there before it writes any, so the move is in place whatever the
+// Moving states.  A block takes the same part of a slab in all beams of a request, U
+// units of a thread.  Where no beam that moves is also one that others continue (beams
+// that go on keep their places), each is copied for itself; otherwise a thread reads all
+// that move to its places before it writes any, so the move is in place whatever the
 // parents are (a permutation too).
 // ---------------------------------------------------------------------------
 template <class T, int WMAX>
 __global__ __launch_bounds__(256) void k_beam_reorder(BeamReorderArgs a) {
+  constexpr int U = kReorderUnits;
   // block: (state, request, slab, part of the slab)
-  int64_t id = blockIdx.x;
-  const int part = (int)(id % a.parts);
+  int id = blockIdx.x;
+  const int part = id % a.parts;
   id /= a.parts;
-  const int slab = (int)(id % a.slabs);
+  const int slab = id % a.slabs;
   id /= a.slabs;
-  const int g = (int)(id % a.groups), x = (int)(id / a.groups);
-  const int64_t i = (int64_t)part * 256 + threadIdx.x;  // place in the slab
-  T* base = reinterpret_cast<T*>(a.state[x]) + (int64_t)g * a.W * a.seq + slab * a.slab + i;
-  T v[WMAX];
-  bool moves[WMAX];
-#pragma unroll
-  for (int w = 0; w < WMAX; ++w) {
-    moves[w] = false;
-    if (w >= a.W) continue;
-    const int row = g * a.W + w, p = a.parent[row] - g * a.W;
+  const int g = id % a.groups, x = id / a.groups;
+  const int lane = threadIdx.x & 63;
+  // lane = place: where its row comes from, and how many units of it
+  int p = -1;
+  int64_t n = 0;
+  if (lane < a.W) {
+    p = a.parent[g * a.W + lane] - g * a.W;
     if ((unsigned)p >= (unsigned)a.W) {
-      if (p != -1 - g * a.W && threadIdx.x == 0 && part == 0) flag_dev_err(a.err, kDevErrBeam);
-      continue;
+      if (p != -1 - g * a.W && threadIdx.x < 64 && part == 0 && slab == 0 && x == 0)
+        flag_dev_err(a.err, kDevErrBeam);
+      p = -1;
     }
-    if (p == w) continue;
-    const int n = a.len != nullptr ? min(max(a.len[g * a.W + p], 0), a.T) : a.T;
-    moves[w] = i < (int64_t)n * a.per;
-    if (moves[w]) v[w] = base[(int64_t)p * a.seq];
+    if (p == lane) p = -1;
+    if (p >= 0) n = (int64_t)(a.len != nullptr ? min(max(a.len[g * a.W + p], 0), a.T) : a.T) * a.per;
   }
+  const int64_t i0 = (int64_t)part * (256 * U);
+  uint64_t moved = __ballot(p >= 0 && n > i0);
+  if (moved == 0) return;
+  bool clash = false;
+  for (uint64_t in = moved; in != 0; in &= in - 1)
+    clash |= (moved >> __builtin_amdgcn_readlane(p, __builtin_ctzll(in)) & 1) != 0;
+  T* base = reinterpret_cast<T*>(a.state[x]) + (int64_t)g * a.W * a.seq + slab * a.slab;
+  auto from = [&](int w) { return base + (int64_t)__builtin_amdgcn_readlane(p, w) * a.seq; };
+  auto units = [&](int w) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)n, w) |
+           (int64_t)__builtin_amdgcn_readlane((int)(n >> 32), w) << 32;
+  };
+  if (!clash) {
+    for (; moved != 0; moved &= moved - 1) {
+      const int w = __builtin_ctzll(moved);
+      const T* src = from(w);
+      T* dst = base + (int64_t)w * a.seq;
+      const int64_t end = units(w);
+      T v[U];
 #pragma unroll
-  for (int w = 0; w < WMAX; ++w)
-    if (moves[w]) base[(int64_t)w * a.seq] = v[w];
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * 256 + threadIdx.x < end) v[u] = src[i0 + u * 256 + threadIdx.x];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * 256 + threadIdx.x < end) stream_store(dst + i0 + u * 256 + threadIdx.x, v[u]);
+    }
+    return;
+  }
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + u * 256 + threadIdx.x;
+    T v[WMAX];
+#pragma unroll
+    for (int w = 0; w < WMAX; ++w)
+      if ((moved >> w & 1) != 0 && i < units(w)) v[w] = from(w)[i];
+#pragma unroll
+    for (int w = 0; w < WMAX; ++w)
+      if ((moved >> w & 1) != 0 && i < units(w)) stream_store(base + (int64_t)w * a.seq + i, v[w]);
+  }
 }
 
 static int64_t reorder_units(const BeamReorderArgs& a) {  // of a slab
   return (int64_t)a.T * (a.row_bytes % 16 == 0 ? a.row_bytes / 16 : a.row_bytes / 4);
 }
 bool beam_reorder_fits(const BeamReorderArgs& a) {
-  const int64_t parts = (reorder_units(a) + 255) / 256;
+  const int64_t parts = (reorder_units(a) + 256 * kReorderUnits - 1) / (256 * kReorderUnits);
   return parts < kBmMaxBlocks && parts * a.slabs < kBmMaxBlocks &&
          parts * a.slabs * a.groups < kBmMaxBlocks;
 }
@@ -576,7 +611,7 @@ void launch_beam_reorder(BeamReorderArgs a, void* const* states, int n_states, h
   a.per = wide ? a.row_bytes / 16 : a.row_bytes / 4;
   a.slab = (int64_t)a.T * a.per;
   a.seq = a.slab * a.slabs;
-  a.parts = (int)((a.slab + 255) / 256);
+  a.parts = (int)((a.slab + 256 * kReorderUnits - 1) / (256 * kReorderUnits));
   const int64_t blocks = (int64_t)a.parts * a.slabs * a.groups;  // of a state
   const int most = (int)std::min<int64_t>(kBeamStates, (kBmMaxBlocks - 1) / blocks);
   for (int x0 = 0, n; x0 < n_states; x0 += n) {

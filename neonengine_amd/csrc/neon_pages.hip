@@ -500,7 +500,7 @@ __device__ __forceinline__ void pg_copy_units(const PagesCopyArgs& a, uint8_t* p
     has &= has - 1;
     const int s = __builtin_amdgcn_readlane(src, e), d = __builtin_amdgcn_readlane(dst, e);
     const int n = __builtin_amdgcn_readlane(rows, e);
-    if (in && row < n) p[(int64_t)d * page_units] = p[(int64_t)s * page_units];
+    if (in && row < n) stream_store(p + (int64_t)d * page_units, p[(int64_t)s * page_units]);
   }
 }
 
