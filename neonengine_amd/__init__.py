@@ -218,15 +218,16 @@ def _nbytes(t):
 _current = None  # (device index, its stream's handle) functions, once a device was
                  # found (a process does not lose it again)
 _fp16 = None     # torch.float16 from then on: it has the size of bf16
+_int32 = _float32 = None  # torch's
 
 
 def _find_current():
     """Functions that give torch's current device, and its current stream there:
     torch's own shortcuts to the bare numbers where it has them
     (torch.cuda.current_stream() makes an object for 3 us)."""
-    global _current, _fp16
+    global _current, _fp16, _int32, _float32
     import torch
-    _fp16 = torch.float16
+    _fp16, _int32, _float32 = torch.float16, torch.int32, torch.float32
     if not torch.cuda.is_available():
         return None
     torch.cuda.init()
@@ -467,6 +468,25 @@ def _arg(t, size, n, name, device, real=None):
     return t.data_ptr()
 
 
+def _i32(t, n, name, device):
+    """_arg of at least n int32: the plans and choices take up to fourteen of these, and
+    one test of the type is half of what _arg costs."""
+    if t.dtype is not _int32 or t.numel() < n or t.get_device() != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{name}: needs {n} contiguous int32 on device {device}, has "
+                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _f32(t, n, name, device):
+    """_arg of at least n float32."""
+    if t.dtype is not _float32 or t.numel() < n or t.get_device() != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{name}: needs {n} contiguous float32 on device {device}, has "
+                         f"{tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
 def _scratch(nbytes, stream, zero=False):
     """_workspace, allocated (and zeroed) on the stream that the call runs on:
     memory of another one could be in use there still, or handed out again
@@ -646,15 +666,17 @@ def beam_select(logits, score, W, token, parent, out_score, stop=None, ended=Non
     n_stop = 0 if stop is None else stop.numel()
     if workspace is None:
         workspace = _scratch(beam_select_workspace(N // W, W, V, n_stop), stream)
-    end = (None,) * 3 if ended is None else (
-        _arg(ended[0], 4, N, "end_token", device, False),
-        _arg(ended[1], 4, N, "end_parent", device, False),
-        _arg(ended[2], 4, N, "end_score", device, True))
+    end_token = end_parent = end_score = None
+    if ended is not None:
+        end_token, end_parent, end_score = ended
+        end_token = _i32(end_token, N, "end_token", device)
+        end_parent = _i32(end_parent, N, "end_parent", device)
+        end_score = _f32(end_score, N, "end_score", device)
     _check(lib().neon_beam_select(
-        rows, stride, N // W, W, V, _arg(score, 4, N, "score", device, True),
-        _arg(stop, 4, n_stop, "stop", device, False) if n_stop else None, n_stop,
-        _arg(token, 4, N, "token", device, False), _arg(parent, 4, N, "parent", device, False),
-        _arg(out_score, 4, N, "out_score", device, True), *end,
+        rows, stride, N // W, W, V, _f32(score, N, "score", device),
+        _i32(stop, n_stop, "stop", device) if n_stop else None, n_stop,
+        _i32(token, N, "token", device), _i32(parent, N, "parent", device),
+        _f32(out_score, N, "out_score", device), end_token, end_parent, end_score,
         _buffer(workspace, "workspace", device), workspace.nbytes, on))
 
 
@@ -681,6 +703,7 @@ class BeamStates:
         for k in row:
             n *= k
         self.ptrs = (C.c_void_p * len(states))(*(_ptr(t) for t in states))
+        self.ref = C.addressof(self.ptrs)
         self.args = (len(states), shape[0] // W, W, slabs, T, n)
 
 
@@ -696,9 +719,9 @@ def beam_reorder(states, parent, length=None, stream=None):
     on = _on_current(device, stream)
     N = states.rows
     _check(lib().neon_beam_reorder(
-        C.addressof(states.ptrs), *states.args,
-        None if length is None else _arg(length, 4, N, "length", device, False),
-        _arg(parent, 4, N, "parent", device, False), on))
+        states.ref, *states.args,
+        None if length is None else _i32(length, N, "length", device),
+        _i32(parent, N, "parent", device), on))
 
 
 def pages_workspace(n_pages, B):
@@ -708,14 +731,17 @@ def pages_workspace(n_pages, B):
     return L.neon_pages_workspace(n_pages, B), L.neon_pages_counters(n_pages)
 
 
-def _pages(refs, table, kv_len, refs_out):
-    """(device, n_pages, rows, max_pages, pointers) of the arrays of a page plan."""
-    if table.dim() != 2 or kv_len.numel() != table.shape[0]:
+def _pages(refs, table, kv_len, refs_out, stream):
+    """(device, stream, n_pages, rows, max_pages, pointers of refs, table, kv_len and
+    refs_out) of a page plan."""
+    device = refs.get_device()
+    shape = table.shape
+    if len(shape) != 2 or kv_len.numel() != shape[0]:
         raise ValueError("table: [B][max_pages], one row per sequence of kv_len")
-    device, n = refs.get_device(), refs.numel()
-    return device, n, *table.shape, (
-        _arg(refs, 4, n, "refs", device, False), _arg(table, 4, 1, "table", device, False),
-        _arg(kv_len, 4, 1, "kv_len", device, False)), _arg(refs_out, 4, n, "refs_out", device, False)
+    n = refs.numel()
+    return (device, _on_current(device, stream), n, shape[0], shape[1],
+            _i32(refs, n, "refs", device), _i32(table, 1, "table", device),
+            _i32(kv_len, 1, "kv_len", device), _i32(refs_out, n, "refs_out", device))
 
 
 def pages_fork(refs, table, kv_len, page_size, refs_out, table_out, len_out, copies, parent=None,
@@ -725,26 +751,27 @@ def pages_fork(refs, table, kv_len, page_size, refs_out, table_out, len_out, cop
     None; table_out int32 [B][max_pages], len_out int32 [B], copies (src, dst, rows)
     int32 [B] each.  counters: zero-filled once by the caller (each call leaves it
     zero)."""
-    device, n, B_in, width, ins, refs_out = _pages(refs, table, kv_len, refs_out)
-    on = _on_current(device, stream)
-    B = table_out.shape[0]
-    if table_out.dim() != 2 or table_out.shape[1] != width:
+    device, on, n, B_in, width, refs, table, kv_len, refs_out = _pages(refs, table, kv_len, refs_out, stream)
+    shape = table_out.shape
+    if len(shape) != 2 or shape[1] != width:
         raise ValueError("table_out: rows of as many entries as table")
+    B = shape[0]
     if workspace is None or counters is None:
         wb, cb = pages_workspace(n, B)
         if workspace is None:
             workspace = _scratch(wb, stream)
         if counters is None:
             counters = _scratch(cb, stream, zero=True)
-
-    def opt(t, name):
-        return None if t is None else _arg(t, 4, B, name, device, False)
-
+    src, dst, rows = copies
     _check(lib().neon_pages_fork(
-        *ins, B_in, opt(parent, "parent"), opt(keep, "keep"), opt(add, "add"), refs_out,
-        _arg(table_out, 4, B * width, "table_out", device, False), opt(len_out, "len_out"),
-        opt(copies[0], "copies[0]"), opt(copies[1], "copies[1]"), opt(copies[2], "copies[2]"), B, n,
-        page_size, width, _buffer(workspace, "workspace", device), workspace.nbytes,
+        refs, table, kv_len, B_in,
+        None if parent is None else _i32(parent, B, "parent", device),
+        None if keep is None else _i32(keep, B, "keep", device),
+        None if add is None else _i32(add, B, "add", device), refs_out,
+        _i32(table_out, B * width, "table_out", device), _i32(len_out, B, "len_out", device),
+        _i32(src, B, "copies[0]", device), _i32(dst, B, "copies[1]", device),
+        _i32(rows, B, "copies[2]", device), B, n, page_size, width,
+        _buffer(workspace, "workspace", device), workspace.nbytes,
         _buffer(counters, "counters", device), counters.nbytes, on))
 
 
@@ -760,6 +787,7 @@ class PagedLayers:
         if any(c.device != first.device for c in self.caches):
             raise ValueError("PagedLayers: caches on one device")
         self.structs = (PagedKVStruct * len(self.caches))(*(c.struct for c in self.caches))
+        self.ref = C.addressof(self.structs)
 
 
 def paged_layers(caches) -> PagedLayers:
@@ -775,24 +803,22 @@ def pages_copy(layers, src, dst, rows=None, stream=None):
     on = _on_current(device, stream)
     n = src.numel()
     _check(lib().neon_pages_copy(
-        C.addressof(layers.structs), len(layers.caches), _arg(src, 4, n, "src", device, False),
-        _arg(dst, 4, n, "dst", device, False),
-        None if rows is None else _arg(rows, 4, n, "rows", device, False), n, on))
+        layers.ref, len(layers.caches), _i32(src, n, "src", device), _i32(dst, n, "dst", device),
+        None if rows is None else _i32(rows, n, "rows", device), n, on))
 
 
 def pages_compact(refs, table, kv_len, page_size, refs_out, table_out, moved_to, copies, stream=None,
                   workspace=None):
     """Moves the used pages of a pool to its lowest ids (neon_pages_compact): moved_to
     int32 [n_pages], copies (src, dst) int32 [n_pages / 2] each, for pages_copy."""
-    device, n, B, width, ins, refs_out = _pages(refs, table, kv_len, refs_out)
-    on = _on_current(device, stream)
+    device, on, n, B, width, refs, table, kv_len, refs_out = _pages(refs, table, kv_len, refs_out, stream)
     if workspace is None:
         workspace = _scratch(pages_workspace(n, B)[0], stream)
+    src, dst = copies
     _check(lib().neon_pages_compact(
-        *ins, refs_out, _arg(table_out, 4, B * width, "table_out", device, False),
-        _arg(moved_to, 4, n, "moved_to", device, False),
-        _arg(copies[0], 4, n // 2, "copies[0]", device, False),
-        _arg(copies[1], 4, n // 2, "copies[1]", device, False), B, n, page_size, width,
+        refs, table, kv_len, refs_out, _i32(table_out, B * width, "table_out", device),
+        _i32(moved_to, n, "moved_to", device), _i32(src, n // 2, "copies[0]", device),
+        _i32(dst, n // 2, "copies[1]", device), B, n, page_size, width,
         _buffer(workspace, "workspace", device), workspace.nbytes, on))
 
 

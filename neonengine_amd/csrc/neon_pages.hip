@@ -312,6 +312,158 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same for small pools in one launch of one block: counts, writers and free pages in
+// LDS, a thread per sequence and eight pages a thread.
+// ---------------------------------------------------------------------------
+constexpr int kPgOneThreads = 1024;
+constexpr int kPgOnePages = 8 * kPgOneThreads;
+constexpr int kPgOneEntries = 65536;  // table entries: B max_pages at most
+
+// exclusive sum over a block of 1024 threads
+__device__ __forceinline__ int pg_scan_one(int v, int* waves, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  const int w = waves[lane & 15];
+  int base = lane < 16 && lane < wave ? w : 0;
+  all = lane < 16 ? w : 0;
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) {
+    base += __shfl_xor(base, d);
+    all += __shfl_xor(all, d);
+  }
+  base = __builtin_amdgcn_readfirstlane(base);
+  all = __builtin_amdgcn_readfirstlane(all);
+  return base + x - v;
+}
+// eight counts of a thread
+__device__ __forceinline__ void pg_load8(const int32_t* refs, int n_pages, int p0, int past, int (&r)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = p0 + j < n_pages ? refs[p0 + j] : past;
+}
+
+__global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs a) {
+  __shared__ int change[kPgOnePages], writers[kPgOnePages], first[kPgOnePages];
+  __shared__ uint16_t free_ids[kPgOnePages];
+  __shared__ int s_parent[kPgOneThreads], s_keep[kPgOneThreads], s_goal[kPgOneThreads];
+  __shared__ int s_before[kPgOneThreads], s_copy[kPgOneThreads];
+  __shared__ int waves[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int p0 = 8 * tid, b = tid;
+  int r[8];
+  pg_load8(a.refs, a.n_pages, p0, 1, r);
+  for (int i = tid; i < a.n_pages; i += kPgOneThreads) change[i] = writers[i] = first[i] = 0;
+  PgSeq q{-1, 0, 0};
+  int held = 0;
+  if (b < a.B) {
+    bool ok;
+    q = pg_seq(a, b, ok);
+    if (!ok) flag_dev_err(a.err, kDevErrPagePlan);
+  }
+  if (b < a.B_in) {
+    const int n = a.len[b];
+    if (!pg_len_ok(a, n)) flag_dev_err(a.err, kDevErrPagePlan);
+    held = pg_len_ok(a, n) ? pg_pages(a.page_log2, n) : 0;
+  }
+  const int kept = pg_pages(a.page_log2, q.keep);
+  int page = -1;  // that the sequence goes on writing
+  if (pg_writes(a, q)) page = a.table[(int64_t)q.parent * a.max_pages + kept - 1];
+  if (q.parent >= 0 && pg_writes(a, q) && (unsigned)page >= (unsigned)a.n_pages) {
+    flag_dev_err(a.err, kDevErrPageId);
+    page = -1;
+  }
+  __syncthreads();
+  if (page >= 0) {
+    atomicAdd(&writers[page], 1);
+    atomicMax(&first[page], a.B - b);
+  }
+  // a wave takes its 64 rows one after another, those with something to change
+  auto count = [&](int row, int i0, int i1, int by) {
+    const int32_t* t = a.table + (int64_t)row * a.max_pages;
+    for (int i = i0 + lane; i < i1; i += 64) {
+      const int p = t[i];
+      if ((unsigned)p < (unsigned)a.n_pages) atomicAdd(&change[p], by);
+      else flag_dev_err(a.err, kDevErrPageId);
+    }
+  };
+  s_parent[tid] = q.parent;
+  s_keep[tid] = kept;
+  s_goal[tid] = held;
+  __syncthreads();
+  const int rows = max(a.B, a.B_in);
+  for (int row = wave; row < rows; row += kPgOneThreads / 64) {
+    const int par = s_parent[row], k = s_keep[row], h = s_goal[row];
+    count(row, par == row ? k : 0, h, -1);
+    if (par >= 0 && par != row) count(par, 0, k, 1);
+  }
+  __syncthreads();
+  // free pages in order
+  int n = 0, n_free;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (p0 + j < a.n_pages) r[j] += change[p0 + j];
+    if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
+    n += r[j] == 0;
+  }
+  int at = pg_scan_one(n, waves[0], n_free);
+  const int free_before = at;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (r[j] == 0) free_ids[at++] = (uint16_t)(p0 + j);
+  // needs
+  const int goal = pg_pages(a.page_log2, q.keep + q.add);
+  int copy = -1, taken;
+  if (page >= 0) {
+    const int holders = a.refs[page] + change[page];
+    if (holders > 1 && !(holders == writers[page] && first[page] == a.B - b)) copy = page;
+  }
+  const int before = pg_scan_one(goal - kept + (copy >= 0), waves[1], taken);
+  s_goal[tid] = goal;
+  s_before[tid] = before;
+  s_copy[tid] = copy;
+  __syncthreads();
+  at = free_before;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int p = p0 + j;
+    if (p >= a.n_pages) break;
+    const int k = writers[p];
+    int out = r[j];
+    if (r[j] == 0) out = at++ < taken ? 1 : 0;
+    else if (k > 0 && r[j] > 1) out -= r[j] == k ? k - 1 : k;
+    a.refs_out[p] = out;
+  }
+  if (b < a.B) {
+    a.len_out[b] = q.keep + q.add;
+    a.copy_src[b] = copy;
+    a.copy_rows[b] = copy >= 0 ? q.keep & ((1 << a.page_log2) - 1) : 0;
+    a.copy_dst[b] = copy >= 0 && before < n_free ? free_ids[before] : -1;
+  }
+  for (int row = wave; row < a.B; row += kPgOneThreads / 64) {
+    const int par = s_parent[row], end = s_goal[row], cp = s_copy[row], base = s_before[row];
+    const int old_end = s_keep[row] - (cp >= 0 ? 1 : 0);
+    int32_t* out = a.table_out + (int64_t)row * a.max_pages;
+    const int32_t* t = a.table + (int64_t)max(par, 0) * a.max_pages;
+    for (int i = (t == out ? old_end : 0) + lane; i < end; i += 64) {
+      int id = -1;
+      if (i < old_end) id = t[i];
+      else if (base + i - old_end < n_free) id = free_ids[base + i - old_end];
+      else flag_dev_err(a.err, kDevErrPagesFull);
+      out[i] = id;
+    }
+  }
+}
+
+static bool pages_one(int n_pages, int B, int max_pages) {
+  return n_pages <= kPgOnePages && B <= kPgOneThreads && (int64_t)B * max_pages <= kPgOneEntries;
+}
 size_t pages_counters(int n_pages) { return (size_t)n_pages * 12; }
 static int64_t pages_parts(int max_pages) { return ((int64_t)max_pages + kPgSpan - 1) / kPgSpan; }
 bool pages_fits(int B, int max_pages) {
@@ -320,6 +472,10 @@ bool pages_fits(int B, int max_pages) {
 void launch_pages_fork(const PagesForkArgs& a, hipStream_t st) {
   const int parts = (int)pages_parts(a.max_pages);
   const int rows = a.B > a.B_in ? a.B : a.B_in;
+  if (pages_one(a.n_pages, rows, a.max_pages)) {
+    hipLaunchKernelGGL(k_pages_fork_one, dim3(1), dim3(kPgOneThreads), 0, st, a);
+    return;
+  }
   const int chunks = (a.n_pages + kPgChunk - 1) / kPgChunk, plans = (a.B + kPgSeqs - 1) / kPgSeqs;
   hipLaunchKernelGGL(k_pages_change, dim3((unsigned)(((int64_t)rows * parts + 3) / 4)), dim3(256), 0, st,
                      a, parts);
@@ -468,7 +624,83 @@ __global__ __launch_bounds__(256) void k_pages_map(PagesCompactArgs a, int parts
   }
 }
 
+// The same for small pools, in one launch of one block.
+__global__ __launch_bounds__(kPgOneThreads) void k_pages_compact_one(PagesCompactArgs a) {
+  __shared__ int fate[kPgOnePages];                                   // new id, -1: free
+  __shared__ uint16_t high[kPgOnePages / 2], low[kPgOnePages / 2];    // ids that move, and where to
+  __shared__ int high_ref[kPgOnePages / 2];
+  __shared__ int waves[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, p0 = 8 * tid;
+  int r[8], n = 0, U, below = 0, n_low;
+  pg_load8(a.refs, a.n_pages, p0, 0, r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
+    n += r[j] != 0;
+  }
+  const int first = pg_scan_one(n, waves[0], U);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) below += r[j] != 0 && p0 + j < U;
+  pg_scan_one(below, waves[1], n_low);
+  const int moves = U - n_low;
+  int rank = first;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int p = p0 + j;
+    if (p < a.n_pages) {
+      if (r[j] != 0 && p >= U) {
+        high[rank - n_low] = (uint16_t)p;
+        high_ref[rank - n_low] = r[j];
+      }
+      if (r[j] == 0 && p < U) low[p - rank] = (uint16_t)p;
+    }
+    rank += r[j] != 0;
+  }
+  __syncthreads();
+  rank = first;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int p = p0 + j;
+    if (p < a.n_pages) {
+      const int to = r[j] == 0 ? -1 : p < U ? p : low[rank - n_low];
+      fate[p] = to;
+      a.moved_to[p] = to;
+      a.refs_out[p] = p >= U ? 0 : r[j] != 0 ? r[j] : high_ref[p - rank];
+    }
+    rank += r[j] != 0;
+  }
+  for (int i = tid; i < a.n_pages / 2; i += kPgOneThreads) {
+    a.copy_src[i] = i < moves ? high[i] : -1;
+    a.copy_dst[i] = i < moves ? low[i] : -1;
+  }
+  __syncthreads();
+  for (int b = wave; b < a.B; b += kPgOneThreads / 64) {
+    const int len = a.len[b];
+    if (len < 0 || len > kPgLongest || (int64_t)len > (int64_t)a.max_pages << a.page_log2) {
+      if (lane == 0) flag_dev_err(a.err, kDevErrPagePlan);
+      continue;
+    }
+    const int end = pg_pages(a.page_log2, len);
+    for (int i = lane; i < end; i += 64) {
+      const int64_t at = (int64_t)b * a.max_pages + i;
+      const int p = a.table[at];
+      int to = p;
+      if ((unsigned)p >= (unsigned)a.n_pages) {
+        flag_dev_err(a.err, kDevErrPageId);
+      } else {
+        to = fate[p];
+        if (to < 0) flag_dev_err(a.err, kDevErrPagePlan);
+      }
+      a.table_out[at] = to;
+    }
+  }
+}
+
 void launch_pages_compact(const PagesCompactArgs& a, hipStream_t st) {
+  if (pages_one(a.n_pages, a.B, a.max_pages)) {
+    hipLaunchKernelGGL(k_pages_compact_one, dim3(1), dim3(kPgOneThreads), 0, st, a);
+    return;
+  }
   const int parts = (int)pages_parts(a.max_pages);
   const unsigned chunks = (unsigned)((a.n_pages + kPgChunk - 1) / kPgChunk);
   hipLaunchKernelGGL(k_pages_used, dim3(chunks), dim3(256), 0, st, a);
