@@ -36,8 +36,9 @@ __device__ __forceinline__ int pg_len(const PagesForkArgs& a, int p) {
   const int n = a.len[p];
   return pg_len_ok(a, n) ? n : 0;
 }
-// ok: false where the numbers are none; the sequence is then left without tokens
-__device__ __forceinline__ PgSeq pg_seq(const PagesForkArgs& a, int b, bool& ok) {
+// ok: false where the numbers are none; the sequence is then left without tokens.
+// len: a.len, or a copy of it
+__device__ __forceinline__ PgSeq pg_seq(const PagesForkArgs& a, const int* len, int b, bool& ok) {
   PgSeq q;
   ok = true;
   q.parent = a.parent != nullptr ? a.parent[b] : b;
@@ -45,7 +46,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PagesForkArgs& a, int b, bool& ok)
     ok = false;
     q.parent = -1;
   }
-  const int raw = q.parent >= 0 ? a.len[q.parent] : 0;
+  const int raw = q.parent >= 0 ? len[q.parent] : 0;
   ok &= pg_len_ok(a, raw);
   const int n = pg_len_ok(a, raw) ? raw : 0;
   q.keep = a.keep != nullptr && q.parent >= 0 ? a.keep[b] : n;
@@ -81,7 +82,6 @@ struct PgWork {  // the workspace
   int* before;    // [B] needs of the sequences before it in its block
   int* keep;      // [B] as the plan has them
   int* add;
-  int* parent;
   int* copy;      // [B] page that is copied (-1: none)
   int* free_ids;  // [chunks][kPgChunk]
   int chunks, plans;
@@ -97,7 +97,6 @@ __host__ __device__ inline PgWork pg_work(void* ws, int n_pages, int B) {
   w.before = p; p += B;
   w.keep = p; p += B;
   w.add = p; p += B;
-  w.parent = p; p += B;
   w.copy = p; p += B;
   w.free_ids = p;
   return w;
@@ -109,7 +108,19 @@ __device__ __forceinline__ int* pg_first(const PagesForkArgs& a) {
   return a.counters + 2 * (int64_t)a.n_pages;
 }
 
-// wave (row, part): entries of old row `row` given up, then of new sequence `row` taken up
+// A row gives up page o and its new sequence takes up page p (where they do).  A page of
+// both changes nothing: most of a prompt is shared by the beams of a request.
+__device__ __forceinline__ void pg_change_of(const PagesForkArgs& a, int o, bool gives, int p, bool takes,
+                                             int* change) {
+  const bool bad_o = gives && (unsigned)o >= (unsigned)a.n_pages;
+  const bool bad_p = takes && (unsigned)p >= (unsigned)a.n_pages;
+  if (bad_o | bad_p) flag_dev_err(a.err, kDevErrPageId);
+  const bool same = gives && takes && o == p;
+  if (gives && !bad_o && !same) atomicAdd(change + o, -1);
+  if (takes && !bad_p && !same) atomicAdd(change + p, 1);
+}
+
+// wave (row, part): what old row `row` gives up and new sequence `row` takes up
 __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts) {
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int row = (int)(id / parts), part = (int)(id % parts), lane = threadIdx.x & 63;
@@ -119,59 +130,85 @@ __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts
   PgSeq q{-1, 0, 0};
   if (row < a.B) {
     bool ok;
-    q = pg_seq(a, row, ok);
+    q = pg_seq(a, a.len, row, ok);
     if (!ok && part == 0 && lane == 0) flag_dev_err(a.err, kDevErrPagePlan);
   }
-  const int kept = pg_pages(a.page_log2, q.keep);
+  const int kept = q.parent >= 0 ? pg_pages(a.page_log2, q.keep) : 0;
+  int held = 0;
   if (row < a.B_in) {
-    const int held = pg_pages(a.page_log2, pg_len(a, row));
-    const int from = q.parent == row ? kept : 0;
+    held = pg_pages(a.page_log2, pg_len(a, row));
     if (part == 0 && lane == 0 && !pg_len_ok(a, a.len[row])) flag_dev_err(a.err, kDevErrPagePlan);
-    for (int i = max(i0, from) + lane; i < min(i1, held); i += 64) {
-      const int p = a.table[(int64_t)row * a.max_pages + i];
-      if ((unsigned)p < (unsigned)a.n_pages) atomicAdd(pg_change(a) + p, -1);
-      else flag_dev_err(a.err, kDevErrPageId);
-    }
   }
-  if (q.parent >= 0) {
-    const int32_t* t = a.table + (int64_t)q.parent * a.max_pages;
-    if (q.parent != row)
-      for (int i = i0 + lane; i < min(i1, kept); i += 64) {
-        const int p = t[i];
-        if ((unsigned)p < (unsigned)a.n_pages) atomicAdd(pg_change(a) + p, 1);
-        else flag_dev_err(a.err, kDevErrPageId);
-      }
-    if (pg_writes(a, q) && part == 0 && lane == 0) {
-      const int p = t[kept - 1];
-      if ((unsigned)p < (unsigned)a.n_pages) {
-        atomicAdd(pg_writers(a) + p, 1);
-        atomicMax(pg_first(a) + p, a.B - row);
-      } else {
-        flag_dev_err(a.err, kDevErrPageId);
-      }
+  const int32_t* old = a.table + (int64_t)min(row, a.B_in - 1) * a.max_pages;
+  const int32_t* now = a.table + (int64_t)max(q.parent, 0) * a.max_pages;
+  const int from = q.parent == row ? min(kept, held) : 0;
+  int32_t* out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
+  const bool moves = now != out && kept > 0;  // the kept entries into a table of their own
+  for (int i = i0 + lane; i < min(i1, max(held, kept)); i += 64) {
+    if (i < from && !moves) continue;
+    const int o = i < held && i >= from ? old[i] : -1, p = i < kept ? now[i] : -1;
+    if (moves && i < kept) out[i] = p;
+    if (i >= from) pg_change_of(a, o, i < held, p, i < kept && q.parent != row, pg_change(a));
+  }
+  if (q.parent >= 0 && pg_writes(a, q) && part == 0 && lane == 0) {
+    const int p = now[kept - 1];
+    if ((unsigned)p < (unsigned)a.n_pages) {
+      atomicAdd(pg_writers(a) + p, 1);
+      atomicMax(pg_first(a) + p, a.B - row);
+    } else {
+      flag_dev_err(a.err, kDevErrPageId);
     }
   }
 }
 
-// exclusive sum over the block's 256 threads; all: the total
-__device__ __forceinline__ int pg_block_scan(int v, int* waves, int& all) {
+// sums over the wave's lanes up to and with each
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int pg_add_from(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int pg_wave_scan(int x) {
+  x = pg_add_from<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x = pg_add_from<0x112, 0xF>(x);
+  x = pg_add_from<0x114, 0xF>(x);
+  x = pg_add_from<0x118, 0xF>(x);
+  x = pg_add_from<0x142, 0xA>(x);     // a row's last lane into the next row
+  return pg_add_from<0x143, 0xC>(x);  // lane 31 into the upper half
+}
+// Before every flag j of a thread, how many are set: the order is j, then the thread (so
+// page j blockDim + thread: loads and stores of a j lie side by side).  Gives the number of
+// all.  sums: LDS, 128 of them, not in use before.
+template <int J, int WAVES>
+__device__ __forceinline__ int pg_ranks(const bool (&is)[J], int (&rank)[J], int* sums) {
+  static_assert(J * WAVES <= 128, "two of a lane");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+  for (int j = 0; j < J; ++j) {
+    const uint64_t in = __ballot(is[j]);
+    rank[j] = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+    if (lane == 0) sums[j * WAVES + wave] = __builtin_popcountll(in);
   }
-  if (lane == 63) waves[wave] = x;
   __syncthreads();
-  int base = 0;
-  all = 0;
+  const int a = 2 * lane < J * WAVES ? sums[2 * lane] : 0, b = 2 * lane + 1 < J * WAVES ? sums[2 * lane + 1] : 0;
+  const int to = pg_wave_scan(a + b);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) base += waves[w];
-    all += waves[w];
+  for (int j = 0; j < J; ++j) {
+    const int at = j * WAVES + wave;
+    const int before = __builtin_amdgcn_ds_bpermute(4 * (at >> 1), to - b - ((at & 1) == 0 ? a : 0));
+    rank[j] += before;
   }
-  return base + x - v;
+  return __builtin_amdgcn_readlane(to, 63);
+}
+// exclusive sum over the block of WAVES waves; all: the total.  sums: LDS, WAVES of them
+template <int WAVES>
+__device__ __forceinline__ int pg_block_scan(int v, int* sums, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = pg_wave_scan(v);
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  const int to = pg_wave_scan(lane < WAVES ? sums[lane] : 0);
+  all = __builtin_amdgcn_readlane(to, 63);
+  const int before = __builtin_amdgcn_readlane(to, __builtin_amdgcn_readfirstlane(max(wave - 1, 0)));
+  return (wave > 0 ? before : 0) + x - v;
 }
 
 __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
@@ -180,22 +217,21 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
   int all;
   if ((int)blockIdx.x < w.chunks) {
     // the chunk's free pages, in order
-    const int p0 = blockIdx.x * kPgChunk + 4 * threadIdx.x;
+    __shared__ int sums[16];
     bool is[4];
-    int n = 0;
+    int rank[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = p0 + j;
+      const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       const int r = p < a.n_pages ? a.refs[p] + pg_change(a)[p] : 1;
       if (r < 0) flag_dev_err(a.err, kDevErrPagePlan);
       is[j] = r == 0;
-      n += is[j];
     }
-    int at = pg_block_scan(n, waves, all);
+    all = pg_ranks<4, 4>(is, rank, sums);
     int* ids = w.free_ids + (int64_t)blockIdx.x * kPgChunk;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (is[j]) ids[at++] = p0 + j;
+      if (is[j]) ids[rank[j]] = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
     if (threadIdx.x == 0) w.free_in[blockIdx.x] = all;
     return;
   }
@@ -204,7 +240,7 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
   int need = 0;
   if (b < a.B) {
     bool ok;
-    const PgSeq q = pg_seq(a, b, ok);
+    const PgSeq q = pg_seq(a, a.len, b, ok);
     const int kept = pg_pages(a.page_log2, q.keep);
     need = pg_pages(a.page_log2, q.keep + q.add) - kept;
     int copy = -1;
@@ -222,10 +258,9 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
     w.need[b] = need;
     w.keep[b] = q.keep;
     w.add[b] = q.add;
-    w.parent[b] = q.parent;
     w.copy[b] = copy;
   }
-  const int before = pg_block_scan(need, waves, all);
+  const int before = pg_block_scan<4>(need, waves, all);
   if (b < a.B) w.before[b] = before;
   if (threadIdx.x == 0) w.need_in[plan] = all;
 }
@@ -240,33 +275,36 @@ __device__ __forceinline__ int64_t pg_wave_total(const int* v, int n) {
   return s;
 }
 
-// blocks 0 .. chunks - 1: the counts; then waves (sequence, part of its row)
+// What a page's count becomes: r without the pages that are taken now, `rank` its place
+// among the free ones; k sequences would go on writing it, and all that get a copy leave.
+__device__ __forceinline__ int pg_count(int r, int64_t rank, int64_t taken, int k) {
+  if (r == 0) return rank < taken ? 1 : 0;
+  return k > 0 && r > 1 ? r - (r == k ? k - 1 : k) : r;
+}
+// blocks 0 .. chunks - 1: the counts; then waves (sequence, part of its row): the new
+// entries
 __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts) {
   const PgWork w = pg_work(a.workspace, a.n_pages, a.B);
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < w.chunks) {
-    __shared__ int waves[4];
+    __shared__ int sums[16];
     const int64_t taken = pg_wave_total(w.need_in, w.plans);
-    const int64_t free_before = pg_wave_total(w.free_in, blockIdx.x);
-    const int p0 = blockIdx.x * kPgChunk + 4 * threadIdx.x;
-    int r[4], n = 0;
+    const int64_t before = pg_wave_total(w.free_in, blockIdx.x);
+    int r[4], k[4], rank[4];
+    bool is[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = p0 + j;
+      const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       r[j] = p < a.n_pages ? a.refs[p] + pg_change(a)[p] : 1;
-      n += r[j] == 0;
+      k[j] = p < a.n_pages ? pg_writers(a)[p] : 0;
+      is[j] = r[j] == 0;
     }
-    int all;
-    int64_t at = free_before + pg_block_scan(n, waves, all);
+    pg_ranks<4, 4>(is, rank, sums);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = p0 + j;
+      const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       if (p >= a.n_pages) break;
-      const int k = pg_writers(a)[p];
-      int out = r[j];
-      if (r[j] == 0) out = at++ < taken ? 1 : 0;
-      else if (k > 0 && r[j] > 1) out -= r[j] == k ? k - 1 : k;  // those that get a copy
-      a.refs_out[p] = out;
+      a.refs_out[p] = pg_count(r[j], before + rank[j], taken, k[j]);
       pg_change(a)[p] = 0;
       pg_writers(a)[p] = 0;
       pg_first(a)[p] = 0;
@@ -276,17 +314,11 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
   const int64_t id = ((int64_t)blockIdx.x - w.chunks) * 4 + (threadIdx.x >> 6);
   const int b = (int)(id / parts), part = (int)(id % parts);
   if (b >= a.B) return;
-  const int keep = w.keep[b], add = w.add[b], parent = w.parent[b], copy = w.copy[b];
+  const int keep = w.keep[b], add = w.add[b], copy = w.copy[b];
   const int goal = pg_pages(a.page_log2, keep + add);
   const int old_end = pg_pages(a.page_log2, keep) - (copy >= 0 ? 1 : 0);
   int32_t* out = a.table_out + (int64_t)b * a.max_pages;
   const int i0 = part * kPgSpan, i1 = min(i0 + kPgSpan, goal);
-  if (i0 < old_end && parent >= 0) {
-    const int32_t* t = a.table + (int64_t)parent * a.max_pages;
-    if (t != out)
-      for (int i = i0 + lane; i < min(i1, old_end); i += 64) out[i] = t[i];
-  }
-  // (a sequence without an entry of its own in this part is done)
   if (part == 0 && lane == 0) {
     a.len_out[b] = keep + add;
     a.copy_src[b] = copy;
@@ -296,19 +328,33 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
   if (i1 <= old_end || i0 >= goal) return;
   const int64_t first = pg_wave_total(w.need_in, b / kPgSeqs) + w.before[b];
   const int64_t n_free = pg_wave_total(w.free_in, w.chunks);
-  for (int i = max(i0, old_end) + lane; i < i1; i += 64) {
+  for (int ib = max(i0, old_end); ib < i1; ib += 64) {
+    const int i = ib + lane;
     const int64_t j = first + i - old_end;
+    // the chunk that holds the j-th free page, chunks 64 at a time
     int id2 = -1;
-    if (j < n_free) {
-      int64_t rest = j;
-      int c = 0;
-      while (rest >= w.free_in[c]) rest -= w.free_in[c++];
-      id2 = w.free_ids[(int64_t)c * kPgChunk + rest];
-    } else {
-      flag_dev_err(a.err, kDevErrPagesFull);
+    const bool mine = i < i1 && j < n_free;
+    int64_t from = 0;
+    for (int c0 = 0; c0 < w.chunks && __any(mine && j >= from); c0 += 64) {
+      const int in = c0 + lane < w.chunks ? w.free_in[c0 + lane] : 0;
+      const int to = pg_wave_scan(in), all = __builtin_amdgcn_readlane(to, 63);
+      const bool now = mine && j >= from && j < from + all;
+      const int want = now ? (int)(j - from) : 0;
+      int c = 0;  // the first of the 64 sums above it
+#pragma unroll
+      for (int step = 32; step > 0; step >>= 1) {
+        const int upto = __builtin_amdgcn_ds_bpermute(4 * (c + step - 1), to);
+        c += upto <= want ? step : 0;
+      }
+      const int before = __builtin_amdgcn_ds_bpermute(4 * c, to - in);
+      if (now) id2 = w.free_ids[(int64_t)(c0 + c) * kPgChunk + want - before];
+      from += all;
     }
-    out[i] = id2;
-    if (copy >= 0 && i == old_end) a.copy_dst[b] = id2;
+    if (i < i1) {
+      if (!mine) flag_dev_err(a.err, kDevErrPagesFull);
+      out[i] = id2;
+      if (copy >= 0 && i == old_end) a.copy_dst[b] = id2;
+    }
   }
 }
 
@@ -320,125 +366,104 @@ constexpr int kPgOneThreads = 1024;
 constexpr int kPgOnePages = 8 * kPgOneThreads;
 constexpr int kPgOneEntries = 65536;  // table entries: B max_pages at most
 
-// exclusive sum over a block of 1024 threads
-__device__ __forceinline__ int pg_scan_one(int v, int* waves, int& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) waves[wave] = x;
-  __syncthreads();
-  const int w = waves[lane & 15];
-  int base = lane < 16 && lane < wave ? w : 0;
-  all = lane < 16 ? w : 0;
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) {
-    base += __shfl_xor(base, d);
-    all += __shfl_xor(all, d);
-  }
-  base = __builtin_amdgcn_readfirstlane(base);
-  all = __builtin_amdgcn_readfirstlane(all);
-  return base + x - v;
-}
-// eight counts of a thread
-__device__ __forceinline__ void pg_load8(const int32_t* refs, int n_pages, int p0, int past, int (&r)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = p0 + j < n_pages ? refs[p0 + j] : past;
-}
-
 __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs a) {
   __shared__ int change[kPgOnePages], writers[kPgOnePages], first[kPgOnePages];
   __shared__ uint16_t free_ids[kPgOnePages];
-  __shared__ int s_parent[kPgOneThreads], s_keep[kPgOneThreads], s_goal[kPgOneThreads];
-  __shared__ int s_before[kPgOneThreads], s_copy[kPgOneThreads];
-  __shared__ int waves[2][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int p0 = 8 * tid, b = tid;
+  __shared__ int s_parent[kPgOneThreads], s_kept[kPgOneThreads], s_held[kPgOneThreads];
+  __shared__ int s_goal[kPgOneThreads], s_before[kPgOneThreads];
+  __shared__ int sums[2][128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int b = tid;
   int r[8];
-  pg_load8(a.refs, a.n_pages, p0, 1, r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = 1024 * j + tid < a.n_pages ? a.refs[1024 * j + tid] : 1;
+  const int len = b < a.B_in ? a.len[b] : 0;
+  s_held[tid] = len;
   for (int i = tid; i < a.n_pages; i += kPgOneThreads) change[i] = writers[i] = first[i] = 0;
+  __syncthreads();
   PgSeq q{-1, 0, 0};
-  int held = 0;
   if (b < a.B) {
     bool ok;
-    q = pg_seq(a, b, ok);
+    q = pg_seq(a, s_held, b, ok);
     if (!ok) flag_dev_err(a.err, kDevErrPagePlan);
   }
-  if (b < a.B_in) {
-    const int n = a.len[b];
-    if (!pg_len_ok(a, n)) flag_dev_err(a.err, kDevErrPagePlan);
-    held = pg_len_ok(a, n) ? pg_pages(a.page_log2, n) : 0;
-  }
-  const int kept = pg_pages(a.page_log2, q.keep);
-  int page = -1;  // that the sequence goes on writing
-  if (pg_writes(a, q)) page = a.table[(int64_t)q.parent * a.max_pages + kept - 1];
-  if (q.parent >= 0 && pg_writes(a, q) && (unsigned)page >= (unsigned)a.n_pages) {
+  if (!pg_len_ok(a, len)) flag_dev_err(a.err, kDevErrPagePlan);
+  const int kept = q.parent >= 0 ? pg_pages(a.page_log2, q.keep) : 0;
+  const bool writes = q.parent >= 0 && pg_writes(a, q);
+  int page = writes ? a.table[(int64_t)q.parent * a.max_pages + kept - 1] : -1;
+  __syncthreads();  // (lengths are read)
+  s_parent[tid] = q.parent;
+  s_kept[tid] = kept;
+  s_held[tid] = pg_len_ok(a, len) ? pg_pages(a.page_log2, len) : 0;
+  if (writes && (unsigned)page >= (unsigned)a.n_pages) {
     flag_dev_err(a.err, kDevErrPageId);
     page = -1;
   }
-  __syncthreads();
   if (page >= 0) {
     atomicAdd(&writers[page], 1);
     atomicMax(&first[page], a.B - b);
   }
-  // a wave takes its 64 rows one after another, those with something to change
-  auto count = [&](int row, int i0, int i1, int by) {
-    const int32_t* t = a.table + (int64_t)row * a.max_pages;
-    for (int i = i0 + lane; i < i1; i += 64) {
-      const int p = t[i];
-      if ((unsigned)p < (unsigned)a.n_pages) atomicAdd(&change[p], by);
-      else flag_dev_err(a.err, kDevErrPageId);
-    }
-  };
-  s_parent[tid] = q.parent;
-  s_keep[tid] = kept;
-  s_goal[tid] = held;
+  const int page_refs = page >= 0 ? a.refs[page] : 0;
   __syncthreads();
+  // a wave takes a row at a time: its changes, and the kept entries into the new table
   const int rows = max(a.B, a.B_in);
   for (int row = wave; row < rows; row += kPgOneThreads / 64) {
-    const int par = s_parent[row], k = s_keep[row], h = s_goal[row];
-    count(row, par == row ? k : 0, h, -1);
-    if (par >= 0 && par != row) count(par, 0, k, 1);
+    const int par = __builtin_amdgcn_readfirstlane(s_parent[row]);
+    const int k = __builtin_amdgcn_readfirstlane(s_kept[row]);
+    const int held = __builtin_amdgcn_readfirstlane(s_held[row]);
+    const int32_t* old = a.table + (int64_t)min(row, a.B_in - 1) * a.max_pages;
+    const int32_t* now = a.table + (int64_t)max(par, 0) * a.max_pages;
+    int32_t* out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
+    const int from = par == row ? min(k, held) : 0;
+    const bool moves = now != out && k > 0;
+    for (int i0 = moves ? 0 : from; i0 < max(held, k); i0 += 256) {
+      int o[4], p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u + lane;
+        o[u] = i < held && i >= from ? old[i] : -1;
+        p[u] = i < k ? now[i] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u + lane;
+        if (moves && i < k) out[i] = p[u];
+        if (i >= from) pg_change_of(a, o[u], i < held, p[u], i < k && par != row, change);
+      }
+    }
   }
   __syncthreads();
   // free pages in order
-  int n = 0, n_free;
+  bool is[8];
+  int rank[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    if (p0 + j < a.n_pages) r[j] += change[p0 + j];
+    const int p = 1024 * j + tid;
+    if (p < a.n_pages) r[j] += change[p];
     if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
-    n += r[j] == 0;
+    is[j] = r[j] == 0;
   }
-  int at = pg_scan_one(n, waves[0], n_free);
-  const int free_before = at;
+  const int n_free = pg_ranks<8, 16>(is, rank, sums[0]);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (r[j] == 0) free_ids[at++] = (uint16_t)(p0 + j);
+    if (is[j]) free_ids[rank[j]] = (uint16_t)(1024 * j + tid);
   // needs
   const int goal = pg_pages(a.page_log2, q.keep + q.add);
   int copy = -1, taken;
   if (page >= 0) {
-    const int holders = a.refs[page] + change[page];
+    const int holders = page_refs + change[page];
     if (holders > 1 && !(holders == writers[page] && first[page] == a.B - b)) copy = page;
   }
-  const int before = pg_scan_one(goal - kept + (copy >= 0), waves[1], taken);
+  const int old_end = kept - (copy >= 0 ? 1 : 0);
+  const int before = pg_block_scan<16>(goal - old_end, sums[1], taken);
   s_goal[tid] = goal;
   s_before[tid] = before;
-  s_copy[tid] = copy;
+  s_kept[tid] = old_end;
   __syncthreads();
-  at = free_before;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int p = p0 + j;
-    if (p >= a.n_pages) break;
-    const int k = writers[p];
-    int out = r[j];
-    if (r[j] == 0) out = at++ < taken ? 1 : 0;
-    else if (k > 0 && r[j] > 1) out -= r[j] == k ? k - 1 : k;
-    a.refs_out[p] = out;
+    const int p = 1024 * j + tid;
+    if (p < a.n_pages) a.refs_out[p] = pg_count(r[j], rank[j], taken, writers[p]);
   }
   if (b < a.B) {
     a.len_out[b] = q.keep + q.add;
@@ -446,17 +471,27 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
     a.copy_rows[b] = copy >= 0 ? q.keep & ((1 << a.page_log2) - 1) : 0;
     a.copy_dst[b] = copy >= 0 && before < n_free ? free_ids[before] : -1;
   }
-  for (int row = wave; row < a.B; row += kPgOneThreads / 64) {
-    const int par = s_parent[row], end = s_goal[row], cp = s_copy[row], base = s_before[row];
-    const int old_end = s_keep[row] - (cp >= 0 ? 1 : 0);
-    int32_t* out = a.table_out + (int64_t)row * a.max_pages;
-    const int32_t* t = a.table + (int64_t)max(par, 0) * a.max_pages;
-    for (int i = (t == out ? old_end : 0) + lane; i < end; i += 64) {
+  // the new entries: a wave's rows side by side while they are few
+  for (int row0 = 64 * wave; row0 < a.B; row0 += kPgOneThreads) {
+    const int row = row0 + lane, end = row < a.B ? s_goal[row] : 0, at = row < a.B ? s_kept[row] : 0;
+    const int base = row < a.B ? s_before[row] : 0;
+    uint64_t some = __ballot(end > at);
+    const bool few = __ballot(end - at > 4) == 0;
+    auto put = [&](int64_t r64, int i, int j) {
       int id = -1;
-      if (i < old_end) id = t[i];
-      else if (base + i - old_end < n_free) id = free_ids[base + i - old_end];
+      if (j < n_free) id = free_ids[j];
       else flag_dev_err(a.err, kDevErrPagesFull);
-      out[i] = id;
+      a.table_out[r64 * a.max_pages + i] = id;
+    };
+    if (few) {
+      for (int i = at; i < end; ++i) put(row, i, base + i - at);
+      continue;
+    }
+    for (; some != 0; some &= some - 1) {
+      const int l = __builtin_ctzll(some);
+      const int e = __builtin_amdgcn_readlane(end, l), f = __builtin_amdgcn_readlane(at, l);
+      const int bs = __builtin_amdgcn_readlane(base, l);
+      for (int i = f + lane; i < e; i += 64) put(row0 + l, i, bs + i - f);
     }
   }
 }
@@ -512,70 +547,70 @@ static size_t pc_bytes(int n_pages) {
   return 4 * (2 + ((size_t)n_pages + kPgChunk - 1) / kPgChunk + (size_t)n_pages / 2 + (size_t)n_pages);
 }
 
-// the thread's four pages' counts (0 past the end)
-__device__ __forceinline__ int pc_load(const int32_t* refs, int n_pages, int p0, int (&r)[4]) {
-  int n = 0;
+// the thread's four counts of a chunk (0 past the end), and which are of used pages
+__device__ __forceinline__ void pc_load(const int32_t* refs, int n_pages, int chunk, int (&r)[4],
+                                        bool (&is)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    r[j] = p0 + j < n_pages ? refs[p0 + j] : 0;
-    n += r[j] != 0;
+    const int p = chunk * kPgChunk + 256 * j + threadIdx.x;
+    r[j] = p < n_pages ? refs[p] : 0;
+    is[j] = r[j] != 0;
   }
-  return n;
 }
 
 __global__ __launch_bounds__(256) void k_pages_used(PagesCompactArgs a) {
-  __shared__ int waves[4];
+  __shared__ int sums[16];
   const PcWork w = pc_work(a.workspace, a.n_pages);
-  int r[4], all;
-  const int n = pc_load(a.refs, a.n_pages, blockIdx.x * kPgChunk + 4 * threadIdx.x, r);
+  int r[4], rank[4];
+  bool is[4];
+  pc_load(a.refs, a.n_pages, blockIdx.x, r, is);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
-  pg_block_scan(n, waves, all);
+  const int all = pg_ranks<4, 4>(is, rank, sums);
   if (threadIdx.x == 0) w.used_in[blockIdx.x] = all;
 }
 
 __global__ __launch_bounds__(256) void k_pages_lists(PagesCompactArgs a) {
-  __shared__ int waves[4], waves2[4];
+  __shared__ int sums[16], sums2[16];
   const PcWork w = pc_work(a.workspace, a.n_pages);
-  const int64_t before = pg_wave_total(w.used_in, blockIdx.x);
+  int r[4], u[4], rank[4], rank2[4];
+  bool is[4], low_is[4];
+  pc_load(a.refs, a.n_pages, blockIdx.x, r, is);
+  const int before = (int)pg_wave_total(w.used_in, blockIdx.x);
   const int U = (int)pg_wave_total(w.used_in, w.chunks);
-  const int p0 = blockIdx.x * kPgChunk + 4 * threadIdx.x;
-  int r[4], u[4], all;
-  const int n = pc_load(a.refs, a.n_pages, p0, r);
-  int rank = (int)before + pg_block_scan(n, waves, all);  // used pages before p0
   // used pages below U: whole chunks, and those of U's own
-  const int cu = U / kPgChunk, q0 = cu * kPgChunk + 4 * threadIdx.x;
-  pc_load(a.refs, a.n_pages, q0, u);
-  int mine = 0;
+  const int cu = U / kPgChunk;
+  pc_load(a.refs, a.n_pages, cu, u, low_is);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) mine += u[j] != 0 && q0 + j < U;
-  pg_block_scan(mine, waves2, all);
-  const int low = (int)pg_wave_total(w.used_in, cu) + all, moves = U - low;
+  for (int j = 0; j < 4; ++j) low_is[j] &= cu * kPgChunk + 256 * j + (int)threadIdx.x < U;
+  pg_ranks<4, 4>(is, rank, sums);
+  const int low = (int)pg_wave_total(w.used_in, cu) + pg_ranks<4, 4>(low_is, rank2, sums2);
+  const int moves = U - low;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     w.sums[0] = U;
     w.sums[1] = low;
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int p = p0 + j;
+    const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
     if (p >= a.n_pages) break;
+    const int at = before + rank[j];  // used pages before it
     int fate = kPcFree;
-    if (r[j] != 0) {
-      fate = p < U ? kPcStays : rank - low;
+    if (is[j]) {
+      fate = p < U ? kPcStays : at - low;
       if (p >= U) {
         a.copy_src[fate] = p;
         w.high_ref[fate] = r[j];
       }
     } else if (p < U) {
-      a.copy_dst[p - rank] = p;  // p - rank free pages before it
+      a.copy_dst[p - at] = p;  // as many free pages before it
     }
     w.fate[p] = fate;
     if (p >= moves && p < a.n_pages / 2) {
       a.copy_src[p] = -1;
       a.copy_dst[p] = -1;
     }
-    rank += r[j] != 0;
   }
 }
 
@@ -583,20 +618,20 @@ __global__ __launch_bounds__(256) void k_pages_lists(PagesCompactArgs a) {
 __global__ __launch_bounds__(256) void k_pages_map(PagesCompactArgs a, int parts) {
   const PcWork w = pc_work(a.workspace, a.n_pages);
   if ((int)blockIdx.x < w.chunks) {
-    __shared__ int waves[4];
+    __shared__ int sums[16];
+    int r[4], rank[4];
+    bool is[4];
+    pc_load(a.refs, a.n_pages, blockIdx.x, r, is);
     const int U = w.sums[0];
-    const int p0 = blockIdx.x * kPgChunk + 4 * threadIdx.x;
-    int r[4], all;
-    const int n = pc_load(a.refs, a.n_pages, p0, r);
-    int rank = (int)pg_wave_total(w.used_in, blockIdx.x) + pg_block_scan(n, waves, all);
+    const int before = (int)pg_wave_total(w.used_in, blockIdx.x);
+    pg_ranks<4, 4>(is, rank, sums);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = p0 + j;
+      const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       if (p >= a.n_pages) break;
       const int f = w.fate[p];
       a.moved_to[p] = f == kPcFree ? -1 : f == kPcStays ? p : a.copy_dst[f];
-      a.refs_out[p] = p >= U ? 0 : r[j] != 0 ? r[j] : w.high_ref[p - rank];
-      rank += r[j] != 0;
+      a.refs_out[p] = p >= U ? 0 : is[j] ? r[j] : w.high_ref[p - before - rank[j]];
     }
     return;
   }
@@ -626,72 +661,75 @@ __global__ __launch_bounds__(256) void k_pages_map(PagesCompactArgs a, int parts
 
 // The same for small pools, in one launch of one block.
 __global__ __launch_bounds__(kPgOneThreads) void k_pages_compact_one(PagesCompactArgs a) {
-  __shared__ int fate[kPgOnePages];                                   // new id, -1: free
-  __shared__ uint16_t high[kPgOnePages / 2], low[kPgOnePages / 2];    // ids that move, and where to
+  __shared__ int fate[kPgOnePages];                                 // new id, -1: free
+  __shared__ uint16_t high[kPgOnePages / 2], low[kPgOnePages / 2];  // ids that move, and where to
   __shared__ int high_ref[kPgOnePages / 2];
-  __shared__ int waves[2][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, p0 = 8 * tid;
-  int r[8], n = 0, U, below = 0, n_low;
-  pg_load8(a.refs, a.n_pages, p0, 0, r);
+  __shared__ int held[kPgOneThreads];
+  __shared__ int sums[2][128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int r[8], rank[8];
+  bool is[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = 1024 * j + tid < a.n_pages ? a.refs[1024 * j + tid] : 0;
+  const int len = tid < a.B ? a.len[tid] : 0;
+  const bool fits = len >= 0 && len <= kPgLongest && (int64_t)len <= (int64_t)a.max_pages << a.page_log2;
+  if (!fits) flag_dev_err(a.err, kDevErrPagePlan);
+  held[tid] = fits ? pg_pages(a.page_log2, len) : 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
-    n += r[j] != 0;
+    is[j] = r[j] != 0;
   }
-  const int first = pg_scan_one(n, waves[0], U);
+  const int U = pg_ranks<8, 16>(is, rank, sums[0]);
+  int below = 0, n_low;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) below += r[j] != 0 && p0 + j < U;
-  pg_scan_one(below, waves[1], n_low);
+  for (int j = 0; j < 8; ++j) below += is[j] && 1024 * j + tid < U;
+  pg_block_scan<16>(below, sums[1], n_low);
   const int moves = U - n_low;
-  int rank = first;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int p = p0 + j;
-    if (p < a.n_pages) {
-      if (r[j] != 0 && p >= U) {
-        high[rank - n_low] = (uint16_t)p;
-        high_ref[rank - n_low] = r[j];
-      }
-      if (r[j] == 0 && p < U) low[p - rank] = (uint16_t)p;
+    const int p = 1024 * j + tid;
+    if (p >= a.n_pages) break;
+    if (is[j] && p >= U) {
+      high[rank[j] - n_low] = (uint16_t)p;
+      high_ref[rank[j] - n_low] = r[j];
     }
-    rank += r[j] != 0;
+    if (!is[j] && p < U) low[p - rank[j]] = (uint16_t)p;
   }
   __syncthreads();
-  rank = first;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int p = p0 + j;
-    if (p < a.n_pages) {
-      const int to = r[j] == 0 ? -1 : p < U ? p : low[rank - n_low];
-      fate[p] = to;
-      a.moved_to[p] = to;
-      a.refs_out[p] = p >= U ? 0 : r[j] != 0 ? r[j] : high_ref[p - rank];
-    }
-    rank += r[j] != 0;
+    const int p = 1024 * j + tid;
+    if (p >= a.n_pages) break;
+    const int to = !is[j] ? -1 : p < U ? p : low[rank[j] - n_low];
+    fate[p] = to;
+    a.moved_to[p] = to;
+    a.refs_out[p] = p >= U ? 0 : is[j] ? r[j] : high_ref[p - rank[j]];
   }
   for (int i = tid; i < a.n_pages / 2; i += kPgOneThreads) {
     a.copy_src[i] = i < moves ? high[i] : -1;
     a.copy_dst[i] = i < moves ? low[i] : -1;
   }
   __syncthreads();
-  for (int b = wave; b < a.B; b += kPgOneThreads / 64) {
-    const int len = a.len[b];
-    if (len < 0 || len > kPgLongest || (int64_t)len > (int64_t)a.max_pages << a.page_log2) {
-      if (lane == 0) flag_dev_err(a.err, kDevErrPagePlan);
-      continue;
-    }
-    const int end = pg_pages(a.page_log2, len);
-    for (int i = lane; i < end; i += 64) {
-      const int64_t at = (int64_t)b * a.max_pages + i;
-      const int p = a.table[at];
-      int to = p;
-      if ((unsigned)p >= (unsigned)a.n_pages) {
-        flag_dev_err(a.err, kDevErrPageId);
-      } else {
-        to = fate[p];
-        if (to < 0) flag_dev_err(a.err, kDevErrPagePlan);
+  for (int row = wave; row < a.B; row += kPgOneThreads / 64) {
+    const int64_t at = (int64_t)row * a.max_pages;
+    const int end = __builtin_amdgcn_readfirstlane(held[row]);
+    for (int i0 = 0; i0 < end; i0 += 256) {
+      int p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[u] = i0 + 64 * u + lane < end ? a.table[at + i0 + 64 * u + lane] : 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i0 + 64 * u + lane >= end) break;
+        int to = p[u];
+        if ((unsigned)to >= (unsigned)a.n_pages) {
+          flag_dev_err(a.err, kDevErrPageId);
+        } else {
+          to = fate[to];
+          if (to < 0) flag_dev_err(a.err, kDevErrPagePlan);
+        }
+        a.table_out[at + i0 + 64 * u + lane] = to;
       }
-      a.table_out[at] = to;
     }
   }
 }
@@ -712,7 +750,7 @@ void launch_pages_compact(const PagesCompactArgs& a, hipStream_t st) {
 size_t pages_workspace(int n_pages, int B) {
   const size_t chunks = ((size_t)n_pages + kPgChunk - 1) / kPgChunk;
   const size_t plans = ((size_t)B + kPgSeqs - 1) / kPgSeqs;
-  const size_t fork = 4 * (chunks + plans + 6 * (size_t)B + chunks * kPgChunk);
+  const size_t fork = 4 * (chunks + plans + 5 * (size_t)B + chunks * kPgChunk);
   return fork > pc_bytes(n_pages) ? fork : pc_bytes(n_pages);
 }
 
