@@ -36,28 +36,31 @@ __device__ __forceinline__ int pg_len(const PagesForkArgs& a, int p) {
   const int n = a.len[p];
   return pg_len_ok(a, n) ? n : 0;
 }
+// Sequence b with its parent's tokens and what keep and add say (where they are given).
 // ok: false where the numbers are none; the sequence is then left without tokens.
-// len: a.len, or a copy of it
-__device__ __forceinline__ PgSeq pg_seq(const PagesForkArgs& a, const int* len, int b, bool& ok) {
+__device__ __forceinline__ int pg_parent(const PagesForkArgs& a, int b) {
+  return a.parent != nullptr ? a.parent[b] : b;
+}
+__device__ __forceinline__ PgSeq pg_seq_of(const PagesForkArgs& a, int parent, int len, int keep, int add,
+                                           bool& ok) {
   PgSeq q;
-  ok = true;
-  q.parent = a.parent != nullptr ? a.parent[b] : b;
-  if (q.parent < -1 || q.parent >= a.B_in) {
-    ok = false;
-    q.parent = -1;
-  }
-  const int raw = q.parent >= 0 ? len[q.parent] : 0;
-  ok &= pg_len_ok(a, raw);
-  const int n = pg_len_ok(a, raw) ? raw : 0;
-  q.keep = a.keep != nullptr && q.parent >= 0 ? a.keep[b] : n;
-  q.add = a.add != nullptr ? a.add[b] : n > 0 ? 1 : 0;
-  ok &= q.keep >= 0 && q.keep <= n && q.add >= 0 && q.add <= kPgLongest &&
-        pg_len_ok(a, (int)min((int64_t)q.keep + q.add, (int64_t)kPgLongest + 1));
+  const int n = pg_len_ok(a, len) ? len : 0;
+  q.parent = parent;
+  q.keep = a.keep != nullptr && parent >= 0 ? keep : n;
+  q.add = a.add != nullptr ? add : n > 0 ? 1 : 0;
+  ok = parent >= -1 && parent < a.B_in && pg_len_ok(a, len) && q.keep >= 0 && q.keep <= n && q.add >= 0 &&
+       q.add <= kPgLongest && pg_len_ok(a, (int)min((int64_t)q.keep + q.add, (int64_t)kPgLongest + 1));
   if (!ok) {
     q.parent = -1;
     q.keep = q.add = 0;
   }
   return q;
+}
+__device__ __forceinline__ PgSeq pg_seq(const PagesForkArgs& a, int b, bool& ok) {
+  const int parent = pg_parent(a, b), keep = a.keep != nullptr ? a.keep[b] : 0;
+  const int add = a.add != nullptr ? a.add[b] : 0;
+  const int len = parent >= 0 && parent < a.B_in ? a.len[parent] : 0;
+  return pg_seq_of(a, parent, len, keep, add, ok);
 }
 // Whether the sequence goes on writing a page that holds tokens already.
 __device__ __forceinline__ bool pg_writes(const PagesForkArgs& a, const PgSeq& q) {
@@ -109,15 +112,15 @@ __device__ __forceinline__ int* pg_first(const PagesForkArgs& a) {
 }
 
 // A row gives up page o and its new sequence takes up page p (where they do).  A page of
-// both changes nothing: most of a prompt is shared by the beams of a request.
+// both changes nothing: most of a prompt is shared by the beams of a request.  bad: an id
+// that is none.
 __device__ __forceinline__ void pg_change_of(const PagesForkArgs& a, int o, bool gives, int p, bool takes,
-                                             int* change) {
-  const bool bad_o = gives && (unsigned)o >= (unsigned)a.n_pages;
-  const bool bad_p = takes && (unsigned)p >= (unsigned)a.n_pages;
-  if (bad_o | bad_p) flag_dev_err(a.err, kDevErrPageId);
-  const bool same = gives && takes && o == p;
-  if (gives && !bad_o && !same) atomicAdd(change + o, -1);
-  if (takes && !bad_p && !same) atomicAdd(change + p, 1);
+                                             int* change, bool& bad) {
+  const bool is_o = (unsigned)o < (unsigned)a.n_pages, is_p = (unsigned)p < (unsigned)a.n_pages;
+  bad |= (gives & !is_o) | (takes & !is_p);
+  const bool same = gives & takes & (o == p);
+  if (gives & is_o & !same) atomicAdd(change + o, -1);
+  if (takes & is_p & !same) atomicAdd(change + p, 1);
 }
 
 // wave (row, part): what old row `row` gives up and new sequence `row` takes up
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts
   PgSeq q{-1, 0, 0};
   if (row < a.B) {
     bool ok;
-    q = pg_seq(a, a.len, row, ok);
+    q = pg_seq(a, row, ok);
     if (!ok && part == 0 && lane == 0) flag_dev_err(a.err, kDevErrPagePlan);
   }
   const int kept = q.parent >= 0 ? pg_pages(a.page_log2, q.keep) : 0;
@@ -144,11 +147,31 @@ __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts
   const int from = q.parent == row ? min(kept, held) : 0;
   int32_t* out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
   const bool moves = now != out && kept > 0;  // the kept entries into a table of their own
-  for (int i = i0 + lane; i < min(i1, max(held, kept)); i += 64) {
-    if (i < from && !moves) continue;
-    const int o = i < held && i >= from ? old[i] : -1, p = i < kept ? now[i] : -1;
-    if (moves && i < kept) out[i] = p;
-    if (i >= from) pg_change_of(a, o, i < held, p, i < kept && q.parent != row, pg_change(a));
+  const int end = min(i1, max(held, kept));
+  if (end > (moves ? i0 : max(i0, from))) {
+    // (inside the row whatever i is: a load under a condition of its own is waited for)
+    int o[kPgSpan / 64], p[kPgSpan / 64];
+#pragma unroll
+    for (int u = 0; u < kPgSpan / 64; ++u) {
+      const int i = min(i0 + 64 * u + lane, a.max_pages - 1);
+      o[u] = old[i];
+      p[u] = now[i];
+    }
+    if (moves) {
+#pragma unroll
+      for (int u = 0; u < kPgSpan / 64; ++u)
+        if (i0 + 64 * u + lane < min(end, kept)) out[i0 + 64 * u + lane] = p[u];
+    }
+    if (from < end) {
+      bool bad = false;
+#pragma unroll
+      for (int u = 0; u < kPgSpan / 64; ++u) {
+        const int i = i0 + 64 * u + lane;
+        pg_change_of(a, o[u], (i >= from) & (i < min(end, held)), p[u],
+                     (i < min(end, kept)) & (q.parent != row), pg_change(a), bad);
+      }
+      if (bad) flag_dev_err(a.err, kDevErrPageId);
+    }
   }
   if (q.parent >= 0 && pg_writes(a, q) && part == 0 && lane == 0) {
     const int p = now[kept - 1];
@@ -240,7 +263,7 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
   int need = 0;
   if (b < a.B) {
     bool ok;
-    const PgSeq q = pg_seq(a, a.len, b, ok);
+    const PgSeq q = pg_seq(a, b, ok);
     const int kept = pg_pages(a.page_log2, q.keep);
     need = pg_pages(a.page_log2, q.keep + q.add) - kept;
     int copy = -1;
@@ -367,70 +390,111 @@ constexpr int kPgOnePages = 8 * kPgOneThreads;
 constexpr int kPgOneEntries = 65536;  // table entries: B max_pages at most
 
 __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs a) {
-  __shared__ int change[kPgOnePages], writers[kPgOnePages], first[kPgOnePages];
+  __shared__ int count[kPgOnePages], writers[kPgOnePages], first[kPgOnePages];
   __shared__ uint16_t free_ids[kPgOnePages];
   __shared__ int s_parent[kPgOneThreads], s_kept[kPgOneThreads], s_held[kPgOneThreads];
   __shared__ int s_goal[kPgOneThreads], s_before[kPgOneThreads];
   __shared__ int sums[2][128];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = tid;
+  // all that depends on nothing, in one round trip
   int r[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) r[j] = 1024 * j + tid < a.n_pages ? a.refs[1024 * j + tid] : 1;
   const int len = b < a.B_in ? a.len[b] : 0;
+  const int parent = b < a.B ? pg_parent(a, b) : -1;
+  const int keep = b < a.B && a.keep != nullptr ? a.keep[b] : 0;
+  const int add = b < a.B && a.add != nullptr ? a.add[b] : 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (1024 * j + tid < a.n_pages) {
+      count[1024 * j + tid] = r[j];
+      writers[1024 * j + tid] = first[1024 * j + tid] = 0;
+    }
   s_held[tid] = len;
-  for (int i = tid; i < a.n_pages; i += kPgOneThreads) change[i] = writers[i] = first[i] = 0;
   __syncthreads();
   PgSeq q{-1, 0, 0};
   if (b < a.B) {
     bool ok;
-    q = pg_seq(a, s_held, b, ok);
+    q = pg_seq_of(a, parent, parent >= 0 && parent < a.B_in ? s_held[parent] : 0, keep, add, ok);
     if (!ok) flag_dev_err(a.err, kDevErrPagePlan);
   }
   if (!pg_len_ok(a, len)) flag_dev_err(a.err, kDevErrPagePlan);
   const int kept = q.parent >= 0 ? pg_pages(a.page_log2, q.keep) : 0;
-  const bool writes = q.parent >= 0 && pg_writes(a, q);
-  int page = writes ? a.table[(int64_t)q.parent * a.max_pages + kept - 1] : -1;
-  __syncthreads();  // (lengths are read)
   s_parent[tid] = q.parent;
   s_kept[tid] = kept;
+  __syncthreads();  // (lengths are read)
   s_held[tid] = pg_len_ok(a, len) ? pg_pages(a.page_log2, len) : 0;
+  __syncthreads();
+  const bool writes = q.parent >= 0 && pg_writes(a, q);
+  int page = writes ? a.table[(int64_t)q.parent * a.max_pages + kept - 1] : -1;
+  // a wave takes two rows at a time: their changes, and the kept entries into the new table
+  const int rows = max(a.B, a.B_in);
+  bool bad = false;
+  struct Row {
+    const int32_t *old, *now;
+    int32_t* out;
+    int k, held, from, i0, end;
+    bool moves, own;
+    int o[4], p[4];
+  };
+  auto open_row = [&](Row& w, int row) {
+    const bool has = row < rows;
+    const int par = has ? __builtin_amdgcn_readfirstlane(s_parent[row]) : -1;
+    w.k = has ? __builtin_amdgcn_readfirstlane(s_kept[row]) : 0;
+    w.held = has ? __builtin_amdgcn_readfirstlane(s_held[row]) : 0;
+    w.old = a.table + (int64_t)min(row, a.B_in - 1) * a.max_pages;
+    w.now = a.table + (int64_t)max(par, 0) * a.max_pages;
+    w.out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
+    w.own = par == row;
+    w.from = w.own ? min(w.k, w.held) : 0;
+    w.moves = w.now != w.out && w.k > 0;
+    w.i0 = w.moves ? 0 : w.from;
+    w.end = max(w.held, w.k);
+  };
+  auto load = [&](Row& w) {
+    // (inside the row whatever i is: a load under a condition of its own is waited for)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(w.i0 + 64 * u + lane, a.max_pages - 1);
+      w.o[u] = w.old[i];
+      w.p[u] = w.now[i];
+    }
+  };
+  auto use = [&](Row& w) {
+    if (w.moves) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (w.i0 + 64 * u + lane < w.k) w.out[w.i0 + 64 * u + lane] = w.p[u];
+    }
+    if (w.from < w.end) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = w.i0 + 64 * u + lane;
+        pg_change_of(a, w.o[u], (i >= w.from) & (i < w.held), w.p[u], (i < w.k) & !w.own, count, bad);
+      }
+    }
+    w.i0 += 256;
+  };
+  for (int row = wave; row < rows; row += 2 * (kPgOneThreads / 64)) {
+    Row x, y;
+    open_row(x, row);
+    open_row(y, row + kPgOneThreads / 64);
+    while (x.i0 < x.end || y.i0 < y.end) {
+      if (x.i0 < x.end) load(x);
+      if (y.i0 < y.end) load(y);
+      if (x.i0 < x.end) use(x);
+      if (y.i0 < y.end) use(y);
+    }
+  }
   if (writes && (unsigned)page >= (unsigned)a.n_pages) {
-    flag_dev_err(a.err, kDevErrPageId);
+    bad = true;
     page = -1;
   }
+  if (bad) flag_dev_err(a.err, kDevErrPageId);
   if (page >= 0) {
     atomicAdd(&writers[page], 1);
     atomicMax(&first[page], a.B - b);
-  }
-  const int page_refs = page >= 0 ? a.refs[page] : 0;
-  __syncthreads();
-  // a wave takes a row at a time: its changes, and the kept entries into the new table
-  const int rows = max(a.B, a.B_in);
-  for (int row = wave; row < rows; row += kPgOneThreads / 64) {
-    const int par = __builtin_amdgcn_readfirstlane(s_parent[row]);
-    const int k = __builtin_amdgcn_readfirstlane(s_kept[row]);
-    const int held = __builtin_amdgcn_readfirstlane(s_held[row]);
-    const int32_t* old = a.table + (int64_t)min(row, a.B_in - 1) * a.max_pages;
-    const int32_t* now = a.table + (int64_t)max(par, 0) * a.max_pages;
-    int32_t* out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
-    const int from = par == row ? min(k, held) : 0;
-    const bool moves = now != out && k > 0;
-    for (int i0 = moves ? 0 : from; i0 < max(held, k); i0 += 256) {
-      int o[4], p[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + 64 * u + lane;
-        o[u] = i < held && i >= from ? old[i] : -1;
-        p[u] = i < k ? now[i] : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + 64 * u + lane;
-        if (moves && i < k) out[i] = p[u];
-        if (i >= from) pg_change_of(a, o[u], i < held, p[u], i < k && par != row, change);
-      }
-    }
   }
   __syncthreads();
   // free pages in order
@@ -439,7 +503,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int p = 1024 * j + tid;
-    if (p < a.n_pages) r[j] += change[p];
+    if (p < a.n_pages) r[j] = count[p];
     if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
     is[j] = r[j] == 0;
   }
@@ -451,7 +515,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
   const int goal = pg_pages(a.page_log2, q.keep + q.add);
   int copy = -1, taken;
   if (page >= 0) {
-    const int holders = page_refs + change[page];
+    const int holders = count[page];
     if (holders > 1 && !(holders == writers[page] && first[page] == a.B - b)) copy = page;
   }
   const int old_end = kept - (copy >= 0 ? 1 : 0);
@@ -717,7 +781,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_compact_one(PagesCompac
     for (int i0 = 0; i0 < end; i0 += 256) {
       int p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = i0 + 64 * u + lane < end ? a.table[at + i0 + 64 * u + lane] : 0;
+      for (int u = 0; u < 4; ++u) p[u] = a.table[at + min(i0 + 64 * u + lane, end - 1)];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (i0 + 64 * u + lane >= end) break;
