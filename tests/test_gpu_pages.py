@@ -36,6 +36,7 @@ def check_fork(pool, B, in_place=False, full=False, counters=None, workspace=Non
     if in_place == "all":
         start = pool.table
     want, ran_out = beam_util.fork(pool.refs, pool.table, pool.length, pool.page, start, **seqs)
+    full = ran_out if full is None else full  # None: as the plain form has it
     assert ran_out == full
     got = run_fork(pool.refs, pool.table, pool.length, pool.page, B, in_place, counters, workspace, **seqs)
     for name, g, w in zip(("refs", "table", "length", "src", "dst", "rows"), got, want):
@@ -58,13 +59,15 @@ def lengths(rng, n, top, page):
     (1, 1, 16, 40, 40), (1, 4, 16, 100, 30), (3, 4, 64, 2000, 100), (16, 4, 16, 3000, 3000),
     (9, 8, 128, 5000, 100), (100, 5, 16, 300, 6000), (2, 3, 16, 9000, 40), (4, 32, 16, 500, 400)])
 @pytest.mark.parametrize("kind", ["beams", "any", "samples", "grow", "drafts", "new"])
-def test_fork(B, W, page, top, spare, kind):
+@pytest.mark.parametrize("wide", [False, True])
+def test_fork(B, W, page, top, spare, kind, wide):
+    """wide: tables of more entries than the launch of one block takes."""
     rng = np.random.default_rng(B * W + top)
     lens = lengths(rng, B, top, page)
-    pool = Pool(rng, lens, W, page, spare + 2 * B * W * (1 + 16 // page + 4), tail=kind in ("any", "grow"),
-                held=min(20, spare), width=(top + 40) // page + 3)
     N = B * W
-    say(f"fork {kind} B={B} W={W} page={page} top={top} pages={pool.n_pages}")
+    pool = Pool(rng, lens, W, page, spare + 2 * B * W * (1 + 16 // page + 4), tail=kind in ("any", "grow"),
+                held=min(20, spare), width=max((top + 40) // page + 3, 65536 // N + 2 if wide else 0))
+    say(f"fork {kind} B={B} W={W} page={page} top={top} pages={pool.n_pages} wide={wide}")
     if kind in ("beams", "any"):
         first = np.repeat(np.arange(B) * W, W)
         parent = first + rng.integers(0, W, N)
@@ -91,20 +94,48 @@ def test_fork(B, W, page, top, spare, kind):
         check_fork(pool, max(1, N // 2), parent=parent[:max(1, N // 2)], add=add[:max(1, N // 2)])
 
 
-def test_fork_without_free_pages():
+@pytest.mark.parametrize("n_pages,used,B", [(8192, 8000, 64), (8193, 8100, 64), (70000, 66000, 300),
+                                            (200000, 150, 1500), (300000, 299000, 40)])
+def test_fork_large_pools(n_pages, used, B):
+    """Most of the pool held by others, the free pages anywhere in it; whole prompts and
+    single tokens."""
+    rng = np.random.default_rng(n_pages)
+    pool = Pool(rng, np.minimum(lengths(rng, B, 60, 16), 60), 1, 16, n_pages, width=30)
+    pool.n_pages = n_pages
+    pool.refs = pool.refs[:n_pages].copy()
+    pool.table[:] = -7
+    ids = rng.permutation(n_pages)
+    at = 0
+    pool.refs[:] = 0
+    for b, n in enumerate(pool.length):
+        k = beam_util.pages(n, 16)
+        pool.table[b, :k] = ids[at:at + k]
+        at += k
+    pool.refs[ids[:at]] = 1
+    pool.refs[ids[:max(at, used)]] += 1
+    parent = np.where(rng.random(B) < 0.5, np.arange(B), rng.integers(-1, B, B))
+    need = np.where(rng.random(B) < 0.2, rng.integers(0, 300, B), 1)
+    say(f"large pool {n_pages} used {used} B={B}")
+    check_fork(pool, B, parent=parent, add=need, full=None)
+    check_fork(pool, B, in_place="all", full=None)
+
+
+@pytest.mark.parametrize("width", [6, 6000])
+def test_fork_without_free_pages(width):
     rng = np.random.default_rng(3)
     for spare in (0, 1, 5):
-        pool = Pool(rng, [32, 32, 20, 16], 3, 16, spare, held=0, width=6)
+        pool = Pool(rng, [32, 32, 20, 16], 3, 16, spare, held=0, width=width)
         say(f"pages run out, {spare} spare")
         check_fork(pool, 12, full=True, add=[17] * 12)
         check_fork(pool, 12, full=True, parent=np.repeat(np.arange(4) * 3, 3), add=[40] * 12)
 
 
-def test_fork_counters_serve_again():
+@pytest.mark.parametrize("width", [40, 9000])
+def test_fork_counters_serve_again(width):
     """One set of counters and workspace for calls of different sizes."""
     torch = torch_cuda()
     rng = np.random.default_rng(4)
-    pools = [Pool(rng, lengths(rng, b, 400, 16), 4, 16, 300, width=40) for b in (30, 2, 11)]
+    pools = [Pool(rng, lengths(rng, b, 400, 16), 4, 16, 300, width=width) for b in (30, 2, 11)]
     n = max(p.n_pages for p in pools)
     wb, cb = ne.pages_workspace(n, 200)
     ws = torch.full((wb,), 0xA5, dtype=torch.uint8, device="cuda")
@@ -116,11 +147,12 @@ def test_fork_counters_serve_again():
             assert not to_host(counters).any()
 
 
-def test_fork_numbers_that_do_not_fit():
+@pytest.mark.parametrize("width", [6, 20000])
+def test_fork_numbers_that_do_not_fit(width):
     """Such a sequence is left without tokens; the others are as they would be."""
     rng = np.random.default_rng(5)
-    pool = Pool(rng, [40, 35, 70, 16], 1, 16, 60, width=6)
-    top = 6 * 16
+    pool = Pool(rng, [40, 35, 70, 16], 1, 16, 60, width=width)
+    top = width * 16
     for what, seqs, good in [
             ("parent", dict(parent=[0, 4, 2, 3]), dict(parent=[0, -1, 2, 3], add=[1, 0, 1, 1])),
             ("parent", dict(parent=[0, -2, 2, 3]), dict(parent=[0, -1, 2, 3], add=[1, 0, 1, 1])),
@@ -130,7 +162,7 @@ def test_fork_numbers_that_do_not_fit():
             ("add", dict(add=[1, top, 1, 1]), dict(parent=[0, -1, 2, 3], add=[1, 0, 1, 1])),
             ("add", dict(add=[1, 2 ** 31 - 1, 1, 1]), dict(parent=[0, -1, 2, 3], add=[1, 0, 1, 1]))]:
         say(f"bad {what} {seqs}")
-        want, _ = beam_util.fork(pool.refs, pool.table, pool.length, 16, np.full((4, 6), -9, np.int32), **good)
+        want, _ = beam_util.fork(pool.refs, pool.table, pool.length, 16, np.full((4, width), -9, np.int32), **good)
         got = run_fork(pool.refs, pool.table, pool.length, 16, 4, **seqs)
         for g, w in zip(got, want):
             assert np.array_equal(g, w)
@@ -145,7 +177,7 @@ def test_fork_numbers_that_do_not_fit():
         say(f"bad length {n}")
         clean = length.copy()
         clean[1] = 0
-        want, _ = beam_util.fork(pool.refs, pool.table, clean, 16, np.full((4, 6), -9, np.int32))
+        want, _ = beam_util.fork(pool.refs, pool.table, clean, 16, np.full((4, width), -9, np.int32))
         got = run_fork(pool.refs, pool.table, length, 16, 4)
         for g, w in zip(got, want):
             assert np.array_equal(g, w)
@@ -165,7 +197,8 @@ def test_fork_numbers_that_do_not_fit():
                                                 (1024, 7, 64, 900), (1025, 30, 16, 100), (5000, 300, 16, 200),
                                                 (70000, 64, 16, 9000)])
 @pytest.mark.parametrize("in_place", [False, True])
-def test_compact(n_pages, B, page, top, in_place):
+@pytest.mark.parametrize("wide", [False, True])
+def test_compact(n_pages, B, page, top, in_place, wide):
     torch = torch_cuda()
     rng = np.random.default_rng(n_pages + B)
     lens = lengths(rng, B, top, page)
@@ -173,7 +206,8 @@ def test_compact(n_pages, B, page, top, in_place):
         lens[rng.integers(0, B)] = 0
     used = sum(beam_util.pages(n, page) for n in lens)
     for held in sorted({0, (n_pages - used) // 3, n_pages}):
-        pool = Pool(rng, lens, 1, page, n_pages - used, held=held, width=top // page + 3)
+        pool = Pool(rng, lens, 1, page, n_pages - used, held=held,
+                    width=max(top // page + 3, 65536 // B + 2 if wide else 0))
         say(f"compact n_pages={n_pages} used={used} held={held} in place {in_place}")
         d = [to_dev(x) for x in (pool.refs, pool.table, pool.length)]
         start = pool.table if in_place else np.full_like(pool.table, -9)
@@ -187,12 +221,13 @@ def test_compact(n_pages, B, page, top, in_place):
         ne.device_check()
 
 
-def test_compact_numbers_that_do_not_fit():
+@pytest.mark.parametrize("width", [6, 30000])
+def test_compact_numbers_that_do_not_fit(width):
     rng = np.random.default_rng(6)
-    pool = Pool(rng, [40, 35, 70], 1, 16, 60, width=6)
+    pool = Pool(rng, [40, 35, 70], 1, 16, 60, width=width)
     refs, table, length = pool.refs.copy(), pool.table.copy(), pool.length.copy()
     table[0, 1] = pool.n_pages + 3
-    length[1] = 97
+    length[1] = 16 * width + 1
     lost = table[2, 2]
     refs[lost] = 0
     d = [to_dev(x) for x in (refs, table, length)]
