@@ -108,6 +108,21 @@ __device__ __forceinline__ int bm_before(const u64* key, int n, u64 mine) {
   return p;
 }
 
+// x[e] for a lane's own e, N a power of two: a choice by each bit of e, as bit masks (a
+// condition on array elements would put the array into memory)
+template <int N>
+__device__ __forceinline__ uint32_t bm_pick(const uint32_t (&x)[N], int e) {
+  if constexpr (N == 1) {
+    return x[0];
+  } else {
+    const uint32_t odd = -(uint32_t)(e & 1);
+    uint32_t y[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = (x[2 * i + 1] & odd) | (x[2 * i] & ~odd);
+    return bm_pick<N / 2>(y, e >> 1);
+  }
+}
+
 // Order of a logit as an integer: larger logit, larger key; both zeros are one, and
 // minus infinity is 0 (no candidate).
 __device__ __forceinline__ uint32_t bm_ordered(float l) {
@@ -180,7 +195,7 @@ __device__ __forceinline__ bool bm_alive(float score) { return score > -INFINITY
 // above (the sum is as exact, and most groups have nothing to rescale).  Then the maxima
 // of the block's lanes give the bound of its list.
 // ---------------------------------------------------------------------------
-constexpr int kBmGroups = 8;
+constexpr int kBmGroups = 8;  // (4 kBmGroups bits of a word)
 constexpr float kBmAbove = 64.0f;
 struct __align__(16) BmSum {
   double s;  // sum of exp(l - m)
@@ -263,19 +278,21 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamSelectArgs a) {
   BmList list(keys[wave]);
   list.bound(bm_ordered(all4), K);
   const float least = bm_logit(list.least);
-  // which of the lane's logits reach the bound: bit 4 NG - 1 - e
-  u64 reach = 0;
+  // which of the lane's logits reach the bound: bit e
+  uint32_t reach = 0;
   if (groups > 0) {
 #pragma unroll
-    for (int e = 0; e < 4 * NG; ++e) reach = reach << 1 | ((x[e] >= least) & (e < 4 * groups));
+    for (int e = 4 * NG - 1; e >= 0; --e) reach = reach + reach + (x[e] >= least ? 1u : 0u);
+    if (groups < NG) reach &= (1u << 4 * groups) - 1;
   }
   while (__any(reach != 0)) {  // every lane its next one
-    const int bit = 63 - __builtin_clzll(reach | 1), e = 4 * NG - 1 - bit;
-    float v = x[0];
+    const int e = __builtin_ctz(reach | 1u << 31);
+    uint32_t bits[4 * NG];
 #pragma unroll
-    for (int i = 1; i < 4 * NG; ++i) v = e == i ? x[i] : v;
+    for (int i = 0; i < 4 * NG; ++i) bits[i] = __float_as_uint(x[i]);
+    const float v = __uint_as_float(bm_pick<4 * NG>(bits, e));
     list.add(reach != 0 ? bm_key(v, first + 256 * (e >> 2) + 4 * lane + (e & 3)) : 0);
-    reach &= ~(1ull << bit);
+    reach &= reach - 1;
     if (list.n > kBmFull) list.cut(K);
   }
   if (list.n > 64) list.cut(K);
@@ -327,13 +344,18 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
   __shared__ int token[kBmOpen];  // | place << 24, negative: a stop token
   __shared__ u64 key_all[kBmOpen + 8], key_live[kBmOpen + 8];
   __shared__ int from[kBmOpen], total;
+  __shared__ uint32_t bound;
+  __shared__ float best;
   __shared__ int stop[kBeamMaxStop];
-  __shared__ int next[kBeamMaxW], over[kBeamMaxW], to_free[kBeamMaxW];
+  __shared__ int next[kBeamMaxW], over[kBeamMaxW], to_free[kBeamMaxW], child[kBeamMaxW];
   const int b = blockIdx.x, W = a.W, K = a.K, waves = blockDim.x >> 6;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const BmExp exp_of;
   if ((int)threadIdx.x < a.n_stop) stop[threadIdx.x] = a.stop[threadIdx.x];
-  if (threadIdx.x < kBeamMaxW) next[threadIdx.x] = over[threadIdx.x] = -1;
+  if (threadIdx.x < kBeamMaxW) {
+    next[threadIdx.x] = over[threadIdx.x] = -1;
+    child[threadIdx.x] = kBeamMaxW;  // the first child of the beam in this place
+  }
   for (int i = threadIdx.x; i < W * K + 8; i += blockDim.x) key_all[i] = key_live[i] = 0;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
@@ -378,15 +400,18 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
           top = max(top, k[h]);
         }
         list.bound((uint32_t)(top >> 32), K);
-        uint32_t reach = 0;  // bit h: the lane's k[h] does
+        uint32_t reach = 0;  // bit h: the lane's k[h] does (past the keys: 0, which does not)
 #pragma unroll
         for (int h = 0; h < kBmAhead; ++h) reach |= (uint32_t)((uint32_t)(k[h] >> 32) >= list.least) << h;
         while (__any(reach != 0)) {  // every lane its next one
-          const int h = __builtin_ctz(reach | 1u << 31);
-          u64 one = k[0];
+          uint32_t lo[kBmAhead], hi[kBmAhead];
 #pragma unroll
-          for (int i = 1; i < kBmAhead; ++i) one = h == i ? k[i] : one;
-          list.add(reach != 0 ? one : 0);
+          for (int h = 0; h < kBmAhead; ++h) {
+            lo[h] = (uint32_t)k[h];
+            hi[h] = (uint32_t)(k[h] >> 32);
+          }
+          const int h = __builtin_ctz(reach | 1u << 31);
+          list.add(reach != 0 ? (u64)bm_pick(hi, h) << 32 | bm_pick(lo, h) : 0);
           reach &= reach - 1;
           if (list.n > kBmFull) list.cut(K);
         }
@@ -413,15 +438,24 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
   // none: larger values before it, and equal ones of a lower index.  Of more than 64, those
   // that cannot be among the W best are left out first.
   const int all = W * K;
-  u64 least = 1;
+  // (as distances from the best, whose upper 16 bits are fine near it)
+  auto near = [&](u64 v) { return v == 0 ? 0u : bm_ordered((float)(bm_value64(v) - (double)best)); };
   if (all > 64) {
-    u64 top = 0;
-    for (int i = lane; i < all; i += 64) top = max(top, token[i] < 0 ? 0 : value[i]);
-    least = max(1ull, (u64)bm_kth((uint32_t)(top >> 32), W) << 32);
+    if (wave == 0) {
+      u64 top = 0;
+      for (int i = lane; i < all; i += 64) top = max(top, token[i] < 0 ? 0 : value[i]);
+      const float x = wave_max(top == 0 ? -INFINITY : (float)bm_value64(top));
+      if (lane == 0) best = x;
+      wave_lds_sync();
+      const uint32_t y = bm_kth(near(top), W);
+      if (lane == 0) bound = y;
+    }
+    __syncthreads();
   }
+  const uint32_t least = all > 64 ? bound : 0;
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
     const u64 v = value[i];
-    if (v < least) continue;
+    if (v == 0 || (least != 0 && near(v) < least)) continue;
     const int at = atomicAdd(&total, 1);
     key_all[at] = v;
     key_live[at] = token[i] < 0 ? 0 : v;
@@ -463,13 +497,10 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
     return;
   }
   // the first child of a beam keeps its place; the others take the free ones in order
-  bool keeps = i >= 0;
-  u64 taken = 0;
-  for (int j = 0; j < W; ++j) {
-    const int p = __builtin_amdgcn_readlane(place, j);
-    if (p >= 0) taken |= 1ull << p;
-    keeps &= !(j < lane && p == place);
-  }
+  if (i >= 0) atomicMin(&child[place], lane);
+  wave_lds_sync();
+  const bool keeps = i >= 0 && child[place] == lane;
+  const u64 taken = __ballot(lane < W && child[min(lane, W - 1)] < W);
   const u64 open = __ballot(lane < W && !(taken >> lane & 1));
   if (open >> lane & 1) to_free[bm_rank(open)] = lane;
   const u64 movers = __ballot(lane < W && !keeps);
