@@ -244,7 +244,9 @@ neon_status neon_tensor_ptr(neon_ctx* ctx, const char* name, void** ptr,
  * kernel-level calls on the current device have set since the last check:
  * NEON_EINVAL when an expert id given in device memory (neon_moe_experts,
  * neon_moe_prefill) lay outside [0, E).  Such a slot is dropped (adds 0)
- * instead of reading past the expert arrays.  The context-level reads
+ * instead of reading past the expert arrays.  (What the calls of a paged cache,
+ * of sampling and of beam search report stands with them; NEON_EKV_FULL: pages
+ * ran out in neon_pages_fork.)  The context-level reads
  * (neon_read_tokens / _logits / _activation) make the same check for the
  * context's own kernels.  (The reference has no counterpart: its Systems
  * throw on the host and do no device-side validation.) */
@@ -591,7 +593,8 @@ neon_status neon_beam_select(const float* logits, int64_t stride, int B, int W, 
 
 /* Moves the states of beams in place: row r of every state becomes what row
  * parent[r] was (device int32 [B W], a row of the same request; -1 or r itself: left
- * as it is).  states: host array of n_states device pointers (16-byte aligned), each
+ * as it is).  states: host array of n_states device pointers (16-byte aligned, to
+ * memory that does not overlap), each
  * [B W][slabs][T][row_bytes] (row_bytes a multiple of 4; a contiguous cache of
  * neon_attn_decode has slabs = Hkv, T = T_max, row_bytes = 2 D).  len [B W] (device
  * int32, or NULL for T): the first min(len[parent[r]], T) rows of each slab are moved,

@@ -191,9 +191,15 @@ __device__ __forceinline__ bool bm_alive(float score) { return score > -INFINITY
 // W + n_stop at least W are no stop tokens, and a stop token that is not among them has W
 // better ones in its own row).  A wave requests all its tokens at once, up to kBmGroups
 // groups of 256 (4 of a lane), and takes the exponentials of a group as it comes: relative
-// to the maximum of the first one, which a later maximum replaces only where it is 64
-// above (the sum is as exact, and most groups have nothing to rescale).  Then the maxima
-// of the block's lanes give the bound of its list.
+// to the maximum of the first one, and only where a later one is more than 64 above are
+// they taken again (the sum is as exact).  Then the maxima of the block's lanes give the
+// bound of its list, which about K of its tokens reach.
+// Bound: the vector units beside the reads.  64 rows of 201088: 19.5 us, 51.5 MB, floor
+// 10.3; 500 vector instructions for 1024 tokens of a wave, 307 of them the exponentials
+// (19 each, 64-bit ones at one in 4 cycles), are 12 us of all SIMDs.  Without the exponentials it takes 16, without the list 16.5, without both
+// 12.  4, 5, 7, 8, 10 and 13 groups, in places for as many blocks as run at once, came to
+// 18 to 21 us; two steps of 1024 with the next on its way to 22.  4 rows: 5.3 us (0.3 until
+// the tokens are there, 0.9 exponentials, 0.5 the bound, 0.3 the list, 0.9 the rest).
 // ---------------------------------------------------------------------------
 constexpr int kBmGroups = 8;  // (4 kBmGroups bits of a word)
 constexpr float kBmAbove = 64.0f;
@@ -333,6 +339,12 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamSelectArgs a) {
 // ---------------------------------------------------------------------------
 // A request: the K best of each row (a wave each), then the W best that go on and the
 // stop tokens among the W best.
+// Bound: a chain of dependent steps of one block (4 beams 5.4 us: 1 until the chunks'
+// results are there, 0.6 the sum, 0.5 the bound, 0.9 the list and its order, 0.8 the places
+// among all, 0.8 the rest, the launch), and from 8 beams on the instructions of four waves
+// a SIMD (16 beams 9.3 us).  A step that goes through scalar registers costs some 40 ns:
+// orders are counted from LDS broadcasts (5 keys put in their places one after another
+// took 1.4 us).
 // ---------------------------------------------------------------------------
 constexpr int kBmMaxK = kBeamMaxW + kBeamMaxStop;
 constexpr int kBmJoinWaves = 16;
@@ -557,13 +569,16 @@ void launch_beam_select(BeamSelectArgs a, hipStream_t st) {
   hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.B), dim3(64 * waves), 0, st, a);
 }
 
-constexpr int kReorderUnits = 4;
+constexpr int kReorderUnits = 4;  // 1, 2, 4, 8: 24, 22.6, 22.6, 31 us (136 MB, see below)
 // ---------------------------------------------------------------------------
 // Moving states.  A block takes the same part of a slab in all beams of a request, U
 // units of a thread.  Where no beam that moves is also one that others continue (beams
 // that go on keep their places), each is copied for itself; otherwise a thread reads all
 // that move to its places before it writes any, so the move is in place whatever the
 // parents are (a permutation too).
+// Bound: the bytes read and written (11 of 32 beams of up to 2000 tokens in four states,
+// 136 MB: 22.5 us, 6.0 TB/s, part of what is read being in the last-level cache; a large
+// copy 4.98).
 // ---------------------------------------------------------------------------
 template <class T, int WMAX>
 __global__ __launch_bounds__(256) void k_beam_reorder(BeamReorderArgs a) {

@@ -76,7 +76,11 @@ __device__ __forceinline__ bool pg_writes(const PagesForkArgs& a, const PgSeq& q
 // 2. Which pages are free then (listed, a chunk of pages by a block), and what each
 //    sequence needs: pages past its last, and one for the page that it would write and
 //    that others hold too (if all holders write, the first keeps it).
-// 3. The counts; the tables: what is kept, then free pages in order.
+// 3. The counts, and the new entries of the tables: free pages in order.  (What is kept is
+//    in them since the first launch.)
+// No order of threads reaches the result: sums, a maximum, and ranks.  Bound: the chain of
+// each launch (lookups of parent, length, entries; then the lists; then a page's place):
+// 1024 sequences of up to 4096 tokens, 45000 pages, 4.8 + 3.9 + 4.8 us for 1.5 MB.
 // ---------------------------------------------------------------------------
 struct PgWork {  // the workspace
   int* free_in;   // [chunks] free pages of a chunk
@@ -594,6 +598,8 @@ void launch_pages_fork(const PagesForkArgs& a, hipStream_t st) {
 // to the free ids below U, both in their order, so that no page is read and written.
 // 1. used pages of each chunk; 2. the lists, and what becomes of every page; 3. the
 // counts and the tables.
+// Bound: the chain of each launch: 131072 pages, 512 sequences, 2.5 + 5.4 + 5.6 us for
+// 2.4 MB.
 // ---------------------------------------------------------------------------
 struct PcWork {
   int* used_in;   // [chunks]
@@ -828,7 +834,10 @@ size_t pages_workspace(int n_pages, int B) {
 
 // ---------------------------------------------------------------------------
 // Copy.  A block takes one 16-byte unit per thread of a page, in one pool, for 64
-// entries of the list: the entries that are none cost a load and a ballot.
+// entries of the list: the entries that are none cost a load and a ballot.  One launch
+// serves up to 64 caches.
+// Bound: the bytes read and written: 600 pages of 256 KB in two layers, 1.26 GB, 257 us,
+// 4.89 TB/s; the first rows of 20 pages in 24 layers, 77 MB, 17 us.
 // ---------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ void pg_copy_units(const PagesCopyArgs& a, uint8_t* pool, int64_t page_units,
