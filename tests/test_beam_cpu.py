@@ -22,7 +22,8 @@ def select(logits=P, stride=100, B=2, W=4, V=100, score=P, stop=P, n_stop=2, tok
     dict(logits=None), dict(score=None), dict(token=None), dict(parent=None), dict(out=None),
     dict(stop=None), dict(stride=99), dict(B=0), dict(B=65536), dict(W=0), dict(W=33), dict(V=0),
     dict(V=(1 << 24) + 1, stride=1 << 30), dict(n_stop=-1), dict(n_stop=17), dict(et=None), dict(ep=None),
-    dict(es=None), dict(et=None, ep=None), dict(ws=None), dict(ws=P + 8), dict(wb=100)], ids=str)
+    dict(es=None), dict(et=None, ep=None), dict(ws=None), dict(ws=P + 8), dict(wb=100),
+    dict(B=65535, W=32, V=1 << 17, stride=1 << 17)], ids=str)
 def test_select_refusals(bad):
     assert select(**bad) == ne.NEON_EINVAL
     assert ne.lib().neon_last_error(None).startswith(b"neon_beam_select")

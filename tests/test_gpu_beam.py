@@ -236,3 +236,100 @@ def test_reorder_shapes_and_bad_parents():
         ne.beam_reorder(ne.beam_states([x], 2), bad, bad.float())
     with pytest.raises(ne.NeonError):
         ne.beam_reorder(ne.beam_states([torch.zeros(4, 3, 1, dtype=torch.uint8, device="cuda")], 2), bad)
+
+
+class Guarded:
+    """A device buffer with a sentinel on both sides."""
+
+    def __init__(self, n, fill=0x5A):
+        torch = torch_cuda()
+        self.all = torch.full((n + 512,), fill, dtype=torch.uint8, device="cuda")
+        self.fill, self.n = fill, n
+        self.mid = self.all[256:256 + n]
+
+    def as_type(self, dtype, *shape):
+        return self.mid.view(dtype).view(*shape)
+
+    def intact(self):
+        a = to_host(self.all)
+        return (a[:256] == self.fill).all() and (a[256 + self.n:] == self.fill).all()
+
+
+@pytest.mark.parametrize("B,W,V,n_stop", [(1, 1, 1, 0), (2, 3, 5000, 2), (3, 32, 2049, 16), (60, 4, 33000, 3)])
+def test_select_stays_inside_its_buffers(B, W, V, n_stop):
+    torch = torch_cuda()
+    rng = np.random.default_rng(V)
+    l, score = case(rng, B, W, V)
+    stop = rng.choice(V, min(V, n_stop), replace=False)
+    N = B * W
+    need = ne.beam_select_workspace(B, W, V, len(stop))
+    ws = Guarded(need)
+    outs = [Guarded(4 * N) for _ in range(6)]
+    t = [g.as_type(torch.float32 if i in (2, 5) else torch.int32, N) for i, g in enumerate(outs)]
+    # rows from an odd place of wider ones
+    wide = torch.full((N, V + 9), float("inf"), device="cuda")
+    wide[:, 3:3 + V] = to_dev(l)
+    say(f"guards B={B} W={W} V={V}")
+    ne.beam_select(wide[:, 3:3 + V], to_dev(score), W, *t[:3], stop=to_dev(stop.astype(np.int32)) if len(stop) else None,
+                   ended=tuple(t[3:]), workspace=ws.mid)
+    check([to_host(x) for x in t], beam_util.select(l, score, W, stop))
+    assert ws.intact() and all(g.intact() for g in outs)
+
+
+@pytest.mark.parametrize("W", [1, 32])
+def test_select_largest_vocabulary(W):
+    torch = torch_cuda()
+    V = 1 << 24
+    g = torch.Generator(device="cuda")
+    g.manual_seed(W)
+    l = torch.randn((W, V), generator=g, device="cuda")
+    score = (-10 - torch.rand(W, generator=g, device="cuda"))
+    token, parent, out = empty_dev(W, np.int32), empty_dev(W, np.int32), empty_dev(W, np.float32)
+    say(f"2^24 tokens, {W} beams")
+    ne.beam_select(l, score, W, token, parent, out)
+    # the candidates that count: the best of each row
+    v = torch.empty(W, W, dtype=torch.float64, device="cuda")
+    at = torch.empty(W, W, dtype=torch.int64, device="cuda")
+    for w in range(W):
+        x = l[w].double()
+        lse = x.max() + (x - x.max()).exp().sum().log()
+        top, at[w] = torch.topk(x, W)
+        v[w] = score[w].double() + (top - lse)
+    v, at = to_host(v).reshape(-1), to_host(at).reshape(-1)
+    best = np.argsort(-v, kind="stable")[:W]
+    place, rest = {}, []
+    for i in best:
+        (rest.append(i) if i // W in place else place.__setitem__(i // W, i))
+    for w in range(W):
+        if w not in place:
+            place[w] = rest.pop(0)
+    for w, i in place.items():
+        assert to_host(token)[w] == at[i] and to_host(parent)[w] == i // W
+        assert abs(to_host(out)[w] - v[i]) <= 2.0 ** -24 * abs(v[i]) + 1e-10
+
+
+def test_select_equal_beams_wherever_their_rows_begin():
+    """Equal rows and scores are ordered by their places, then tokens, whatever the
+    alignment of the rows: their 64-bit values are bit-equal."""
+    rng = np.random.default_rng(12)
+    for V in (1001, 4099, 20003):
+        one = rng.normal(0, 2, V).astype(np.float32)
+        l = np.repeat(one[None], 8, 0)
+        token, parent, out = run(l, np.full(8, -1.5, np.float32), 8, ended=False)
+        assert np.array_equal(token, np.full(8, one.argmax())) and np.array_equal(parent, np.arange(8))
+        assert (out == out[0]).all()
+
+
+@pytest.mark.parametrize("row", [4, 16, 48])
+def test_reorder_stays_inside_its_states(row):
+    torch = torch_cuda()
+    rng = np.random.default_rng(row)
+    N, slabs, T = 6, 3, 37
+    x = rng.integers(-2 ** 31, 2 ** 31, (N, slabs, T, row // 4)).astype(np.int32)
+    g = Guarded(x.nbytes)
+    d = g.as_type(torch.int32, *x.shape)
+    d.copy_(to_dev(x))
+    parent = np.array([1, 2, 0, 3, 3, 4], np.int32)
+    length = np.array([37, 5, 0, 37, 36, 1], np.int32)
+    ne.beam_reorder(ne.beam_states([d], 3), to_dev(parent), to_dev(length))
+    assert np.array_equal(to_host(d), beam_util.reorder(x, parent, length, 3)) and g.intact()

@@ -329,3 +329,65 @@ def test_refusals_python():
     with pytest.raises(ValueError):
         ne.paged_layers([])
     ne.device_check()
+
+
+def guarded(n, dtype):
+    """(the whole buffer, its middle of n elements) with a sentinel on both sides."""
+    torch = torch_cuda()
+    whole = torch.full((n + 128,), 0x5A5A5A5A if dtype is torch.int32 else 0x5A, dtype=dtype, device="cuda")
+    return whole, whole[64:64 + n]
+
+
+def untouched(whole, n):
+    a = to_host(whole)
+    return (a[:64] == a[0]).all() and (a[64 + n:] == a[0]).all() and a[0] in (0x5A5A5A5A, 0x5A)
+
+
+@pytest.mark.parametrize("n_pages,B,W,width", [(97, 2, 3, 8), (900, 16, 4, 30), (9000, 3, 4, 40), (1100, 30, 8, 20),
+                                               (2049, 1, 1, 70000)])
+def test_plans_stay_inside_their_buffers(n_pages, B, W, width):
+    torch = torch_cuda()
+    rng = np.random.default_rng(n_pages)
+    lens = np.minimum(lengths(rng, B, 100, 16), 100)
+    while sum(beam_util.pages(n, 16) * W for n in lens) + 2 * B * W > n_pages:
+        lens[rng.integers(0, B)] = 0
+    pool = Pool(rng, lens, W, 16, n_pages, width=width)
+    pool.n_pages = n_pages
+    keep = pool.table[pool.table >= 0]
+    remap = np.full(len(pool.refs), -1)
+    used = np.unique(keep)
+    remap[used] = rng.permutation(n_pages)[:len(used)]
+    pool.table = np.where(pool.table >= 0, remap[np.clip(pool.table, 0, None)], -7).astype(np.int32)
+    refs = np.zeros(n_pages, np.int32)
+    np.add.at(refs, pool.table[pool.table >= 0], 1)
+    pool.refs = refs
+    N = B * W
+    parent = np.repeat(np.arange(B) * W, W) + rng.integers(0, W, N)
+    want, full = beam_util.fork(refs, pool.table, pool.length, 16, np.full((N, width), 0x5A5A5A5A, np.int32),
+                                parent=parent)
+    wb, cb = ne.pages_workspace(n_pages, N)
+    i32, u8 = torch.int32, torch.uint8
+    sizes = [n_pages, N * width, N, N, N, N]
+    bufs = [guarded(n, i32) for n in sizes]
+    ws = guarded(-(-wb // 16) * 16, u8)
+    ws_mid = ws[1][:wb]
+    counters = guarded(cb, u8)
+    counters[1].zero_()
+    d = [to_dev(x) for x in (refs, pool.table, pool.length)]
+    m = [b[1] for b in bufs]
+    say(f"guards n_pages={n_pages} B={B} W={W} width={width}")
+    ne.pages_fork(*d, 16, m[0], m[1].view(N, width), m[2], m[3:], parent=to_dev(parent.astype(np.int32)),
+                  workspace=ws_mid, counters=counters[1])
+    for g, w in zip(m, want):
+        assert np.array_equal(to_host(g), w.reshape(-1))
+    assert all(untouched(b[0], n) for b, n in zip(bufs, sizes))
+    assert untouched(ws[0], len(ws[1])) and untouched(counters[0], cb) and not to_host(counters[1]).any()
+    sizes = [n_pages, N * width, n_pages, n_pages // 2, n_pages // 2]
+    bufs = [guarded(n, i32) for n in sizes]
+    m = [b[1] for b in bufs]
+    ne.pages_compact(*d, 16, m[0], m[1].view(N, width), m[2], m[3:], workspace=ws_mid)
+    want = beam_util.compact(refs, pool.table, pool.length, 16, np.full((N, width), 0x5A5A5A5A, np.int32))
+    for g, w in zip(m, want):
+        assert np.array_equal(to_host(g), w.reshape(-1))
+    assert all(untouched(b[0], n) for b, n in zip(bufs, sizes)) and untouched(ws[0], len(ws[1]))
+    ne.device_check()
