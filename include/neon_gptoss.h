@@ -609,7 +609,8 @@ neon_status neon_beam_reorder(void* const* states, int n_states, int B, int W, i
  * and others (a prefix that is kept); 0: free.  A sequence of n tokens holds the
  * pages of the first ceil(n / page_size) entries of its page table row.  One table
  * serves the caches of all layers.  n_pages is up to 2^24, page_size a power of two
- * from 16 to 65536, B and B_in 1 to 65535.
+ * from 16 to 65536, B and B_in 1 to 65535, a table has fewer than 2^31 entries.  Calls
+ * that may run at once need a workspace and counters each.
  *
  * neon_pages_fork: which pages the sequences hold next.  Sequence b < B continues the
  * first keep[b] tokens (NULL: all) of row parent[b] of page_table (B_in rows; NULL: its

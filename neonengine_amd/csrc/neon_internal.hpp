@@ -524,7 +524,7 @@ struct PagesCompactArgs {
 constexpr int kPagesMax = 1 << 24;
 size_t pages_workspace(int n_pages, int B);
 size_t pages_counters(int n_pages);
-bool pages_fits(int B, int max_pages);  // the launches' grids hold them
+bool pages_fits(int B, int max_pages);  // tables of as many entries are taken
 void launch_pages_fork(const PagesForkArgs& a, hipStream_t st);
 void launch_pages_compact(const PagesCompactArgs& a, hipStream_t st);
 

@@ -575,9 +575,9 @@ static bool pages_one(int n_pages, int B, int most, int max_pages) {
 }
 size_t pages_counters(int n_pages) { return (size_t)n_pages * 12; }
 static int64_t pages_parts(int max_pages) { return ((int64_t)max_pages + kPgSpan - 1) / kPgSpan; }
-bool pages_fits(int B, int max_pages) {
-  return pages_parts(max_pages) * B / 4 + (kPagesMax / kPgChunk) + 2 < 1 << 24;
-}
+// All entries of a table count in 32 bits (what the sequences need is summed), and then
+// the grids hold them too.
+bool pages_fits(int B, int max_pages) { return (int64_t)B * max_pages < (int64_t)1 << 31; }
 void launch_pages_fork(const PagesForkArgs& a, hipStream_t st) {
   const int parts = (int)pages_parts(a.max_pages);
   const int rows = a.B > a.B_in ? a.B : a.B_in;

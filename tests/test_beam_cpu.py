@@ -74,7 +74,7 @@ def fork(refs=P, table=P, length=P, B_in=3, parent=P, keep=P, add=P, refs_out=P,
 
 SHAPES = [dict(B=0), dict(B=65536), dict(n_pages=0), dict(n_pages=(1 << 24) + 1), dict(page=8),
           dict(page=48), dict(page=1 << 17), dict(page=-16), dict(width=0), dict(width=-1),
-          dict(B=65535, width=1 << 30), dict(ws=None), dict(ws=P + 4), dict(wb=10), dict(refs=None),
+          dict(B=65535, width=1 << 30), dict(B=200, width=1 << 26), dict(B=32, width=1 << 26), dict(ws=None), dict(ws=P + 4), dict(wb=10), dict(refs=None),
           dict(table=None), dict(length=None), dict(refs_out=None), dict(table_out=None), dict(src=None),
           dict(dst=None)]
 
