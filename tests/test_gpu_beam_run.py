@@ -332,3 +332,115 @@ def test_states_in_contiguous_caches(W, T):
             got = out[b, h * D:(h + 1) * D].float().cpu().numpy()
             assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -12).all()
     ne.device_check()
+
+
+class Calls:
+    """A choice, a fork and a compaction, each from fixed inputs into outputs of its own."""
+
+    def __init__(self, seed, B, W, vocab, n_pages, width):
+        torch = torch_cuda()
+        rng = np.random.default_rng(seed)
+        self.W, N = W, B * W
+        logits = rng.normal(0, 2.5, (N, vocab)).astype(np.float32)
+        score = (-3 - rng.random(N)).astype(np.float32)
+        # one sequence of each request has tokens, the others continue it
+        length = np.zeros(N, np.int32)
+        length[::W] = rng.integers(1, 60, B)
+        table, refs = np.full((N, width), -1, np.int32), np.zeros(n_pages, np.int32)
+        free = rng.permutation(n_pages)
+        for b in range(0, N, W):
+            k = beam_util.pages(length[b], PAGE)
+            table[b, :k], free = free[:k], free[k:]
+            refs[table[b, :k]] = 1
+        parent = np.repeat(np.arange(0, N, W), W).astype(np.int32)
+        fill = np.full((N, width), -9, np.int32)
+        fork, out_of_pages = beam_util.fork(refs, table, length, PAGE, fill, parent=parent)
+        assert not out_of_pages
+        self.want = [*beam_util.select(logits, score, W)[:2], *fork,
+                     *beam_util.compact(refs, table, length, PAGE, fill)]
+        self.ins = [to_dev(x) for x in (logits, score, refs, table, length, parent)]
+        self.out_score = torch.empty(N, device="cuda")
+        shapes = [(N,), (N,), (n_pages,), (N, width), (N,), (N,), (N,), (N,), (n_pages,), (N, width), (n_pages,),
+                  (n_pages // 2,), (n_pages // 2,)]
+        self.outs = [torch.empty(s, dtype=torch.int32, device="cuda") for s in shapes]
+        wb, cb = ne.pages_workspace(n_pages, N)
+        self.needs = ne.beam_select_workspace(B, W, vocab, 0), wb, cb
+
+    def __call__(self, select_ws, plan_ws, counters):
+        logits, score, refs, table, length, parent = self.ins
+        o = self.outs
+        ne.beam_select(logits, score, self.W, o[0], o[1], self.out_score, workspace=select_ws)
+        ne.pages_fork(refs, table, length, PAGE, o[2], o[3], o[4], o[5:8], parent=parent, workspace=plan_ws,
+                      counters=counters)
+        ne.pages_compact(refs, table, length, PAGE, *o[8:11], o[11:13], workspace=plan_ws)
+
+    def clear(self):
+        for o in self.outs:
+            o.fill_(-9)
+
+    def check(self):
+        assert len(self.outs) == len(self.want)
+        for i, (o, w) in enumerate(zip(self.outs, self.want)):
+            assert np.array_equal(to_host(o), w), i
+
+
+# (one block each, and several launches each)
+SIZES = [[(3, 4, 5000, 200, 8), (7, 2, 900, 90, 5)], [(40, 8, 3000, 9000, 12), (100, 3, 20011, 30000, 7)]]
+
+
+def buffers(needs):
+    torch = torch_cuda()
+    s, w, c = needs
+    return (torch.full((s,), 0xA5, dtype=torch.uint8, device="cuda"),
+            torch.full((w,), 0xA5, dtype=torch.uint8, device="cuda"),
+            torch.zeros(c, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=["small", "large"])
+def test_graphs_share_workspaces(sizes):
+    """Two captured graphs of calls of different sizes with one set of workspaces and
+    counters, replayed in turn with an eager call in between."""
+    torch = torch_cuda()
+    calls = [Calls(20 + i, *s) for i, s in enumerate(sizes)]
+    shared = buffers([max(n) for n in zip(*(c.needs for c in calls))])
+    for c in calls:
+        c(*shared)
+    torch.cuda.synchronize()
+    graphs = []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c(*shared)
+    for replay in range(5):
+        say("replay", replay)
+        for c in calls:
+            c.clear()
+        for g in graphs if replay % 2 else graphs[::-1]:
+            g.replay()
+        for c in calls:
+            c.check()
+        calls[replay % 2].clear()
+        calls[replay % 2](*shared)
+        calls[replay % 2].check()
+    assert not shared[2].any()
+    ne.device_check()
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=["small", "large"])
+def test_two_streams_at_once(sizes):
+    """The same calls on two streams, each with workspaces and counters of its own."""
+    torch = torch_cuda()
+    calls = [Calls(30 + i, *s) for i, s in enumerate(sizes)]
+    own = [buffers(c.needs) for c in calls]
+    for c in calls:
+        c.clear()
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, b, s in zip(calls, own, streams):
+            with torch.cuda.stream(s):
+                c(*b)
+    torch.cuda.synchronize()
+    for c in calls:
+        c.check()
+    ne.device_check()
