@@ -342,14 +342,16 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamSelectArgs a) {
 // Bound: a chain of dependent steps of one block (4 beams 5.4 us: 1 until the chunks'
 // results are there, 0.6 the sum, 0.5 the bound, 0.9 the list and its order, 0.8 the places
 // among all, 0.8 the rest, the launch), and from 8 beams on the instructions of four waves
-// a SIMD (16 beams 9.3 us).  A step that goes through scalar registers costs some 40 ns:
+// a SIMD (16 beams 8.6 us).  A step that goes through scalar registers costs some 40 ns:
 // orders are counted from LDS broadcasts (5 keys put in their places one after another
 // took 1.4 us).
 // ---------------------------------------------------------------------------
 constexpr int kBmMaxK = kBeamMaxW + kBeamMaxStop;
 constexpr int kBmJoinWaves = 16;
-constexpr int kBmAhead = 8;  // keys of a lane that are requested at once
 constexpr int kBmOpen = kBeamMaxW * kBmMaxK;
+// AHEAD: keys of a lane that are requested at once, 4 where all of a row are so (16 beams
+// 8.6 us, with 8 9.1; 4 beams of 25 chunks 5.7 and 5.8).
+template <int AHEAD>
 __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs a) {
   __shared__ u64 lists[kBmJoinWaves][kBmList + 8];
   __shared__ u64 value[kBmOpen];  // of (place, rank), ordered; 0: none
@@ -379,9 +381,9 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
     // there that is used)
     const float score = a.score[row];
     BmSum sum = sums[min(lane, a.chunks - 1)];
-    u64 k[kBmAhead];
+    u64 k[AHEAD];
 #pragma unroll
-    for (int h = 0; h < kBmAhead; ++h) k[h] = keys[min(64 * h + lane, all - 1)];
+    for (int h = 0; h < AHEAD; ++h) k[h] = keys[min(64 * h + lane, all - 1)];
     bool alive = bm_alive(score);
     if (lane == 0 && (score != score || score == INFINITY)) flag_dev_err(a.err, kDevErrBeam);
     double lse = 0.0;
@@ -401,24 +403,24 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
       lse = (double)m + log(s);
     }
     if (alive) {
-      for (int i0 = 0; i0 < all; i0 += 64 * kBmAhead) {
+      for (int i0 = 0; i0 < all; i0 += 64 * AHEAD) {
         if (i0 > 0)
 #pragma unroll
-          for (int h = 0; h < kBmAhead; ++h) k[h] = keys[min(i0 + 64 * h + lane, all - 1)];
+          for (int h = 0; h < AHEAD; ++h) k[h] = keys[min(i0 + 64 * h + lane, all - 1)];
         u64 top = 0;
 #pragma unroll
-        for (int h = 0; h < kBmAhead; ++h) {
+        for (int h = 0; h < AHEAD; ++h) {
           k[h] = i0 + 64 * h + lane < all ? k[h] : 0;
           top = max(top, k[h]);
         }
         list.bound((uint32_t)(top >> 32), K);
         uint32_t reach = 0;  // bit h: the lane's k[h] does (past the keys: 0, which does not)
 #pragma unroll
-        for (int h = 0; h < kBmAhead; ++h) reach |= (uint32_t)((uint32_t)(k[h] >> 32) >= list.least) << h;
+        for (int h = 0; h < AHEAD; ++h) reach |= (uint32_t)((uint32_t)(k[h] >> 32) >= list.least) << h;
         while (__any(reach != 0)) {  // every lane its next one
-          uint32_t lo[kBmAhead], hi[kBmAhead];
+          uint32_t lo[AHEAD], hi[AHEAD];
 #pragma unroll
-          for (int h = 0; h < kBmAhead; ++h) {
+          for (int h = 0; h < AHEAD; ++h) {
             lo[h] = (uint32_t)k[h];
             hi[h] = (uint32_t)(k[h] >> 32);
           }
@@ -566,7 +568,9 @@ void launch_beam_select(BeamSelectArgs a, hipStream_t st) {
   if (a.groups > 4) hipLaunchKernelGGL(k_beam_part<kBmGroups>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(k_beam_part<4>, grid, dim3(256), 0, st, a);
   const int waves = std::min(std::max(a.W, 2), kBmJoinWaves);
-  hipLaunchKernelGGL(k_beam_join, dim3((unsigned)a.B), dim3(64 * waves), 0, st, a);
+  const dim3 requests((unsigned)a.B), threads(64 * waves);
+  if (a.chunks * a.K > 256) hipLaunchKernelGGL(k_beam_join<8>, requests, threads, 0, st, a);
+  else hipLaunchKernelGGL(k_beam_join<4>, requests, threads, 0, st, a);
 }
 
 constexpr int kReorderUnits = 4;  // 1, 2, 4, 8: 24, 22.6, 22.6, 31 us (136 MB, see below)
