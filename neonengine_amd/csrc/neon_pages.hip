@@ -292,19 +292,17 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
   if (threadIdx.x == 0) w.need_in[plan] = all;
 }
 
-// sum of n numbers, by the wave
-__device__ __forceinline__ int64_t pg_wave_total(const int* v, int n) {
+// sum of n numbers, by the wave (of pages or of table entries: 32 bits)
+__device__ __forceinline__ int pg_wave_total(const int* v, int n) {
   const int lane = threadIdx.x & 63;
-  int64_t s = 0;
+  int s = 0;
   for (int i = lane; i < n; i += 64) s += v[i];
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-  return s;
+  return __builtin_amdgcn_readlane(pg_wave_scan(s), 63);
 }
 
 // What a page's count becomes: r without the pages that are taken now, `rank` its place
 // among the free ones; k sequences would go on writing it, and all that get a copy leave.
-__device__ __forceinline__ int pg_count(int r, int64_t rank, int64_t taken, int k) {
+__device__ __forceinline__ int pg_count(int r, int rank, int taken, int k) {
   if (r == 0) return rank < taken ? 1 : 0;
   return k > 0 && r > 1 ? r - (r == k ? k - 1 : k) : r;
 }
@@ -315,8 +313,8 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < w.chunks) {
     __shared__ int sums[16];
-    const int64_t taken = pg_wave_total(w.need_in, w.plans);
-    const int64_t before = pg_wave_total(w.free_in, blockIdx.x);
+    const int taken = pg_wave_total(w.need_in, w.plans);
+    const int before = pg_wave_total(w.free_in, blockIdx.x);
     int r[4], k[4], rank[4];
     bool is[4];
 #pragma unroll
@@ -353,20 +351,20 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
     if (copy < 0) a.copy_dst[b] = -1;
   }
   if (i1 <= old_end || i0 >= goal) return;
-  const int64_t first = pg_wave_total(w.need_in, b / kPgSeqs) + w.before[b];
-  const int64_t n_free = pg_wave_total(w.free_in, w.chunks);
+  const int first = pg_wave_total(w.need_in, b / kPgSeqs) + w.before[b];
+  const int n_free = pg_wave_total(w.free_in, w.chunks);
   for (int ib = max(i0, old_end); ib < i1; ib += 64) {
     const int i = ib + lane;
-    const int64_t j = first + i - old_end;
+    const int j = first + (i - old_end);
     // the chunk that holds the j-th free page, chunks 64 at a time
     int id2 = -1;
     const bool mine = i < i1 && j < n_free;
-    int64_t from = 0;
+    int from = 0;
     for (int c0 = 0; c0 < w.chunks && __any(mine && j >= from); c0 += 64) {
       const int in = c0 + lane < w.chunks ? w.free_in[c0 + lane] : 0;
       const int to = pg_wave_scan(in), all = __builtin_amdgcn_readlane(to, 63);
       const bool now = mine && j >= from && j < from + all;
-      const int want = now ? (int)(j - from) : 0;
+      const int want = now ? j - from : 0;
       int c = 0;  // the first of the 64 sums above it
 #pragma unroll
       for (int step = 32; step > 0; step >>= 1) {
@@ -598,7 +596,7 @@ void launch_pages_fork(const PagesForkArgs& a, hipStream_t st) {
 // to the free ids below U, both in their order, so that no page is read and written.
 // 1. used pages of each chunk; 2. the lists, and what becomes of every page; 3. the
 // counts and the tables.
-// Bound: the chain of each launch: 131072 pages, 512 sequences, 2.5 + 5.4 + 5.6 us for
+// Bound: the chain of each launch: 131072 pages, 512 sequences, 2.4 + 5.0 + 5.6 us for
 // 2.4 MB.
 // ---------------------------------------------------------------------------
 struct PcWork {
@@ -653,15 +651,15 @@ __global__ __launch_bounds__(256) void k_pages_lists(PagesCompactArgs a) {
   int r[4], u[4], rank[4], rank2[4];
   bool is[4], low_is[4];
   pc_load(a.refs, a.n_pages, blockIdx.x, r, is);
-  const int before = (int)pg_wave_total(w.used_in, blockIdx.x);
-  const int U = (int)pg_wave_total(w.used_in, w.chunks);
+  const int before = pg_wave_total(w.used_in, blockIdx.x);
+  const int U = pg_wave_total(w.used_in, w.chunks);
   // used pages below U: whole chunks, and those of U's own
   const int cu = U / kPgChunk;
   pc_load(a.refs, a.n_pages, cu, u, low_is);
 #pragma unroll
   for (int j = 0; j < 4; ++j) low_is[j] &= cu * kPgChunk + 256 * j + (int)threadIdx.x < U;
   pg_ranks<4, 4>(is, rank, sums);
-  const int low = (int)pg_wave_total(w.used_in, cu) + pg_ranks<4, 4>(low_is, rank2, sums2);
+  const int low = pg_wave_total(w.used_in, cu) + pg_ranks<4, 4>(low_is, rank2, sums2);
   const int moves = U - low;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     w.sums[0] = U;
@@ -699,7 +697,7 @@ __global__ __launch_bounds__(256) void k_pages_map(PagesCompactArgs a, int parts
     bool is[4];
     pc_load(a.refs, a.n_pages, blockIdx.x, r, is);
     const int U = w.sums[0];
-    const int before = (int)pg_wave_total(w.used_in, blockIdx.x);
+    const int before = pg_wave_total(w.used_in, blockIdx.x);
     pg_ranks<4, 4>(is, rank, sums);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
