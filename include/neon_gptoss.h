@@ -246,7 +246,8 @@ neon_status neon_tensor_ptr(neon_ctx* ctx, const char* name, void** ptr,
  * neon_moe_prefill) lay outside [0, E).  Such a slot is dropped (adds 0)
  * instead of reading past the expert arrays.  (What the calls of a paged cache,
  * of sampling and of beam search report stands with them; NEON_EKV_FULL: pages
- * ran out in neon_pages_fork.)  The context-level reads
+ * ran out in neon_pages_fork, given before the page ids that later calls missed
+ * for it.)  The context-level reads
  * (neon_read_tokens / _logits / _activation) make the same check for the
  * context's own kernels.  (The reference has no counterpart: its Systems
  * throw on the host and do no device-side validation.) */

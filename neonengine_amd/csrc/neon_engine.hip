@@ -1722,15 +1722,17 @@ extern "C" neon_status neon_device_check(void* stream) {
   if (bits & kDevErrSyncTimeout)
     KFAIL(NEON_EHIP, "a grid-wide wait inside a kernel-level call timed out (status bits 0x%x); "
           "its results are invalid", bits);
+  // (before what follows from it: the step's append and attention, and the next fork, meet
+  // the entries without a page)
+  if (bits & kDevErrPagesFull)
+    KFAIL(NEON_EKV_FULL, "neon_pages_fork needed more pages than are free (status bits 0x%x); the "
+          "entries without one are -1", bits);
   if (bits & kDevErrPagedRows)
     KFAIL(NEON_EINVAL, "a paged call saw row starts or lengths outside its buffers (status bits "
           "0x%x); that sequence was left out", bits);
   if (bits & kDevErrPageId)
     KFAIL(NEON_EINVAL, "a paged call needed a page id outside [0, n_pages) (status bits 0x%x); "
           "that page's rows were dropped or hidden", bits);
-  if (bits & kDevErrPagesFull)
-    KFAIL(NEON_EKV_FULL, "neon_pages_fork needed more pages than are free (status bits 0x%x); the "
-          "entries without one are -1", bits);
   if (bits & kDevErrPagePlan)
     KFAIL(NEON_EINVAL, "neon_pages_fork or neon_pages_compact saw a parent, length, keep, add or "
           "reference count out of range (status bits 0x%x); that sequence was left out", bits);

@@ -444,3 +444,27 @@ def test_two_streams_at_once(sizes):
     for c in calls:
         c.check()
     ne.device_check()
+
+
+@pytest.mark.parametrize("max_pages", [10, 9000])
+@pytest.mark.parametrize("steps", [1, 2])
+def test_pages_run_out_in_a_run(max_pages, steps):
+    """The fork of a step needs more pages than are free; the append and the attention that
+    follow, and the fork of the next step, meet the entries without one.  The check names
+    the cause, once.  (max_pages: a plan of one launch, and of three.)"""
+    rng = np.random.default_rng(12)
+    prompts = [rng.integers(0, V, n) for n in (16, 31)]
+    # 3 pages of the prompts; 4 and 3 more for the first tokens; then 4 more for the second
+    s = Search(prompts, 4, 12, max_pages, [], seed=13)
+    s.choose()
+    s.advance(first=True)
+    ne.device_check()
+    assert int((s.refs == 0).sum()) == 2
+    say(f"pages run out, width {max_pages}, {steps} steps")
+    for _ in range(steps):
+        s.choose()
+        s.advance()
+    with pytest.raises(ne.NeonError) as e:
+        ne.device_check()
+    assert e.value.status == ne.NEON_EKV_FULL
+    ne.device_check()
