@@ -310,6 +310,7 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamSelectArgs a) {
     ms[wave] = m;
   }
   base = uni(base);
+  wave_lds_sync();  // the list's keys are other lanes'
   if (lane < list.n) joint[base + lane] = keys[wave][lane];
   __syncthreads();
   const int all = total, i = threadIdx.x;
