@@ -595,7 +595,7 @@ neon_status neon_beam_select(const float* logits, int64_t stride, int B, int W, 
 /* Moves the states of beams in place: row r of every state becomes what row
  * parent[r] was (device int32 [B W], a row of the same request; -1 or r itself: left
  * as it is).  states: host array of n_states device pointers (16-byte aligned, to
- * memory that does not overlap), each
+ * memory that does not overlap: NEON_EINVAL), each
  * [B W][slabs][T][row_bytes] (row_bytes a multiple of 4; a contiguous cache of
  * neon_attn_decode has slabs = Hkv, T = T_max, row_bytes = 2 D).  len [B W] (device
  * int32, or NULL for T): the first min(len[parent[r]], T) rows of each slab are moved,

@@ -696,6 +696,9 @@ class BeamStates:
         if any(tuple(t.shape) != shape or t.element_size() != size or
                t.get_device() != self.device for t in states):
             raise ValueError("BeamStates: states of one shape and type, on one device")
+        starts, nbytes = sorted(t.data_ptr() for t in states), _nbytes(states[0])
+        if any(b - a < nbytes for a, b in zip(starts, starts[1:])):
+            raise ValueError("BeamStates: two states overlap")
         self.states = states  # keeps them alive
         self.W, self.rows = W, shape[0]
         slabs, T, row = (1, shape[1], shape[2:]) if len(shape) < 4 else (shape[1], shape[2], shape[3:])

@@ -2463,6 +2463,22 @@ extern "C" neon_status neon_beam_reorder(void* const* states, int n_states, int 
       row_bytes % 4 || !beam_reorder_fits(a))
     KFAIL(NEON_EINVAL, "neon_beam_reorder: bad shape B=%d W=%d slabs=%d T=%d row_bytes=%d (a "
           "multiple of 4)", B, W, slabs, T, row_bytes);
+  // (a state moved twice at once would read what it has written)
+  if (n_states > 1) {
+    std::vector<uintptr_t> at;
+    try {
+      at.resize((size_t)n_states);
+    } catch (...) {
+      KFAIL(NEON_ENOMEM, "neon_beam_reorder: no memory for %d states", n_states);
+    }
+    for (int x = 0; x < n_states; ++x) at[x] = (uintptr_t)states[x];
+    std::sort(at.begin(), at.end());
+    // (the launch holds them, so this fits)
+    const uint64_t bytes = (uint64_t)B * W * slabs * T * row_bytes;
+    for (int x = 1; x < n_states; ++x)
+      if (at[x] - at[x - 1] < bytes)
+        KFAIL(NEON_EINVAL, "neon_beam_reorder: two states overlap");
+  }
   a.err = device_status_word();
   if (n_states > 0) launch_beam_reorder(a, states, n_states, S(stream));
   KLAUNCHED();

@@ -178,3 +178,25 @@ def test_plain_compact():
                             [20, 16], 16, np.full((2, 2), -9, np.int32))
     assert [x.tolist() for x in out] == [[1, 2, 1, 0, 0, 0], [[0, 1], [1, -9]], [-1, 1, -1, -1, 0, 2],
                                          [4, 5, -1], [0, 2, -1]]
+
+
+# ---------------------------------------------------------------------------
+# states that overlap would be moved twice at once
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("others", [(Q,), (Q + 16,), (Q + 16384 - 16,), (Q - 16384 + 16,), (1 << 30, Q + 8192),
+                                    tuple((1 << 30) + 16384 * i for i in range(70)) + (Q + 16,)])
+def test_reorder_refuses_states_that_overlap(others):
+    # 2 requests of 4 places, 2 slabs of 8 rows of 128 bytes: 16384 bytes
+    assert reorder(states=(Q, *others)) == ne.NEON_EINVAL
+    assert b"overlap" in ne.lib().neon_last_error(None)
+
+
+def test_beam_states_refuse_tensors_that_overlap():
+    torch = pytest.importorskip("torch")
+    x, y = torch.zeros(8, 2, 6, 4), torch.zeros(8, 2, 6, 4)
+    whole = torch.zeros(9, 2, 6, 4)
+    for states in ([x, x], [x, y, x], [whole[:8], whole[1:]], [whole[1:], y, whole[:8]]):
+        with pytest.raises(ValueError, match="overlap"):
+            ne.beam_states(states, 4)
+    both = torch.zeros(2, 8, 2, 6, 4)
+    assert ne.beam_states([both[1], x, both[0]], 4).rows == 8
