@@ -238,6 +238,12 @@ __device__ __forceinline__ int pg_block_scan(int v, int* sums, int& all) {
   return (wave > 0 ? before : 0) + x - v;
 }
 
+// A page's holders: its count after the change, and no fewer than go on writing it (a count
+// that says less is wrong: the page is neither free nor written by two).
+__device__ __forceinline__ int pg_holders(int count, int writers) {
+  return writers > 0 ? max(count, writers) : count;
+}
+
 __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
   __shared__ int waves[4];
   const PgWork w = pg_work(a.workspace, a.n_pages, a.B);
@@ -251,8 +257,9 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
     for (int j = 0; j < 4; ++j) {
       const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       const int r = p < a.n_pages ? a.refs[p] + pg_change(a)[p] : 1;
-      if (r < 0) flag_dev_err(a.err, kDevErrPagePlan);
-      is[j] = r == 0;
+      const int k = p < a.n_pages ? pg_writers(a)[p] : 0;
+      if (r < k) flag_dev_err(a.err, kDevErrPagePlan);
+      is[j] = pg_holders(r, k) == 0;
     }
     all = pg_ranks<4, 4>(is, rank, sums);
     int* ids = w.free_ids + (int64_t)blockIdx.x * kPgChunk;
@@ -274,8 +281,8 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
     if (pg_writes(a, q)) {
       const int p = a.table[(int64_t)q.parent * a.max_pages + kept - 1];
       if ((unsigned)p < (unsigned)a.n_pages) {
-        const int r = a.refs[p] + pg_change(a)[p];
-        const bool mine = r == pg_writers(a)[p] && pg_first(a)[p] == a.B - b;
+        const int k = pg_writers(a)[p], r = pg_holders(a.refs[p] + pg_change(a)[p], k);
+        const bool mine = r == k && pg_first(a)[p] == a.B - b;
         if (r > 1 && !mine) {
           copy = p;
           ++need;
@@ -300,8 +307,8 @@ __device__ __forceinline__ int pg_wave_total(const int* v, int n) {
   return __builtin_amdgcn_readlane(pg_wave_scan(s), 63);
 }
 
-// What a page's count becomes: r without the pages that are taken now, `rank` its place
-// among the free ones; k sequences would go on writing it, and all that get a copy leave.
+// What the count of a page of r holders becomes: `rank` is the place of a free one, k
+// sequences would go on writing it, and all that get a copy leave.
 __device__ __forceinline__ int pg_count(int r, int rank, int taken, int k) {
   if (r == 0) return rank < taken ? 1 : 0;
   return k > 0 && r > 1 ? r - (r == k ? k - 1 : k) : r;
@@ -320,8 +327,8 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
-      r[j] = p < a.n_pages ? a.refs[p] + pg_change(a)[p] : 1;
       k[j] = p < a.n_pages ? pg_writers(a)[p] : 0;
+      r[j] = p < a.n_pages ? pg_holders(a.refs[p] + pg_change(a)[p], k[j]) : 1;
       is[j] = r[j] == 0;
     }
     pg_ranks<4, 4>(is, rank, sums);
@@ -511,8 +518,11 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int p = 1024 * j + tid;
-    if (p < a.n_pages) r[j] = count[p];
-    if (r[j] < 0) flag_dev_err(a.err, kDevErrPagePlan);
+    if (p < a.n_pages) {
+      const int k = writers[p];
+      if (count[p] < k) flag_dev_err(a.err, kDevErrPagePlan);
+      r[j] = pg_holders(count[p], k);
+    }
     is[j] = r[j] == 0;
   }
   const int n_free = pg_ranks<8, 16>(is, rank, sums[0]);
@@ -523,7 +533,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
   const int goal = pg_pages(a.page_log2, q.keep + q.add);
   int copy = -1, taken;
   if (page >= 0) {
-    const int holders = count[page];
+    const int holders = pg_holders(count[page], writers[page]);
     if (holders > 1 && !(holders == writers[page] && first[page] == a.B - b)) copy = page;
   }
   const int old_end = kept - (copy >= 0 ? 1 : 0);

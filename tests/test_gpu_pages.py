@@ -193,6 +193,57 @@ def test_fork_numbers_that_do_not_fit(width):
         ne.device_check()
 
 
+def check_wrong_counts(refs, table, length, want, page=16, **seqs):
+    """A fork whose counts are not those of the table: its outputs (entries past a row's
+    pages are -9), and the error, once."""
+    start = np.full_like(table, -9)
+    for name, w in zip(("refs", "table", "length", "src", "dst", "rows"), want):
+        if name == "table":
+            for row, ids in zip(start, w):
+                row[:len(ids)] = ids
+    want = [w if i != 1 else start for i, w in enumerate(want)]
+    got = run_fork(refs, table, length, page, len(want[2]), **seqs)
+    for name, g, w in zip(("refs", "table", "length", "src", "dst", "rows"), got, want):
+        assert np.array_equal(g, w), (name, g, w)
+    with pytest.raises(ne.NeonError) as e:
+        ne.device_check()
+    assert e.value.status == ne.NEON_EINVAL
+    ne.device_check()
+
+
+WIDTHS = [4, 40000]  # a plan of one launch, and of three
+
+
+def wide_table(rows, width):
+    t = np.full((len(rows), width), -7, np.int32)
+    for r, ids in zip(t, rows):
+        r[:len(ids)] = ids
+    return t
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+def test_fork_counts_below_the_writers(width):
+    """A page that goes on being written by more sequences than its count says: the first
+    keeps it, the others get a copy, its count is 1, and the error is set."""
+    i32 = lambda *x: np.array(x, np.int32)
+    for count in (1, 2):
+        refs = i32(0, 0, 0, 0, 0, count)
+        say(f"count {count} of a page of three writers")
+        check_wrong_counts(refs, wide_table([[5]] * 3, width), i32(10, 4, 7),
+                           (i32(1, 1, 0, 0, 0, 1), [[5], [0], [1]], i32(11, 5, 8), i32(-1, 5, 5),
+                            i32(-1, 0, 1), i32(0, 4, 7)))
+    # children of one row, which the count leaves out
+    say("count 0 of a page of two writers")
+    check_wrong_counts(i32(0, 1, 0), wide_table([[2], [1]], width), i32(10, 16),
+                       (i32(1, 0, 1), [[2], [0]], i32(11, 11), i32(-1, 2), i32(-1, 0), i32(0, 10)),
+                       parent=[0, 0])
+    # a writer whose page has no count at all
+    say("count 0 of a page that is written")
+    check_wrong_counts(i32(0, 0, 0), wide_table([[0], []], width), i32(10, 0),
+                       (i32(1, 1, 0), [[0], [1]], i32(11, 5), i32(-1, -1), i32(-1, -1), i32(0, 0)),
+                       add=[1, 5])
+
+
 @pytest.mark.parametrize("n_pages,B,page,top", [(1, 1, 16, 10), (2, 1, 16, 16), (5, 2, 16, 30), (1023, 7, 16, 900),
                                                 (1024, 7, 64, 900), (1025, 30, 16, 100), (5000, 300, 16, 200),
                                                 (70000, 64, 16, 9000)])
