@@ -634,8 +634,8 @@ neon_status neon_beam_reorder(void* const* states, int n_states, int B, int W, i
  * Where no page is left the entry is -1 and neon_device_check gives NEON_EKV_FULL; a
  * sequence whose numbers do not fit (parent, keep, add, a length) is left without
  * tokens, entries outside [0, n_pages) are passed on and not counted, and a count below
- * the sequences that go on writing the page is taken as theirs
- * (neon_device_check NEON_EINVAL, also for a count that falls below 0).
+ * the sequences that go on writing the page, or of none where one keeps it, is taken as
+ * that many (neon_device_check NEON_EINVAL, also for a count that falls below 0).
  *   workspace  neon_pages_workspace(n_pages, B) bytes, 16-byte aligned, any contents;
  *   counters   neon_pages_counters(n_pages) bytes, zero before their first use and
  *              left zero by every call. */

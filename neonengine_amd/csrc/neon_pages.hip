@@ -108,11 +108,15 @@ __host__ __device__ inline PgWork pg_work(void* ws, int n_pages, int B) {
   w.free_ids = p;
   return w;
 }
-// counters: [n_pages] change of the count, [n_pages] writers, [n_pages] B - first writer
+// counters: [n_pages] change of the count, [n_pages] writers, [n_pages] B - first writer,
+// [n_pages] bytes: 1 where a sequence of the result keeps the page
 __device__ __forceinline__ int* pg_change(const PagesForkArgs& a) { return a.counters; }
 __device__ __forceinline__ int* pg_writers(const PagesForkArgs& a) { return a.counters + a.n_pages; }
 __device__ __forceinline__ int* pg_first(const PagesForkArgs& a) {
   return a.counters + 2 * (int64_t)a.n_pages;
+}
+__device__ __forceinline__ uint8_t* pg_held(const PagesForkArgs& a) {
+  return reinterpret_cast<uint8_t*>(a.counters + 3 * (int64_t)a.n_pages);
 }
 
 // A row gives up page o and its new sequence takes up page p (where they do).  A page of
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts
   int32_t* out = a.table_out + (int64_t)min(row, a.B - 1) * a.max_pages;
   const bool moves = now != out && kept > 0;  // the kept entries into a table of their own
   const int end = min(i1, max(held, kept));
-  if (end > (moves ? i0 : max(i0, from))) {
+  if (end > i0) {
     // (inside the row whatever i is: a load under a condition of its own is waited for)
     int o[kPgSpan / 64], p[kPgSpan / 64];
 #pragma unroll
@@ -166,6 +170,9 @@ __global__ __launch_bounds__(256) void k_pages_change(PagesForkArgs a, int parts
       for (int u = 0; u < kPgSpan / 64; ++u)
         if (i0 + 64 * u + lane < min(end, kept)) out[i0 + 64 * u + lane] = p[u];
     }
+#pragma unroll
+    for (int u = 0; u < kPgSpan / 64; ++u)
+      if (i0 + 64 * u + lane < min(end, kept) && (unsigned)p[u] < (unsigned)a.n_pages) pg_held(a)[p[u]] = 1;
     if (from < end) {
       bool bad = false;
 #pragma unroll
@@ -238,10 +245,12 @@ __device__ __forceinline__ int pg_block_scan(int v, int* sums, int& all) {
   return (wave > 0 ? before : 0) + x - v;
 }
 
-// A page's holders: its count after the change, and no fewer than go on writing it (a count
-// that says less is wrong: the page is neither free nor written by two).
-__device__ __forceinline__ int pg_holders(int count, int writers) {
-  return writers > 0 ? max(count, writers) : count;
+// A page's holders: its count after the change, and no fewer than go on writing it, or than
+// one that keeps it (a count that says less is wrong: the page is neither free nor written
+// by two).  Of these `least` are known.
+__device__ __forceinline__ int pg_least(int writers, int held) { return max(writers, held); }
+__device__ __forceinline__ int pg_holders(int count, int least) {
+  return least > 0 ? max(count, least) : count;
 }
 
 __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
@@ -257,9 +266,9 @@ __global__ __launch_bounds__(256) void k_pages_plan(PagesForkArgs a) {
     for (int j = 0; j < 4; ++j) {
       const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       const int r = p < a.n_pages ? a.refs[p] + pg_change(a)[p] : 1;
-      const int k = p < a.n_pages ? pg_writers(a)[p] : 0;
-      if (r < k) flag_dev_err(a.err, kDevErrPagePlan);
-      is[j] = pg_holders(r, k) == 0;
+      const int least = p < a.n_pages ? pg_least(pg_writers(a)[p], pg_held(a)[p]) : 0;
+      if (r < least) flag_dev_err(a.err, kDevErrPagePlan);
+      is[j] = pg_holders(r, least) == 0;
     }
     all = pg_ranks<4, 4>(is, rank, sums);
     int* ids = w.free_ids + (int64_t)blockIdx.x * kPgChunk;
@@ -328,7 +337,7 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
     for (int j = 0; j < 4; ++j) {
       const int p = blockIdx.x * kPgChunk + 256 * j + threadIdx.x;
       k[j] = p < a.n_pages ? pg_writers(a)[p] : 0;
-      r[j] = p < a.n_pages ? pg_holders(a.refs[p] + pg_change(a)[p], k[j]) : 1;
+      r[j] = p < a.n_pages ? pg_holders(a.refs[p] + pg_change(a)[p], pg_least(k[j], pg_held(a)[p])) : 1;
       is[j] = r[j] == 0;
     }
     pg_ranks<4, 4>(is, rank, sums);
@@ -340,6 +349,7 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
       pg_change(a)[p] = 0;
       pg_writers(a)[p] = 0;
       pg_first(a)[p] = 0;
+      pg_held(a)[p] = 0;
     }
     return;
   }
@@ -407,6 +417,7 @@ constexpr int kPcOneRows = 256;       // of the compaction
 __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs a) {
   __shared__ int count[kPgOnePages], writers[kPgOnePages], first[kPgOnePages];
   __shared__ uint16_t free_ids[kPgOnePages];
+  __shared__ uint8_t keeps[kPgOnePages];  // 1 where a sequence of the result keeps the page
   __shared__ int s_parent[kPgOneThreads], s_kept[kPgOneThreads], s_held[kPgOneThreads];
   __shared__ int s_goal[kPgOneThreads], s_before[kPgOneThreads];
   __shared__ int sums[2][128];
@@ -425,6 +436,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
     if (1024 * j + tid < a.n_pages) {
       count[1024 * j + tid] = r[j];
       writers[1024 * j + tid] = first[1024 * j + tid] = 0;
+      keeps[1024 * j + tid] = 0;
     }
   s_held[tid] = len;
   __syncthreads();
@@ -464,7 +476,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
     w.own = par == row;
     w.from = w.own ? min(w.k, w.held) : 0;
     w.moves = w.now != w.out && w.k > 0;
-    w.i0 = w.moves ? 0 : w.from;
+    w.i0 = 0;
     w.end = max(w.held, w.k);
   };
   auto load = [&](Row& w) {
@@ -482,6 +494,9 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
       for (int u = 0; u < 4; ++u)
         if (w.i0 + 64 * u + lane < w.k) w.out[w.i0 + 64 * u + lane] = w.p[u];
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (w.i0 + 64 * u + lane < w.k && (unsigned)w.p[u] < (unsigned)a.n_pages) keeps[w.p[u]] = 1;
     if (w.from < w.end) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -519,9 +534,9 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
   for (int j = 0; j < 8; ++j) {
     const int p = 1024 * j + tid;
     if (p < a.n_pages) {
-      const int k = writers[p];
-      if (count[p] < k) flag_dev_err(a.err, kDevErrPagePlan);
-      r[j] = pg_holders(count[p], k);
+      const int least = pg_least(writers[p], keeps[p]);
+      if (count[p] < least) flag_dev_err(a.err, kDevErrPagePlan);
+      r[j] = pg_holders(count[p], least);
     }
     is[j] = r[j] == 0;
   }
@@ -581,7 +596,7 @@ __global__ __launch_bounds__(kPgOneThreads) void k_pages_fork_one(PagesForkArgs 
 static bool pages_one(int n_pages, int B, int most, int max_pages) {
   return n_pages <= kPgOnePages && B <= most && (int64_t)B * max_pages <= kPgOneEntries;
 }
-size_t pages_counters(int n_pages) { return (size_t)n_pages * 12; }
+size_t pages_counters(int n_pages) { return (size_t)n_pages * 12 + ((size_t)n_pages + 3) / 4 * 4; }
 static int64_t pages_parts(int max_pages) { return ((int64_t)max_pages + kPgSpan - 1) / kPgSpan; }
 // All entries of a table count in 32 bits (what the sequences need is summed), and then
 // the grids hold them too.

@@ -244,6 +244,39 @@ def test_fork_counts_below_the_writers(width):
                        add=[1, 5])
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_fork_held_pages_without_a_count(width, in_place):
+    """A page that a sequence of the result holds is not handed out, whatever its count
+    says: it stays with a count of 1, and the error is set."""
+    torch = torch_cuda()
+    i32 = lambda *x: np.array(x, np.int32)
+    # the full page 0 of the first sequence was never counted; the second grows
+    cases = [("never counted", i32(0, 1, 1, 0), [[0, 2], [1]], i32(20, 16), None, i32(1, 16),
+              i32(1, 1, 1, 1), [[0, 2], [1, 3]], i32(21, 32)),
+             # a page of two sequences that was released twice: one leaves, the other stays
+             ("released twice", i32(1, 1, 0), [[0], [0, 1]], i32(16, 20), i32(0, 20), i32(0, 13),
+              i32(1, 1, 1), [[], [0, 1, 2]], i32(0, 33))]
+    for what, refs, rows, length, keep, add, refs_out, rows_out, len_out in cases:
+        if in_place:
+            table = wide_table(rows, width)
+            d = [to_dev(x) for x in (refs, table, length)]
+            copies = [torch.full((2,), 99, dtype=torch.int32, device="cuda") for _ in range(3)]
+            ne.pages_fork(*d, 16, *d, copies, keep=None if keep is None else to_dev(keep), add=to_dev(add))
+            got = [to_host(x) for x in d]
+            assert np.array_equal(got[0], refs_out) and np.array_equal(got[2], len_out), (what, got)
+            for row, ids in zip(got[1], rows_out):
+                assert row[:len(ids)].tolist() == ids
+            with pytest.raises(ne.NeonError) as e:
+                ne.device_check()
+            assert e.value.status == ne.NEON_EINVAL
+            ne.device_check()
+        else:
+            check_wrong_counts(refs, wide_table(rows, width), length,
+                               (refs_out, rows_out, len_out, i32(-1, -1), i32(-1, -1), i32(0, 0)),
+                               keep=keep, add=add)
+
+
 @pytest.mark.parametrize("n_pages,B,page,top", [(1, 1, 16, 10), (2, 1, 16, 16), (5, 2, 16, 30), (1023, 7, 16, 900),
                                                 (1024, 7, 64, 900), (1025, 30, 16, 100), (5000, 300, 16, 200),
                                                 (70000, 64, 16, 9000)])
