@@ -95,6 +95,34 @@ def test_select_orders(form, V):
     ne.device_check()
 
 
+# Plateaus of 256 tokens (a group of a wave, whose first one the exponentials are relative
+# to until another is more than 64 above it), repeated along the row
+RISES = {"mask of -1e9": [-1e9, 0.0], "mask of the lowest": [np.finfo(np.float32).min, 0.0],
+         "just below": [-63.0, 0.0], "just above": [-66.0, 0.0], "by 100": [-100.0, 0.0],
+         "stairs": [-1e30, -1e9, -2e4, -500.0, -100.0, 0.0, -3.0], "fall and rise": [0.0, -1e4, 90.0, -1e9],
+         "past the exponent": [0.0, 710.0, 1500.0, 3000.0], "huge": [-1e38, 1e38, 3e38, -3e38],
+         "open": [-np.inf, -1e9, 0.0, np.nan, 200.0]}
+
+
+@pytest.mark.parametrize("V", [300, 1500, 8000, 40000, 600011])
+@pytest.mark.parametrize("form", list(RISES))
+def test_select_logits_that_rise_by_much(form, V):
+    """Tokens far above those before them; one group of a wave, and several (up to 4 and up
+    to 8 of them: 12 and 360 rows)."""
+    for B in (3, 90) if V < 50000 else (3,):
+        W = 4
+        rng = np.random.default_rng(V + B)
+        steps = np.array(RISES[form])[np.arange(V) // 256 % len(RISES[form])]
+        l = (steps + rng.normal(0, 2.0, (B * W, V))).astype(np.float32)
+        l[1] = np.roll(l[1], 256)
+        l[2] = l[2, ::-1]
+        score = (-12 - 2 * rng.random(B * W)).astype(np.float32)
+        stop = [int(l[0].argmax()) if form != "open" else int(np.nanargmax(l[0])), V - 1]
+        say(f"rises {form} V={V} B={B}")
+        check(run(l, score, W, stop), beam_util.select(l, score, W, stop))
+        ne.device_check()
+
+
 def test_select_first_step_and_dead_requests():
     rng = np.random.default_rng(5)
     l, score = case(rng, 6, 4, 3001)
