@@ -566,7 +566,8 @@ neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
 
 /* The next beams from logits (device fp32, rows [B W] `stride` >= V elements
  * apart).  A candidate (place w, token t) has the value
- *   v = score[w] + l[w][t] - log sum_u exp(l[w][u])   (64 bits, rounded once),
+ *   v = score[w] + l[w][t] - log sum_u exp(l[w][u])   (64 bits, rounded once; the
+ *       exponentials near the largest to 2^-45),
  * candidates are ordered by (v descending, place ascending, token ascending), those
  * of one place by their logit.
  *   - The W best candidates that are no stop token (stop [n_stop], device ids, at
@@ -580,9 +581,10 @@ neon_status neon_sample_rows(const float* logits, int64_t stride, int B, int V,
  *     end_score [B W], a request's in their order from its first entry on, then -1,
  *     -1, -inf.  All three may be NULL.
  * A first step has one beam per request: the others' scores are -inf.  Logits of
- * -inf and NaN are never chosen.  A beam with a score of NaN or +inf or a logit of
- * +inf, or with nothing above -inf, has no candidates (neon_device_check gives
- * NEON_EINVAL for the first three).  B is 1 to 65535, V up to 2^24.
+ * -inf and NaN are never chosen and add nothing to the sum.  A beam with a score of
+ * NaN or +inf or a logit of +inf, or with nothing above -inf, has no candidates
+ * (neon_device_check gives NEON_EINVAL for the first three).  B is 1 to 65535, V up to
+ * 2^24.
  * workspace: neon_beam_select_workspace(...) bytes, 16-byte aligned, any contents;
  * they serve every call of up to B requests of the same W, V and n_stop. */
 size_t neon_beam_select_workspace(int B, int W, int V, int n_stop);

@@ -19,9 +19,13 @@ typedef unsigned long long u64;
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---------------------------------------------------------------------------
-// The K best of what a wave sees.  The K-th largest of the lanes' maxima is a bound that
-// few others reach (K lanes hold something at least as large), so what reaches it goes
-// into a list in LDS, and its order is found by counting.
+// The K best of what a wave sees.  The K-th largest of the lanes' maxima is a bound (K
+// lanes hold something at least as large): what reaches it goes into a list in LDS, and its
+// order is found by counting.  Few others reach it where the lanes see alike.  They do in a
+// row's tokens; in the join lane i reads keys 64 h + i of ordered lists of K, so where K
+// divides 64 a lane sees one rank of all lists and the bound is loose (2 requests of 32
+// beams, 88480 tokens: 62 us with K = 32, 43 with 33; one of 16, 201088: 25.5 with 16,
+// 19.7 with 17).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ u64 bm_lane_key(u64 v, int lane) {
   return (u64)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
@@ -146,9 +150,11 @@ __device__ __forceinline__ double bm_value64(u64 k) {
   return __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
 }
 
-// exp(x) for x <= 0, to 2^-45: 2^f by a polynomial of degree 9 on [-1/2, 1/2]
-// (interpolated at the Chebyshev points, 1.9e-14), the exponent added as an integer.
-// 2^-1020 stands for all below it.  The coefficients stay in scalar registers: as
+// exp(x) for x up to kBmAbove: 2^f by a polynomial of degree 9 on [-1/2, 1/2]
+// (interpolated at the Chebyshev points, 1.9e-14), the exponent added as an integer.  x / ln 2
+// is rounded, so the error is 1.9e-14 + |x| 2^-53 of the value: 2^-45 near the largest, whose
+// sum this is for, under 1e-13 at -700.  2^-1020 stands for all below it; what comes of larger x
+// (past the exponents, garbage) is not used.  The coefficients stay in scalar registers: as
 // literals each would be moved into vector registers first.
 struct BmExp {
   double c[10];
@@ -490,7 +496,7 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
         more += x > v;
         as_much += x >= v;
       }
-    if (as_much - more > 1)  // (a stop token is not among its own, with equal ones it is)
+    if (as_much - more > 1)  // (itself, and equal ones)
       for (int j = 0; j < n; ++j) more += among[j] == v && from[j] < from[c];
     if (more < W) (is ? over : next)[more] = from[c];
   }
@@ -528,8 +534,11 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void k_beam_join(BeamSelectArgs 
   }
 }
 
-// Groups of a wave: as many blocks as run at once, where there are enough tokens; no fewer
-// than 4 groups, since the join takes the chunks' keys one row after another.
+// Groups of a wave: about as many blocks as run at once, where there are enough tokens, 6
+// of each CU (k_beam_part<4> in 64 registers has 8 places there, <8> in 87 5: 16 requests of 4
+// beams, 201088 tokens, take 24.9 us in a graph with 1280 as with 1536, 2 of 32 beams, 88480
+// tokens, 53.5 and 62.3); no fewer than 4 groups, since the join takes the chunks' keys one
+// row after another.
 constexpr int64_t kBmPlaces = 1536;
 static int beam_groups(int64_t rows, int V) {
   const int64_t chunks = std::max<int64_t>(1, kBmPlaces / rows);

@@ -72,7 +72,8 @@ __device__ __forceinline__ bool pg_writes(const PagesForkArgs& a, const PgSeq& q
 // 1. What the change adds to and takes from the counts: a sequence that goes on in its
 //    own row gives up what it does not keep; another row is given up whole, and taken up
 //    by its continuations.  And who writes where: per page the number of sequences that
-//    will, and the first of them.
+//    will, and the first of them; and which pages are kept, so that none of them is handed
+//    out if its count is wrong.
 // 2. Which pages are free then (listed, a chunk of pages by a block), and what each
 //    sequence needs: pages past its last, and one for the page that it would write and
 //    that others hold too (if all holders write, the first keeps it).
@@ -80,7 +81,8 @@ __device__ __forceinline__ bool pg_writes(const PagesForkArgs& a, const PgSeq& q
 //    in them since the first launch.)
 // No order of threads reaches the result: sums, a maximum, and ranks.  Bound: the chain of
 // each launch (lookups of parent, length, entries; then the lists; then a page's place):
-// 1024 sequences of up to 4096 tokens, 45000 pages, 4.8 + 3.9 + 4.8 us for 1.5 MB.
+// 1024 sequences of up to 4096 tokens, 45000 pages, 5.0 + 5.0 + 4.7 us for 1.5 MB (without
+// the marks of the kept pages 4.8 + 3.9 + 4.8).
 // ---------------------------------------------------------------------------
 struct PgWork {  // the workspace
   int* free_in;   // [chunks] free pages of a chunk
@@ -403,10 +405,12 @@ __global__ __launch_bounds__(256) void k_pages_apply(PagesForkArgs a, int parts)
 // ---------------------------------------------------------------------------
 // The same for small pools and few sequences in one launch of one block: counts, writers
 // and free pages in LDS, a thread per sequence and eight pages a thread.
-// Bound: the chain of loads of a row, four rows a wave one after another (4.6 us of the
-// 9.6 that 64 beams of up to 8192 tokens take), and the host: in a graph 4 / 64 / 128 / 256
-// rows take 6.3 / 10.1 / 14 / 22 us against 8.6 / 10.2 / 10.8 / 10.8 in three launches,
-// and a call is enqueued in 8.4 us against 13.
+// Bound: the chain of loads of a row, a wave's four rows in two pairs one after another (4.6
+// us of the 9.6 that 64 beams of up to 8192 tokens take), and the host: in a graph 4 / 64 /
+// 128 / 256 rows take 5.8 / 9.9 to 10.5 / 15 / 24 us against 8.2 / 10.4 to 11.4 / 11.6 / 11.7
+// in three launches, and a call is enqueued in 9 us against 13.  (64 rows of 4003 tokens grown
+// in place: 8.8; their kept entries are read only so that no page among them is handed out,
+// 6.8 without.)
 // ---------------------------------------------------------------------------
 constexpr int kPgOneThreads = 1024;
 constexpr int kPgOnePages = 8 * kPgOneThreads;
